@@ -38,9 +38,10 @@ def cutlass_include() -> list:
                     "-I" + os.path.join(root, "tools", "util", "include")]
     raise RuntimeError("CUTLASS headers (sm100 collectives) not found")
 CUDA_SOURCES = ["kernels.cu", "engine.cu", "ops.cu", "noalloc.cu",
-                "prefill.cu", "gemm_sm100.cu", "safetensors.cpp", "tp.cpp"]
+                "prefill.cu", "gemm_sm100.cu", "paged.cu", "paged_attn.cu", "logits.cu",
+                "safetensors.cpp", "tp.cpp"]
 HEADERS = ["common.cuh", "kernels.h", "safetensors.h", "prefill.h",
-           "gemm_sm100.h", "tp.h"]
+           "gemm_sm100.h", "paged.h", "tp.h"]
 
 
 def nvcc() -> str:

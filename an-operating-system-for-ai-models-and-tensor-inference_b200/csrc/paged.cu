@@ -1,0 +1,438 @@
+// Serving over a paged KV cache: block tables and slot maps from request
+// lengths, and the pass that norms, rotates and stores q, k and v.
+#include <math.h>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "paged.h"
+
+namespace myos {
+
+int paged_check(const myos_paged_kv* kv) {
+  if (!kv || !kv->k || !kv->v) return MYOS_ERR_ARG;
+  if (kv->kv_dtype != MYOS_KV_F32 && kv->kv_dtype != MYOS_KV_BF16) return MYOS_ERR_ARG;
+  if (kv->reserved != 0) return MYOS_ERR_ARG;
+  if (kv->num_pages == 0 || kv->num_pages > 0x7fffffffu || kv->page_size == 0 ||
+      kv->page_size > 65536 || kv->num_kv_heads == 0 || kv->num_kv_heads > 65535 ||
+      kv->head_dim == 0 || kv->head_dim % 8 != 0 || kv->head_dim > 256)
+    return MYOS_ERR_SHAPE;
+  if (kv->slot_stride < kv->head_dim || kv->head_stride < kv->head_dim ||
+      kv->page_stride < kv->head_dim)
+    return MYOS_ERR_SHAPE;
+  // every element offset fits 62 bits
+  const uint64_t most = (uint64_t)1 << 60;
+  uint64_t pages, heads, slots;
+  if (__builtin_mul_overflow(kv->page_stride, (uint64_t)kv->num_pages, &pages) ||
+      __builtin_mul_overflow(kv->head_stride, (uint64_t)kv->num_kv_heads, &heads) ||
+      __builtin_mul_overflow(kv->slot_stride, (uint64_t)kv->page_size, &slots) || pages > most ||
+      heads > most || slots > most)
+    return MYOS_ERR_SHAPE;
+  const uint64_t per16 = kv->kv_dtype == MYOS_KV_F32 ? 4 : 8;
+  if (!aligned(kv->k, 16) || !aligned(kv->v, 16) || kv->page_stride % per16 != 0 ||
+      kv->head_stride % per16 != 0 || kv->slot_stride % per16 != 0)
+    return MYOS_ERR_ARG;
+  return MYOS_OK;
+}
+
+namespace {
+
+// ------------------------------------------------------------------ tables
+// Every block runs the two prefix sums over all requests itself (8 bytes a
+// request from L2), so one launch with no meeting of the blocks does the
+// whole step: block i then writes the table entries of every gridDim-th
+// request and its share of the rows.
+struct TablesArgs {
+  int32_t* table;
+  int64_t table_stride, max_blocks;
+  const int32_t *ctx, *add;
+  int nseq;
+  const int32_t* free_pages;
+  int64_t free_cap;
+  const int32_t* num_free;
+  uint32_t page_size, num_pages;
+  int64_t* slots;
+  int32_t *positions, *row_seq;
+  int64_t max_rows;
+  int32_t *kv_lens, *seq_starts, *result;
+};
+
+MYOS_DEV int64_t warp_scan(int64_t v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Inclusive sum over the block; *total is the block's. red: 33 values.
+MYOS_DEV int64_t block_scan(int64_t v, int64_t* red, int64_t* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  v = warp_scan(v);
+  if (lane == 31) red[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    const int64_t t = warp_scan(lane < nwarps ? red[lane] : 0);
+    red[lane] = t;
+  }
+  __syncthreads();
+  if (warp > 0) v += red[warp - 1];
+  *total = red[nwarps - 1];
+  __syncthreads();
+  return v;
+}
+
+__global__ void __launch_bounds__(1024) k_paged_tables(TablesArgs a) {
+  // end[b]: row behind request b's last, clipped to max_rows; first[b]: pages
+  // taken by the requests before b, or -1 for a refused one.
+  extern __shared__ int32_t smem[];
+  int32_t* end = smem;
+  int32_t* first = smem + a.nseq;
+  __shared__ int64_t red[32];
+  __shared__ int refused_s;
+  const int64_t P = a.page_size;
+  const bool writer = blockIdx.x == 0;
+  const int64_t nfree = min((int64_t)max(*a.num_free, 0), a.free_cap);
+  if (threadIdx.x == 0) refused_s = 0;
+  int64_t rows0 = 0, pages0 = 0, taken = 0;
+  int refused = 0;
+  for (int base = 0; base < a.nseq; base += blockDim.x) {
+    const int b = base + threadIdx.x;
+    int64_t ctx = 0, add = 0;
+    if (b < a.nseq) {
+      ctx = max(a.ctx[b], 0);
+      add = max(a.add[b], 0);
+    }
+    int64_t total;
+    const int64_t e = rows0 + block_scan(add, red, &total);
+    rows0 += total;
+    const bool fits = add == 0 || (ctx + add <= a.max_blocks * P && e <= a.max_rows);
+    const int64_t held = (ctx + P - 1) / P;
+    const int64_t need = add > 0 && fits ? (ctx + add + P - 1) / P - held : 0;
+    const int64_t upto = pages0 + block_scan(need, red, &total);
+    pages0 += total;
+    const bool ok = fits && (need == 0 || upto <= nfree);
+    if (b < a.nseq) {
+      end[b] = (int32_t)min(e, a.max_rows);
+      first[b] = ok ? (int32_t)min(upto - need, (int64_t)0x7fffffff) : -1;
+      if (ok) taken = max(taken, need > 0 ? upto : 0);
+      refused += !ok;
+      if (writer) {
+        a.kv_lens[b] = (int32_t)(ok ? ctx + add : ctx);
+        a.seq_starts[b + 1] = (int32_t)min(e, a.max_rows);
+        if (b == 0) a.seq_starts[0] = 0;
+      }
+    }
+  }
+  __syncthreads();
+  if (writer) {
+    // the admitted requests' running sum is largest at the last of them
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      taken = max(taken, __shfl_xor_sync(0xffffffffu, taken, o));
+      refused += __shfl_xor_sync(0xffffffffu, refused, o);
+    }
+    if ((threadIdx.x & 31) == 0) {
+      red[threadIdx.x >> 5] = taken;
+      atomicAdd(&refused_s, refused);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 0; w < (int)(blockDim.x >> 5); ++w) taken = max(taken, red[w]);
+      a.result[0] = (int32_t)(nfree - taken);
+      a.result[1] = refused_s;
+    }
+  }
+  // new table entries: one warp per request
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  for (int b = blockIdx.x * warps + (threadIdx.x >> 5); b < a.nseq; b += gridDim.x * warps) {
+    const int64_t ctx = max(a.ctx[b], 0), add = max(a.add[b], 0);
+    if (first[b] < 0 || add == 0) continue;
+    const int64_t held = (ctx + P - 1) / P, need = (ctx + add + P - 1) / P - held;
+    for (int64_t j = lane; j < need; j += 32)
+      a.table[b * a.table_stride + held + j] = a.free_pages[nfree - 1 - first[b] - j];
+  }
+  // rows: the request is the first whose end lies behind the row
+  for (int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; r < a.max_rows;
+       r += (int64_t)gridDim.x * blockDim.x) {
+    int lo = 0, hi = a.nseq;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (end[mid] > r) hi = mid;
+      else lo = mid + 1;
+    }
+    int64_t slot = -1, pos = 0;
+    if (lo < a.nseq && first[lo] >= 0) {
+      const int64_t ctx = max(a.ctx[lo], 0), held = (ctx + P - 1) / P;
+      pos = ctx + r - (lo > 0 ? end[lo - 1] : 0);
+      const int64_t pg = pos / P;
+      const int32_t page = pg < held ? a.table[lo * a.table_stride + pg]
+                                     : a.free_pages[nfree - 1 - first[lo] - (pg - held)];
+      if (page >= 0 && (uint32_t)page < a.num_pages) slot = (int64_t)page * P + pos % P;
+    }
+    a.slots[r] = slot;
+    a.positions[r] = (int32_t)pos;
+    a.row_seq[r] = lo < a.nseq ? lo : -1;
+  }
+}
+
+// ------------------------------------------------------- norm, rotate, store
+// A head is handled by `1 << lanes_log2` >= d / 8 lanes, each with two chunks
+// of four values: chunk j and its rotation partner j + rot / 8, or (behind the
+// rotated part) two neighbouring chunks.
+struct StoreArgs {
+  float* q;
+  const float* qkv;
+  int64_t q_stride, qkv_stride, rows;
+  const uint16_t *q_gamma, *k_gamma;
+  float eps;
+  const float *cos_t, *sin_t;
+  int64_t num_pos;
+  const int32_t* positions;
+  const int64_t* slots;
+  int hq, rot, lanes_log2;
+};
+
+MYOS_DEV void put4(float* p, const float4& v) { *reinterpret_cast<float4*>(p) = v; }
+// bf16 cache: round to nearest even, at most half a step (2^-9 of the value's
+// binade) off the f32 value; the cache type asks for it.
+MYOS_DEV void put4(__nv_bfloat16* p, const float4& v) {
+  __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+  uint2 u;
+  u.x = *reinterpret_cast<uint32_t*>(&lo);
+  u.y = *reinterpret_cast<uint32_t*>(&hi);
+  *reinterpret_cast<uint2*>(p) = u;
+}
+
+MYOS_DEV float sq4(const float4& v) { return v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w; }
+
+MYOS_DEV float4 scale4(const float4& v, float inv, const uint16_t* g) {
+  const uint2 u = *reinterpret_cast<const uint2*>(g);
+  float4 r;
+  r.x = __fmul_rn(bf16_lo(u.x), __fmul_rn(v.x, inv));
+  r.y = __fmul_rn(bf16_hi(u.x), __fmul_rn(v.y, inv));
+  r.z = __fmul_rn(bf16_lo(u.y), __fmul_rn(v.z, inv));
+  r.w = __fmul_rn(bf16_hi(u.y), __fmul_rn(v.w, inv));
+  return r;
+}
+
+MYOS_DEV float rot_lo(float x, float y, float c, float s) {
+  return __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
+}
+MYOS_DEV float rot_hi(float x, float y, float c, float s) {
+  return __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
+}
+
+template <class KT>
+__global__ void __launch_bounds__(256) k_paged_store(StoreArgs a, PagedKv<KT> kv) {
+  const int lanes = 1 << a.lanes_log2, d = (int)kv.d, heads = a.hq + 2 * (int)kv.heads;
+  const int j = threadIdx.x & (lanes - 1);
+  const bool on = j < d / 8;
+  const int pairs = a.rot / 8;
+  const bool turn = j < pairs;
+  const int c0 = 4 * (turn ? j : 2 * pairs + 2 * (j - pairs));
+  const int c1 = turn ? c0 + 4 * pairs : c0 + 4;
+  const int64_t units = a.rows * heads;
+  const int64_t per = (int64_t)gridDim.x * (blockDim.x >> a.lanes_log2);
+  for (int64_t base = 0; base < units; base += per) {
+    // every lane of a warp goes through the shuffles, with or without a head
+    const int64_t u = base + (((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> a.lanes_log2);
+    const bool live = u < units && on;
+    const int64_t row = u / heads;
+    const int head = (int)(u - row * heads);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+    if (live) {
+      const float* src = a.qkv + row * a.qkv_stride + (int64_t)head * d;
+      x = *reinterpret_cast<const float4*>(src + c0);
+      y = *reinterpret_cast<const float4*>(src + c1);
+    }
+    const bool is_q = head < a.hq, is_v = head >= a.hq + (int)kv.heads;
+    const uint16_t* gamma = is_q ? a.q_gamma : is_v ? nullptr : a.k_gamma;
+    if (a.q_gamma || a.k_gamma) {
+      float ss = sq4(x) + sq4(y);
+      for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (live && gamma) {
+        const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)d), a.eps)));
+        x = scale4(x, inv, gamma + c0);
+        y = scale4(y, inv, gamma + c1);
+      }
+    }
+    if (!live) continue;
+    bool placed = true;
+    if (a.rot > 0) {
+      const int64_t pos = a.positions[row];
+      placed = pos >= 0 && pos < a.num_pos;
+      if (placed && turn && !is_v) {
+        const float4 c = *reinterpret_cast<const float4*>(a.cos_t + pos * (a.rot / 2) + c0);
+        const float4 s = *reinterpret_cast<const float4*>(a.sin_t + pos * (a.rot / 2) + c0);
+        const float4 p = x, r = y;
+        x.x = rot_lo(p.x, r.x, c.x, s.x);
+        x.y = rot_lo(p.y, r.y, c.y, s.y);
+        x.z = rot_lo(p.z, r.z, c.z, s.z);
+        x.w = rot_lo(p.w, r.w, c.w, s.w);
+        y.x = rot_hi(p.x, r.x, c.x, s.x);
+        y.y = rot_hi(p.y, r.y, c.y, s.y);
+        y.z = rot_hi(p.z, r.z, c.z, s.z);
+        y.w = rot_hi(p.w, r.w, c.w, s.w);
+      }
+    }
+    if (is_q) {
+      float* dst = a.q + row * a.q_stride + (int64_t)head * d;
+      if (!placed) {
+        const float n = __int_as_float(0x7fc00000);
+        x = y = make_float4(n, n, n, n);
+      }
+      put4(dst + c0, x);
+      put4(dst + c1, y);
+      continue;
+    }
+    const int64_t slot = a.slots[row];
+    if (!placed || slot < 0 || slot >= (int64_t)kv.num_pages * kv.page_size) continue;
+    const int64_t page = slot / kv.page_size;
+    const int h = head - a.hq - (is_v ? (int)kv.heads : 0);
+    KT* dst = (is_v ? kv.v : kv.k) + page * kv.page_stride + h * kv.head_stride +
+              (slot - page * kv.page_size) * kv.slot_stride;
+    put4(dst + c0, x);
+    put4(dst + c1, y);
+  }
+}
+
+template <class KT>
+cudaError_t launch_store(const StoreArgs& a, const myos_paged_kv* kv, cudaStream_t st) {
+  const int64_t units = a.rows * (a.hq + 2 * (int64_t)kv->num_kv_heads);
+  const int64_t blocks = (units + (256 >> a.lanes_log2) - 1) / (256 >> a.lanes_log2);
+  const int grid = (int)(blocks < 148 * 8 ? blocks : 148 * 8);
+  k_paged_store<KT><<<grid, 256, 0, st>>>(a, paged_view<KT>(kv));
+  return counted(cudaGetLastError());
+}
+
+}  // namespace
+}  // namespace myos
+
+using namespace myos;
+
+extern "C" {
+
+int myos_dev_paged_tables(int32_t* d_block_table, size_t table_stride, size_t max_blocks,
+                          const int32_t* d_ctx_lens, const int32_t* d_new_lens, size_t nseq,
+                          const int32_t* d_free_pages, size_t free_cap,
+                          const int32_t* d_num_free, uint32_t page_size, uint32_t num_pages,
+                          int64_t* d_slots, int32_t* d_positions, int32_t* d_row_seq,
+                          size_t max_rows, int32_t* d_kv_lens, int32_t* d_seq_starts,
+                          int32_t* d_result, void* stream) {
+  if (nseq == 0) return MYOS_OK;
+  if (!d_block_table || !d_ctx_lens || !d_new_lens || (!d_free_pages && free_cap > 0) ||
+      !d_num_free || (max_rows > 0 && (!d_slots || !d_positions || !d_row_seq)) || !d_kv_lens ||
+      !d_seq_starts || !d_result)
+    return MYOS_ERR_ARG;
+  const uintptr_t words = (uintptr_t)d_block_table | (uintptr_t)d_ctx_lens |
+                          (uintptr_t)d_new_lens | (uintptr_t)d_free_pages |
+                          (uintptr_t)d_num_free | (uintptr_t)d_positions | (uintptr_t)d_row_seq |
+                          (uintptr_t)d_kv_lens | (uintptr_t)d_seq_starts | (uintptr_t)d_result;
+  if ((words & 3) != 0 || !aligned(d_slots, 8)) return MYOS_ERR_ARG;
+  if (d_kv_lens == d_ctx_lens || d_kv_lens == d_new_lens || d_result == d_num_free ||
+      d_result + 1 == d_num_free)
+    return MYOS_ERR_ARG;
+  if (nseq > 16384 || page_size == 0 || page_size > 65536 || num_pages > 0x7fffffffu ||
+      max_blocks == 0 || max_blocks > 0x7fffffff || table_stride < max_blocks ||
+      table_stride > ((size_t)1 << 40) || max_rows > 0x7fffffff || free_cap > 0x7fffffff)
+    return MYOS_ERR_SHAPE;
+  const size_t smem = 8 * nseq;
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(k_paged_tables, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           8 * 16384) != cudaSuccess)
+    return MYOS_ERR_CUDA;
+  TablesArgs a;
+  a.table = d_block_table;
+  a.table_stride = (int64_t)table_stride;
+  a.max_blocks = (int64_t)max_blocks;
+  a.ctx = d_ctx_lens;
+  a.add = d_new_lens;
+  a.nseq = (int)nseq;
+  a.free_pages = d_free_pages;
+  a.free_cap = (int64_t)free_cap;
+  a.num_free = d_num_free;
+  a.page_size = page_size;
+  a.num_pages = num_pages;
+  a.slots = d_slots;
+  a.positions = d_positions;
+  a.row_seq = d_row_seq;
+  a.max_rows = (int64_t)max_rows;
+  a.kv_lens = d_kv_lens;
+  a.seq_starts = d_seq_starts;
+  a.result = d_result;
+  const int threads = nseq <= 256 && max_rows <= 4096 ? 256 : 1024;
+  const size_t work = max_rows > nseq ? max_rows : nseq;
+  size_t grid = (work + threads - 1) / threads;
+  if (grid > 148) grid = 148;
+  k_paged_tables<<<(int)grid, threads, smem, (cudaStream_t)stream>>>(a);
+  return counted(cudaGetLastError()) == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
+}
+
+int myos_dev_qk_norm_rope_store(float* d_q, size_t q_stride, const float* d_qkv,
+                                size_t qkv_stride, size_t rows, size_t num_q_heads,
+                                const myos_paged_kv* kv, const void* d_q_gamma,
+                                const void* d_k_gamma, float eps, const float* d_cos,
+                                const float* d_sin, size_t num_pos, size_t rot_dim,
+                                const int32_t* d_positions, const int64_t* d_slots,
+                                void* stream) {
+  if (int st = paged_check(kv)) return st;
+  if (rows == 0) return MYOS_OK;
+  if (!d_q || !d_qkv || !d_slots || (rot_dim > 0 && (!d_cos || !d_sin || !d_positions)))
+    return MYOS_ERR_ARG;
+  const size_t d = kv->head_dim;
+  if (num_q_heads == 0 || num_q_heads > 65535 || rot_dim % 8 != 0 || rot_dim > d ||
+      rows > 0x7fffffff || num_pos > 0x7fffffff || (rot_dim > 0 && num_pos == 0) ||
+      q_stride < num_q_heads * d || qkv_stride < (num_q_heads + 2 * (size_t)kv->num_kv_heads) * d ||
+      q_stride > ((size_t)1 << 30) || qkv_stride > ((size_t)1 << 30))
+    return MYOS_ERR_SHAPE;
+  if (!aligned(d_q, 16) || !aligned(d_qkv, 16) || q_stride % 4 != 0 || qkv_stride % 4 != 0 ||
+      !aligned(d_q_gamma, 8) || !aligned(d_k_gamma, 8) || !aligned(d_slots, 8))
+    return MYOS_ERR_ARG;
+  if (rot_dim > 0 && (!aligned(d_cos, 16) || !aligned(d_sin, 16) || !aligned(d_positions, 4)))
+    return MYOS_ERR_ARG;
+  if (d_q == d_qkv && rows > 1 && q_stride != qkv_stride) return MYOS_ERR_ARG;
+  StoreArgs a;
+  a.q = d_q;
+  a.qkv = d_qkv;
+  a.q_stride = (int64_t)q_stride;
+  a.qkv_stride = (int64_t)qkv_stride;
+  a.rows = (int64_t)rows;
+  a.q_gamma = static_cast<const uint16_t*>(d_q_gamma);
+  a.k_gamma = static_cast<const uint16_t*>(d_k_gamma);
+  a.eps = eps;
+  a.cos_t = d_cos;
+  a.sin_t = d_sin;
+  a.num_pos = (int64_t)num_pos;
+  a.positions = d_positions;
+  a.slots = d_slots;
+  a.hq = (int)num_q_heads;
+  a.rot = (int)rot_dim;
+  a.lanes_log2 = 0;
+  while ((8u << a.lanes_log2) < d) ++a.lanes_log2;
+  const cudaError_t e = kv->kv_dtype == MYOS_KV_F32
+                            ? launch_store<float>(a, kv, (cudaStream_t)stream)
+                            : launch_store<__nv_bfloat16>(a, kv, (cudaStream_t)stream);
+  return e == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
+}
+
+// rope.rs:186-194, one row per position: libm in f32, each step rounded.
+int myos_rope_table(float* cos_out, float* sin_out, size_t num_pos, size_t rot_dim, float theta) {
+  if (!cos_out || !sin_out) return MYOS_ERR_ARG;
+  if (rot_dim == 0 || rot_dim % 2 != 0 || rot_dim > 65536 || num_pos > 0x7fffffff)
+    return MYOS_ERR_SHAPE;
+  const size_t half = rot_dim / 2;
+  for (size_t i = 0; i < half; ++i) {
+    volatile float exponent = (float)(2 * i) / (float)rot_dim;
+    volatile float inv = 1.0f / powf(theta, exponent);
+    for (size_t p = 0; p < num_pos; ++p) {
+      volatile float angle = (float)p * inv;
+      cos_out[p * half + i] = cosf(angle);
+      sin_out[p * half + i] = sinf(angle);
+    }
+  }
+  return MYOS_OK;
+}
+
+}  // extern "C"

@@ -5,6 +5,7 @@ binds it with ctypes and mirrors the reference's crate APIs:
 
   myos.engine   model_core: Engine.prefill / forward_token / greedy_decode / KV access
   myos.ops      tensor_core operators on host arrays (run on the GPU)
+  myos.dev      serving operators over a paged KV cache, on tensors in device memory
   myos.synth    seeded synthetic weights and prompts for the benchmark configs
   myos.tp       tensor-parallel generation, one process per GPU (torchrun)
 """

@@ -82,6 +82,48 @@ class TPPart(C.Structure):
     ]
 
 
+class PagedKV(C.Structure):
+    """myos_paged_kv: one layer's paged K/V cache in device memory."""
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("page_stride", C.c_uint64),
+        ("head_stride", C.c_uint64),
+        ("slot_stride", C.c_uint64),
+        ("num_pages", C.c_uint32),
+        ("page_size", C.c_uint32),
+        ("num_kv_heads", C.c_uint32),
+        ("head_dim", C.c_uint32),
+        ("kv_dtype", C.c_int32),
+        ("reserved", C.c_uint32),
+    ]
+
+
+class LogitControls(C.Structure):
+    """myos_logit_controls_args: device pointers (or null) and their sizes."""
+    _fields_ = [
+        ("history", C.c_void_p),
+        ("history_stride", C.c_uint64),
+        ("history_width", C.c_uint64),
+        ("prompt_lens", C.c_void_p),
+        ("history_lens", C.c_void_p),
+        ("repetition", C.c_void_p),
+        ("frequency", C.c_void_p),
+        ("presence", C.c_void_p),
+        ("bias_starts", C.c_void_p),
+        ("bias_ids", C.c_void_p),
+        ("bias_vals", C.c_void_p),
+        ("num_bias", C.c_uint64),
+        ("mask", C.c_void_p),
+        ("mask_stride", C.c_uint64),
+        ("num_masks", C.c_uint64),
+        ("mask_rows", C.c_void_p),
+    ]
+
+
+PAGED_WORK_BYTES = 16 << 20  # MYOS_PAGED_WORK_BYTES
+_dp = C.c_void_p  # a device pointer
+
 # Every symbol include/myos_cuda.h declares, with (restype, argtypes).
 SIGNATURES = {
     "myos_version": (C.c_char_p, []),
@@ -125,6 +167,15 @@ SIGNATURES = {
     "myos_batch_forced_decode": (C.c_int, [C.c_void_p, sz, _u32p, _u32p, sz, _u32p, _u32p, _f32p]),
     "myos_dev_gqa_attn_f32_noalloc": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                                 sz, sz, sz, sz, C.c_int32, sz, C.c_void_p]),
+    "myos_dev_paged_tables": (C.c_int, [_dp, sz, sz, _dp, _dp, sz, _dp, sz, _dp, C.c_uint32,
+                                        C.c_uint32, _dp, _dp, _dp, sz, _dp, _dp, _dp, _dp]),
+    "myos_dev_qk_norm_rope_store": (C.c_int, [_dp, sz, _dp, sz, sz, sz, C.POINTER(PagedKV), _dp,
+                                              _dp, C.c_float, _dp, _dp, sz, sz, _dp, _dp, _dp]),
+    "myos_dev_paged_attn": (C.c_int, [_dp, sz, _dp, _dp, sz, sz, sz, C.POINTER(PagedKV), _dp, sz,
+                                      sz, _dp, C.c_float, C.c_uint32, _dp, sz, _dp]),
+    "myos_dev_logit_controls": (C.c_int, [_dp, sz, _dp, sz, sz, sz, C.POINTER(LogitControls),
+                                          _dp, _dp]),
+    "myos_rope_table": (C.c_int, [_f32p, _f32p, sz, sz, C.c_float]),
 }
 
 _lib = None

@@ -17,6 +17,9 @@ const SOURCES: &[&str] = &[
     "noalloc.cu",
     "prefill.cu",
     "gemm_sm100.cu",
+    "paged.cu",
+    "paged_attn.cu",
+    "logits.cu",
     "safetensors.cpp",
     "tp.cpp",
 ];

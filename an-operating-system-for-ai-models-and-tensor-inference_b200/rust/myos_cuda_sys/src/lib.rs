@@ -48,6 +48,7 @@ pub mod ffi {
     pub const MYOS_KV_F32: i32 = 0;
     pub const MYOS_KV_BF16: i32 = 1;
     pub const MYOS_NOALLOC_SCRATCH_BYTES: usize = 2 << 20;
+    pub const MYOS_PAGED_WORK_BYTES: usize = 16 << 20;
 
     #[repr(C)]
     #[derive(Clone, Copy, Debug, Default, PartialEq)]
@@ -97,6 +98,43 @@ pub mod ffi {
     }
 
     #[repr(C)]
+    #[derive(Clone, Copy, Debug)]
+    pub struct myos_paged_kv {
+        pub k: *mut c_void,
+        pub v: *mut c_void,
+        pub page_stride: u64,
+        pub head_stride: u64,
+        pub slot_stride: u64,
+        pub num_pages: u32,
+        pub page_size: u32,
+        pub num_kv_heads: u32,
+        pub head_dim: u32,
+        pub kv_dtype: i32,
+        pub reserved: u32,
+    }
+
+    #[repr(C)]
+    #[derive(Clone, Copy, Debug)]
+    pub struct myos_logit_controls_args {
+        pub history: *const i32,
+        pub history_stride: u64,
+        pub history_width: u64,
+        pub prompt_lens: *const i32,
+        pub history_lens: *const i32,
+        pub repetition: *const f32,
+        pub frequency: *const f32,
+        pub presence: *const f32,
+        pub bias_starts: *const i32,
+        pub bias_ids: *const i32,
+        pub bias_vals: *const f32,
+        pub num_bias: u64,
+        pub mask: *const u32,
+        pub mask_stride: u64,
+        pub num_masks: u64,
+        pub mask_rows: *const i32,
+    }
+
+    #[repr(C)]
     pub struct myos_ctx {
         _private: [u8; 0],
     }
@@ -137,6 +175,11 @@ pub mod ffi {
         pub fn myos_batch_generate(ctx: *mut myos_ctx, nseq: usize, ids: *const u32, lens: *const u32, steps: usize, out_ids: *mut u32) -> c_int;
         pub fn myos_batch_forced_decode(ctx: *mut myos_ctx, nseq: usize, ids: *const u32, lens: *const u32, steps: usize, feed: *const u32, argmax_out: *mut u32, logits: *mut f32) -> c_int;
         pub fn myos_dev_gqa_attn_f32_noalloc(d_y: *mut f32, d_q: *const f32, d_k: *const f32, d_v: *const f32, hq: usize, hkv: usize, d: usize, seq: usize, mask_kind: i32, query_pos: usize, stream: *mut c_void) -> c_int;
+        pub fn myos_dev_paged_tables(d_block_table: *mut i32, table_stride: usize, max_blocks: usize, d_ctx_lens: *const i32, d_new_lens: *const i32, nseq: usize, d_free_pages: *const i32, free_cap: usize, d_num_free: *const i32, page_size: u32, num_pages: u32, d_slots: *mut i64, d_positions: *mut i32, d_row_seq: *mut i32, max_rows: usize, d_kv_lens: *mut i32, d_seq_starts: *mut i32, d_result: *mut i32, stream: *mut c_void) -> c_int;
+        pub fn myos_dev_qk_norm_rope_store(d_q: *mut f32, q_stride: usize, d_qkv: *const f32, qkv_stride: usize, rows: usize, num_q_heads: usize, kv: *const myos_paged_kv, d_q_gamma: *const c_void, d_k_gamma: *const c_void, eps: f32, d_cos: *const f32, d_sin: *const f32, num_pos: usize, rot_dim: usize, d_positions: *const i32, d_slots: *const i64, stream: *mut c_void) -> c_int;
+        pub fn myos_dev_paged_attn(d_out: *mut f32, out_stride: usize, d_lse: *mut f32, d_q: *const f32, q_stride: usize, nseq: usize, num_q_heads: usize, kv: *const myos_paged_kv, d_block_table: *const i32, table_stride: usize, max_blocks: usize, d_kv_lens: *const i32, scale: f32, window: u32, d_work: *mut c_void, work_bytes: usize, stream: *mut c_void) -> c_int;
+        pub fn myos_dev_logit_controls(d_out: *mut f32, out_stride: usize, d_logits: *const f32, logits_stride: usize, rows: usize, vocab: usize, c: *const myos_logit_controls_args, d_ids: *mut u32, stream: *mut c_void) -> c_int;
+        pub fn myos_rope_table(cos_out: *mut f32, sin_out: *mut f32, num_pos: usize, rot_dim: usize, theta: f32) -> c_int;
         pub fn myos_version() -> *const c_char;
     }
 }

@@ -346,6 +346,176 @@ int myos_dev_gqa_attn_f32_noalloc(float* d_y, const float* d_q, const float* d_k
                                   const float* d_v, size_t hq, size_t hkv, size_t d, size_t seq,
                                   int32_t mask_kind, size_t query_pos, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Serving over a paged KV cache (device pointers). No counterpart in the
+ * reference, whose cache is one contiguous f32 slab for one sequence
+ * (crates/model_core/src/kv_cache.rs:89-125). One serving step of a batch is:
+ * tables and slot maps from the requests' lengths (myos_dev_paged_tables);
+ * per layer the q/k/v rows normed, rotated and stored into the pages
+ * (myos_dev_qk_norm_rope_store) and the attention of each sequence's newest
+ * token over its pages (myos_dev_paged_attn); the head's logits put under the
+ * requests' controls, with the greedy id (myos_dev_logit_controls).
+ *
+ * Common rules: the calls run on the current device, on `stream` (0: the
+ * default stream) of that device, and every pointer is memory of that device.
+ * They allocate nothing, do not synchronize, and can be captured into a graph;
+ * the first call on a device belongs outside a capture (it raises the kernels'
+ * shared-memory limits). Arguments that the host can see are checked before
+ * any device work: MYOS_ERR_ARG for null pointers, invalid options and
+ * misaligned addresses or strides, MYOS_ERR_SHAPE for sizes. What only the
+ * device can see (lengths, page ids, slots, positions, token ids) is checked
+ * there, and never read or written through when out of range; each call says
+ * what happens then. Unless a call says otherwise its outputs overlap neither
+ * each other nor its inputs. Strides count elements, not bytes. A call with no
+ * rows returns MYOS_OK and does nothing.
+ * ------------------------------------------------------------------------- */
+
+/* One layer's paged K/V cache. Element (page, head, slot, i) of K is
+ * k[page * page_stride + head * head_stride + slot * slot_stride + i] (V the
+ * same, with the same strides), so [page][head][slot][dim] and
+ * [page][slot][head][dim] are both possible. head_dim is a multiple of 8, at
+ * most 256; page_size at most 65536, a power of two or not; k, v and the
+ * strides are multiples of 16 bytes. The token at position p of a sequence
+ * lies in page table[p / page_size], slot p % page_size. */
+typedef struct myos_paged_kv {
+  void* k;
+  void* v;
+  uint64_t page_stride;
+  uint64_t head_stride;
+  uint64_t slot_stride;
+  uint32_t num_pages;
+  uint32_t page_size;
+  uint32_t num_kv_heads;
+  uint32_t head_dim;
+  int32_t kv_dtype; /* enum myos_kv_dtype */
+  uint32_t reserved; /* 0 */
+} myos_paged_kv;
+
+/* Gives each of nseq requests (at most 16384) the pages that its new tokens
+ * need, and maps the step's token rows to cache slots. Request b holds
+ * d_ctx_lens[b] tokens in the pages of table row b (d_block_table +
+ * b * table_stride, max_blocks entries) and adds d_new_lens[b]; negative
+ * lengths count as 0. Rows of the step are packed: request b's are
+ * d_seq_starts[b] .. d_seq_starts[b + 1] (written here, nseq + 1 values,
+ * clipped to max_rows). New pages come from the END of d_free_pages
+ * [0 .. *d_num_free) (free_cap entries; *d_num_free is clipped to it), in
+ * request order, and are appended to the table row in place.
+ * A request is admitted when its tokens fit the table row (max_blocks *
+ * page_size) and the row buffer (max_rows), and the pages needed by the
+ * requests up to and including it (those that fit) do not exceed *d_num_free;
+ * a request that needs no page is not held up by the free list. A refused
+ * request keeps its length, takes no page, and its rows get slot -1. Outputs:
+ * per row d_slots (page * page_size + slot in page; -1: none, also where the
+ * page id is outside 0 .. num_pages), d_positions (0 without a slot's
+ * request), d_row_seq (the request; -1 for rows behind the last one, whose
+ * slot is -1 and position 0); per request d_kv_lens, its length after the
+ * step; d_result[2]: the free pages left (the next call's *d_num_free, same
+ * d_free_pages) and the number of refused requests. d_kv_lens must not be
+ * d_ctx_lens and d_result must not hold d_num_free (MYOS_ERR_ARG): blocks of
+ * one launch read the one while another block writes the other. */
+int myos_dev_paged_tables(int32_t* d_block_table, size_t table_stride, size_t max_blocks,
+                          const int32_t* d_ctx_lens, const int32_t* d_new_lens, size_t nseq,
+                          const int32_t* d_free_pages, size_t free_cap,
+                          const int32_t* d_num_free, uint32_t page_size, uint32_t num_pages,
+                          int64_t* d_slots, int32_t* d_positions, int32_t* d_row_seq,
+                          size_t max_rows, int32_t* d_kv_lens, int32_t* d_seq_starts,
+                          int32_t* d_result, void* stream);
+
+/* One pass over the q|k|v rows of a projection (f32; row r at d_qkv +
+ * r * qkv_stride: num_q_heads, then kv->num_kv_heads key heads, then as many
+ * value heads, head_dim each): per-head RMSNorm of q and k with a BF16 weight
+ * of head_dim values (d_q_gamma, d_k_gamma; null: that one is not normed, the
+ * Qwen2.5 form), NeoX rotation of each q and k head's first rot_dim values
+ * (pairs i, i + rot_dim / 2; the rest passes through; 0: no rotation) by row
+ * d_positions[r] of the tables d_cos, d_sin [num_pos][rot_dim / 2]
+ * (myos_rope_table), then q to d_q (row r at r * q_stride, num_q_heads *
+ * head_dim values) and K, V to slot d_slots[r] of the cache, in its type
+ * (bf16: round to nearest even). A row whose slot is outside the cache
+ * (negative: padding) is not stored, its q is computed. A row whose position
+ * is outside the tables is not stored and its q is NaN. d_q may be d_qkv (same
+ * stride, in place); two rows of one call must not name the same slot.
+ * rot_dim is a multiple of 8 and at most head_dim; all f32 pointers and row
+ * strides are multiples of 16 bytes, the weights 8-byte aligned. Order of the
+ * steps as in myos_rmsnorm_bf16_weight and myos_rope_f32. */
+int myos_dev_qk_norm_rope_store(float* d_q, size_t q_stride, const float* d_qkv,
+                                size_t qkv_stride, size_t rows, size_t num_q_heads,
+                                const myos_paged_kv* kv, const void* d_q_gamma,
+                                const void* d_k_gamma, float eps, const float* d_cos,
+                                const float* d_sin, size_t num_pos, size_t rot_dim,
+                                const int32_t* d_positions, const int64_t* d_slots, void* stream);
+
+/* Bytes of the work buffer of myos_dev_paged_attn. */
+#define MYOS_PAGED_WORK_BYTES (16u << 20)
+
+/* Attention of one new token per sequence over the cache: out[b] (num_q_heads
+ * * head_dim f32 at b * out_stride) = softmax(scale * q[b] . K) V over the keys
+ * at positions [max(0, len - window), len) of sequence b, len = d_kv_lens[b]
+ * clipped to [0, max_blocks * page_size], window 0: all; query head h reads
+ * KV head h / (num_q_heads / num_kv_heads), a group of at most 8 (as in
+ * tensor_core::gqa_attn_f32). d_lse (nullable, [nseq][num_q_heads]) receives
+ * the natural log of the sum of exp(scale * q . k). Keys of a page whose table
+ * entry is outside the cache are left out. A sequence with no keys gives zeros
+ * and lse -inf. Slots behind len are never read, whatever they hold; the keys
+ * and values that are attended to, q and scale are finite.
+ * d_work: MYOS_PAGED_WORK_BYTES of device memory, 16-byte aligned, zeroed once
+ * before its first use; each call leaves it ready for the next. Calls that may
+ * run at the same time (other streams, graphs) need buffers of their own.
+ * Deterministic: the same inputs give the same bits. q and out pointers and row
+ * strides are multiples of 16 bytes. */
+int myos_dev_paged_attn(float* d_out, size_t out_stride, float* d_lse, const float* d_q,
+                        size_t q_stride, size_t nseq, size_t num_q_heads,
+                        const myos_paged_kv* kv, const int32_t* d_block_table,
+                        size_t table_stride, size_t max_blocks, const int32_t* d_kv_lens,
+                        float scale, uint32_t window, void* d_work, size_t work_bytes,
+                        void* stream);
+
+/* The controls of myos_dev_logit_controls; every pointer may be null. */
+typedef struct myos_logit_controls_args {
+  /* Tokens of each row so far, prompt first: row r at r * history_stride,
+   * history_lens[r] of them (clipped to 0 .. history_width; null: all), the
+   * first prompt_lens[r] the prompt (null: none). Ids outside the vocabulary
+   * are passed over. */
+  const int32_t* history;
+  uint64_t history_stride;
+  uint64_t history_width;
+  const int32_t* prompt_lens;
+  const int32_t* history_lens;
+  /* Per row: a token seen in prompt or output has x / r where x > 0, else
+   * x * r; then x - frequency * (times in the output); then x - presence if it
+   * is in the output. Null: the step is left out. They need `history`. */
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+  /* Row r adds bias_vals[e] to token bias_ids[e] for e in bias_starts[r] ..
+   * bias_starts[r + 1] (clipped to 0 .. num_bias); of several entries of one
+   * token the last counts. */
+  const int32_t* bias_starts;
+  const int32_t* bias_ids;
+  const float* bias_vals;
+  uint64_t num_bias;
+  /* Grammar masks: bit t % 32 of word t / 32 set: token t is allowed, else its
+   * logit becomes -inf. Row r uses mask mask_rows[r] (outside 0 .. num_masks:
+   * none; null: mask r, for num_masks >= rows). */
+  const uint32_t* mask;
+  uint64_t mask_stride;
+  uint64_t num_masks;
+  const int32_t* mask_rows;
+} myos_logit_controls_args;
+
+/* Puts the rows of logits [rows][vocab] under the requests' controls, in the
+ * order penalties, bias, mask, each step rounded to f32, and picks the greedy
+ * id of the result (myos_greedy_token's rule: the first maximum; NaN and -inf
+ * never win, a row of nothing else gives 0). d_out receives the controlled
+ * logits (may be d_logits with the same stride: in place; null: only the ids),
+ * d_ids the ids (null: none); not both null. c null: no controls. */
+int myos_dev_logit_controls(float* d_out, size_t out_stride, const float* d_logits,
+                            size_t logits_stride, size_t rows, size_t vocab,
+                            const myos_logit_controls_args* c, uint32_t* d_ids, void* stream);
+
+/* Host: cos and sin of the rotary angles, [num_pos][rot_dim / 2] f32 each,
+ * built as tensor_core::rope_f32 builds its row (rope.rs:186-194). */
+int myos_rope_table(float* cos_out, float* sin_out, size_t num_pos, size_t rot_dim, float theta);
+
 /* Library version string and the build's target architecture. */
 const char* myos_version(void);
 
