@@ -16,7 +16,9 @@
 //
 // Each warp streams keys of its own through its own stages of shared memory
 // (cp.async, three deep, pages looked up one tile ahead), so warps never wait
-// for one another inside an item.
+// for one another inside an item. A copy instruction takes 64 bytes of each of
+// eight rows: a lane stays with one or two rows of a tile, and all its
+// addresses are one base each and constants.
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.h"
@@ -77,6 +79,45 @@ MYOS_DEV void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+MYOS_DEV void mma16816_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                            uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// The same in tf32, A 16 x 8, B 8 x 8.
+MYOS_DEV void mma1688(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                      uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+MYOS_DEV void mma1688_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                           uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+MYOS_DEV void lds4(float4& x, uint32_t addr) {
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "r"(addr)
+               : "memory");
+}
+// Bits 0, 4, .., 28 next to each other.
+MYOS_DEV uint32_t gather_rows(uint32_t x) {
+  x &= 0x11111111u;
+  x = (x | x >> 3) & 0x03030303u;
+  x = (x | x >> 6) & 0x000f000fu;
+  return (x | x >> 12) & 0xffu;
+}
+
 // x = hi + mid + lo, exactly: three times the leading 8 significand bits, by
 // truncation (two values at a time, packed as bf16 pairs).
 struct Split3 {
@@ -98,24 +139,120 @@ MYOS_DEV Split3 split3(float x, float y) {
   return s;
 }
 
+MYOS_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Rescaling of a part with maximum m to the common maximum top.
-MYOS_DEV float weight_of(float m, float top) { return top == -INFINITY ? 0.f : exp2f(m - top); }
+MYOS_DEV float weight_of(float m, float top) { return top == -INFINITY ? 0.f : ex2(m - top); }
 
 // ---------------------------------------------------------- a warp's state
-// bf16 cache: 16 keys a tile through mma. The A operand's 16 rows hold the
-// group's (at most 8) heads twice, the hi terms in rows 0-7 and the mid terms
-// in rows 8-15, and a second mma adds the lo terms, so the f32 queries and
-// weights enter exactly; a lane's c0, c1 and c2, c3 belong to the same head
-// (lane / 4). The tensor core truncates its f32 sums, so no long chain runs
-// through it: four steps of a score, one tile of an output, the rest are f32
-// adds, rounded to nearest.
+// The group's (at most 8) heads are rows 0-7 of an mma's A operand, with the
+// leading part of the f32 queries (or weights); rows 8-15 take the next part
+// of the same heads, so a lane's c0, c1 and c2, c3 belong to one head
+// (lane / 4) and are added up. The tensor core truncates its f32 sums, so no
+// long chain runs through it: four steps of a score, one tile of an output;
+// the rest are f32 adds, rounded to nearest.
+//
+// o[2 t + i] is value i of column tile t (8 of the head's dims).
 template <int DH>
-struct MmaWarp {
-  static constexpr int kKeys = 16, kRegs = DH / 4, kSteps = DH / 16;
-  using KT = __nv_bfloat16;
-  Split3 q[kSteps][2];
+struct WarpState {
+  static constexpr int kRegs = DH / 4;
   float o[kRegs];
   float m, l;
+
+  MYOS_DEV void clear() {
+#pragma unroll
+    for (int r = 0; r < kRegs; ++r) o[r] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+  }
+  // Sums over the lanes of a head, once per piece.
+  MYOS_DEV void finish() {
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+  }
+  MYOS_DEV void put(float* ms, float* ls, float* os) const {
+    const int lane = threadIdx.x & 31;
+    if ((lane & 3) == 0) {
+      ms[lane >> 2] = m;
+      ls[lane >> 2] = l;
+    }
+#pragma unroll
+    for (int r = 0; r < kRegs; r += 4)
+      *reinterpret_cast<float4*>(os + r * 32 + lane * 4) =
+          make_float4(o[r], o[r + 1], o[r + 2], o[r + 3]);
+  }
+  MYOS_DEV void join(const float* ms, const float* ls, const float* os) {
+    const int lane = threadIdx.x & 31, g = lane >> 2;
+    const float pm = ms[g], top = fmaxf(m, pm);
+    const float a = weight_of(m, top), b = weight_of(pm, top);
+    m = top;
+    l = l * a + ls[g] * b;
+#pragma unroll
+    for (int r = 0; r < kRegs; r += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(os + r * 32 + lane * 4);
+      o[r] = o[r] * a + x.x * b;
+      o[r + 1] = o[r + 1] * a + x.y * b;
+      o[r + 2] = o[r + 2] * a + x.z * b;
+      o[r + 3] = o[r + 3] * a + x.w * b;
+    }
+  }
+  MYOS_DEV void rescale(float a) {
+#pragma unroll
+    for (int r = 0; r < kRegs; ++r) o[r] *= a;
+  }
+  MYOS_DEV void add(const float* os, float b) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int r = 0; r < kRegs; r += 4) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(os + r * 32 + lane * 4));
+      o[r] = fmaf(x.x, b, o[r]);
+      o[r + 1] = fmaf(x.y, b, o[r + 1]);
+      o[r + 2] = fmaf(x.z, b, o[r + 2]);
+      o[r + 3] = fmaf(x.w, b, o[r + 3]);
+    }
+  }
+  // Maximum and weights of a tile's scores s (in powers of two, -inf: no key;
+  // the tile has one); the factor for what came before.
+  template <int N>
+  MYOS_DEV float weigh(float (&s)[N]) {
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, s[i]);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    top = fmaxf(top, m);
+    const float keep = ex2(m - top);
+    m = top;
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t += s[i] = ex2(s[i] - top);
+    l = fmaf(l, keep, t);
+    return keep;
+  }
+  MYOS_DEV float inverse() const { return l > 0.f ? __fdiv_rn(1.0f, l) : 0.f; }
+  MYOS_DEV void put_lse(float* lse, int G) const {
+    const int lane = threadIdx.x & 31;
+    if (lse && (lane & 3) == 0 && (lane >> 2) < G)
+      lse[lane >> 2] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  }
+};
+
+// bf16 cache, 16 keys a tile: queries and weights enter as three bf16 terms
+// that sum to them exactly, hi and mid in the A operand's two halves, lo in a
+// second mma. 64 mma of 2048 products a tile at head_dim 128: a third of the
+// tile's share of the memory's time.
+template <int DH>
+struct Bf16Warp : WarpState<DH> {
+  using KT = __nv_bfloat16;
+  using WarpState<DH>::o;
+  static constexpr int kKeys = 16, kSteps = DH / 16;
+  static constexpr bool kLate = DH > 128;  // queries split at each use: registers
+  Split3 q[kLate ? 1 : kSteps][2];
+  float2 raw[kLate ? kSteps : 1][2];
 
   MYOS_DEV void begin(const float* q_row, int G, int d) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = (lane & 3) * 2;
@@ -126,17 +263,16 @@ struct MmaWarp {
         const int at = 16 * k + 8 * u + c;
         float2 x = make_float2(0.f, 0.f);
         if (g < G && at < d) x = *reinterpret_cast<const float2*>(q_row + g * d + at);
-        q[k][u] = split3(x.x, x.y);
+        if constexpr (kLate) raw[k][u] = x;
+        else q[k][u] = split3(x.x, x.y);
       }
-#pragma unroll
-    for (int r = 0; r < kRegs; ++r) o[r] = 0.f;
-    m = -INFINITY;
-    l = 0.f;
+    this->clear();
   }
 
-  // Chunks of 16 bytes; row r keeps chunk i at i ^ (r & 7): the eight rows
-  // that an ldmatrix reads at one chunk lie in different banks.
-  static MYOS_DEV int place(int row, int chunk) { return row * (DH / 8) + (chunk ^ (row & 7)); }
+  // Row r keeps 16-byte chunk i at i ^ (r & 7), so the eight rows that an
+  // ldmatrix reads at one chunk lie in different banks.
+  static MYOS_DEV uint32_t flip_k(int row) { return row & 7; }
+  static MYOS_DEV uint32_t flip_v(int row) { return row & 7; }
 
   MYOS_DEV void tile(uint32_t ks, uint32_t vs, uint32_t ok, float scale2) {
     const int lane = threadIdx.x & 31, c = (lane & 3) * 2;
@@ -147,16 +283,24 @@ struct MmaWarp {
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[n][0][i] = a[n][1][i] = lo[n][i] = 0.f;
-      const int row = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+      const int row = (lane & 7) + ((lane >> 4) << 3);
+      const uint32_t base = ks + row * (DH * 2) + ((((lane >> 3) & 1) ^ (row & 7)) << 4);
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
         uint32_t b[4];
-        ldmatrix4(b, ks + 16 * place(row, 2 * k + half));
+        ldmatrix4(b, (base ^ ((2 * k & 6) << 4)) + (k >> 2) * 128);
+        Split3 q0, q1;
+        if constexpr (kLate) {
+          q0 = split3(raw[k][0].x, raw[k][0].y);
+          q1 = split3(raw[k][1].x, raw[k][1].y);
+        } else {
+          q0 = q[k][0];
+          q1 = q[k][1];
+        }
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          mma16816(lo[n], q[k][0].lo, 0u, q[k][1].lo, 0u, b[2 * n], b[2 * n + 1]);
-          mma16816(a[n][(k >> 2) & 1], q[k][0].hi, q[k][0].mid, q[k][1].hi, q[k][1].mid, b[2 * n],
-                   b[2 * n + 1]);
+          mma16816(lo[n], q0.lo, 0u, q1.lo, 0u, b[2 * n], b[2 * n + 1]);
+          mma16816(a[n][(k >> 2) & 1], q0.hi, q0.mid, q1.hi, q1.mid, b[2 * n], b[2 * n + 1]);
         }
       }
 #pragma unroll
@@ -167,26 +311,18 @@ struct MmaWarp {
           s[2 * n + i] = (ok >> (8 * n + c + i)) & 1u ? x * scale2 : -INFINITY;
         }
     }
-    float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    top = fmaxf(top, m);  // finite: the tile has a key
-    const float keep = exp2f(m - top);
-    m = top;
-    float p[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[i] = exp2f(s[i] - top);
-    l = fmaf(l, keep, (p[0] + p[1]) + (p[2] + p[3]));
-    const Split3 w0 = split3(p[0], p[1]), w1 = split3(p[2], p[3]);
-    const int row = lane & 15, half = lane >> 4;
+    const float keep = this->weigh(s);
+    const Split3 w0 = split3(s[0], s[1]), w1 = split3(s[2], s[3]);
+    const int row = lane & 15;
+    const uint32_t base = vs + row * (DH * 2) + (((lane >> 4) ^ (row & 7)) << 4);
 #pragma unroll
     for (int j = 0; j < DH / 16; ++j) {
       uint32_t b[4];
-      ldmatrix4t(b, vs + 16 * place(row, 2 * j + half));
+      ldmatrix4t(b, (base ^ ((2 * j & 6) << 4)) + (j >> 2) * 128);
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        float t[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816(t, w0.lo, 0u, w1.lo, 0u, b[2 * n], b[2 * n + 1]);
+        float t[4];
+        mma16816_zero(t, w0.lo, 0u, w1.lo, 0u, b[2 * n], b[2 * n + 1]);
         mma16816(t, w0.hi, w0.mid, w1.hi, w1.mid, b[2 * n], b[2 * n + 1]);
         float* x = &o[4 * j + 2 * n];
         x[0] = fmaf(x[0], keep, t[0] + t[2]);
@@ -195,199 +331,150 @@ struct MmaWarp {
     }
   }
 
-  // Sums over the lanes of a head, once per piece.
-  MYOS_DEV void finish() {
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-  }
-  MYOS_DEV void put_ml(float* ms, float* ls) const {
-    const int lane = threadIdx.x & 31;
-    if ((lane & 3) == 0) {
-      ms[lane >> 2] = m;
-      ls[lane >> 2] = l;
-    }
-  }
-  // o of a part (regs apart by 32 lanes) into this state; m, l per head.
-  MYOS_DEV void join(const float* part, const float* ms, const float* ls) {
-    const int lane = threadIdx.x & 31, g = lane >> 2;
-    const float pm = ms[g], top = fmaxf(m, pm);
-    const float a = weight_of(m, top), b = weight_of(pm, top);
-    m = top;
-    l = l * a + ls[g] * b;
-#pragma unroll
-    for (int r = 0; r < kRegs; r += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(part + r * 32 + lane * 4);
-      o[r] = o[r] * a + x.x * b;
-      o[r + 1] = o[r + 1] * a + x.y * b;
-      o[r + 2] = o[r + 2] * a + x.z * b;
-      o[r + 3] = o[r + 3] * a + x.w * b;
-    }
-  }
-  MYOS_DEV void write(float* out, float* lse, int G, int d) const {
+  MYOS_DEV void write(float* out, int G, int d) const {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = (lane & 3) * 2;
     if (g >= G) return;
-    const float inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
+    const float inv = this->inverse();
 #pragma unroll
     for (int j = 0; j < DH / 8; ++j)
       if (8 * j < d)
         *reinterpret_cast<float2*>(out + g * d + 8 * j + c) =
             make_float2(o[2 * j] * inv, o[2 * j + 1] * inv);
-    if (lse && c == 0) lse[g] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
   }
 };
 
-// f32 cache: 8 keys a tile on the FMA units; a lane holds DH / 32 dims of
-// every head. The products of 32 (head, key) pairs are summed over the lanes
-// by a halving exchange that leaves one pair in each lane.
-template <int DH, int GP>
-struct FmaWarp {
-  static constexpr int kKeys = 8, kDims = DH / 32, kRegs = GP * kDims;
-  static constexpr int kVec = kDims < 4 ? kDims : 4, kJ = 32 / GP;  // kJ keys at a time
+// x = hi + lo for a tf32 mma: hi the nearest value of 11 significand bits, lo
+// the rest cut to 11 bits, off by at most one step (2^-23) of x.
+MYOS_DEV void split2(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+}
+
+// f32 cache, 8 keys a tile: both sides as two tf32 terms, all four products
+// (hi and lo of the queries in the A operand's two halves, hi and lo of the
+// keys in two mma). On the FMA units a tile cost 1700 instructions, and 64
+// sequences of 512 to 640 keys (12/2 heads of 128) took 37 us.
+//
+// The order in which an mma takes its summed index is free, as long as both
+// operands agree: step s of a score sums dims 16 (s / 2) + 4 c + 2 (s % 2) and
+// the next (c: lane % 4), so a lane reads its keys 16 bytes at a time; an
+// output's step sums key 2 c, which the lane's score is for, and 2 c + 1, and
+// column n of tile t is dim 32 (t / 4) + 4 n + t % 4.
+template <int DH>
+struct F32Warp : WarpState<DH> {
   using KT = float;
-  float q[GP][kDims];
-  float o[kRegs];
-  float m[GP], l[GP];
+  using WarpState<DH>::o;
+  static constexpr int kKeys = 8, kChunks = DH / 16;
+  static constexpr bool kLate = DH > 128;
+  uint32_t q[kLate ? 1 : kChunks][8];
+  float4 raw[kLate ? kChunks : 1];
 
-  // dims of a lane: kVec at lane * kVec, then (DH 256) at 128 + lane * kVec
-  static MYOS_DEV int dim(int i) { return (i / kVec) * 32 * kVec + (threadIdx.x & 31) * kVec + i % kVec; }
-
+  static MYOS_DEV void split_q(const float4& x, uint32_t (&y)[8]) {
+    split2(x.x, y[0], y[1]);
+    split2(x.y, y[2], y[3]);
+    split2(x.z, y[4], y[5]);
+    split2(x.w, y[6], y[7]);
+  }
   MYOS_DEV void begin(const float* q_row, int G, int d) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
 #pragma unroll
-    for (int g = 0; g < GP; ++g) {
-#pragma unroll
-      for (int i = 0; i < kDims; ++i) {
-        q[g][i] = g < G && dim(i) < d ? q_row[g * d + dim(i)] : 0.f;
-        o[g * kDims + i] = 0.f;
-      }
-      m[g] = -INFINITY;
-      l[g] = 0.f;
+    for (int k = 0; k < kChunks; ++k) {
+      const int at = 16 * k + 4 * c;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (g < G && at < d) x = *reinterpret_cast<const float4*>(q_row + g * d + at);
+      if constexpr (kLate) raw[k] = x;
+      else split_q(x, q[k]);
     }
+    this->clear();
   }
-  static MYOS_DEV int place(int row, int chunk) { return row * (DH / 4) + chunk; }
 
-  static MYOS_DEV void row_of(float (&x)[kDims], uint32_t base, int row) {
-    const uint32_t at = base + (row * DH + (threadIdx.x & 31) * kVec) * 4;
-    if constexpr (kVec == 2) {
-      asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(x[0]), "=f"(x[1]) : "r"(at) : "memory");
-    } else {
-#pragma unroll
-      for (int i = 0; i < kDims; i += 4)
-        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
-                     : "=f"(x[i]), "=f"(x[i + 1]), "=f"(x[i + 2]), "=f"(x[i + 3])
-                     : "r"(at + i * 128)
-                     : "memory");
-    }
-  }
+  // Chunks of a row are exchanged so that the 8 lanes of a 16-byte read phase
+  // (two keys x four chunks of K, four even or odd keys x two chunks of V)
+  // lie in different banks.
+  static MYOS_DEV uint32_t flip_k(int row) { return (row & 1) << 2; }
+  static MYOS_DEV uint32_t flip_v(int row) { return (row & 6); }
 
   MYOS_DEV void tile(uint32_t ks, uint32_t vs, uint32_t ok, float scale2) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int j0 = 0; j0 < kKeys; j0 += kJ) {
-      const uint32_t now = (ok >> j0) & ((1u << kJ) - 1u);
-      if (now == 0) continue;
-      float d[32];  // (head, key) pair g * kJ + j
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) {
-        float x[kDims];
-        row_of(x, ks, j0 + j);
-#pragma unroll
-        for (int g = 0; g < GP; ++g) {
-          float s = 0.f;
-#pragma unroll
-          for (int i = 0; i < kDims; ++i) s = fmaf(q[g][i], x[i], s);
-          d[g * kJ + j] = s;
-        }
-      }
-#pragma unroll
-      for (int w = 16; w > 0; w >>= 1) {
-        const bool up = (lane & w) != 0;
-#pragma unroll
-        for (int i = 0; i < w; ++i) {
-          const float give = up ? d[i] : d[i + w];
-          const float have = up ? d[i + w] : d[i];
-          d[i] = have + __shfl_xor_sync(0xffffffffu, give, w);
-        }
-      }
-      // lane g * kJ + j has the score of head g, key j0 + j
-      const float s = (now >> (lane % kJ)) & 1u ? d[0] * scale2 : -INFINITY;
-      float top = s;
-#pragma unroll
-      for (int w = 1; w < kJ; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-      float keep[GP];
-      float mine = -INFINITY;
-#pragma unroll
-      for (int g = 0; g < GP; ++g) {
-        const float t = fmaxf(m[g], __shfl_sync(0xffffffffu, top, g * kJ));
-        keep[g] = exp2f(m[g] - t);
-        m[g] = t;
-        if (lane / kJ == g) mine = t;
-      }
-      const float p = exp2f(s - mine);
-      float w[GP][kJ];
-#pragma unroll
-      for (int g = 0; g < GP; ++g) {
-        float t = 0.f;
-#pragma unroll
-        for (int j = 0; j < kJ; ++j) {
-          w[g][j] = __shfl_sync(0xffffffffu, p, g * kJ + j);
-          t += w[g][j];
-        }
-        l[g] = fmaf(l[g], keep[g], t);
-#pragma unroll
-        for (int i = 0; i < kDims; ++i) o[g * kDims + i] *= keep[g];
-      }
-#pragma unroll
-      for (int j = 0; j < kJ; ++j) {
-        float x[kDims];
-        row_of(x, vs, j0 + j);
-#pragma unroll
-        for (int g = 0; g < GP; ++g)
-#pragma unroll
-          for (int i = 0; i < kDims; ++i) o[g * kDims + i] = fmaf(w[g][j], x[i], o[g * kDims + i]);
-      }
-    }
-  }
-  MYOS_DEV void finish() {}
-  MYOS_DEV void put_ml(float* ms, float* ls) const {
-    if ((threadIdx.x & 31) == 0)
-#pragma unroll
-      for (int g = 0; g < GP; ++g) {
-        ms[g] = m[g];
-        ls[g] = l[g];
-      }
-  }
-  MYOS_DEV void join(const float* part, const float* ms, const float* ls) {
-    const int lane = threadIdx.x & 31;
-    float a[GP], b[GP];
-#pragma unroll
-    for (int g = 0; g < GP; ++g) {
-      const float pm = ms[g], top = fmaxf(m[g], pm);
-      a[g] = weight_of(m[g], top);
-      b[g] = weight_of(pm, top);
-      m[g] = top;
-      l[g] = l[g] * a[g] + ls[g] * b[g];
-    }
-#pragma unroll
-    for (int r = 0; r < kRegs; r += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(part + r * 32 + lane * 4);
-      const float y[4] = {x.x, x.y, x.z, x.w};
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    float s[2];
+    {
+      constexpr int kChains = DH / 32 < 4 ? DH / 32 : 4;
+      float a[kChains][4], lo[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int g = (r + i) / kDims;
-        o[r + i] = o[r + i] * a[g] + y[i] * b[g];
+        lo[i] = 0.f;
+#pragma unroll
+        for (int n = 0; n < kChains; ++n) a[n][i] = 0.f;
+      }
+      const uint32_t base = ks + g * (DH * 4) + ((c ^ flip_k(g)) << 4);
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+        float4 x;
+        lds4(x, (base ^ ((4 * k & 4) << 4)) + (k >> 1) * 128);
+        uint32_t y[8], qs[8];
+        split_q(x, y);
+        if constexpr (kLate) {
+          split_q(raw[k], qs);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) qs[i] = q[k][i];
+        }
+        float(&m4)[4] = a[k * kChains / kChunks];
+        mma1688(lo, qs[0], qs[1], qs[2], qs[3], y[1], y[3]);
+        mma1688(m4, qs[0], qs[1], qs[2], qs[3], y[0], y[2]);
+        mma1688(lo, qs[4], qs[5], qs[6], qs[7], y[5], y[7]);
+        mma1688(m4, qs[4], qs[5], qs[6], qs[7], y[4], y[6]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x = a[0][i], y = a[0][i + 2];
+#pragma unroll
+        for (int n = 1; n < kChains; ++n) {
+          x += a[n][i];
+          y += a[n][i + 2];
+        }
+        x += y + (lo[i] + lo[i + 2]);
+        s[i] = (ok >> (2 * c + i)) & 1u ? x * scale2 : -INFINITY;
+      }
+    }
+    const float keep = this->weigh(s);
+    uint32_t w[4];
+    split2(s[0], w[0], w[1]);
+    split2(s[1], w[2], w[3]);
+    // rows 2 c and 2 c + 1 have the same exchange
+    const uint32_t base = vs + 2 * c * (DH * 4) + ((g ^ flip_v(2 * c)) << 4);
+#pragma unroll
+    for (int j = 0; j < DH / 32; ++j) {
+      float4 x, y;
+      lds4(x, base + j * 128);
+      lds4(y, base + j * 128 + DH * 4);
+      uint32_t u[8], v[8];
+      split_q(x, u);
+      split_q(y, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float t[4];
+        mma1688_zero(t, w[0], w[1], w[2], w[3], u[2 * e + 1], v[2 * e + 1]);
+        mma1688(t, w[0], w[1], w[2], w[3], u[2 * e], v[2 * e]);
+        float* r = &o[8 * j + 2 * e];
+        r[0] = fmaf(r[0], keep, t[0] + t[2]);
+        r[1] = fmaf(r[1], keep, t[1] + t[3]);
       }
     }
   }
-  MYOS_DEV void write(float* out, float* lse, int G, int d) const {
+
+  MYOS_DEV void write(float* out, int G, int d) const {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    if (g >= G) return;
+    const float inv = this->inverse();
 #pragma unroll
-    for (int g = 0; g < GP; ++g) {
-      if (g >= G) break;
-      const float inv = l[g] > 0.f ? __fdiv_rn(1.0f, l[g]) : 0.f;
-#pragma unroll
-      for (int i = 0; i < kDims; ++i)
-        if (dim(i) < d) out[g * d + dim(i)] = o[g * kDims + i] * inv;
-      if (lse && (threadIdx.x & 31) == 0)
-        lse[g] = l[g] > 0.f ? (m[g] + log2f(l[g])) * kLn2 : -INFINITY;
+    for (int j = 0; j < DH / 32; ++j) {
+      const float* r = &o[8 * j];
+      float* to = out + g * d + 32 * j + 8 * c;
+      if (32 * j + 8 * c >= d) continue;
+      *reinterpret_cast<float4*>(to) = make_float4(r[0] * inv, r[2] * inv, r[4] * inv, r[6] * inv);
+      *reinterpret_cast<float4*>(to + 4) =
+          make_float4(r[1] * inv, r[3] * inv, r[5] * inv, r[7] * inv);
     }
   }
 };
@@ -422,6 +509,10 @@ MYOS_DEV void advance(const PagedAttnArgs& a, int heads, Cursor* c) {
 }
 
 constexpr int kStages = 3, kWarps = 4;
+// An item of at most kWholeTiles tiles costs less in one block than the
+// meeting of several (about 2 us), when there are blocks for all items; and a
+// share of fewer than kMinTiles tiles less than the part it adds to the join.
+constexpr int kWholeTiles = 12, kMinTiles = 4;
 
 template <class W, int DH>
 constexpr size_t attn_smem() {
@@ -429,32 +520,37 @@ constexpr size_t attn_smem() {
          (kWarps - 1) * W::kRegs * 32 * 4;
 }
 
-template <class W, int DH>
+// kFull: head_dim is DH itself (else the chunks behind it are zero-filled).
+template <class W, int DH, bool kFull>
 __global__ void __launch_bounds__(kWarps * 32)
     k_paged_attn(const PagedAttnArgs a, const PagedKv<typename W::KT> kv) {
   using KT = typename W::KT;
   constexpr int T = W::kKeys * kWarps, kThreads = kWarps * 32;
   constexpr int kRowBytes = DH * (int)sizeof(KT), kHalf = W::kKeys * kRowBytes;
-  constexpr int kPart = kMaxGroup * DH + 16;
+  constexpr int kStageBytes = kWarps * 2 * kHalf, kPart = kMaxGroup * DH + 16;
+  constexpr int kRowsEach = W::kKeys / 8, kSegs = kRowBytes / 64;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float ms[kWarps][kMaxGroup], ls[kWarps][kMaxGroup];
-  __shared__ uint32_t okay[kWarps][kStages];
-  __shared__ int64_t sums[33];
+  __shared__ float weights[kWarps][32][kMaxGroup];
+  __shared__ int64_t sums[kWarps];
+  __shared__ int longs[kWarps];
   __shared__ Cursor first_s;
   __shared__ int last_s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int heads = (int)kv.heads, G = a.group, d = (int)kv.d;
+  const int heads = (int)kv.heads, G = a.group, d = kFull ? DH : (int)kv.d;
   const int64_t me = blockIdx.x;
-  float* swap = reinterpret_cast<float*>(smem + (size_t)kStages * kWarps * 2 * kHalf);
+  float* swap = reinterpret_cast<float*>(smem + kStages * kStageBytes);
 
   // this block's share [lo, hi) of the tiles, and where it begins
   const int per = (a.nseq + kThreads - 1) / kThreads;
   const int b0 = min(a.nseq, (int)threadIdx.x * per), b1 = min(a.nseq, b0 + per);
   int64_t mine = 0;
+  int longest = 0;
   for (int b = b0; b < b1; ++b) {
     Cursor c;
     span_of<T>(a, b, &c);
     mine += c.t1 - c.t0;
+    longest = max(longest, c.t1 - c.t0);
   }
   int64_t upto = mine;
 #pragma unroll
@@ -462,32 +558,10 @@ __global__ void __launch_bounds__(kWarps * 32)
     const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += u;
   }
-  if (lane == 31) sums[warp] = upto;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += sums[w];
-    total += sums[w];
-  }
-  total *= heads;
-  // as many shares as blocks, or as tiles if those are fewer: none is empty
-  const int64_t n = max((int64_t)1, min((int64_t)gridDim.x, total));
-  const int64_t lo = min(total, me * total / n), hi = min(total, (me + 1) * total / n);
-  if (lo < hi && (upto - mine) * heads <= lo && lo < upto * heads) {
-    int64_t at = (upto - mine) * heads;
-    Cursor c;
-    int b = b0;
-    for (;; ++b) {
-      span_of<T>(a, b, &c);
-      const int64_t next = at + (int64_t)(c.t1 - c.t0) * heads;
-      if (lo < next) break;
-      at = next;
-    }
-    c.b = b;
-    c.h = (int)((lo - at) / (c.t1 - c.t0));
-    c.t = c.t0 + (int)((lo - at) % (c.t1 - c.t0));
-    first_s = c;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 31) {
+    sums[warp] = upto;
+    longs[warp] = longest;
   }
   // sequences without a key have no tile: their outputs are spread over the blocks
   for (int b = (int)me; b < a.nseq; b += (int)gridDim.x) {
@@ -499,131 +573,217 @@ __global__ void __launch_bounds__(kWarps * 32)
       for (int i = threadIdx.x; i < a.hq; i += kThreads) a.lse[(int64_t)b * a.hq + i] = -INFINITY;
   }
   __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) upto += sums[w];
+    total += sums[w];
+    longest = max(longest, longs[w]);
+  }
+  total *= heads;
+  // n shares, none of them empty; or one for each item
+  const int64_t items = (int64_t)a.nseq * heads;
+  const bool by_item = items <= gridDim.x && longest <= kWholeTiles;
+  const int64_t n = by_item ? items : max((int64_t)1, min((int64_t)gridDim.x, total / kMinTiles));
+  int64_t lo, hi;
+  Cursor ahead;
+  if (by_item) {
+    if (me >= items) return;
+    ahead.b = (int)(me / heads);
+    ahead.h = (int)(me % heads);
+    span_of<T>(a, ahead.b, &ahead);
+    ahead.t = ahead.t0;
+    lo = 0;
+    hi = ahead.t1 - ahead.t0;
+  } else {
+    lo = min(total, me * total / n);
+    hi = min(total, (me + 1) * total / n);
+    if (lo < hi && (upto - mine) * heads <= lo && lo < upto * heads) {
+      int64_t at = (upto - mine) * heads;
+      Cursor c;
+      int b = b0;
+      for (;; ++b) {
+        span_of<T>(a, b, &c);
+        const int64_t next = at + (int64_t)(c.t1 - c.t0) * heads;
+        if (lo < next) break;
+        at = next;
+      }
+      c.b = b;
+      c.h = (int)((lo - at) / (c.t1 - c.t0));
+      c.t = c.t0 + (int)((lo - at) % (c.t1 - c.t0));
+      first_s = c;
+    }
+    __syncthreads();
+    ahead = first_s;
+  }
   if (lo >= hi) return;
 
-  Cursor ahead = first_s, c = first_s;
-  const uint32_t stage0 = smem_u32(smem) + warp * 2 * kHalf;
-  // the page of this lane's key in a tile (lanes past the tile's keys: none)
-  auto look = [&](const Cursor& x) -> int {
-    const int key = x.t * T + warp * W::kKeys + lane;
-    if (lane >= W::kKeys || key < x.start || key >= x.len) return -1;
-    const int pg = a.page_shift >= 0 ? key >> a.page_shift : key / (int)kv.page_size;
-    return a.table[x.b * a.table_stride + pg];
-  };
-  auto issue = [&](const Cursor& x, int page, int stage) {
-    const int key = x.t * T + warp * W::kKeys + lane;
-    const bool on = page >= 0 && (uint32_t)page < kv.num_pages;
-    const int in = a.page_shift >= 0 ? key & ((1 << a.page_shift) - 1) : key % (int)kv.page_size;
-    const int64_t off =
-        on ? page * kv.page_stride + x.h * kv.head_stride + in * kv.slot_stride : -1;
-    const uint32_t ok = __ballot_sync(0xffffffffu, on);
-    if (lane == 0) okay[warp][stage] = ok;
-    constexpr int kChunks = kRowBytes / 16, kEach = 16 / (int)sizeof(KT);
-    const uint32_t dst = stage0 + stage * (kWarps * 2 * kHalf);
+  Cursor c = ahead;
+  const uint32_t stages = smem_u32(smem) + warp * 2 * kHalf;
+  // this lane's copies: rows lane / 4 (+ 8), 16-byte chunks 4 j + lane % 4
+  const int row = lane >> 2, seg = lane & 3;
+  uint32_t to_k[2], to_v[2];
 #pragma unroll
-    for (int i = 0; i < W::kKeys * kChunks / 32; ++i) {
-      const int row = (i * 32 + lane) / kChunks, ch = (i * 32 + lane) % kChunks;
-      const int64_t from = __shfl_sync(0xffffffffu, off, row);
-      const bool load = from >= 0 && ch * kEach < d;
-      const int64_t at = load ? from + ch * kEach : 0;
-      const uint32_t to = dst + 16 * W::place(row, ch);
-      cp_async16(to, kv.k + at, load);
-      cp_async16(to + kHalf, kv.v + at, load);
+  for (int u = 0; u < 2; ++u) {
+    to_k[u] = row * kRowBytes + (((4 * u + seg) ^ W::flip_k(row)) << 4);
+    to_v[u] = kHalf + row * kRowBytes + (((4 * u + seg) ^ W::flip_v(row)) << 4);
+  }
+  // the pages of this lane's rows in a tile
+  int page[kRowsEach];
+  auto look = [&](const Cursor& x) {
+#pragma unroll
+    for (int r = 0; r < kRowsEach; ++r) {
+      const int key = x.t * T + warp * W::kKeys + row + 8 * r;
+      const int pg = a.page_shift >= 0 ? key >> a.page_shift : key / (int)kv.page_size;
+      page[r] = key >= x.start && key < x.len ? a.table[x.b * a.table_stride + pg] : -1;
     }
   };
-  int page = look(ahead);
   int64_t next = lo;  // the tile that is copied next; `page` belongs to it
-  auto step = [&]() {
+  int put_at = 0;     // its stage
+  auto step = [&]() -> uint32_t {  // the keys of the copied tile
+    uint32_t ok = 0;
     if (next < hi) {
-      const Cursor x = ahead;
-      const int pg = page;
+      const uint32_t dst = stages + put_at * kStageBytes;
+      const KT *src_k[kRowsEach], *src_v[kRowsEach];
+      bool on[kRowsEach];
+#pragma unroll
+      for (int r = 0; r < kRowsEach; ++r) {
+        const int key = ahead.t * T + warp * W::kKeys + row + 8 * r;
+        const int in =
+            a.page_shift >= 0 ? key & ((1 << a.page_shift) - 1) : key % (int)kv.page_size;
+        on[r] = (uint32_t)page[r] < kv.num_pages;
+        const int64_t at = on[r] ? page[r] * kv.page_stride + ahead.h * kv.head_stride +
+                                       in * kv.slot_stride + seg * (16 / (int)sizeof(KT))
+                                 : 0;
+        src_k[r] = kv.k + at;
+        src_v[r] = kv.v + at;
+        const uint32_t rows8 = __ballot_sync(0xffffffffu, on[r]);  // bit 4 i: row i
+        ok |= gather_rows(rows8) << (8 * r);
+      }
+#pragma unroll
+      for (int r = 0; r < kRowsEach; ++r)
+#pragma unroll
+        for (int j = 0; j < kSegs; ++j) {
+          const bool load = on[r] && (kFull || (4 * j + seg) * (16 / (int)sizeof(KT)) < d);
+          const uint32_t off = dst + r * 8 * kRowBytes + (j >> 1) * 128;
+          const int from = j * (64 / (int)sizeof(KT));
+          cp_async16(off + to_k[j & 1], kFull ? src_k[r] + from : load ? src_k[r] + from : kv.k, load);
+          cp_async16(off + to_v[j & 1], kFull ? src_v[r] + from : load ? src_v[r] + from : kv.v, load);
+        }
       advance<T>(a, heads, &ahead);
-      if (next + 1 < hi) page = look(ahead);
-      issue(x, pg, (int)((next - lo) % kStages));
+      if (++next < hi) look(ahead);
     }
     cp_commit();
-    ++next;
+    put_at = put_at == kStages - 1 ? 0 : put_at + 1;
+    return ok;
   };
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) step();
+  static_assert(kStages == 3, "key bits of three tiles in one word");
+  look(ahead);
+  uint64_t okay = step();
+  okay |= (uint64_t)step() << 16;
 
   W w;
+  int take_at = 0;
   for (int64_t i = lo; i < hi; ++i) {
-    if (i == lo || c.t == c.t0)
-      w.begin(a.q + c.b * a.q_stride + (int64_t)c.h * G * d, G, d);
+    if (i == lo || c.t == c.t0) w.begin(a.q + c.b * a.q_stride + (int64_t)c.h * G * d, G, d);
     cp_wait<kStages - 2>();
     __syncwarp();
-    step();
-    const int stage = (int)((i - lo) % kStages);
-    const uint32_t ok = okay[warp][stage];
-    const uint32_t base = stage0 + stage * (kWarps * 2 * kHalf);
+    okay |= (uint64_t)step() << 32;
+    const uint32_t base = stages + take_at * kStageBytes, ok = (uint32_t)okay & 0xffffu;
+    take_at = take_at == kStages - 1 ? 0 : take_at + 1;
+    okay >>= 16;
     if (ok) w.tile(base, base + kHalf, ok, a.scale2);
     __syncwarp();
     if (c.t + 1 == c.t1 || i + 1 == hi) {
-      // the piece's end: the warps' states into warp 0's
-      w.finish();
-      __syncthreads();  // the swap space of the piece before is free
-      w.put_ml(ms[warp], ls[warp]);
-      if (warp > 0) {
-        float* s = swap + (warp - 1) * W::kRegs * 32;
-#pragma unroll
-        for (int r = 0; r < W::kRegs; r += 4)
-          *reinterpret_cast<float4*>(s + r * 32 + lane * 4) =
-              make_float4(w.o[r], w.o[r + 1], w.o[r + 2], w.o[r + 3]);
-      }
-      __syncthreads();
       const int64_t i0 = i - (c.t - c.t0), i1 = i0 + (c.t1 - c.t0);
       const bool whole = i0 >= lo && i1 <= hi;
-      if (warp == 0)
-#pragma unroll 1
-        for (int u = 1; u < kWarps; ++u) w.join(swap + (u - 1) * W::kRegs * 32, ms[u], ls[u]);
-      if (!whole) {
-        const int64_t c0 = ((i0 + 1) * n - 1) / total, c1 = (i1 * n - 1) / total;
+      w.finish();
+      // the warps' states into warp 0's; for the last block of a split item a
+      // second time, with the states of the parts
+      for (bool done = whole;; done = true) {
+        __syncthreads();  // the swap space is free
+        if (warp > 0) w.put(ms[warp], ls[warp], swap + (warp - 1) * W::kRegs * 32);
+        __syncthreads();
         if (warp == 0) {
-          float* part = a.parts + (me * 2 + (i0 < lo ? 0 : 1)) * kPart;
-          w.put_ml(part, part + kMaxGroup);
-          part += 16;
-#pragma unroll
-          for (int r = 0; r < W::kRegs; r += 4)
-            *reinterpret_cast<float4*>(part + r * 32 + lane * 4) =
-                make_float4(w.o[r], w.o[r + 1], w.o[r + 2], w.o[r + 3]);
+#pragma unroll 1
+          for (int u = 1; u < kWarps; ++u) w.join(ms[u], ls[u], swap + (u - 1) * W::kRegs * 32);
+          if (done) {
+            w.write(a.out + c.b * a.out_stride + (int64_t)c.h * G * d, G, d);
+            w.put_lse(a.lse ? a.lse + (int64_t)c.b * a.hq + c.h * G : nullptr, G);
+          }
+        }
+        if (done) break;
+        const int64_t c0 = ((i0 + 1) * n - 1) / total, c1 = (i1 * n - 1) / total;
+        auto part_of = [&](int64_t p) {
+          return a.parts + (p * 2 + (i0 < p * total / n ? 0 : 1)) * kPart;
+        };
+        if (warp == 0) {
+          float* part = part_of(me);
+          w.put(part, part + kMaxGroup, part + 16);
           __threadfence();
           __syncwarp();
           if (lane == 0) {
             const unsigned before = atomicAdd(&a.arrived[c0], 1u);
             last_s = before == (unsigned)(c1 - c0);
             if (last_s) a.arrived[c0] = 0;
+            __threadfence();
           }
-          __threadfence();
         }
         __syncthreads();
-        if (last_s) {
-          // the parts in the order of their shares, a run of them for each warp
-          __threadfence();
-          const int64_t count = c1 - c0 + 1, run = (count + kWarps - 1) / kWarps;
-          const int64_t p0 = c0 + min(count, warp * run), p1 = c0 + min(count, (warp + 1) * run);
-          w.begin(a.q, 0, 0);
-          for (int64_t p = p0; p < p1; ++p) {
-            const float* part = a.parts + (p * 2 + (i0 < p * total / n ? 0 : 1)) * kPart;
-            w.join(part + 16, part, part + kMaxGroup);
-          }
-          w.put_ml(ms[warp], ls[warp]);
-          if (warp > 0) {
-            float* s = swap + (warp - 1) * W::kRegs * 32;
+        if (!last_s) break;
+        // the parts in the order of their shares, a run of them for each warp,
+        // 32 at a time: a lane weighs one of them, then all add them up
+        const int64_t count = c1 - c0 + 1, run = (count + kWarps - 1) / kWarps;
+        const int64_t p0 = c0 + min(count, warp * run), p1 = c0 + min(count, (warp + 1) * run);
+        w.clear();
+        float top[kMaxGroup], sum[kMaxGroup];
 #pragma unroll
-            for (int r = 0; r < W::kRegs; r += 4)
-              *reinterpret_cast<float4*>(s + r * 32 + lane * 4) =
-                  make_float4(w.o[r], w.o[r + 1], w.o[r + 2], w.o[r + 3]);
-          }
-          __syncthreads();
-          if (warp == 0)
-#pragma unroll 1
-            for (int u = 1; u < kWarps; ++u) w.join(swap + (u - 1) * W::kRegs * 32, ms[u], ls[u]);
+        for (int g = 0; g < kMaxGroup; ++g) {
+          top[g] = -INFINITY;
+          sum[g] = 0.f;
         }
+#pragma unroll 1
+        for (int64_t p = p0; p < p1; p += 32) {
+          const int now = (int)min((int64_t)32, p1 - p);
+          float pm[kMaxGroup], pl[kMaxGroup];
+#pragma unroll
+          for (int g = 0; g < kMaxGroup; ++g) {
+            pm[g] = -INFINITY;
+            pl[g] = 0.f;
+          }
+          if (lane < now) {
+            const float* head = part_of(p + lane);
+#pragma unroll
+            for (int g = 0; g < kMaxGroup; g += 4) {
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(head + g));
+              const float4 y = __ldcg(reinterpret_cast<const float4*>(head + kMaxGroup + g));
+              pm[g] = x.x, pm[g + 1] = x.y, pm[g + 2] = x.z, pm[g + 3] = x.w;
+              pl[g] = y.x, pl[g + 1] = y.y, pl[g + 2] = y.z, pl[g + 3] = y.w;
+            }
+          }
+          __syncwarp();
+          float mine_keep = 1.f;
+#pragma unroll
+          for (int g = 0; g < kMaxGroup; ++g) {
+            const float t = fmaxf(top[g], warp_max(pm[g]));
+            const float keep = weight_of(top[g], t), f = weight_of(pm[g], t);
+            if (g == lane >> 2) mine_keep = keep;
+            sum[g] = sum[g] * keep + warp_sum(pl[g] * f);
+            top[g] = t;
+            weights[warp][lane][g] = f;
+          }
+          __syncwarp();
+          if (p > p0) w.rescale(mine_keep);
+#pragma unroll 2
+          for (int u = 0; u < now; ++u) w.add(part_of(p + u) + 16, weights[warp][u][lane >> 2]);
+        }
+#pragma unroll
+        for (int g = 0; g < kMaxGroup; ++g)
+          if (g == lane >> 2) {
+            w.m = top[g];
+            w.l = sum[g];
+          }
       }
-      if (warp == 0 && (whole || last_s))
-        w.write(a.out + c.b * a.out_stride + (int64_t)c.h * G * d,
-                a.lse ? a.lse + (int64_t)c.b * a.hq + c.h * G : nullptr, G, d);
     }
     advance<T>(a, heads, &c);
   }
@@ -636,34 +796,37 @@ int sm_count() {
   return sms;
 }
 
-template <class W, int DH>
+template <class W, int DH, bool kFull>
 cudaError_t launch(PagedAttnArgs a, const myos_paged_kv* kv, void* work, cudaStream_t st) {
-  constexpr size_t smem = attn_smem<W, DH>();
+  constexpr size_t smem = attn_smem<W, DH>(), kCounters = 16 * 1024;
   constexpr int T = W::kKeys * kWarps;
-  static_assert(256 * 4 * 16 + (size_t)kMaxShares * 2 * (kMaxGroup * DH + 16) * 4 <=
+  static_assert(kCounters + (size_t)kMaxShares * 2 * (kMaxGroup * DH + 16) * 4 <=
                 MYOS_PAGED_WORK_BYTES);
-  cudaError_t e = cudaFuncSetAttribute(k_paged_attn<W, DH>,
+  cudaError_t e = cudaFuncSetAttribute(k_paged_attn<W, DH, kFull>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   a.arrived = static_cast<unsigned*>(work);
-  a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + 256 * 4 * 16);
-  // a share per resident block, and never more shares than there can be tiles
+  a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + kCounters);
+  // a share per resident block, and never more than there can be tiles
   int64_t keys = a.max_keys;
   if (a.window > 0 && (int64_t)a.window + T < keys) keys = (int64_t)a.window + T;
   const int64_t most = (int64_t)a.nseq * kv->num_kv_heads * ((keys + T - 1) / T);
   int64_t grid = (int64_t)sm_count() * (smem <= 110 * 1024 ? 2 : 1);
   if (grid > kMaxShares) grid = kMaxShares;
   if (grid > most) grid = most;
-  k_paged_attn<W, DH><<<(int)grid, kWarps * 32, smem, st>>>(a, paged_view<typename W::KT>(kv));
+  k_paged_attn<W, DH, kFull>
+      <<<(int)grid, kWarps * 32, smem, st>>>(a, paged_view<typename W::KT>(kv));
   return counted(cudaGetLastError());
 }
 
 template <int DH>
 cudaError_t launch_d(const PagedAttnArgs& a, const myos_paged_kv* kv, void* work,
                      cudaStream_t st) {
-  if (kv->kv_dtype == MYOS_KV_BF16) return launch<MmaWarp<DH>, DH>(a, kv, work, st);
-  return a.group <= 4 ? launch<FmaWarp<DH, 4>, DH>(a, kv, work, st)
-                      : launch<FmaWarp<DH, 8>, DH>(a, kv, work, st);
+  if (kv->kv_dtype == MYOS_KV_BF16)
+    return kv->head_dim == DH ? launch<Bf16Warp<DH>, DH, true>(a, kv, work, st)
+                              : launch<Bf16Warp<DH>, DH, false>(a, kv, work, st);
+  return kv->head_dim == DH ? launch<F32Warp<DH>, DH, true>(a, kv, work, st)
+                            : launch<F32Warp<DH>, DH, false>(a, kv, work, st);
 }
 
 }  // namespace

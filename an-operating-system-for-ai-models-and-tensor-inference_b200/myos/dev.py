@@ -17,7 +17,6 @@ raises MyosError with the C call's status and has no effect.
 from __future__ import annotations
 
 import ctypes as C
-import math
 
 import numpy as np
 import torch
@@ -27,70 +26,94 @@ from ._lib import ERR_ARG, ERR_SHAPE, MyosError
 
 WORK_BYTES = _lib.PAGED_WORK_BYTES
 _KV = {torch.float32: _lib.KV_F32, torch.bfloat16: _lib.KV_BF16}
-_W32 = (torch.int32, torch.uint32)
+_F32, _I32, _W32 = (torch.float32,), (torch.int32,), (torch.int32, torch.uint32)
+_I64, _BF16, _U8 = (torch.int64,), (torch.bfloat16,), (torch.uint8,)
+
+# A serving step makes these calls once per layer and token, each a few
+# microseconds of device time, so the checks below ask a tensor the fewest
+# questions that settle them; _refusal finds the reason after one failed.
 
 
 def _refuse(code, msg):
     raise MyosError(code, msg)
 
 
-class _Call:
-    """Pointers of one call's tensors, all on the first one's device."""
-    __slots__ = ("dev",)
+def _refusal(t, what, dtypes, dev, shape):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _refuse(ERR_ARG, f"{what}: not a CUDA tensor")
+    if t.get_device() != dev:
+        _refuse(ERR_ARG, f"{what}: on cuda:{t.get_device()}, not cuda:{dev}")
+    if t.dtype not in dtypes:
+        _refuse(ERR_ARG, f"{what}: dtype {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        _refuse(ERR_SHAPE, f"{what}: {list(shape)} wanted, got {list(t.shape)}")
+    _refuse(ERR_ARG, f"{what}: strides {t.stride()}")
 
-    def __init__(self, first):
-        if not isinstance(first, torch.Tensor) or not first.is_cuda:
-            _refuse(ERR_ARG, "tensors live on a CUDA device")
-        self.dev = first.get_device()
 
-    def ptr(self, t, what, dtypes, ndim=1):
-        """The address of t (0 for None)."""
-        if t is None:
-            return None
-        if not isinstance(t, torch.Tensor) or t.get_device() != self.dev:
-            _refuse(ERR_ARG, f"{what}: not a tensor on cuda:{self.dev}")
-        if t.dtype is not dtypes and not (type(dtypes) is tuple and t.dtype in dtypes):
-            _refuse(ERR_ARG, f"{what}: dtype {t.dtype}")
-        if t.dim() != ndim:
-            _refuse(ERR_SHAPE, f"{what}: {ndim} dimensions wanted, got {t.dim()}")
-        if t.stride(-1) != 1 and t.size(-1) > 1:
-            _refuse(ERR_ARG, f"{what}: the last dimension is not contiguous")
-        return t.data_ptr()
+def _device(t, what):
+    """The ordinal of a CUDA tensor's device."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _refuse(ERR_ARG, f"{what}: not a CUDA tensor")
+    return t.get_device()
 
-    def vec(self, t, what, dtypes, n):
-        """The address of a 1-D tensor of n values (None stays None)."""
-        p = self.ptr(t, what, dtypes)
-        if t is not None and t.size(0) != n:
-            _refuse(ERR_SHAPE, f"{what}: {n} values wanted, got {t.size(0)}")
-        return p
 
-    def run(self, what, fn, *args, stream=None):
-        if stream is None:
-            stream = torch.cuda.current_stream(self.dev)
-        stream = getattr(stream, "cuda_stream", stream)
-        if self.dev == torch.cuda.current_device():
+def _vec(t, what, dtypes, dev, n):
+    """The address of n contiguous values; None stays None."""
+    if t is None:
+        return None
+    try:
+        if t.dtype in dtypes and t.get_device() == dev and t.numel() == n and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refusal(t, what, dtypes, dev, (n,))
+
+
+def _rows(t, what, dtypes, dev, shape):
+    """(address, elements from row to row) of a tensor of this shape whose rows
+    are contiguous; a single row has no stride of its own."""
+    try:
+        if t.dtype in dtypes and t.get_device() == dev and t.shape == shape:
+            if t.is_contiguous():
+                n = t.numel()
+                return t.data_ptr(), n // shape[0] if n else 0
+            st = t.stride()
+            if len(shape) == 2:
+                row = shape[1]
+                ok = st[1] == 1 or row == 1
+            else:
+                row = shape[1] * shape[2]
+                ok = (st[2] == 1 or shape[2] == 1) and (st[1] == shape[2] or shape[1] == 1)
+            if ok:
+                return t.data_ptr(), st[0] if shape[0] > 1 else row
+    except AttributeError:
+        pass
+    _refusal(t, what, dtypes, dev, shape)
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+
+_fns = {}
+
+
+def _fn(name):
+    f = _fns.get(name)
+    if f is None:
+        f = _fns[name] = getattr(_lib.load(), name)
+    return f
+
+
+def _run(what, dev, stream, fn, *args):
+    stream = _raw_stream(dev) if stream is None else getattr(stream, "cuda_stream", stream)
+    if dev == torch.cuda.current_device():
+        st = fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
             st = fn(*args, stream)
-        else:
-            with torch.cuda.device(self.dev):
-                st = fn(*args, stream)
-        if st != 0:
-            _refuse(st, what)
-
-
-def _row_stride(t):
-    """Elements from one row of t to the next; a single row has none of its own."""
-    if t.size(0) > 1:
-        return t.stride(0)
-    n = 1
-    for s in t.shape[1:]:
-        n *= s
-    return max(t.stride(0), n)
-
-
-def _packed(t, what):
-    """[rows, heads, d] with the heads of a row next to each other."""
-    if t.size(1) > 1 and t.stride(1) != t.size(2):
-        _refuse(ERR_ARG, f"{what}: the heads of a row are not contiguous")
+    if st != 0:
+        _refuse(st, what)
 
 
 class PagedKV:
@@ -99,21 +122,28 @@ class PagedKV:
     [num_pages, page_size, num_kv_heads, head_dim] is passed as
     ``t.permute(0, 2, 1, 3)``). Holds the tensors, copies nothing."""
 
+    __slots__ = ("k", "v", "dev", "num_kv_heads", "head_dim", "c", "ref")
+
     def __init__(self, k, v):
-        c = _Call(k)
-        kp, vp = c.ptr(k, "k", (torch.float32, torch.bfloat16), 4), c.ptr(v, "v", k.dtype, 4)
-        pages, heads, slots, d = k.shape
-        sp, sh, ss, _ = k.stride()
-        if v.shape != k.shape or v.stride() != k.stride():
-            _refuse(ERR_SHAPE, "k and v differ in shape or strides")
-        if max(pages, heads, slots, d) > 0x7fffffff:
-            _refuse(ERR_SHAPE, "cache dimensions")
-        # a dimension of one element has no stride of its own
-        n = max(d, ss if slots > 1 else 0, sh if heads > 1 else 0)
-        self.k, self.v, self.dev = k, v, c.dev
+        dev = _device(k, "k")
+        kind, shape, st = _KV.get(k.dtype), k.shape, k.stride()
+        if kind is None:
+            _refuse(ERR_ARG, f"k: dtype {k.dtype}")
+        if len(shape) != 4 or max(shape) > 0x7fffffff:
+            _refuse(ERR_SHAPE, f"k: [pages, heads, slots, dim] wanted, got {list(shape)}")
+        pages, heads, slots, d = shape
+        sp, sh, ss, sd = st
+        if (getattr(v, "shape", None) != shape or v.dtype is not k.dtype or v.get_device() != dev
+                or v.stride() != st):
+            _refuse(ERR_ARG, "k and v differ in shape, strides, dtype or device")
+        if sd != 1 and d > 1:
+            _refuse(ERR_ARG, "the last dimension is not contiguous")
+        if 1 in shape:  # a dimension of one element has no stride of its own
+            n = max(d, ss if slots > 1 else 0, sh if heads > 1 else 0)
+            sp, sh, ss = (x if m > 1 else n for x, m in ((sp, pages), (sh, heads), (ss, slots)))
+        self.k, self.v, self.dev = k, v, dev
         self.num_kv_heads, self.head_dim = heads, d
-        self.c = _lib.PagedKV(kp, vp, sp if pages > 1 else n, sh if heads > 1 else n,
-                              ss if slots > 1 else n, pages, slots, heads, d, _KV[k.dtype], 0)
+        self.c = _lib.PagedKV(k.data_ptr(), v.data_ptr(), sp, sh, ss, pages, slots, heads, d, kind, 0)
         self.ref = C.byref(self.c)
 
 
@@ -139,18 +169,17 @@ def paged_tables(block_table, ctx_lens, new_lens, free_pages, num_free, page_siz
     slots (int64), positions, row_seq [max_rows], kv_lens [nseq], seq_starts
     [nseq + 1] and result [2] (pages left, requests refused) are written. All
     integers but slots are int32."""
-    c, i32 = _Call(block_table), torch.int32
-    table = c.ptr(block_table, "block_table", i32, 2)
+    dev = _device(block_table, "block_table")
+    table, stride = _rows(block_table, "block_table", _I32, dev, block_table.shape)
     nseq, blocks = block_table.shape
-    rows = slots.size(0)
-    c.run("paged_tables", _lib.load().myos_dev_paged_tables, table, _row_stride(block_table), blocks,
-          c.vec(ctx_lens, "ctx_lens", i32, nseq), c.vec(new_lens, "new_lens", i32, nseq), nseq,
-          c.ptr(free_pages, "free_pages", i32), free_pages.size(0),
-          c.vec(num_free, "num_free", i32, 1), page_size, num_pages,
-          c.ptr(slots, "slots", torch.int64), c.vec(positions, "positions", i32, rows),
-          c.vec(row_seq, "row_seq", i32, rows), rows, c.vec(kv_lens, "kv_lens", i32, nseq),
-          c.vec(seq_starts, "seq_starts", i32, nseq + 1), c.vec(result, "result", i32, 2),
-          stream=stream)
+    rows, cap = slots.numel(), free_pages.numel()
+    _run("paged_tables", dev, stream, _fn("myos_dev_paged_tables"), table, stride, blocks,
+         _vec(ctx_lens, "ctx_lens", _I32, dev, nseq), _vec(new_lens, "new_lens", _I32, dev, nseq),
+         nseq, _vec(free_pages, "free_pages", _I32, dev, cap), cap,
+         _vec(num_free, "num_free", _I32, dev, 1), page_size, num_pages,
+         _vec(slots, "slots", _I64, dev, rows), _vec(positions, "positions", _I32, dev, rows),
+         _vec(row_seq, "row_seq", _I32, dev, rows), rows, _vec(kv_lens, "kv_lens", _I32, dev, nseq),
+         _vec(seq_starts, "seq_starts", _I32, dev, nseq + 1), _vec(result, "result", _I32, dev, 2))
 
 
 def qk_norm_rope_store(q_out, qkv, kv: PagedKV, positions, slots, cos=None, sin=None,
@@ -161,28 +190,25 @@ def qk_norm_rope_store(q_out, qkv, kv: PagedKV, positions, slots, cos=None, sin=
     k_gamma, then k and v into the cache at slots [rows] (int64, negative: not
     stored): myos_dev_qk_norm_rope_store. q_out may be a view of qkv's own q
     part."""
-    c, f32 = _Call(qkv), torch.float32
-    rows, width = qkv.size(0), qkv.size(-1)
-    qp, ip = c.ptr(q_out, "q_out", f32, 3), c.ptr(qkv, "qkv", f32, 2)
-    hq, d = q_out.size(1), kv.head_dim
-    if kv.dev != c.dev:
-        _refuse(ERR_ARG, f"kv: not on cuda:{c.dev}")
-    if q_out.size(0) != rows or q_out.size(2) != d or width != (hq + 2 * kv.num_kv_heads) * d:
-        _refuse(ERR_SHAPE, "q_out, qkv and the cache disagree")
-    _packed(q_out, "q_out")
-    half = npos = 0
+    dev = _device(qkv, "qkv")
+    if kv.dev != dev:
+        _refuse(ERR_ARG, f"kv: on cuda:{kv.dev}, not cuda:{dev}")
+    rows, hq, d = q_out.shape
+    qp, qs = _rows(q_out, "q_out", _F32, dev, (rows, hq, kv.head_dim))
+    ip, istride = _rows(qkv, "qkv", _F32, dev, (rows, (hq + 2 * kv.num_kv_heads) * d))
+    npos = rot = 0
+    cp = sp = None
     if cos is not None or sin is not None:
-        if cos is None or sin is None or cos.shape != sin.shape:
-            _refuse(ERR_SHAPE, "cos and sin come together, of one shape")
-        npos, half = cos.shape
-        if not cos.is_contiguous() or not sin.is_contiguous():
+        npos, half = (cos if cos is not None else sin).shape
+        rot = 2 * half
+        cp, cstride = _rows(cos, "cos", _F32, dev, (npos, half))
+        sp, sstride = _rows(sin, "sin", _F32, dev, (npos, half))
+        if npos > 1 and not cstride == sstride == half:
             _refuse(ERR_ARG, "cos and sin are contiguous")
-    c.run("qk_norm_rope_store", _lib.load().myos_dev_qk_norm_rope_store, qp, _row_stride(q_out), ip,
-          _row_stride(qkv), rows, hq, kv.ref, c.vec(q_gamma, "q_gamma", torch.bfloat16, d),
-          c.vec(k_gamma, "k_gamma", torch.bfloat16, d), eps, c.ptr(cos, "cos", f32, 2),
-          c.ptr(sin, "sin", f32, 2), npos, 2 * half,
-          c.vec(positions, "positions", torch.int32, rows),
-          c.vec(slots, "slots", torch.int64, rows), stream=stream)
+    _run("qk_norm_rope_store", dev, stream, _fn("myos_dev_qk_norm_rope_store"), qp, qs, ip, istride,
+         rows, hq, kv.ref, _vec(q_gamma, "q_gamma", _BF16, dev, d),
+         _vec(k_gamma, "k_gamma", _BF16, dev, d), eps, cp, sp, npos, rot,
+         _vec(positions, "positions", _I32, dev, rows), _vec(slots, "slots", _I64, dev, rows))
 
 
 def paged_attention(out, q, kv: PagedKV, block_table, kv_lens, work, scale=None, window: int = 0,
@@ -192,26 +218,25 @@ def paged_attention(out, q, kv: PagedKV, block_table, kv_lens, work, scale=None,
     (optional) their log-sum-exp. scale defaults to 1 / sqrt(d). work: at least
     WORK_BYTES of uint8, zeroed once before its first use, not shared by calls
     that may run at the same time: myos_dev_paged_attn."""
-    c, f32 = _Call(q), torch.float32
-    qp, op = c.ptr(q, "q", f32, 3), c.ptr(out, "out", f32, 3)
-    nseq, hq, d = q.shape
-    if kv.dev != c.dev:
-        _refuse(ERR_ARG, f"kv: not on cuda:{c.dev}")
-    if out.shape != q.shape or d != kv.head_dim:
-        _refuse(ERR_SHAPE, "out, q and the cache disagree")
-    _packed(q, "q")
-    _packed(out, "out")
-    lp = c.ptr(lse, "lse", f32, 2)
-    if lse is not None and (lse.shape != (nseq, hq) or not lse.is_contiguous()):
-        _refuse(ERR_SHAPE, "lse: [nseq, num_q_heads], contiguous")
-    table = c.ptr(block_table, "block_table", torch.int32, 2)
-    if block_table.size(0) != nseq:
-        _refuse(ERR_SHAPE, "block_table: one row per sequence")
-    c.run("paged_attention", _lib.load().myos_dev_paged_attn, op, _row_stride(out), lp, qp,
-          _row_stride(q), nseq, hq, kv.ref, table, _row_stride(block_table), block_table.size(1),
-          c.vec(kv_lens, "kv_lens", torch.int32, nseq),
-          1.0 / math.sqrt(d) if scale is None else scale, window,
-          c.ptr(work, "work", torch.uint8), work.size(0), stream=stream)
+    dev = _device(q, "q")
+    if kv.dev != dev:
+        _refuse(ERR_ARG, f"kv: on cuda:{kv.dev}, not cuda:{dev}")
+    nseq, hq, d = shape = q.shape
+    if d != kv.head_dim:
+        _refuse(ERR_SHAPE, f"q: head_dim {d}, the cache's is {kv.head_dim}")
+    qp, qs = _rows(q, "q", _F32, dev, shape)
+    op, ostride = _rows(out, "out", _F32, dev, shape)
+    lp = None
+    if lse is not None:
+        lp, lstride = _rows(lse, "lse", _F32, dev, (nseq, hq))
+        if nseq > 1 and lstride != hq:
+            _refuse(ERR_ARG, "lse is contiguous")
+    blocks = block_table.shape[-1]
+    tp, ts = _rows(block_table, "block_table", _I32, dev, (nseq, blocks))
+    bytes_ = work.numel()
+    _run("paged_attention", dev, stream, _fn("myos_dev_paged_attn"), op, ostride, lp, qp, qs, nseq,
+         hq, kv.ref, tp, ts, blocks, _vec(kv_lens, "kv_lens", _I32, dev, nseq),
+         d ** -0.5 if scale is None else scale, window, _vec(work, "work", _U8, dev, bytes_), bytes_)
 
 
 def logit_controls(out, logits, history=None, prompt_lens=None, hist_lens=None, repetition=None,
@@ -224,29 +249,34 @@ def logit_controls(out, logits, history=None, prompt_lens=None, hist_lens=None, 
     mask_rows[r], negative: none); ids [rows] (int32 or uint32) the greedy ids
     of the result: myos_dev_logit_controls. out may be logits (in place) or
     None (only ids)."""
-    c, f32, i32 = _Call(logits), torch.float32, torch.int32
-    lp, op = c.ptr(logits, "logits", f32, 2), c.ptr(out, "out", f32, 2)
-    rows, vocab = logits.shape
-    if out is not None and out.shape != logits.shape:
-        _refuse(ERR_SHAPE, "out and logits differ in shape")
-    hp, mp = c.ptr(history, "history", i32, 2), c.ptr(mask, "mask", _W32, 2)
-    if history is not None and history.size(0) != rows:
-        _refuse(ERR_SHAPE, "history: one row per row of logits")
-    nb = 0
+    dev = _device(logits, "logits")
+    rows, vocab = shape = logits.shape
+    lp, ls = _rows(logits, "logits", _F32, dev, shape)
+    op = ostride = hp = hs = width = mp = ms = masks = nb = 0
+    if out is not None:
+        op, ostride = _rows(out, "out", _F32, dev, shape)
+    if history is not None:
+        width = history.shape[-1]
+        hp, hs = _rows(history, "history", _I32, dev, (rows, width))
     if bias_starts is not None:
-        if bias_ids is None or bias_vals is None or bias_ids.shape != bias_vals.shape:
-            _refuse(ERR_SHAPE, "bias_ids and bias_vals come together, of one shape")
-        nb = bias_ids.size(0)
-    if mask is not None and mask.size(1) * 32 < vocab:
-        _refuse(ERR_SHAPE, "mask: fewer bits than the vocabulary")
+        if bias_ids is None or bias_vals is None:
+            _refuse(ERR_ARG, "bias_starts, bias_ids and bias_vals come together")
+        nb = bias_ids.numel()
+    if mask is not None:
+        masks, words = mask.shape
+        mp, ms = _rows(mask, "mask", _W32, dev, (masks, words))
+        if words * 32 < vocab:
+            _refuse(ERR_SHAPE, "mask: fewer bits than the vocabulary")
     a = _lib.LogitControls(
-        hp, 0 if history is None else _row_stride(history), 0 if history is None else history.size(1),
-        c.vec(prompt_lens, "prompt_lens", i32, rows), c.vec(hist_lens, "hist_lens", i32, rows),
-        c.vec(repetition, "repetition", f32, rows), c.vec(frequency, "frequency", f32, rows),
-        c.vec(presence, "presence", f32, rows), c.vec(bias_starts, "bias_starts", i32, rows + 1),
-        c.ptr(bias_ids, "bias_ids", i32), c.ptr(bias_vals, "bias_vals", f32), nb,
-        mp, 0 if mask is None else _row_stride(mask), 0 if mask is None else mask.size(0),
-        c.vec(mask_rows, "mask_rows", i32, rows))
-    c.run("logit_controls", _lib.load().myos_dev_logit_controls, op,
-          0 if out is None else _row_stride(out), lp, _row_stride(logits), rows, vocab, C.byref(a),
-          c.vec(ids, "ids", _W32, rows), stream=stream)
+        hp, hs, width, _vec(prompt_lens, "prompt_lens", _I32, dev, rows),
+        _vec(hist_lens, "hist_lens", _I32, dev, rows),
+        _vec(repetition, "repetition", _F32, dev, rows),
+        _vec(frequency, "frequency", _F32, dev, rows), _vec(presence, "presence", _F32, dev, rows),
+        _vec(bias_starts, "bias_starts", _I32, dev, rows + 1),
+        _vec(bias_ids, "bias_ids", _I32, dev, nb) if nb else None,
+        _vec(bias_vals, "bias_vals", _F32, dev, nb) if nb else None, nb,
+        mp, ms, masks, _vec(mask_rows, "mask_rows", _I32, dev, rows))
+    if not nb:
+        a.bias_starts = None
+    _run("logit_controls", dev, stream, _fn("myos_dev_logit_controls"), op, ostride, lp, ls, rows,
+         vocab, C.byref(a), _vec(ids, "ids", _W32, dev, rows))
