@@ -110,6 +110,11 @@ MYOS_DEV void lds4(float4& x, uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
+MYOS_DEV unsigned arrive(unsigned* count) {
+  unsigned before;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(count) : "memory");
+  return before;
+}
 // Bits 0, 4, .., 28 next to each other.
 MYOS_DEV uint32_t gather_rows(uint32_t x) {
   x &= 0x11111111u;
@@ -204,15 +209,13 @@ struct WarpState {
 #pragma unroll
     for (int r = 0; r < kRegs; ++r) o[r] *= a;
   }
-  MYOS_DEV void add(const float* os, float b) {
-    const int lane = threadIdx.x & 31;
+  MYOS_DEV void add(const float4 (&x)[kRegs / 4], float b) {
 #pragma unroll
-    for (int r = 0; r < kRegs; r += 4) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(os + r * 32 + lane * 4));
-      o[r] = fmaf(x.x, b, o[r]);
-      o[r + 1] = fmaf(x.y, b, o[r + 1]);
-      o[r + 2] = fmaf(x.z, b, o[r + 2]);
-      o[r + 3] = fmaf(x.w, b, o[r + 3]);
+    for (int r = 0; r < kRegs / 4; ++r) {
+      o[4 * r] = fmaf(x[r].x, b, o[4 * r]);
+      o[4 * r + 1] = fmaf(x[r].y, b, o[4 * r + 1]);
+      o[4 * r + 2] = fmaf(x[r].z, b, o[4 * r + 2]);
+      o[4 * r + 3] = fmaf(x[r].w, b, o[4 * r + 3]);
     }
   }
   // Maximum and weights of a tile's scores s (in powers of two, -inf: no key;
@@ -509,10 +512,109 @@ MYOS_DEV void advance(const PagedAttnArgs& a, int heads, Cursor* c) {
 }
 
 constexpr int kStages = 3, kWarps = 4;
-// An item of at most kWholeTiles tiles costs less in one block than the
-// meeting of several (about 2 us), when there are blocks for all items; and a
-// share of fewer than kMinTiles tiles less than the part it adds to the join.
-constexpr int kWholeTiles = 12, kMinTiles = 4;
+// The meeting of several blocks costs about as much as kJoinTiles tiles, and a
+// share of fewer than kMinTiles tiles saves less than the part it adds to it.
+constexpr int kJoinTiles = 5, kMinTiles = 2;
+
+// The parts of one split item: shares first .. last. All but the first share
+// begin inside the item, so their part is their first piece (slot 0); the
+// first share's is its last piece (slot 1).
+struct Parts {
+  int64_t first, last;
+  bool second;  // whether the first share's part is in slot 1
+};
+
+template <int DH>
+MYOS_DEV float* part_of(float* parts, const Parts& ps, int64_t share) {
+  const int slot = share == ps.first && ps.second ? 1 : 0;
+  return parts + (share * 2 + slot) * (kMaxGroup * DH + 16);
+}
+
+// By the last block of a split item: its parts in the order of their shares, a
+// run of them for each warp, 32 at a time (a lane weighs one of them, then all
+// add them up), then the warps' sums in order. Out of line: its registers are
+// not the main loop's.
+template <class W, int DH>
+__device__ __noinline__ void join_parts(float* parts, const Parts ps, float* swap, float* out,
+                                        float* lse, int G, int d) {
+  __shared__ float ms[kWarps][kMaxGroup], ls[kWarps][kMaxGroup];
+  __shared__ float weights[kWarps][32][kMaxGroup];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t count = ps.last - ps.first + 1, run = (count + kWarps - 1) / kWarps;
+  const int64_t p0 = ps.first + min(count, warp * run);
+  const int64_t p1 = ps.first + min(count, (warp + 1) * run);
+  W w;
+  w.clear();
+  float top[kMaxGroup], sum[kMaxGroup];
+#pragma unroll
+  for (int g = 0; g < kMaxGroup; ++g) {
+    top[g] = -INFINITY;
+    sum[g] = 0.f;
+  }
+#pragma unroll 1
+  for (int64_t p = p0; p < p1; p += 32) {
+    const int now = (int)min((int64_t)32, p1 - p);
+    float pm[kMaxGroup], pl[kMaxGroup];
+#pragma unroll
+    for (int g = 0; g < kMaxGroup; ++g) {
+      pm[g] = -INFINITY;
+      pl[g] = 0.f;
+    }
+    if (lane < now) {
+      const float* head = part_of<DH>(parts, ps, p + lane);
+#pragma unroll
+      for (int g = 0; g < kMaxGroup; g += 4) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(head + g));
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(head + kMaxGroup + g));
+        pm[g] = x.x, pm[g + 1] = x.y, pm[g + 2] = x.z, pm[g + 3] = x.w;
+        pl[g] = y.x, pl[g + 1] = y.y, pl[g + 2] = y.z, pl[g + 3] = y.w;
+      }
+    }
+    // two parts' values are on their way while the weights are made
+    float4 x[2][W::kRegs / 4];
+    auto fetch = [&](int u, float4(&to)[W::kRegs / 4]) {
+      const float* os = part_of<DH>(parts, ps, p + min(u, now - 1)) + 16 + lane * 4;
+#pragma unroll
+      for (int r = 0; r < W::kRegs / 4; ++r)
+        to[r] = __ldcg(reinterpret_cast<const float4*>(os + r * 128));
+    };
+    fetch(0, x[0]);
+    fetch(1, x[1]);
+    float keep = 1.f;
+#pragma unroll
+    for (int g = 0; g < kMaxGroup; ++g) {
+      const float t = fmaxf(top[g], warp_max(pm[g]));
+      const float old = weight_of(top[g], t), f = weight_of(pm[g], t);
+      if (g == lane >> 2) keep = old;
+      sum[g] = sum[g] * old + warp_sum(pl[g] * f);
+      top[g] = t;
+      weights[warp][lane][g] = f;
+    }
+    __syncwarp();
+    w.rescale(keep);
+    for (int u = 0; u < now; u += 2) {
+      w.add(x[0], weights[warp][u][lane >> 2]);
+      fetch(u + 2, x[0]);
+      if (u + 1 < now) w.add(x[1], weights[warp][u + 1][lane >> 2]);
+      fetch(u + 3, x[1]);
+    }
+    __syncwarp();
+  }
+#pragma unroll
+  for (int g = 0; g < kMaxGroup; ++g)
+    if (g == lane >> 2) {
+      w.m = top[g];
+      w.l = sum[g];
+    }
+  if (warp > 0) w.put(ms[warp], ls[warp], swap + (warp - 1) * W::kRegs * 32);
+  __syncthreads();
+  if (warp == 0) {
+#pragma unroll 1
+    for (int u = 1; u < kWarps; ++u) w.join(ms[u], ls[u], swap + (u - 1) * W::kRegs * 32);
+    w.write(out, G, d);
+    w.put_lse(lse, G);
+  }
+}
 
 template <class W, int DH>
 constexpr size_t attn_smem() {
@@ -527,11 +629,10 @@ __global__ void __launch_bounds__(kWarps * 32)
   using KT = typename W::KT;
   constexpr int T = W::kKeys * kWarps, kThreads = kWarps * 32;
   constexpr int kRowBytes = DH * (int)sizeof(KT), kHalf = W::kKeys * kRowBytes;
-  constexpr int kStageBytes = kWarps * 2 * kHalf, kPart = kMaxGroup * DH + 16;
+  constexpr int kStageBytes = kWarps * 2 * kHalf;
   constexpr int kRowsEach = W::kKeys / 8, kSegs = kRowBytes / 64;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float ms[kWarps][kMaxGroup], ls[kWarps][kMaxGroup];
-  __shared__ float weights[kWarps][32][kMaxGroup];
   __shared__ int64_t sums[kWarps];
   __shared__ int longs[kWarps];
   __shared__ Cursor first_s;
@@ -581,10 +682,11 @@ __global__ void __launch_bounds__(kWarps * 32)
     longest = max(longest, longs[w]);
   }
   total *= heads;
-  // n shares, none of them empty; or one for each item
+  // n shares, none of them empty; or one for each item, where that is sooner done
   const int64_t items = (int64_t)a.nseq * heads;
-  const bool by_item = items <= gridDim.x && longest <= kWholeTiles;
-  const int64_t n = by_item ? items : max((int64_t)1, min((int64_t)gridDim.x, total / kMinTiles));
+  int64_t n = max((int64_t)1, min((int64_t)gridDim.x, total / kMinTiles));
+  const bool by_item = items <= gridDim.x && longest <= total / n + kJoinTiles;
+  if (by_item) n = items;
   int64_t lo, hi;
   Cursor ahead;
   if (by_item) {
@@ -682,109 +784,57 @@ __global__ void __launch_bounds__(kWarps * 32)
   uint64_t okay = step();
   okay |= (uint64_t)step() << 16;
 
-  W w;
   int take_at = 0;
-  for (int64_t i = lo; i < hi; ++i) {
-    if (i == lo || c.t == c.t0) w.begin(a.q + c.b * a.q_stride + (int64_t)c.h * G * d, G, d);
-    cp_wait<kStages - 2>();
-    __syncwarp();
-    okay |= (uint64_t)step() << 32;
-    const uint32_t base = stages + take_at * kStageBytes, ok = (uint32_t)okay & 0xffffu;
-    take_at = take_at == kStages - 1 ? 0 : take_at + 1;
-    okay >>= 16;
-    if (ok) w.tile(base, base + kHalf, ok, a.scale2);
-    __syncwarp();
-    if (c.t + 1 == c.t1 || i + 1 == hi) {
-      const int64_t i0 = i - (c.t - c.t0), i1 = i0 + (c.t1 - c.t0);
-      const bool whole = i0 >= lo && i1 <= hi;
-      w.finish();
-      // the warps' states into warp 0's; for the last block of a split item a
-      // second time, with the states of the parts
-      for (bool done = whole;; done = true) {
-        __syncthreads();  // the swap space is free
-        if (warp > 0) w.put(ms[warp], ls[warp], swap + (warp - 1) * W::kRegs * 32);
-        __syncthreads();
-        if (warp == 0) {
-#pragma unroll 1
-          for (int u = 1; u < kWarps; ++u) w.join(ms[u], ls[u], swap + (u - 1) * W::kRegs * 32);
-          if (done) {
-            w.write(a.out + c.b * a.out_stride + (int64_t)c.h * G * d, G, d);
-            w.put_lse(a.lse ? a.lse + (int64_t)c.b * a.hq + c.h * G : nullptr, G);
-          }
-        }
-        if (done) break;
-        const int64_t c0 = ((i0 + 1) * n - 1) / total, c1 = (i1 * n - 1) / total;
-        auto part_of = [&](int64_t p) {
-          return a.parts + (p * 2 + (i0 < p * total / n ? 0 : 1)) * kPart;
-        };
-        if (warp == 0) {
-          float* part = part_of(me);
-          w.put(part, part + kMaxGroup, part + 16);
-          __threadfence();
-          __syncwarp();
-          if (lane == 0) {
-            const unsigned before = atomicAdd(&a.arrived[c0], 1u);
-            last_s = before == (unsigned)(c1 - c0);
-            if (last_s) a.arrived[c0] = 0;
-            __threadfence();
-          }
-        }
-        __syncthreads();
-        if (!last_s) break;
-        // the parts in the order of their shares, a run of them for each warp,
-        // 32 at a time: a lane weighs one of them, then all add them up
-        const int64_t count = c1 - c0 + 1, run = (count + kWarps - 1) / kWarps;
-        const int64_t p0 = c0 + min(count, warp * run), p1 = c0 + min(count, (warp + 1) * run);
-        w.clear();
-        float top[kMaxGroup], sum[kMaxGroup];
-#pragma unroll
-        for (int g = 0; g < kMaxGroup; ++g) {
-          top[g] = -INFINITY;
-          sum[g] = 0.f;
-        }
-#pragma unroll 1
-        for (int64_t p = p0; p < p1; p += 32) {
-          const int now = (int)min((int64_t)32, p1 - p);
-          float pm[kMaxGroup], pl[kMaxGroup];
-#pragma unroll
-          for (int g = 0; g < kMaxGroup; ++g) {
-            pm[g] = -INFINITY;
-            pl[g] = 0.f;
-          }
-          if (lane < now) {
-            const float* head = part_of(p + lane);
-#pragma unroll
-            for (int g = 0; g < kMaxGroup; g += 4) {
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(head + g));
-              const float4 y = __ldcg(reinterpret_cast<const float4*>(head + kMaxGroup + g));
-              pm[g] = x.x, pm[g + 1] = x.y, pm[g + 2] = x.z, pm[g + 3] = x.w;
-              pl[g] = y.x, pl[g + 1] = y.y, pl[g + 2] = y.z, pl[g + 3] = y.w;
-            }
-          }
-          __syncwarp();
-          float mine_keep = 1.f;
-#pragma unroll
-          for (int g = 0; g < kMaxGroup; ++g) {
-            const float t = fmaxf(top[g], warp_max(pm[g]));
-            const float keep = weight_of(top[g], t), f = weight_of(pm[g], t);
-            if (g == lane >> 2) mine_keep = keep;
-            sum[g] = sum[g] * keep + warp_sum(pl[g] * f);
-            top[g] = t;
-            weights[warp][lane][g] = f;
-          }
-          __syncwarp();
-          if (p > p0) w.rescale(mine_keep);
-#pragma unroll 2
-          for (int u = 0; u < now; ++u) w.add(part_of(p + u) + 16, weights[warp][u][lane >> 2]);
-        }
-#pragma unroll
-        for (int g = 0; g < kMaxGroup; ++g)
-          if (g == lane >> 2) {
-            w.m = top[g];
-            w.l = sum[g];
-          }
-      }
+  for (int64_t i = lo; i < hi;) {
+    // one piece: the tiles of item (c.b, c.h) from c.t on in this share
+    const int64_t i0 = i - (c.t - c.t0), i1 = i0 + (c.t1 - c.t0);
+    W w;
+    w.begin(a.q + c.b * a.q_stride + (int64_t)c.h * G * d, G, d);
+    for (const int64_t end = min(hi, i1); i < end; ++i) {
+      cp_wait<kStages - 2>();
+      __syncwarp();
+      okay |= (uint64_t)step() << 32;
+      const uint32_t base = stages + take_at * kStageBytes, ok = (uint32_t)okay & 0xffffu;
+      take_at = take_at == kStages - 1 ? 0 : take_at + 1;
+      okay >>= 16;
+      if (ok) w.tile(base, base + kHalf, ok, a.scale2);
+      __syncwarp();
     }
+    w.finish();
+    // the warps' states into warp 0's
+    __syncthreads();  // the swap space is free
+    if (warp > 0) w.put(ms[warp], ls[warp], swap + (warp - 1) * W::kRegs * 32);
+    __syncthreads();
+    if (warp == 0)
+#pragma unroll 1
+      for (int u = 1; u < kWarps; ++u) w.join(ms[u], ls[u], swap + (u - 1) * W::kRegs * 32);
+    const int64_t head = (int64_t)c.h * G;
+    float* lse = a.lse ? a.lse + (int64_t)c.b * a.hq + head : nullptr;
+    float* out = a.out + c.b * a.out_stride + head * d;
+    if (i0 >= lo && i1 <= hi) {
+      if (warp == 0) {
+        w.write(out, G, d);
+        w.put_lse(lse, G);
+      }
+    } else {
+      Parts ps;
+      ps.first = ((i0 + 1) * n - 1) / total;
+      ps.last = (i1 * n - 1) / total;
+      ps.second = i0 >= ps.first * total / n;
+      if (warp == 0) {
+        float* part = part_of<DH>(a.parts, ps, me);
+        w.put(part, part + kMaxGroup, part + 16);
+        __syncwarp();
+        if (lane == 0) {
+          // the warp's stores before the arrival, the others' parts after it
+          last_s = arrive(&a.arrived[ps.first]) == (unsigned)(ps.last - ps.first);
+          if (last_s) a.arrived[ps.first] = 0;
+        }
+      }
+      __syncthreads();
+      if (last_s) join_parts<W, DH>(a.parts, ps, swap, out, lse, G, d);
+    }
+    c.t = c.t1 - 1;
     advance<T>(a, heads, &c);
   }
 }
