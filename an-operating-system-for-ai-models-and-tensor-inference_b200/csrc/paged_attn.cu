@@ -28,6 +28,7 @@ namespace {
 
 constexpr int kMaxGroup = 8;  // query heads per KV head, as tensor_core::gqa_attn_f32 here
 constexpr int kMaxShares = 592;
+constexpr int kStages = 3, kWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct PagedAttnArgs {
@@ -41,7 +42,8 @@ struct PagedAttnArgs {
   const int32_t* kv_lens;
   float scale2;  // scale * log2(e): scores are kept in powers of two
   uint32_t window;
-  int page_shift;  // log2 of the page size, or -1
+  uint32_t page_mul;  // key / page_size = key * page_mul >> page_shift, keys below 2^31
+  int page_shift;
   unsigned* arrived;  // [shares], zero between launches
   float* parts;       // [shares][2][8 * DH + 16]
 };
@@ -179,43 +181,68 @@ struct WarpState {
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
   }
-  MYOS_DEV void put(float* ms, float* ls, float* os) const {
+  MYOS_DEV void put_ml(float* ms, float* ls) const {
     const int lane = threadIdx.x & 31;
     if ((lane & 3) == 0) {
       ms[lane >> 2] = m;
       ls[lane >> 2] = l;
     }
-#pragma unroll
-    for (int r = 0; r < kRegs; r += 4)
-      *reinterpret_cast<float4*>(os + r * 32 + lane * 4) =
-          make_float4(o[r], o[r + 1], o[r + 2], o[r + 3]);
   }
-  MYOS_DEV void join(const float* ms, const float* ls, const float* os) {
-    const int lane = threadIdx.x & 31, g = lane >> 2;
-    const float pm = ms[g], top = fmaxf(m, pm);
-    const float a = weight_of(m, top), b = weight_of(pm, top);
-    m = top;
-    l = l * a + ls[g] * b;
+  // The meeting of a block's warps: warp u < kOwners ends with values
+  // [u kOwn, (u + 1) kOwn) of o, summed over the warps in their order (m and l
+  // in every warp). A warp first leaves the others' shares in `swap`,
+  // kOwners * (kWarps - 1) blocks of kOwn * 32 floats.
+  static constexpr int kOwners = kRegs / 8 < kWarps ? kRegs / 8 : kWarps, kOwn = kRegs / kOwners;
+  MYOS_DEV void leave(float* ms, float* ls, float* swap) const {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    put_ml(ms + warp * kMaxGroup, ls + warp * kMaxGroup);
 #pragma unroll
-    for (int r = 0; r < kRegs; r += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(os + r * 32 + lane * 4);
-      o[r] = o[r] * a + x.x * b;
-      o[r + 1] = o[r + 1] * a + x.y * b;
-      o[r + 2] = o[r + 2] * a + x.z * b;
-      o[r + 3] = o[r + 3] * a + x.w * b;
+    for (int u = 0; u < kOwners; ++u) {
+      if (u == warp) continue;
+      float* to = swap + (u * (kWarps - 1) + (warp < u ? warp : warp - 1)) * kOwn * 32 + lane * 4;
+#pragma unroll
+      for (int r = 0; r < kOwn; r += 4)
+        *reinterpret_cast<float4*>(to + r * 32) = make_float4(
+            o[u * kOwn + r], o[u * kOwn + r + 1], o[u * kOwn + r + 2], o[u * kOwn + r + 3]);
     }
   }
-  MYOS_DEV void rescale(float a) {
+  MYOS_DEV void meet(const float* ms, const float* ls, const float* swap, float (&own)[kOwn]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
+    float top = -INFINITY, f[kWarps];
 #pragma unroll
-    for (int r = 0; r < kRegs; ++r) o[r] *= a;
-  }
-  MYOS_DEV void add(const float4 (&x)[kRegs / 4], float b) {
+    for (int v = 0; v < kWarps; ++v) top = fmaxf(top, f[v] = ms[v * kMaxGroup + g]);
+    l = 0.f;
 #pragma unroll
-    for (int r = 0; r < kRegs / 4; ++r) {
-      o[4 * r] = fmaf(x[r].x, b, o[4 * r]);
-      o[4 * r + 1] = fmaf(x[r].y, b, o[4 * r + 1]);
-      o[4 * r + 2] = fmaf(x[r].z, b, o[4 * r + 2]);
-      o[4 * r + 3] = fmaf(x[r].w, b, o[4 * r + 3]);
+    for (int v = 0; v < kWarps; ++v) {
+      f[v] = weight_of(f[v], top);
+      l = fmaf(ls[v * kMaxGroup + g], f[v], l);
+    }
+    m = top;
+    float mine[kOwn];
+#pragma unroll
+    for (int r = 0; r < kOwn; ++r) {
+      mine[r] = o[r];
+#pragma unroll
+      for (int u = 1; u < kOwners; ++u) mine[r] = warp == u ? o[u * kOwn + r] : mine[r];
+      own[r] = 0.f;
+    }
+    const float* from = swap + warp * (kWarps - 1) * kOwn * 32 + lane * 4;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) {
+      if (v == warp) {
+#pragma unroll
+        for (int r = 0; r < kOwn; ++r) own[r] = fmaf(mine[r], f[v], own[r]);
+        continue;
+      }
+#pragma unroll
+      for (int r = 0; r < kOwn; r += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(from + r * 32);
+        own[r] = fmaf(x.x, f[v], own[r]);
+        own[r + 1] = fmaf(x.y, f[v], own[r + 1]);
+        own[r + 2] = fmaf(x.z, f[v], own[r + 2]);
+        own[r + 3] = fmaf(x.w, f[v], own[r + 3]);
+      }
+      from += kOwn * 32;
     }
   }
   // Maximum and weights of a tile's scores s (in powers of two, -inf: no key;
@@ -236,7 +263,13 @@ struct WarpState {
     l = fmaf(l, keep, t);
     return keep;
   }
-  MYOS_DEV float inverse() const { return l > 0.f ? __fdiv_rn(1.0f, l) : 0.f; }
+  // 1 / l, or 0 without a key. l is at least 1 (the largest weight), at most the
+  // number of keys: an approximate reciprocal and one Newton step, no special cases.
+  MYOS_DEV float inverse() const {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(l));
+    return l > 0.f ? fmaf(r, fmaf(-l, r, 1.0f), r) : 0.f;
+  }
   MYOS_DEV void put_lse(float* lse, int G) const {
     const int lane = threadIdx.x & 31;
     if (lse && (lane & 3) == 0 && (lane >> 2) < G)
@@ -334,15 +367,17 @@ struct Bf16Warp : WarpState<DH> {
     }
   }
 
-  MYOS_DEV void write(float* out, int G, int d) const {
+  static constexpr int kOwn = WarpState<DH>::kOwn;
+  MYOS_DEV void write(const float (&own)[kOwn], float* out, int G, int d) const {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = (lane & 3) * 2;
     if (g >= G) return;
     const float inv = this->inverse();
+    const int at = (threadIdx.x >> 5) * kOwn * 4;
 #pragma unroll
-    for (int j = 0; j < DH / 8; ++j)
-      if (8 * j < d)
-        *reinterpret_cast<float2*>(out + g * d + 8 * j + c) =
-            make_float2(o[2 * j] * inv, o[2 * j + 1] * inv);
+    for (int j = 0; j < kOwn / 2; ++j)
+      if (at + 8 * j < d)
+        *reinterpret_cast<float2*>(out + g * d + at + 8 * j + c) =
+            make_float2(own[2 * j] * inv, own[2 * j + 1] * inv);
   }
 };
 
@@ -466,19 +501,38 @@ struct F32Warp : WarpState<DH> {
     }
   }
 
-  MYOS_DEV void write(float* out, int G, int d) const {
+  static constexpr int kOwn = WarpState<DH>::kOwn;
+  MYOS_DEV void write(const float (&own)[kOwn], float* out, int G, int d) const {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     if (g >= G) return;
     const float inv = this->inverse();
 #pragma unroll
-    for (int j = 0; j < DH / 32; ++j) {
-      const float* r = &o[8 * j];
-      float* to = out + g * d + 32 * j + 8 * c;
-      if (32 * j + 8 * c >= d) continue;
+    for (int j = 0; j < kOwn / 8; ++j) {
+      const float* r = &own[8 * j];
+      const int at = (threadIdx.x >> 5) * kOwn * 4 + 32 * j + 8 * c;
+      if (at >= d) continue;
+      float* to = out + g * d + at;
       *reinterpret_cast<float4*>(to) = make_float4(r[0] * inv, r[2] * inv, r[4] * inv, r[6] * inv);
       *reinterpret_cast<float4*>(to + 4) =
           make_float4(r[1] * inv, r[3] * inv, r[5] * inv, r[7] * inv);
     }
+  }
+};
+
+// n shares of a row of `total` tiles, the first `more` of them one tile longer
+// than `each`.
+struct Shares {
+  uint32_t each, more;
+  MYOS_DEV void cut(uint32_t total, uint32_t n) {
+    each = total / n;
+    more = total - each * n;
+  }
+  MYOS_DEV uint32_t begin(uint32_t i) const { return i * each + min(i, more); }
+  MYOS_DEV uint32_t of(uint32_t tile) const {
+    const uint32_t longer = more * (each + 1);
+    const bool in = tile < longer;
+    const uint32_t at = (in ? tile : tile - longer) / (in ? each + 1 : each);
+    return in ? at : at + more;
   }
 };
 
@@ -500,6 +554,7 @@ MYOS_DEV void advance(const PagedAttnArgs& a, int heads, Cursor* c) {
   if (++c->t < c->t1) return;
   if (++c->h == heads) {
     c->h = 0;
+#pragma unroll 1
     do {
       if (++c->b >= a.nseq) {
         c->t0 = c->t1 = c->len = c->start = 0;
@@ -511,109 +566,83 @@ MYOS_DEV void advance(const PagedAttnArgs& a, int heads, Cursor* c) {
   c->t = c->t0;
 }
 
-constexpr int kStages = 3, kWarps = 4;
-// The meeting of several blocks costs about as much as kJoinTiles tiles, and a
-// share of fewer than kMinTiles tiles saves less than the part it adds to it.
-constexpr int kJoinTiles = 5, kMinTiles = 2;
+// The meeting of several blocks costs about as much as kJoinTiles tiles (2 us),
+// and each of its parts (0.06 us) about a sixth of one: an item of L tiles is
+// soonest done in sqrt(kPartsPerTile * L) shares.
+constexpr int kJoinTiles = 5, kPartsPerTile = 6;
 
 // The parts of one split item: shares first .. last. All but the first share
 // begin inside the item, so their part is their first piece (slot 0); the
 // first share's is its last piece (slot 1).
-struct Parts {
-  int64_t first, last;
+struct Split {
+  int first, last;
+  int b, h;
   bool second;  // whether the first share's part is in slot 1
 };
 
-template <int DH>
-MYOS_DEV float* part_of(float* parts, const Parts& ps, int64_t share) {
+template <int DH, class P>
+MYOS_DEV P* part_of(P* parts, const Split& ps, int share) {
   const int slot = share == ps.first && ps.second ? 1 : 0;
-  return parts + (share * 2 + slot) * (kMaxGroup * DH + 16);
+  return parts + (size_t)(share * 2 + slot) * (kMaxGroup * DH + 16);
 }
 
-// By the last block of a split item: its parts in the order of their shares, a
-// run of them for each warp, 32 at a time (a lane weighs one of them, then all
-// add them up), then the warps' sums in order. Out of line: its registers are
-// not the main loop's.
+// By the last block of a split item: its parts through the stages, as many at
+// a time as fit (their copies all in flight at once), then warp u adds up
+// values [u kOwn, (u + 1) kOwn) of them in the order of their shares. Out of
+// line: its registers are not the main loop's.
 template <class W, int DH>
-__device__ __noinline__ void join_parts(float* parts, const Parts ps, float* swap, float* out,
-                                        float* lse, int G, int d) {
-  __shared__ float ms[kWarps][kMaxGroup], ls[kWarps][kMaxGroup];
-  __shared__ float weights[kWarps][32][kMaxGroup];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t count = ps.last - ps.first + 1, run = (count + kWarps - 1) / kWarps;
-  const int64_t p0 = ps.first + min(count, warp * run);
-  const int64_t p1 = ps.first + min(count, (warp + 1) * run);
+__device__ __noinline__ void join_parts(const float* parts, const Split ps, float* room,
+                                        float* out, float* lse, int G, int d) {
+  constexpr int kOwn = W::kOwn, kPart = kMaxGroup * DH + 16, kChunks = kPart / 4;
+  constexpr int kFit = kStages * kWarps * 2 * W::kKeys * DH * (int)sizeof(typename W::KT) / (kPart * 4);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
+  const int count = ps.last - ps.first + 1;
   W w;
-  w.clear();
-  float top[kMaxGroup], sum[kMaxGroup];
+  w.m = -INFINITY;
+  w.l = 0.f;
+  float own[kOwn];
 #pragma unroll
-  for (int g = 0; g < kMaxGroup; ++g) {
-    top[g] = -INFINITY;
-    sum[g] = 0.f;
-  }
+  for (int r = 0; r < kOwn; ++r) own[r] = 0.f;
 #pragma unroll 1
-  for (int64_t p = p0; p < p1; p += 32) {
-    const int now = (int)min((int64_t)32, p1 - p);
-    float pm[kMaxGroup], pl[kMaxGroup];
-#pragma unroll
-    for (int g = 0; g < kMaxGroup; ++g) {
-      pm[g] = -INFINITY;
-      pl[g] = 0.f;
+  for (int p0 = 0; p0 < count; p0 += kFit) {
+    const int now = min(kFit, count - p0);
+    __syncthreads();  // the stages are free
+#pragma unroll 4
+    for (int i = threadIdx.x; i < now * kChunks; i += kWarps * 32) {
+      const int p = i / kChunks;
+      cp_async16(smem_u32(room) + i * 16,
+                 part_of<DH>(parts, ps, ps.first + p0 + p) + (i - p * kChunks) * 4, true);
     }
-    if (lane < now) {
-      const float* head = part_of<DH>(parts, ps, p + lane);
+    cp_commit();
+    cp_wait<0>();
+    __syncthreads();
+    if (warp >= W::kOwners) continue;
+    float top = w.m;
+#pragma unroll 4
+    for (int p = 0; p < now; ++p) top = fmaxf(top, room[p * kPart + g]);
+    const float keep = weight_of(w.m, top);
+    w.m = top;
+    w.l *= keep;
 #pragma unroll
-      for (int g = 0; g < kMaxGroup; g += 4) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(head + g));
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(head + kMaxGroup + g));
-        pm[g] = x.x, pm[g + 1] = x.y, pm[g + 2] = x.z, pm[g + 3] = x.w;
-        pl[g] = y.x, pl[g + 1] = y.y, pl[g + 2] = y.z, pl[g + 3] = y.w;
+    for (int r = 0; r < kOwn; ++r) own[r] *= keep;
+#pragma unroll 2
+    for (int p = 0; p < now; ++p) {
+      const float* part = room + p * kPart;
+      const float f = weight_of(part[g], top);
+      w.l = fmaf(part[kMaxGroup + g], f, w.l);
+      part += 16 + warp * kOwn * 32 + lane * 4;
+#pragma unroll
+      for (int r = 0; r < kOwn; r += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(part + r * 32);
+        own[r] = fmaf(x.x, f, own[r]);
+        own[r + 1] = fmaf(x.y, f, own[r + 1]);
+        own[r + 2] = fmaf(x.z, f, own[r + 2]);
+        own[r + 3] = fmaf(x.w, f, own[r + 3]);
       }
     }
-    // two parts' values are on their way while the weights are made
-    float4 x[2][W::kRegs / 4];
-    auto fetch = [&](int u, float4(&to)[W::kRegs / 4]) {
-      const float* os = part_of<DH>(parts, ps, p + min(u, now - 1)) + 16 + lane * 4;
-#pragma unroll
-      for (int r = 0; r < W::kRegs / 4; ++r)
-        to[r] = __ldcg(reinterpret_cast<const float4*>(os + r * 128));
-    };
-    fetch(0, x[0]);
-    fetch(1, x[1]);
-    float keep = 1.f;
-#pragma unroll
-    for (int g = 0; g < kMaxGroup; ++g) {
-      const float t = fmaxf(top[g], warp_max(pm[g]));
-      const float old = weight_of(top[g], t), f = weight_of(pm[g], t);
-      if (g == lane >> 2) keep = old;
-      sum[g] = sum[g] * old + warp_sum(pl[g] * f);
-      top[g] = t;
-      weights[warp][lane][g] = f;
-    }
-    __syncwarp();
-    w.rescale(keep);
-    for (int u = 0; u < now; u += 2) {
-      w.add(x[0], weights[warp][u][lane >> 2]);
-      fetch(u + 2, x[0]);
-      if (u + 1 < now) w.add(x[1], weights[warp][u + 1][lane >> 2]);
-      fetch(u + 3, x[1]);
-    }
-    __syncwarp();
   }
-#pragma unroll
-  for (int g = 0; g < kMaxGroup; ++g)
-    if (g == lane >> 2) {
-      w.m = top[g];
-      w.l = sum[g];
-    }
-  if (warp > 0) w.put(ms[warp], ls[warp], swap + (warp - 1) * W::kRegs * 32);
-  __syncthreads();
-  if (warp == 0) {
-#pragma unroll 1
-    for (int u = 1; u < kWarps; ++u) w.join(ms[u], ls[u], swap + (u - 1) * W::kRegs * 32);
-    w.write(out, G, d);
-    w.put_lse(lse, G);
-  }
+  if (warp < W::kOwners) w.write(own, out, G, d);
+  if (warp == 0) w.put_lse(lse, G);
 }
 
 template <class W, int DH>
@@ -633,30 +662,34 @@ __global__ void __launch_bounds__(kWarps * 32)
   constexpr int kRowsEach = W::kKeys / 8, kSegs = kRowBytes / 64;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float ms[kWarps][kMaxGroup], ls[kWarps][kMaxGroup];
-  __shared__ int64_t sums[kWarps];
+  __shared__ uint32_t sums[kWarps];
   __shared__ int longs[kWarps];
   __shared__ Cursor first_s;
-  __shared__ int last_s;
+  __shared__ Split splits[2];  // split items that this block was the last to arrive at
+  __shared__ int ready[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int heads = (int)kv.heads, G = a.group, d = kFull ? DH : (int)kv.d;
-  const int64_t me = blockIdx.x;
+  const uint32_t me = blockIdx.x;
   float* swap = reinterpret_cast<float*>(smem + kStages * kStageBytes);
+  if (threadIdx.x < 2) ready[threadIdx.x] = 0;
 
-  // this block's share [lo, hi) of the tiles, and where it begins
+  // this block's share [lo, hi) of the tiles (fewer than 2^31 in all), and
+  // where it begins
   const int per = (a.nseq + kThreads - 1) / kThreads;
   const int b0 = min(a.nseq, (int)threadIdx.x * per), b1 = min(a.nseq, b0 + per);
-  int64_t mine = 0;
+  uint32_t mine = 0;
   int longest = 0;
+#pragma unroll 1
   for (int b = b0; b < b1; ++b) {
     Cursor c;
     span_of<T>(a, b, &c);
     mine += c.t1 - c.t0;
     longest = max(longest, c.t1 - c.t0);
   }
-  int64_t upto = mine;
+  uint32_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+    const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += u;
   }
   longest = __reduce_max_sync(0xffffffffu, longest);
@@ -665,16 +698,19 @@ __global__ void __launch_bounds__(kWarps * 32)
     longs[warp] = longest;
   }
   // sequences without a key have no tile: their outputs are spread over the blocks
+#pragma unroll 1
   for (int b = (int)me; b < a.nseq; b += (int)gridDim.x) {
     Cursor c;
     span_of<T>(a, b, &c);
     if (c.t0 < c.t1) continue;
-    for (int i = threadIdx.x; i < a.hq * d; i += kThreads) a.out[b * a.out_stride + i] = 0.f;
-    if (a.lse)
-      for (int i = threadIdx.x; i < a.hq; i += kThreads) a.lse[(int64_t)b * a.hq + i] = -INFINITY;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < a.hq * d; i += kThreads) {
+      a.out[b * a.out_stride + i] = 0.f;
+      if (a.lse && i < a.hq) a.lse[(int64_t)b * a.hq + i] = -INFINITY;
+    }
   }
   __syncthreads();
-  int64_t total = 0;
+  uint32_t total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) upto += sums[w];
@@ -683,36 +719,40 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
   total *= heads;
   // n shares, none of them empty; or one for each item, where that is sooner done
-  const int64_t items = (int64_t)a.nseq * heads;
-  int64_t n = max((int64_t)1, min((int64_t)gridDim.x, total / kMinTiles));
-  const bool by_item = items <= gridDim.x && longest <= total / n + kJoinTiles;
-  if (by_item) n = items;
-  int64_t lo, hi;
+  const uint32_t items = (uint32_t)a.nseq * heads;
+  const uint32_t best = items * sqrtf(kPartsPerTile * ((float)total / items));
+  const uint32_t n = max(1u, min(min(gridDim.x, total), best));
+  Shares shares;
+  shares.cut(total, n);
+  const bool by_item = items <= gridDim.x && (uint32_t)longest <= shares.each + kJoinTiles;
+  uint32_t lo = 0, hi = 0;
   Cursor ahead;
   if (by_item) {
     if (me >= items) return;
-    ahead.b = (int)(me / heads);
-    ahead.h = (int)(me % heads);
+    ahead.b = me / heads;
+    ahead.h = me - ahead.b * heads;
     span_of<T>(a, ahead.b, &ahead);
     ahead.t = ahead.t0;
-    lo = 0;
     hi = ahead.t1 - ahead.t0;
   } else {
-    lo = min(total, me * total / n);
-    hi = min(total, (me + 1) * total / n);
+    if (me < n) {
+      lo = shares.begin(me);
+      hi = shares.begin(me + 1);
+    }
     if (lo < hi && (upto - mine) * heads <= lo && lo < upto * heads) {
-      int64_t at = (upto - mine) * heads;
+      uint32_t at = lo - (upto - mine) * heads;  // tiles between b0's first and the share
       Cursor c;
       int b = b0;
+#pragma unroll 1
       for (;; ++b) {
         span_of<T>(a, b, &c);
-        const int64_t next = at + (int64_t)(c.t1 - c.t0) * heads;
-        if (lo < next) break;
-        at = next;
+        const uint32_t all = (uint32_t)(c.t1 - c.t0) * heads;
+        if (at < all) break;
+        at -= all;
       }
       c.b = b;
-      c.h = (int)((lo - at) / (c.t1 - c.t0));
-      c.t = c.t0 + (int)((lo - at) % (c.t1 - c.t0));
+      c.h = at / (uint32_t)(c.t1 - c.t0);
+      c.t = c.t0 + at - c.h * (c.t1 - c.t0);
       first_s = c;
     }
     __syncthreads();
@@ -730,38 +770,47 @@ __global__ void __launch_bounds__(kWarps * 32)
     to_k[u] = row * kRowBytes + (((4 * u + seg) ^ W::flip_k(row)) << 4);
     to_v[u] = kHalf + row * kRowBytes + (((4 * u + seg) ^ W::flip_v(row)) << 4);
   }
-  // the pages of this lane's rows in a tile
-  int page[kRowsEach];
-  auto look = [&](const Cursor& x) {
+  // where this lane's rows of a tile lie, up to the page, which is on its way
+  struct Rows {
+    int page[kRowsEach];
+    int64_t in[kRowsEach];
+  };
+  int left = (int)(hi - lo);  // tiles not looked up yet
+  auto look = [&](Rows& x) {
 #pragma unroll
     for (int r = 0; r < kRowsEach; ++r) {
-      const int key = x.t * T + warp * W::kKeys + row + 8 * r;
-      const int pg = a.page_shift >= 0 ? key >> a.page_shift : key / (int)kv.page_size;
-      page[r] = key >= x.start && key < x.len ? a.table[x.b * a.table_stride + pg] : -1;
+      const int key = ahead.t * T + warp * W::kKeys + row + 8 * r;
+      const int pg = (int)((uint64_t)(uint32_t)key * a.page_mul >> a.page_shift);
+      x.in[r] = ahead.h * kv.head_stride + (key - pg * (int)kv.page_size) * kv.slot_stride +
+                seg * (16 / (int)sizeof(KT));
+      x.page[r] = left > 0 && key >= ahead.start && key < ahead.len
+                      ? a.table[ahead.b * a.table_stride + pg]
+                      : -1;
     }
+    if (left > 1) advance<T>(a, heads, &ahead);
+    if (left > 0) --left;
   };
-  int64_t next = lo;  // the tile that is copied next; `page` belongs to it
-  int put_at = 0;     // its stage
-  auto step = [&]() -> uint32_t {  // the keys of the copied tile
-    uint32_t ok = 0;
-    if (next < hi) {
-      const uint32_t dst = stages + put_at * kStageBytes;
-      const KT *src_k[kRowsEach], *src_v[kRowsEach];
-      bool on[kRowsEach];
+  Rows soon, later;
 #pragma unroll
-      for (int r = 0; r < kRowsEach; ++r) {
-        const int key = ahead.t * T + warp * W::kKeys + row + 8 * r;
-        const int in =
-            a.page_shift >= 0 ? key & ((1 << a.page_shift) - 1) : key % (int)kv.page_size;
-        on[r] = (uint32_t)page[r] < kv.num_pages;
-        const int64_t at = on[r] ? page[r] * kv.page_stride + ahead.h * kv.head_stride +
-                                       in * kv.slot_stride + seg * (16 / (int)sizeof(KT))
-                                 : 0;
-        src_k[r] = kv.k + at;
-        src_v[r] = kv.v + at;
-        const uint32_t rows8 = __ballot_sync(0xffffffffu, on[r]);  // bit 4 i: row i
-        ok |= gather_rows(rows8) << (8 * r);
-      }
+  for (int r = 0; r < kRowsEach; ++r) soon.page[r] = later.page[r] = -1;
+  int put_at = 1;     // the stage of the tile that is copied next: 0 for the first
+  uint64_t okay = 0;  // 16 bits of keys for each tile in flight, the newest on top
+  static_assert(kStages == 3, "key bits of three tiles in one word");
+  // copies the tile that was looked up two calls before, looks the next one up
+  auto pump = [&]() {
+    uint32_t ok = 0;
+    const uint32_t dst = stages + put_at * kStageBytes;
+    const KT *src_k[kRowsEach], *src_v[kRowsEach];
+    bool on[kRowsEach];
+#pragma unroll
+    for (int r = 0; r < kRowsEach; ++r) {
+      on[r] = (uint32_t)soon.page[r] < kv.num_pages;
+      const int64_t at = on[r] ? soon.page[r] * kv.page_stride + soon.in[r] : 0;
+      src_k[r] = kv.k + at;
+      src_v[r] = kv.v + at;
+      ok |= gather_rows(__ballot_sync(0xffffffffu, on[r])) << (8 * r);  // bit 4 i: row i
+    }
+    if (ok) {
 #pragma unroll
       for (int r = 0; r < kRowsEach; ++r)
 #pragma unroll
@@ -769,73 +818,87 @@ __global__ void __launch_bounds__(kWarps * 32)
           const bool load = on[r] && (kFull || (4 * j + seg) * (16 / (int)sizeof(KT)) < d);
           const uint32_t off = dst + r * 8 * kRowBytes + (j >> 1) * 128;
           const int from = j * (64 / (int)sizeof(KT));
-          cp_async16(off + to_k[j & 1], kFull ? src_k[r] + from : load ? src_k[r] + from : kv.k, load);
-          cp_async16(off + to_v[j & 1], kFull ? src_v[r] + from : load ? src_v[r] + from : kv.v, load);
+          cp_async16(off + to_k[j & 1], kFull || load ? src_k[r] + from : kv.k, load);
+          cp_async16(off + to_v[j & 1], kFull || load ? src_v[r] + from : kv.v, load);
         }
-      advance<T>(a, heads, &ahead);
-      if (++next < hi) look(ahead);
     }
     cp_commit();
     put_at = put_at == kStages - 1 ? 0 : put_at + 1;
-    return ok;
+    okay = okay >> 16 | (uint64_t)ok << 32;
+    soon = later;
+    look(later);
   };
-  static_assert(kStages == 3, "key bits of three tiles in one word");
-  look(ahead);
-  uint64_t okay = step();
-  okay |= (uint64_t)step() << 16;
+#pragma unroll 1
+  for (int s = 0; s < 4; ++s) pump();  // two calls copy nothing yet
 
   int take_at = 0;
-  for (int64_t i = lo; i < hi;) {
+#pragma unroll 1
+  for (uint32_t i = lo; i < hi;) {
     // one piece: the tiles of item (c.b, c.h) from c.t on in this share
-    const int64_t i0 = i - (c.t - c.t0), i1 = i0 + (c.t1 - c.t0);
+    const uint32_t i0 = i - (c.t - c.t0), i1 = i0 + (c.t1 - c.t0);
     W w;
     w.begin(a.q + c.b * a.q_stride + (int64_t)c.h * G * d, G, d);
-    for (const int64_t end = min(hi, i1); i < end; ++i) {
+#pragma unroll 1
+    for (const uint32_t end = min(hi, i1); i < end; ++i) {
       cp_wait<kStages - 2>();
       __syncwarp();
-      okay |= (uint64_t)step() << 32;
+      pump();
       const uint32_t base = stages + take_at * kStageBytes, ok = (uint32_t)okay & 0xffffu;
       take_at = take_at == kStages - 1 ? 0 : take_at + 1;
-      okay >>= 16;
       if (ok) w.tile(base, base + kHalf, ok, a.scale2);
       __syncwarp();
     }
     w.finish();
-    // the warps' states into warp 0's
     __syncthreads();  // the swap space is free
-    if (warp > 0) w.put(ms[warp], ls[warp], swap + (warp - 1) * W::kRegs * 32);
+    w.leave(&ms[0][0], &ls[0][0], swap);
     __syncthreads();
-    if (warp == 0)
-#pragma unroll 1
-      for (int u = 1; u < kWarps; ++u) w.join(ms[u], ls[u], swap + (u - 1) * W::kRegs * 32);
-    const int64_t head = (int64_t)c.h * G;
-    float* lse = a.lse ? a.lse + (int64_t)c.b * a.hq + head : nullptr;
-    float* out = a.out + c.b * a.out_stride + head * d;
-    if (i0 >= lo && i1 <= hi) {
-      if (warp == 0) {
-        w.write(out, G, d);
-        w.put_lse(lse, G);
-      }
-    } else {
-      Parts ps;
-      ps.first = ((i0 + 1) * n - 1) / total;
-      ps.last = (i1 * n - 1) / total;
-      ps.second = i0 >= ps.first * total / n;
-      if (warp == 0) {
-        float* part = part_of<DH>(a.parts, ps, me);
-        w.put(part, part + kMaxGroup, part + 16);
+    const bool whole = i0 >= lo && i1 <= hi;
+    if (warp < W::kOwners) {
+      float own[W::kOwn];
+      w.meet(&ms[0][0], &ls[0][0], swap, own);
+      const int64_t head = (int64_t)c.h * G;
+      if (whole) {
+        w.write(own, a.out + c.b * a.out_stride + head * d, G, d);
+        if (warp == 0) w.put_lse(a.lse ? a.lse + (int64_t)c.b * a.hq + head : nullptr, G);
+      } else {
+        Split sp;
+        sp.first = (int)shares.of(i0);
+        sp.last = (int)shares.of(i1 - 1);
+        sp.second = i0 >= shares.begin(sp.first);
+        sp.b = c.b;
+        sp.h = c.h;
+        float* part = part_of<DH>(a.parts, sp, (int)me);
+        if (warp == 0) w.put_ml(part, part + kMaxGroup);
+        part += 16 + warp * W::kOwn * 32 + lane * 4;
+#pragma unroll
+        for (int r = 0; r < W::kOwn; r += 4)
+          *reinterpret_cast<float4*>(part + r * 32) =
+              make_float4(own[r], own[r + 1], own[r + 2], own[r + 3]);
         __syncwarp();
         if (lane == 0) {
-          // the warp's stores before the arrival, the others' parts after it
-          last_s = arrive(&a.arrived[ps.first]) == (unsigned)(ps.last - ps.first);
-          if (last_s) a.arrived[ps.first] = 0;
+          // the warp's stores before its arrival, the others' parts after it
+          const unsigned all = (unsigned)(sp.last - sp.first + 1) * W::kOwners;
+          if (arrive(&a.arrived[sp.first]) == all - 1) {
+            a.arrived[sp.first] = 0;
+            splits[i0 < lo ? 0 : 1] = sp;
+            ready[i0 < lo ? 0 : 1] = 1;
+          }
         }
       }
-      __syncthreads();
-      if (last_s) join_parts<W, DH>(a.parts, ps, swap, out, lse, G, d);
     }
     c.t = c.t1 - 1;
     advance<T>(a, heads, &c);
+  }
+  // the joins that fell to this block, once its own tiles are done
+  cp_wait<0>();
+  __syncthreads();
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    if (!ready[k]) continue;
+    const Split sp = splits[k];
+    const int64_t head = (int64_t)sp.h * G;
+    join_parts<W, DH>(a.parts, sp, reinterpret_cast<float*>(smem), a.out + sp.b * a.out_stride + head * d,
+                      a.lse ? a.lse + (int64_t)sp.b * a.hq + head : nullptr, G, d);
   }
 }
 
@@ -897,7 +960,8 @@ extern "C" int myos_dev_paged_attn(float* d_out, size_t out_stride, float* d_lse
   if (num_q_heads == 0 || num_q_heads % kv->num_kv_heads != 0 ||
       num_q_heads / kv->num_kv_heads > (size_t)kMaxGroup || nseq > 65535 || max_blocks == 0 ||
       max_blocks > 0x7fffffff || table_stride < max_blocks || table_stride > ((size_t)1 << 40) ||
-      max_blocks * kv->page_size > 0x7fffff00 || q_stride < num_q_heads * d ||
+      max_blocks * kv->page_size > 0x7fffff00 ||
+      (max_blocks * kv->page_size / 32 + 1) * nseq * kv->num_kv_heads > 0x7fffffff || q_stride < num_q_heads * d ||
       out_stride < num_q_heads * d || q_stride > ((size_t)1 << 30) ||
       out_stride > ((size_t)1 << 30))
     return MYOS_ERR_SHAPE;
@@ -921,9 +985,12 @@ extern "C" int myos_dev_paged_attn(float* d_out, size_t out_stride, float* d_lse
   a.kv_lens = d_kv_lens;
   a.scale2 = scale * kLog2e;
   a.window = window;
-  a.page_shift = -1;
-  if ((kv->page_size & (kv->page_size - 1)) == 0)
-    for (a.page_shift = 0; (1u << a.page_shift) < kv->page_size;) ++a.page_shift;
+  // ceil(2^s / P) with s = 31 + ceil(log2 P): its error times any key is below 2^s
+  int log2 = 0;
+  while ((1u << log2) < kv->page_size) ++log2;
+  a.page_shift = 31 + log2;
+  a.page_mul =
+      (uint32_t)((((uint64_t)1 << a.page_shift) + kv->page_size - 1) / kv->page_size);
   const cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = d <= 64    ? launch_d<64>(a, kv, d_work, st)
                         : d <= 128 ? launch_d<128>(a, kv, d_work, st)

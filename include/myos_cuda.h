@@ -452,7 +452,8 @@ int myos_dev_qk_norm_rope_store(float* d_q, size_t q_stride, const float* d_qkv,
  * at positions [max(0, len - window), len) of sequence b, len = d_kv_lens[b]
  * clipped to [0, max_blocks * page_size], window 0: all; query head h reads
  * KV head h / (num_q_heads / num_kv_heads), a group of at most 8 (as in
- * tensor_core::gqa_attn_f32). d_lse (nullable, [nseq][num_q_heads]) receives
+ * tensor_core::gqa_attn_f32); (max_blocks * page_size / 32 + 1) * nseq *
+ * num_kv_heads is below 2^31. d_lse (nullable, [nseq][num_q_heads]) receives
  * the natural log of the sum of exp(scale * q . k). Keys of a page whose table
  * entry is outside the cache are left out. A sequence with no keys gives zeros
  * and lse -inf. Slots behind len are never read, whatever they hold; the keys
