@@ -1,18 +1,22 @@
-"""Build the in-tree native libraries with nvcc / g++ (no PyTorch involved).
+"""Build the in-tree native libraries with nvcc / g++. PyTorch is needed only by
+the last one, the tensor binding, which is left out where torch is not installed.
 
 Outputs (git-ignored, carried to the GPU box with the tree):
   lib/libmyos_cuda.so   CUDA kernels + the C ABI of include/myos_cuda.h (sm_100a)
   lib/libmyos_synth.so  seeded synthetic weights/prompts (host C++)
   lib/myos              C++ command-line runner mirroring the reference CLI
+  lib/_myos_dev.so      myos.dev: the device-pointer operators on torch tensors
 
 Usage: python build.py [--force]
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
@@ -98,7 +102,24 @@ def build(force: bool = False, verbose: bool = False) -> dict:
     if os.path.exists(cli_src) and (force or _stale(cli_bin, [cli_src, so])):
         _run(["g++", "-O2", "-std=c++17", "-I" + INCLUDE, "-o", cli_bin, cli_src,
               "-L" + LIB, "-lmyos_cuda", "-Wl,-rpath,$ORIGIN", "-pthread"])
-    return {"cuda": so, "synth": synth_so, "cli": cli_bin}
+    out = {"cuda": so, "synth": synth_so, "cli": cli_bin}
+    torch = importlib.util.find_spec("torch")
+    if torch is not None:
+        root = torch.submodule_search_locations[0]
+        dev_src = os.path.join(CSRC, "dev_torch.cpp")
+        dev_so = os.path.join(LIB, "_myos_dev.so")
+        if force or _stale(dev_so, [dev_src, os.path.join(INCLUDE, "myos_cuda.h"),
+                                    os.path.join(root, "version.py")]):
+            cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+            inc = [os.path.join(root, "include"),
+                   os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                   os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+            _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
+                 + ["-I" + d for d in inc] + [dev_src, "-o", dev_so, "-L" + LIB, "-lmyos_cuda",
+                 "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+                 "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
+        out["dev"] = dev_so
+    return out
 
 
 if __name__ == "__main__":

@@ -165,8 +165,8 @@ extern "C" int myos_dev_logit_controls(float* d_out, size_t out_stride, const fl
     a.c = *c;
   }
   constexpr int smem = 2 * kChunk * 4;
-  if (cudaFuncSetAttribute(k_logit_controls, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
-      cudaSuccess)
+  static std::atomic<uint64_t> raised{0};
+  if (raise_smem_limit((const void*)k_logit_controls, smem, &raised) != cudaSuccess)
     return MYOS_ERR_CUDA;
   k_logit_controls<<<(unsigned)rows, kThreads, smem, (cudaStream_t)stream>>>(a);
   return counted(cudaGetLastError()) == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;

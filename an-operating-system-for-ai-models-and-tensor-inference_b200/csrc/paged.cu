@@ -34,6 +34,18 @@ int paged_check(const myos_paged_kv* kv) {
   return MYOS_OK;
 }
 
+int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int sms = known[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    known[dev].store(sms, std::memory_order_relaxed);
+  }
+  return sms;
+}
+
 namespace {
 
 // ------------------------------------------------------------------ tables
@@ -339,9 +351,9 @@ int myos_dev_paged_tables(int32_t* d_block_table, size_t table_stride, size_t ma
       table_stride > ((size_t)1 << 40) || max_rows > 0x7fffffff || free_cap > 0x7fffffff)
     return MYOS_ERR_SHAPE;
   const size_t smem = 8 * nseq;
+  static std::atomic<uint64_t> raised{0};
   if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(k_paged_tables, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           8 * 16384) != cudaSuccess)
+      raise_smem_limit((const void*)k_paged_tables, 8 * 16384, &raised) != cudaSuccess)
     return MYOS_ERR_CUDA;
   TablesArgs a;
   a.table = d_block_table;

@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/myos_cuda.h"
 
 namespace myos {
@@ -35,6 +37,22 @@ inline PagedKv<KT> paged_view(const myos_paged_kv* kv) {
 
 // The header's rules for a cache; MYOS_OK or the status to return.
 int paged_check(const myos_paged_kv* kv);
+
+// Raises a kernel's dynamic shared-memory limit, once per device; `done` is the
+// kernel's own mask of devices.
+inline cudaError_t raise_smem_limit(const void* kernel, size_t bytes, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if (bit && (done->load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done->fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
+// Multiprocessors of the current device (148 where it cannot be asked).
+int sm_count();
 
 inline bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 

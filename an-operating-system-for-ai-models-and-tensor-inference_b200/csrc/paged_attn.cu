@@ -902,21 +902,14 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 template <class W, int DH, bool kFull>
 cudaError_t launch(PagedAttnArgs a, const myos_paged_kv* kv, void* work, cudaStream_t st) {
   constexpr size_t smem = attn_smem<W, DH>(), kCounters = 16 * 1024;
   constexpr int T = W::kKeys * kWarps;
   static_assert(kCounters + (size_t)kMaxShares * 2 * (kMaxGroup * DH + 16) * 4 <=
                 MYOS_PAGED_WORK_BYTES);
-  cudaError_t e = cudaFuncSetAttribute(k_paged_attn<W, DH, kFull>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> raised{0};
+  const cudaError_t e = raise_smem_limit((const void*)k_paged_attn<W, DH, kFull>, smem, &raised);
   if (e != cudaSuccess) return e;
   a.arrived = static_cast<unsigned*>(work);
   a.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(work) + kCounters);
