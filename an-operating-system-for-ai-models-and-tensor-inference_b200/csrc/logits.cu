@@ -12,20 +12,36 @@ struct LogitArgs {
   const float* logits;
   int64_t out_stride, logits_stride;
   int vocab;
-  int slice, chunk;  // ids of a block, and of a pass over its tables: multiples of 4
+  int slice, chunk, slots;  // ids of a block, and of a pass (multiples of 4); table slots
   uint32_t* ids;
   myos_logit_controls_args c;
 };
 
 // A row is shared by a cluster of blocks, a slice of the vocabulary each. A
-// slice goes by in chunks whose history and biases are first sorted into tables
-// in shared memory, one word an id, by integer atomics (the result does not
-// depend on their order); a chunk's logits are loaded before that, kGroups
-// 16-byte groups a thread, so the tables are built while they come. The blocks'
-// best ids meet in the first block's shared memory.
-constexpr int kThreads = 512, kGroups = 4, kMaxChunk = kThreads * kGroups * 4;
+// block sorts the row's tokens and biases that fall into its slice into a hash
+// table in shared memory by integer atomics (the result does not depend on their
+// order); then the slice passes once, four ids a thread and load, with nothing
+// to wait for between them: out = logits under the mask, and the largest of the
+// ids that no token or bias touches; then the touched ids are computed one to a
+// thread, over what that pass wrote. A history longer than the table has room
+// for is handled in chunks of as many ids as the table has slots, each id in the
+// slot of its own number. The blocks' best ids meet in the first block's shared
+// memory.
+//
+// What this replaces: tables of one word an id, chunk by chunk, with the
+// penalties in the pass over all ids, 59 instructions an id (64 rows of 152064:
+// 52 us), and with the touched ids computed before that pass from lists, 40
+// instructions (39 us): zeroing and reading the tables and looking through the
+// lists for every chunk cost more than the pass.
+#ifndef SLOTS
+#define SLOTS 2
+#define VT 512
+#endif
 constexpr int kMaxCluster = 8;
+constexpr int kTokens = 4096, kBiases = 1024;  // of a row: room in the table
+constexpr int kMaxChunk = 65536;
 constexpr uint32_t kSeen = 0x80000000u;  // in the prompt; the low bits count the output
+constexpr uint32_t kNoId = 0xffffffffu;
 
 // x under the penalties: each step rounded, as a chain of elementwise passes
 // would round it.
@@ -44,11 +60,13 @@ MYOS_DEV void better(float& v, int& i, float ov, int oi) {
   }
 }
 
-__global__ void __launch_bounds__(kThreads, 2) k_logit_controls(const LogitArgs a) {
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) {
   extern __shared__ __align__(16) uint32_t tables[];
   __shared__ float best_v[32];
   __shared__ int best_i[32];
   __shared__ unsigned long long found[kMaxCluster];
+  __shared__ int listed;
   const int tid = threadIdx.x, lane = tid & 31;
   uint32_t rank, ranks;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -61,13 +79,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_logit_controls(const LogitArgs 
   float* y = a.out ? a.out + row * a.out_stride : nullptr;
   // Ids count from `shift` on, so that groups of four lie on 16 bytes of x.
   const int shift = (int)((uintptr_t)x >> 2 & 3);
-  const bool together = y && (((uintptr_t)x ^ (uintptr_t)y) & 15) == 0;
-  const bool in_place = y == x;
+  const bool together = (((uintptr_t)x ^ (uintptr_t)y) & 15) == 0;
 
-  const bool pen = c.history && (c.repetition || c.frequency || c.presence);
   int hist = 0, prompt = 0;
   float rep = 1.f, freq = 0.f, pres = 0.f;
-  if (pen) {
+  if (c.history && (c.repetition || c.frequency || c.presence)) {
     hist = (int)c.history_width;
     if (c.history_lens) hist = min(hist, max(c.history_lens[row], 0));
     if (c.prompt_lens) prompt = c.prompt_lens[row];
@@ -75,135 +91,191 @@ __global__ void __launch_bounds__(kThreads, 2) k_logit_controls(const LogitArgs 
     if (c.frequency) freq = c.frequency[row];
     if (c.presence) pres = c.presence[row];
   }
-  const int32_t* said_ids = pen ? c.history + row * (int64_t)c.history_stride : nullptr;
+  const int32_t* said = c.history + row * (int64_t)c.history_stride;
   int e0 = 0, e1 = 0;
   if (c.bias_starts) {
     e0 = min(max(c.bias_starts[row], 0), (int)c.num_bias);
     e1 = min(max(c.bias_starts[row + 1], 0), (int)c.num_bias);
   }
-  const bool has_bias = e1 > e0;
+  const bool touched = hist > 0 || e1 > e0;
+  const bool hashed = hist <= kTokens && e1 - e0 <= kBiases;
   const uint32_t* mask = nullptr;
   if (c.mask) {
     const int64_t g = c.mask_rows ? c.mask_rows[row] : row;
     if (g >= 0 && g < (int64_t)c.num_masks) mask = c.mask + g * (int64_t)c.mask_stride;
   }
-  uint32_t* said = tables;
-  uint32_t* bias = tables + (pen ? a.chunk : 0);
+  // the chunk's mask and touched ids, a bit each (two mask words more than full
+  // ones: a chunk may begin inside a word); the table: an id's place in the
+  // chunk, the history's word, 1 + its last bias entry; the slots in use
+  const uint32_t slots = a.slots;
+  const int words = a.chunk / 32 + 2;
+  uint32_t* mask_s = tables;
+  uint32_t* bits = mask_s + words;
+  uint32_t* key = bits + words;
+  uint32_t* word = key + slots;
+  uint32_t* bias = word + slots;
+  uint16_t* used = reinterpret_cast<uint16_t*>(bias + slots);
 
   float bv = -INFINITY;
   int bi = 0;
   const int s0 = rank * a.slice, s1 = min(s0 + a.slice, a.vocab + shift);
+  const int step = hashed || !touched ? a.chunk : min(a.chunk, (int)slots & ~3);
 #pragma unroll 1
-  for (int base = s0; base < s1; base += a.chunk) {
-    const int n = min(a.chunk, s1 - base);  // shifted ids base .. base + n
-    const uint32_t first = (uint32_t)(base - shift);
-    float4 v[kGroups];
+  for (int base = s0; base < s1; base += step) {
+    const int n = min(step, s1 - base);  // shifted ids base .. base + n
+    const int first = base - shift;      // the id of the first
+    const int word0 = max(first, 0) >> 5;
+    if (base > s0) __syncthreads();
+    if (mask)
+#pragma unroll 1
+      for (int k = tid; k < n / 32 + 2; k += kThreads)
+        mask_s[k] = (word0 + k) * 32 < a.vocab ? mask[word0 + k] : 0u;
+    if (touched) {
+#pragma unroll 1
+      for (int k = tid; k < (int)slots; k += kThreads) {
+        key[k] = kNoId;
+        word[k] = 0;
+        bias[k] = 0;
+      }
+#pragma unroll 1
+      for (int k = tid; k < n / 32 + 1; k += kThreads) bits[k] = 0;
+      if (tid == 0) listed = 0;
+      __syncthreads();
+      // the slot of an id of this chunk, or -1
+      auto slot_of = [&](int32_t id) -> int {
+        const uint32_t t = (uint32_t)id - (uint32_t)first;
+        if ((uint32_t)id >= (uint32_t)a.vocab || t >= (uint32_t)n) return -1;
+        uint32_t h = hashed ? __umulhi(t * 2654435761u, slots) : t;
+        for (;;) {
+          const uint32_t was = atomicCAS(&key[h], kNoId, t);
+          if (was == kNoId) {
+            atomicOr(&bits[t >> 5], 1u << (t & 31));
+            used[atomicAdd(&listed, 1)] = (uint16_t)h;
+            break;
+          }
+          if (was == t) break;
+          if (++h == slots) h = 0;
+        }
+        return (int)h;
+      };
+      constexpr int kBatch = 4;
+#pragma unroll 1
+      for (int i0 = tid; i0 < hist; i0 += kBatch * kThreads) {
+        int32_t id[kBatch];
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-      const int at = 4 * (tid + k * kThreads), i = base + at - shift;  // ids i .. i + 3
-      v[k] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      if (at >= n) continue;
-      if (i >= 0 && i + 3 < a.vocab) {
-        v[k] = *reinterpret_cast<const float4*>(x + i);
-      } else {
-        if (i >= 0 && i < a.vocab) v[k].x = x[i];
-        if (i + 1 >= 0 && i + 1 < a.vocab) v[k].y = x[i + 1];
-        if (i + 2 >= 0 && i + 2 < a.vocab) v[k].z = x[i + 2];
-        if (i + 3 >= 0 && i + 3 < a.vocab) v[k].w = x[i + 3];
+        for (int k = 0; k < kBatch; ++k) id[k] = i0 + k * kThreads < hist ? said[i0 + k * kThreads] : -1;
+#pragma unroll 1
+        for (int k = 0; k < kBatch; ++k) {
+          const int32_t now = id[0];
+          id[0] = id[1], id[1] = id[2], id[2] = id[3];
+          const int h = slot_of(now);
+          if (h < 0) continue;
+          if (i0 + k * kThreads < prompt) atomicOr(&word[h], kSeen);
+          else atomicAdd(&word[h], 1u);
+        }
+      }
+      // the last entry of an id counts: entries leave their number, the largest stays
+#pragma unroll 1
+      for (int e = e0 + tid; e < e1; e += kThreads) {
+        const int h = slot_of(c.bias_ids[e]);
+        if (h >= 0) atomicMax(&bias[h], (uint32_t)(e - e0 + 1));
       }
     }
-    if (hist > 0 || has_bias) {
-      const uint4 none = make_uint4(0, 0, 0, 0);
-      if (base > s0) __syncthreads();
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
-        const int at = 4 * (tid + k * kThreads);
-        if (at >= n) break;
-        if (pen) *reinterpret_cast<uint4*>(said + at) = none;
-        if (has_bias) *reinterpret_cast<uint4*>(bias + at) = none;
-      }
-      __syncthreads();
-#pragma unroll 4
-      for (int i = tid; i < hist; i += kThreads) {
-        const uint32_t t = (uint32_t)said_ids[i] - first;
-        // ids of this chunk; not those below 0, which the first chunk's shift would let in
-        if (t >= (uint32_t)n || (uint32_t)said_ids[i] >= (uint32_t)a.vocab) continue;
-        if (i >= prompt) atomicAdd(&said[t], 1u);
-        else atomicOr(&said[t], kSeen);
-      }
-      if (has_bias) {
-        // the last entry of an id counts: entries leave their number, the largest stays ...
-#pragma unroll 1
-        for (int e = e0 + tid; e < e1; e += kThreads) {
-          const uint32_t t = (uint32_t)c.bias_ids[e] - first;
-          if (t < (uint32_t)n && (uint32_t)c.bias_ids[e] < (uint32_t)a.vocab)
-            atomicMax(&bias[t], (uint32_t)(e - e0 + 1));
-        }
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-      const int at = 4 * (tid + k * kThreads), i = base + at - shift;
-      if (at >= n) break;
-      float r[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-      if (hist > 0) {
-        const uint4 w = *reinterpret_cast<const uint4*>(said + at);
-        if ((w.x | w.y | w.z | w.w) != 0) {
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (u[j]) r[j] = penalised(r[j], u[j], rep, freq, pres, c.repetition != nullptr);
-        }
-      }
-      if (has_bias) {
-        const uint4 w = *reinterpret_cast<const uint4*>(bias + at);
-        if ((w.x | w.y | w.z | w.w) != 0) {
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j)  // ... and is looked up here
-            if (u[j]) r[j] = __fadd_rn(r[j], c.bias_vals[e0 + u[j] - 1]);
-        }
-      }
+    if (touched || mask) __syncthreads();
+
+    // ids i .. i + 3 at place `at` of the chunk: the value of an id, edge or not
+    auto pass = [&](int at, float (&r)[4]) -> uint32_t {  // the untouched ones
+      uint32_t keep = 15u;
+      if (touched) keep = ~(bits[at >> 5] >> (at & 31));  // at is a multiple of 4
       if (mask) {
-        // bits of ids i .. i + 3, which may lie in two words; none of ids out of range is used
-        const int w0 = max(i, 0) >> 5, w1 = min(i + 3, a.vocab - 1) >> 5;
-        uint32_t bits = mask[w0];
-        const uint32_t more = w1 > w0 ? mask[w1] : 0u;
-        bits = i >= 0 ? __funnelshift_r(bits, more, i & 31) : bits << -i;
+        // their bits may lie in two words; bits of ids out of range are not used
+        const int i = first + at, w0 = (max(i, 0) >> 5) - word0;
+        const uint32_t m = mask_s[w0];
+        const uint32_t m4 = i >= 0 ? __funnelshift_r(m, mask_s[w0 + 1], i & 31) : m << -i;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (!((bits >> j) & 1u)) r[j] = -INFINITY;
+          if (!((m4 >> j) & 1u)) r[j] = -INFINITY;
       }
-      if (i >= 0 && i + 3 < a.vocab) {
+      return keep;
+    };
+    auto take = [&](float v, int i) {  // ids come in rising order
+      if (v > bv) {
+        bv = v;
+        bi = i;
+      }
+    };
+    // groups [g0, g1) lie within the row; at most one before and one behind do not
+    const int g0 = first < 0 ? 1 : 0, g1 = min((n + 3) / 4, (a.vocab - first) / 4);
+    const float* xc = x + first;
+    float* yc = y + first;
+    constexpr int kUnroll = 4;
+#pragma unroll 1
+    for (int gr = g0 + tid; gr < g1; gr += kUnroll * kThreads) {
+      float4 v[kUnroll];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k)
+        if (gr + k * kThreads < g1)
+          v[k] = *reinterpret_cast<const float4*>(xc + 4 * (gr + k * kThreads));
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        if (gr + k * kThreads >= g1) break;
+        const int at = 4 * (gr + k * kThreads);
+        float r[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        const uint32_t keep = pass(at, r);
         if (y) {
-          const bool same = in_place && __float_as_uint(r[0]) == __float_as_uint(v[k].x) &&
-                            __float_as_uint(r[1]) == __float_as_uint(v[k].y) &&
-                            __float_as_uint(r[2]) == __float_as_uint(v[k].z) &&
-                            __float_as_uint(r[3]) == __float_as_uint(v[k].w);
           if (together) {
-            if (!same) *reinterpret_cast<float4*>(y + i) = make_float4(r[0], r[1], r[2], r[3]);
+            *reinterpret_cast<float4*>(yc + at) = make_float4(r[0], r[1], r[2], r[3]);
           } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[i + j] = r[j];
+            for (int j = 0; j < 4; ++j) yc[at + j] = r[j];
           }
         }
+        if (fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])) > bv) {  // NaN is passed over
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (r[j] > bv) {
-            bv = r[j];
-            bi = i + j;
-          }
-      } else {
+          for (int j = 0; j < 4; ++j)
+            if (keep >> j & 1u) take(r[j], first + at + j);
+        }
+      }
+    }
+    // the groups that reach over the row's ends
+    if (tid < 2) {
+      const int gr = tid == 0 ? 0 : g1;
+      if ((tid == 0 ? g0 == 1 : 4 * g1 < n) && (tid == 0 || g1 >= g0)) {
+        float r[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (i + j < 0 || i + j >= a.vocab) continue;
-          if (y) y[i + j] = r[j];
-          if (r[j] > bv) {
+          const int i = first + 4 * gr + j;
+          r[j] = i >= 0 && i < a.vocab ? x[i] : -INFINITY;
+        }
+        const uint32_t keep = pass(4 * gr, r);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = first + 4 * gr + j;
+          if (i < 0 || i >= a.vocab) continue;
+          if (y) y[i] = r[j];
+          if ((keep >> j & 1u) && (r[j] > bv || (r[j] == bv && i < bi))) {
             bv = r[j];
-            bi = i + j;
+            bi = i;
           }
         }
+      }
+    }
+    if (!touched) continue;
+    __syncthreads();
+    // the touched ids, over what the pass wrote (an id that the mask takes out
+    // is -inf whatever it was, any other still holds its logit)
+#pragma unroll 1
+    for (int k = tid; k < listed; k += kThreads) {
+      const int h = used[k], i = first + (int)key[h];
+      float r = x[i];
+      const uint32_t w = word[h], e = bias[h];
+      if (w) r = penalised(r, w, rep, freq, pres, c.repetition != nullptr);
+      if (e) r = __fadd_rn(r, c.bias_vals[e0 + e - 1]);
+      if (mask && !(mask_s[(i >> 5) - word0] >> (i & 31) & 1u)) r = -INFINITY;
+      if (y) y[i] = r;
+      if (r > bv || (r == bv && i < bi)) {
+        bv = r;
+        bi = i;
       }
     }
   }
@@ -241,6 +313,46 @@ __global__ void __launch_bounds__(kThreads, 2) k_logit_controls(const LogitArgs 
         better(bv, bi, __uint_as_float((uint32_t)(found[u] >> 32)), (int)(uint32_t)found[u]);
   }
   if (tid == 0) a.ids[row] = bv == -INFINITY ? 0u : (uint32_t)bi;
+}
+
+template <int kThreads>
+cudaError_t launch_controls(LogitArgs a, size_t rows, cudaStream_t st) {
+  // As many blocks a row as are resident at once, slices of at least 2048 ids;
+  // slices and chunks in multiples of four (three ids more: a row's shift).
+  const int ids = a.vocab + 3;
+  int cluster = kMaxCluster;
+  while (cluster > 1 &&
+         (rows * cluster > (size_t)sm_count() * SLOTS || ids / cluster < 2048))
+    cluster /= 2;
+  a.slice = ((ids + cluster - 1) / cluster + 3) & ~3;
+  const int passes = (a.slice + kMaxChunk - 1) / kMaxChunk;
+  a.chunk = ((a.slice + passes - 1) / passes + 3) & ~3;
+  const bool pen = a.c.history && (a.c.repetition || a.c.frequency || a.c.presence);
+  // room for every id that the listed tokens and biases can name, and a quarter more
+  size_t room = 0;
+  if (pen) room += a.c.history_width < kTokens ? a.c.history_width : kTokens;
+  if (a.c.bias_starts) room += a.c.num_bias < kBiases ? a.c.num_bias : kBiases;
+  a.slots = room ? (int)((room + room / 4 + 31) & ~(size_t)31) : 0;
+  const auto bytes = [](size_t chunk, size_t slots) { return 8 * (chunk / 32 + 2) + 14 * slots; };
+  const size_t smem = bytes(a.chunk, a.slots);
+  constexpr size_t kMostSlots = (kTokens + kBiases) * 5 / 4;
+  static_assert(kMostSlots % 32 == 0 && kMostSlots <= 65536);
+  static std::atomic<uint64_t> raised{0};
+  const cudaError_t e = raise_smem_limit((const void*)k_logit_controls<kThreads>,
+                                         bytes(kMaxChunk, kMostSlots), &raised);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return counted(cudaLaunchKernelEx(&cfg, k_logit_controls<kThreads>, a));
 }
 
 }  // namespace
@@ -285,31 +397,8 @@ extern "C" int myos_dev_logit_controls(float* d_out, size_t out_stride, const fl
       return MYOS_ERR_SHAPE;
     a.c = *c;
   }
-  // As many blocks a row as keep the device busy, slices of at least 2048 ids;
-  // slices and chunks in multiples of four (three ids more: a row's shift).
-  const size_t ids_shifted = vocab + 3;
-  int cluster = kMaxCluster;
-  while (cluster > 1 && (rows * cluster > (size_t)sm_count() * 8 || ids_shifted / cluster < 2048))
-    cluster /= 2;
-  a.slice = (int)((ids_shifted + cluster - 1) / cluster + 3) & ~3;
-  const int passes = (a.slice + kMaxChunk - 1) / kMaxChunk;
-  a.chunk = ((a.slice + passes - 1) / passes + 3) & ~3;
-  const bool pen = a.c.history && (a.c.repetition || a.c.frequency || a.c.presence);
-  const size_t smem = 4 * (size_t)a.chunk * ((pen ? 1 : 0) + (a.c.bias_starts ? 1 : 0));
-  static std::atomic<uint64_t> raised{0};
-  if (raise_smem_limit((const void*)k_logit_controls, 2 * kMaxChunk * 4, &raised) != cudaSuccess)
-    return MYOS_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return counted(cudaLaunchKernelEx(&cfg, k_logit_controls, a)) == cudaSuccess ? MYOS_OK
-                                                                               : MYOS_ERR_CUDA;
+  const cudaError_t e = rows * kMaxCluster <= (size_t)sm_count()
+                            ? launch_controls<1024>(a, rows, (cudaStream_t)stream)
+                            : launch_controls<VT>(a, rows, (cudaStream_t)stream);
+  return e == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
 }
