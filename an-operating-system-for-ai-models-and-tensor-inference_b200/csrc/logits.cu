@@ -12,21 +12,22 @@ struct LogitArgs {
   const float* logits;
   int64_t out_stride, logits_stride;
   int vocab;
-  int slice, chunk, slots;  // ids of a block, and of a pass (multiples of 4); table slots
+  int chunk, slots, room;  // ids of a pass (a multiple of kRun), table slots (of 4), list
   uint32_t* ids;
   myos_logit_controls_args c;
 };
 
-// A row is shared by a cluster of blocks, a slice of the vocabulary each. A
-// block sorts the row's tokens and biases that fall into its slice into a hash
-// table in shared memory by integer atomics (the result does not depend on their
-// order); then the slice passes once, four ids a thread and load, with nothing
-// to wait for between them: out = logits under the mask, and the largest of the
-// ids that no token or bias touches; then the touched ids are computed one to a
-// thread, over what that pass wrote. A history longer than the table has room
-// for is handled in chunks of as many ids as the table has slots, each id in the
-// slot of its own number. The blocks' best ids meet in the first block's shared
-// memory.
+// A row is shared by a cluster of blocks, every so many-th run of 128 ids each
+// (common tokens have low ids: in plain slices the first block had most of the
+// work). A block lists the row's tokens and biases among its ids and sorts them
+// into a hash table in shared memory by integer atomics (the result does not
+// depend on their order); then its ids pass once, four a thread and load, with nothing to wait
+// for between them: out = logits under the mask, and the largest of the ids that
+// no token or bias touches; then the touched ids are computed one to a thread,
+// over what that pass wrote. Where the list runs over, the block's ids go in
+// chunks of as many as the table has slots, each id in the slot of its own
+// number, and the whole history is looked through for each. The blocks' best ids
+// meet in the first block's shared memory.
 //
 // What this replaces: tables of one word an id, chunk by chunk, with the
 // penalties in the pass over all ids, 59 instructions an id (64 rows of 152064:
@@ -38,8 +39,8 @@ struct LogitArgs {
 #define VT 512
 #endif
 constexpr int kMaxCluster = 8;
-constexpr int kTokens = 4096, kBiases = 1024;  // of a row: room in the table
-constexpr int kMaxChunk = 65536;
+constexpr int kMaxChunk = 65536, kRun = 128, kRunWords = kRun / 32 + 1;
+static_assert(kRunWords <= 8);
 constexpr uint32_t kSeen = 0x80000000u;  // in the prompt; the low bits count the output
 constexpr uint32_t kNoId = 0xffffffffu;
 
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
   __shared__ float best_v[32];
   __shared__ int best_i[32];
   __shared__ unsigned long long found[kMaxCluster];
-  __shared__ int listed;
+  __shared__ int listed, in_use;
   const int tid = threadIdx.x, lane = tid & 31;
   uint32_t rank, ranks;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -98,164 +99,196 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
     e1 = min(max(c.bias_starts[row + 1], 0), (int)c.num_bias);
   }
   const bool touched = hist > 0 || e1 > e0;
-  const bool hashed = hist <= kTokens && e1 - e0 <= kBiases;
   const uint32_t* mask = nullptr;
   if (c.mask) {
     const int64_t g = c.mask_rows ? c.mask_rows[row] : row;
     if (g >= 0 && g < (int64_t)c.num_masks) mask = c.mask + g * (int64_t)c.mask_stride;
   }
-  // the chunk's mask and touched ids, a bit each (two mask words more than full
-  // ones: a chunk may begin inside a word); the table: an id's place in the
-  // chunk, the history's word, 1 + its last bias entry; the slots in use
+  // the chunk's touched ids, a bit each; the table: an id's place among the
+  // block's, the history's word, 1 + its last bias entry; the slots in use
   const uint32_t slots = a.slots;
-  const int words = a.chunk / 32 + 2;
-  uint32_t* mask_s = tables;
-  uint32_t* bits = mask_s + words;
-  uint32_t* key = bits + words;
+  uint32_t* key = tables;
   uint32_t* word = key + slots;
   uint32_t* bias = word + slots;
-  uint16_t* used = reinterpret_cast<uint16_t*>(bias + slots);
+  uint32_t* bits = bias + slots;
+  uint32_t* mask_s = bits + (slots ? a.chunk / 32 : 0);
+  uint2* list = reinterpret_cast<uint2*>(mask_s + (c.mask ? (a.chunk / kRun * kRunWords + 2) & ~1 : 0));
+  uint16_t* used = reinterpret_cast<uint16_t*>(list + a.room);
+
+  // The block's ids: place l is id (l / kRun * ranks + rank) * kRun + l % kRun - shift.
+  const uint32_t log_ranks = __ffs(ranks) - 1;
+  const int runs = (a.vocab + shift + kRun - 1) / kRun;
+  const int places = (runs - (int)rank + (int)ranks - 1) / (int)ranks * kRun;
+  auto id_at = [&](int l) -> int {
+    return (((l / kRun) << log_ranks | (int)rank) * kRun | (l & (kRun - 1))) - shift;
+  };
+  // the first 3 ids of a row may come before it, and any behind it
+  const uint32_t whole = a.vocab > 3 ? a.vocab - 3 : 0;  // ids from which four on are in the row
 
   float bv = -INFINITY;
   int bi = 0;
-  const int s0 = rank * a.slice, s1 = min(s0 + a.slice, a.vocab + shift);
-  const int step = hashed || !touched ? a.chunk : min(a.chunk, (int)slots & ~3);
+  auto take = [&](float v, int i) {
+    if (v > bv || (v == bv && i < bi)) {
+      bv = v;
+      bi = i;
+    }
+  };
+  // An id's place among the block's, or -1.
+  auto place = [&](int32_t id) -> int {
+    const uint32_t t = (uint32_t)id + (uint32_t)shift, run = t / kRun;
+    const bool ours = (uint32_t)id < (uint32_t)a.vocab && (run & (ranks - 1)) == rank;
+    return ours ? (int)((run >> log_ranks) * kRun + t % kRun) : -1;
+  };
+  // All tokens f(id, kSeen or 0, 0) and biases f(id, 0, 1 + entry) of the row,
+  // whole warps at a time (id -1: none).
+  constexpr int kBatch = 4;
+  const int warp_at = tid & ~31;
+  auto all_of_row = [&](auto&& f) {
 #pragma unroll 1
-  for (int base = s0; base < s1; base += step) {
-    const int n = min(step, s1 - base);  // shifted ids base .. base + n
-    const int first = base - shift;      // the id of the first
-    const int word0 = max(first, 0) >> 5;
-    if (base > s0) __syncthreads();
-    if (mask)
-#pragma unroll 1
-      for (int k = tid; k < n / 32 + 2; k += kThreads)
-        mask_s[k] = (word0 + k) * 32 < a.vocab ? mask[word0 + k] : 0u;
-    if (touched) {
-#pragma unroll 1
-      for (int k = tid; k < (int)slots; k += kThreads) {
-        key[k] = kNoId;
-        word[k] = 0;
-        bias[k] = 0;
+    for (int i0 = warp_at; i0 < hist; i0 += kBatch * kThreads) {
+      int32_t id[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = i0 + lane + k * kThreads;
+        id[k] = i < hist ? said[i] : -1;
       }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        f(id[k], i0 + lane + k * kThreads < prompt ? kSeen : 0u, 0u);
+    }
 #pragma unroll 1
-      for (int k = tid; k < n / 32 + 1; k += kThreads) bits[k] = 0;
-      if (tid == 0) listed = 0;
+    for (int e = e0 + warp_at; e < e1; e += kThreads)
+      f(e + lane < e1 ? c.bias_ids[e + lane] : -1, 0u, (uint32_t)(e + lane - e0 + 1));
+  };
+  bool hashed = true;
+  if (touched) {
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    all_of_row([&](int32_t id, uint32_t flag, uint32_t e) {
+      const int l = place(id);
+      const uint32_t who = __ballot_sync(0xffffffffu, l >= 0);
+      if (who == 0) return;
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&listed, __popc(who));
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+      if (l >= 0 && at < a.room) list[at] = make_uint2((uint32_t)l | flag, e);
+    });
+    __syncthreads();
+    hashed = listed <= a.room;
+  }
+  const int step = hashed ? a.chunk : min(a.chunk, (int)slots & ~(kRun - 1));
+#pragma unroll 1
+  for (int base = 0; base < places; base += step) {
+    const int n = min(step, places - base);
+    if (base > 0) __syncthreads();
+    if (mask) {
+      // the mask's words of each run, from the one with its first id on; that id
+      // is the word's bit -shift % 32 in every run
+      const int all = (a.vocab + 31) / 32;
+#pragma unroll 1
+      for (int k = tid; k < n / kRun * 8; k += kThreads) {  // eight threads a run
+        const int at = k & 7, w = (id_at(base + (k >> 3) * kRun) >> 5) + at;  // -1: before the row
+        if (at < kRunWords)
+          mask_s[(k >> 3) * kRunWords + at] = (uint32_t)w < (uint32_t)all ? mask[w] : 0u;
+      }
+    }
+    if (touched) {
+      const uint4 none = make_uint4(0, 0, 0, 0), no_id = make_uint4(kNoId, kNoId, kNoId, kNoId);
+#pragma unroll 1
+      for (int k = tid; k < (int)slots / 4; k += kThreads) reinterpret_cast<uint4*>(key)[k] = no_id;
+      // word, bias and bits lie behind one another
+#pragma unroll 1
+      for (int k = tid; k < (int)slots / 2 + a.chunk / 128; k += kThreads)
+        reinterpret_cast<uint4*>(word)[k] = none;
+      if (tid == 0) in_use = 0;
       __syncthreads();
-      // the slot of an id of this chunk, or -1
-      auto slot_of = [&](int32_t id) -> int {
-        const uint32_t t = (uint32_t)id - (uint32_t)first;
-        if ((uint32_t)id >= (uint32_t)a.vocab || t >= (uint32_t)n) return -1;
-        uint32_t h = hashed ? __umulhi(t * 2654435761u, slots) : t;
+      // a token (kSeen or 0: of the prompt or the output) or a bias entry of place l
+      auto enter = [&](uint32_t l, uint32_t flag, uint32_t e) {
+        if (l >= (uint32_t)n) return;
+        uint32_t h = hashed ? __umulhi(l * 2654435761u, slots) : l;
         for (;;) {
-          const uint32_t was = atomicCAS(&key[h], kNoId, t);
+          const uint32_t was = atomicCAS(&key[h], kNoId, l);
           if (was == kNoId) {
-            atomicOr(&bits[t >> 5], 1u << (t & 31));
-            used[atomicAdd(&listed, 1)] = (uint16_t)h;
+            atomicOr(&bits[l >> 5], 1u << (l & 31));
+            used[atomicAdd(&in_use, 1)] = (uint16_t)h;
             break;
           }
-          if (was == t) break;
+          if (was == l) break;
           if (++h == slots) h = 0;
         }
-        return (int)h;
+        // the last entry of an id counts: entries leave their number, the largest stays
+        if (e) atomicMax(&bias[h], e);
+        else if (flag) atomicOr(&word[h], kSeen);
+        else atomicAdd(&word[h], 1u);
       };
-      constexpr int kBatch = 4;
+      if (hashed) {
 #pragma unroll 1
-      for (int i0 = tid; i0 < hist; i0 += kBatch * kThreads) {
-        int32_t id[kBatch];
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) id[k] = i0 + k * kThreads < hist ? said[i0 + k * kThreads] : -1;
-#pragma unroll 1
-        for (int k = 0; k < kBatch; ++k) {
-          const int32_t now = id[0];
-          id[0] = id[1], id[1] = id[2], id[2] = id[3];
-          const int h = slot_of(now);
-          if (h < 0) continue;
-          if (i0 + k * kThreads < prompt) atomicOr(&word[h], kSeen);
-          else atomicAdd(&word[h], 1u);
-        }
-      }
-      // the last entry of an id counts: entries leave their number, the largest stays
-#pragma unroll 1
-      for (int e = e0 + tid; e < e1; e += kThreads) {
-        const int h = slot_of(c.bias_ids[e]);
-        if (h >= 0) atomicMax(&bias[h], (uint32_t)(e - e0 + 1));
+        for (int k = tid; k < listed; k += kThreads)
+          enter(list[k].x & ~kSeen, list[k].x & kSeen, list[k].y);
+      } else {
+        all_of_row([&](int32_t id, uint32_t flag, uint32_t e) {
+          const int l = place(id);
+          if (l >= base) enter((uint32_t)(l - base), flag, e);
+        });
       }
     }
     if (touched || mask) __syncthreads();
+    // the mask's bits from place l on, at least four of them
+    const int lead = -shift & 31;
+    auto allowed = [&](int l) -> uint32_t {
+      const int at = (l & (kRun - 1)) + lead;
+      const uint32_t* w = mask_s + l / kRun * kRunWords + (at >> 5);
+      return __funnelshift_r(w[0], w[1], at & 31);  // a run's last word is not needed at its end
+    };
 
-    // ids i .. i + 3 at place `at` of the chunk: the value of an id, edge or not
-    auto pass = [&](int at, float (&r)[4]) -> uint32_t {  // the untouched ones
-      uint32_t keep = 15u;
-      if (touched) keep = ~(bits[at >> 5] >> (at & 31));  // at is a multiple of 4
-      if (mask) {
-        // their bits may lie in two words; bits of ids out of range are not used
-        const int i = first + at, w0 = (max(i, 0) >> 5) - word0;
-        const uint32_t m = mask_s[w0];
-        const uint32_t m4 = i >= 0 ? __funnelshift_r(m, mask_s[w0 + 1], i & 31) : m << -i;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (!((m4 >> j) & 1u)) r[j] = -INFINITY;
-      }
-      return keep;
-    };
-    auto take = [&](float v, int i) {  // ids come in rising order
-      if (v > bv) {
-        bv = v;
-        bi = i;
-      }
-    };
-    // groups [g0, g1) lie within the row; at most one before and one behind do not
-    const int g0 = first < 0 ? 1 : 0, g1 = min((n + 3) / 4, (a.vocab - first) / 4);
-    const float* xc = x + first;
-    float* yc = y + first;
     constexpr int kUnroll = 4;
+    static_assert(4 * kThreads % kRun == 0);
+    const int far = (4 * kThreads) << log_ranks;  // from a thread's group to its next
 #pragma unroll 1
-    for (int gr = g0 + tid; gr < g1; gr += kUnroll * kThreads) {
+    for (int l0 = 4 * tid; l0 < n; l0 += 4 * kUnroll * kThreads) {
+      const int i0 = id_at(base + l0);
       float4 v[kUnroll];
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k)
-        if (gr + k * kThreads < g1)
-          v[k] = *reinterpret_cast<const float4*>(xc + 4 * (gr + k * kThreads));
+      for (int k = 0; k < kUnroll; ++k) {
+        const int i = i0 + k * far;
+        if ((uint32_t)i < whole && l0 + 4 * k * kThreads < n)
+          v[k] = *reinterpret_cast<const float4*>(x + i);
+      }
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
-        if (gr + k * kThreads >= g1) break;
-        const int at = 4 * (gr + k * kThreads);
-        float r[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-        const uint32_t keep = pass(at, r);
-        if (y) {
-          if (together) {
-            *reinterpret_cast<float4*>(yc + at) = make_float4(r[0], r[1], r[2], r[3]);
-          } else {
+        const int l = l0 + 4 * k * kThreads, i = i0 + k * far;
+        if (l >= n) break;
+        const uint32_t b4 = touched ? bits[l >> 5] >> (l & 31) & 15u : 0u;  // l: a multiple of 4
+        if ((uint32_t)i < whole) {
+          float r[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          if (mask) {
+            const uint32_t m = allowed(l);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) yc[at + j] = r[j];
+            for (int j = 0; j < 4; ++j)
+              if (!(m >> j & 1u)) r[j] = -INFINITY;
           }
-        }
-        if (fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])) > bv) {  // NaN is passed over
+          if (y) {
+            if (together) {
+              *reinterpret_cast<float4*>(y + i) = make_float4(r[0], r[1], r[2], r[3]);
+            } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (keep >> j & 1u) take(r[j], first + at + j);
-        }
-      }
-    }
-    // the groups that reach over the row's ends
-    if (tid < 2) {
-      const int gr = tid == 0 ? 0 : g1;
-      if ((tid == 0 ? g0 == 1 : 4 * g1 < n) && (tid == 0 || g1 >= g0)) {
-        float r[4];
+              for (int j = 0; j < 4; ++j) y[i + j] = r[j];
+            }
+          }
+          if (fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])) >= bv) {  // NaN is passed over
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = first + 4 * gr + j;
-          r[j] = i >= 0 && i < a.vocab ? x[i] : -INFINITY;
-        }
-        const uint32_t keep = pass(4 * gr, r);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = first + 4 * gr + j;
-          if (i < 0 || i >= a.vocab) continue;
-          if (y) y[i] = r[j];
-          if ((keep >> j & 1u) && (r[j] > bv || (r[j] == bv && i < bi))) {
-            bv = r[j];
-            bi = i;
+            for (int j = 0; j < 4; ++j)
+              if (!(b4 >> j & 1u)) take(r[j], i + j);
+          }
+        } else {  // the group reaches over the row's ends, or lies behind it
+#pragma unroll 1
+          for (int j = 0; j < 4; ++j) {
+            const int id = i + j;
+            if ((uint32_t)id >= (uint32_t)a.vocab) continue;
+            float r = x[id];
+            if (mask && !(allowed(l + j) & 1u)) r = -INFINITY;
+            if (y) y[id] = r;
+            if (!(b4 >> j & 1u)) take(r, id);
           }
         }
       }
@@ -264,19 +297,16 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
     __syncthreads();
     // the touched ids, over what the pass wrote (an id that the mask takes out
     // is -inf whatever it was, any other still holds its logit)
-#pragma unroll 1
-    for (int k = tid; k < listed; k += kThreads) {
-      const int h = used[k], i = first + (int)key[h];
+#pragma unroll 2
+    for (int k = tid; k < in_use; k += kThreads) {
+      const int h = used[k], l = (int)key[h], i = id_at(base + l);
       float r = x[i];
       const uint32_t w = word[h], e = bias[h];
       if (w) r = penalised(r, w, rep, freq, pres, c.repetition != nullptr);
       if (e) r = __fadd_rn(r, c.bias_vals[e0 + e - 1]);
-      if (mask && !(mask_s[(i >> 5) - word0] >> (i & 31) & 1u)) r = -INFINITY;
+      if (mask && !(allowed(l) & 1u)) r = -INFINITY;
       if (y) y[i] = r;
-      if (r > bv || (r == bv && i < bi)) {
-        bv = r;
-        bi = i;
-      }
+      take(r, i);
     }
   }
   if (!a.ids) return;
@@ -317,29 +347,36 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
 
 template <int kThreads>
 cudaError_t launch_controls(LogitArgs a, size_t rows, cudaStream_t st) {
-  // As many blocks a row as are resident at once, slices of at least 2048 ids;
-  // slices and chunks in multiples of four (three ids more: a row's shift).
-  const int ids = a.vocab + 3;
+  // As many blocks a row as are resident at once, with 2048 ids at least
   int cluster = kMaxCluster;
   while (cluster > 1 &&
-         (rows * cluster > (size_t)sm_count() * SLOTS || ids / cluster < 2048))
+         (rows * cluster > (size_t)sm_count() * SLOTS || a.vocab / cluster < 2048))
     cluster /= 2;
-  a.slice = ((ids + cluster - 1) / cluster + 3) & ~3;
-  const int passes = (a.slice + kMaxChunk - 1) / kMaxChunk;
-  a.chunk = ((a.slice + passes - 1) / passes + 3) & ~3;
+  const int most = ((a.vocab + 3 + kRun - 1) / kRun + cluster - 1) / cluster * kRun;
+  const int passes = (most + kMaxChunk - 1) / kMaxChunk;
+  a.chunk = ((most / kRun + passes - 1) / passes) * kRun;
   const bool pen = a.c.history && (a.c.repetition || a.c.frequency || a.c.presence);
-  // room for every id that the listed tokens and biases can name, and a quarter more
-  size_t room = 0;
-  if (pen) room += a.c.history_width < kTokens ? a.c.history_width : kTokens;
-  if (a.c.bias_starts) room += a.c.num_bias < kBiases ? a.c.num_bias : kBiases;
-  a.slots = room ? (int)((room + room / 4 + 31) & ~(size_t)31) : 0;
-  const auto bytes = [](size_t chunk, size_t slots) { return 8 * (chunk / 32 + 2) + 14 * slots; };
-  const size_t smem = bytes(a.chunk, a.slots);
-  constexpr size_t kMostSlots = (kTokens + kBiases) * 5 / 4;
-  static_assert(kMostSlots % 32 == 0 && kMostSlots <= 65536);
+  // a table for three times a block's share of the longest history and of the mean
+  // number of biases, and four slots for five entries
+  size_t share = 0;
+  if (pen) share += a.c.history_width;
+  if (a.c.bias_starts) share += a.c.num_bias / rows + 32;
+  constexpr size_t kLeastRoom = 512, kMostRoom = 5120;
+  static_assert(kLeastRoom * 5 / 4 >= kRun && kMostRoom * 5 / 4 <= 65536);
+  size_t room = share == 0 ? 0 : 3 * share / cluster;
+  if (room > kMostRoom) room = kMostRoom;
+  if (room > 0 && room < kLeastRoom) room = kLeastRoom;
+  room = (room + 15) & ~(size_t)15;
+  a.room = (int)room;
+  a.slots = (int)(room + room / 4);
+  const auto bytes = [](size_t chunk, size_t room, bool mask) {
+    return (room ? chunk / 8 : 0) + (mask ? 4 * (chunk / kRun * kRunWords + 2) : 0) +
+           14 * (room + room / 4) + 8 * room;
+  };
+  const size_t smem = bytes(a.chunk, room, a.c.mask);
   static std::atomic<uint64_t> raised{0};
   const cudaError_t e = raise_smem_limit((const void*)k_logit_controls<kThreads>,
-                                         bytes(kMaxChunk, kMostSlots), &raised);
+                                         bytes(kMaxChunk, kMostRoom, true), &raised);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * cluster));
