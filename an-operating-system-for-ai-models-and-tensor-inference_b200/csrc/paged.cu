@@ -49,144 +49,185 @@ int sm_count() {
 namespace {
 
 // ------------------------------------------------------------------ tables
-// Every block runs the two prefix sums over all requests itself (8 bytes a
-// request from L2), so one launch with no meeting of the blocks does the
-// whole step: block i then writes the table entries of every gridDim-th
-// request and its share of the rows.
+// Every block runs the prefix sums over all requests itself (8 bytes a request
+// from L2), so one launch with no meeting of the blocks does the whole step:
+// block i then writes the table entries and rows of its share. A request of one
+// or two rows (decode) is written by the thread that scanned it, which has
+// looked its last page up meanwhile; the rows of longer ones find their request
+// by a binary search. What is left is latency: two loads on one another
+// (lengths, then pages), one barrier, the stores.
 struct TablesArgs {
   int32_t* table;
-  int64_t table_stride, max_blocks;
+  int64_t table_stride;
+  int max_blocks;
   const int32_t *ctx, *add;
   int nseq;
   const int32_t* free_pages;
-  int64_t free_cap;
+  int free_cap;
   const int32_t* num_free;
   uint32_t page_size, num_pages;
   int64_t* slots;
   int32_t *positions, *row_seq;
-  int64_t max_rows;
+  int max_rows;
   int32_t *kv_lens, *seq_starts, *result;
 };
 
-MYOS_DEV int64_t warp_scan(int64_t v) {
+struct Sums {
+  int64_t rows, pages;
+};
+MYOS_DEV Sums warp_scan(Sums v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
+    const int64_t r = __shfl_up_sync(0xffffffffu, v.rows, o);
+    const int64_t p = __shfl_up_sync(0xffffffffu, v.pages, o);
+    if (lane >= o) {
+      v.rows += r;
+      v.pages += p;
+    }
   }
   return v;
 }
 
-// Inclusive sum over the block; *total is the block's. red: 33 values.
-MYOS_DEV int64_t block_scan(int64_t v, int64_t* red, int64_t* total) {
+constexpr int kSmall = 2;  // rows that a request's thread writes itself
+constexpr uint32_t kLong = 0x80000000u;
+
+// A request: its first row, the pages taken by the requests before it (-1: it is
+// refused), and its length, with kLong where its rows are not written yet.
+struct Span {
+  int start, first;
+  uint32_t ctx;
+};
+MYOS_DEV uint32_t ceil_div(uint32_t a, uint32_t b) { return a / b + (a % b != 0); }
+
+__global__ void __launch_bounds__(1024) k_paged_tables(const TablesArgs a) {
+  extern __shared__ Span spans[];
+  __shared__ Sums parts[2][32];
+  __shared__ int64_t taken_s[32];
+  __shared__ int refused_s[32];
+  const uint32_t P = a.page_size;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
-  v = warp_scan(v);
-  if (lane == 31) red[warp] = v;
-  __syncthreads();
-  if (warp == 0) {
-    const int64_t t = warp_scan(lane < nwarps ? red[lane] : 0);
-    red[lane] = t;
-  }
-  __syncthreads();
-  if (warp > 0) v += red[warp - 1];
-  *total = red[nwarps - 1];
-  __syncthreads();
-  return v;
-}
-
-__global__ void __launch_bounds__(1024) k_paged_tables(TablesArgs a) {
-  // end[b]: row behind request b's last, clipped to max_rows; first[b]: pages
-  // taken by the requests before b, or -1 for a refused one.
-  extern __shared__ int32_t smem[];
-  int32_t* end = smem;
-  int32_t* first = smem + a.nseq;
-  __shared__ int64_t red[32];
-  __shared__ int refused_s;
-  const int64_t P = a.page_size;
-  const bool writer = blockIdx.x == 0;
-  const int64_t nfree = min((int64_t)max(*a.num_free, 0), a.free_cap);
-  if (threadIdx.x == 0) refused_s = 0;
-  int64_t rows0 = 0, pages0 = 0, taken = 0;
-  int refused = 0;
-  for (int base = 0; base < a.nseq; base += blockDim.x) {
+  const int nfree = min(max(*a.num_free, 0), a.free_cap);
+  const int64_t room = (int64_t)a.max_blocks * P;
+  Sums before = {0, 0};  // of the requests of earlier rounds
+  int64_t taken = 0;
+  int refused = 0, longer = 0;
+  // the page of a position of a request with `held` pages and `first` taken before
+  auto page_of = [&](int b, uint32_t pg, uint32_t held, int first) -> int32_t {
+    return pg < held ? a.table[b * a.table_stride + pg]
+                     : a.free_pages[nfree - 1 - first - (int)(pg - held)];
+  };
+  auto row = [&](int r, int b, uint32_t pos, uint32_t in, int32_t page) {
+    a.slots[r] = page >= 0 && (uint32_t)page < a.num_pages ? (int64_t)page * P + in : -1;
+    a.positions[r] = (int32_t)pos;
+    a.row_seq[r] = b;
+  };
+#pragma unroll 1
+  for (int base = 0, round = 0; base < a.nseq; base += blockDim.x, ++round) {
     const int b = base + threadIdx.x;
-    int64_t ctx = 0, add = 0;
+    const bool mine = b % (int)(gridDim.x * 32) / 32 == (int)blockIdx.x;  // 32 in turn
+    uint32_t ctx = 0, add = 0;
     if (b < a.nseq) {
       ctx = max(a.ctx[b], 0);
       add = max(a.add[b], 0);
     }
-    int64_t total;
-    const int64_t e = rows0 + block_scan(add, red, &total);
-    rows0 += total;
-    const bool fits = add == 0 || (ctx + add <= a.max_blocks * P && e <= a.max_rows);
-    const int64_t held = (ctx + P - 1) / P;
-    const int64_t need = add > 0 && fits ? (ctx + add + P - 1) / P - held : 0;
-    const int64_t upto = pages0 + block_scan(need, red, &total);
-    pages0 += total;
-    const bool ok = fits && (need == 0 || upto <= nfree);
-    if (b < a.nseq) {
-      end[b] = (int32_t)min(e, a.max_rows);
-      first[b] = ok ? (int32_t)min(upto - need, (int64_t)0x7fffffff) : -1;
-      if (ok) taken = max(taken, need > 0 ? upto : 0);
-      refused += !ok;
-      if (writer) {
-        a.kv_lens[b] = (int32_t)(ok ? ctx + add : ctx);
-        a.seq_starts[b + 1] = (int32_t)min(e, a.max_rows);
-        if (b == 0) a.seq_starts[0] = 0;
+    // lengths are below 2^31, their sum below 2^32
+    const uint32_t held = ceil_div(ctx, P), all = ceil_div(ctx + add, P);
+    const bool fits = (int64_t)ctx + add <= room;
+    // the page that a decode row goes to, on its way during the scan
+    const bool look = mine && fits && add > 0 && add <= kSmall && ctx % P != 0;
+    const int32_t last = look ? a.table[b * a.table_stride + ctx / P] : -1;
+    // A request that the row buffer has no room for is behind every admitted one
+    // (the rows only grow), so its need may stand in the sum.
+    const uint32_t need = add > 0 && fits ? all - held : 0;
+    const Sums own = {(int64_t)add, (int64_t)need};
+    Sums s = warp_scan(own);
+    if (lane == 31) parts[round & 1][warp] = s;
+    __syncthreads();
+    const Sums upto = warp_scan(lane < nwarps ? parts[round & 1][lane] : Sums{0, 0});
+    s.rows += before.rows + (warp ? __shfl_sync(0xffffffffu, upto.rows, max(warp, 1) - 1) : 0);
+    s.pages += before.pages + (warp ? __shfl_sync(0xffffffffu, upto.pages, max(warp, 1) - 1) : 0);
+    before.rows += __shfl_sync(0xffffffffu, upto.rows, 31);
+    before.pages += __shfl_sync(0xffffffffu, upto.pages, 31);
+    if (b >= a.nseq) continue;
+    const int end = (int)min(s.rows, (int64_t)a.max_rows);
+    const int start = (int)min(s.rows - own.rows, (int64_t)a.max_rows);
+    const bool ok = add == 0 || (fits && s.rows <= a.max_rows && (need == 0 || s.pages <= nfree));
+    const int first = ok ? (int)min(s.pages - own.pages, (int64_t)nfree) : -1;
+    if (ok && need > 0) taken = s.pages;  // a later request's is larger
+    refused += !ok;
+    spans[b] = Span{start, first, ctx | (add > kSmall ? kLong : 0u)};
+    longer |= add > kSmall;
+    if (!mine) continue;
+    a.kv_lens[b] = (int32_t)(ok ? ctx + add : ctx);
+    a.seq_starts[b + 1] = end;
+    if (b == 0) a.seq_starts[0] = 0;
+    if (add == 0 || add > kSmall) continue;
+#pragma unroll 1
+    for (int r = start; r < end; ++r) {
+      if (!ok) {
+        row(r, b, 0, 0, -1);
+        continue;
       }
+      const uint32_t pos = ctx + (r - start), pg = pos / P;
+      const int32_t page = look && pg == ctx / P ? last : page_of(b, pg, held, first);
+      if (pg >= held && pos % P == 0) a.table[b * a.table_stride + pg] = page;
+      row(r, b, pos, pos - pg * P, page);
     }
   }
-  __syncthreads();
-  if (writer) {
+  if (blockIdx.x == 0) {
     // the admitted requests' running sum is largest at the last of them
-#pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       taken = max(taken, __shfl_xor_sync(0xffffffffu, taken, o));
       refused += __shfl_xor_sync(0xffffffffu, refused, o);
     }
-    if ((threadIdx.x & 31) == 0) {
-      red[threadIdx.x >> 5] = taken;
-      atomicAdd(&refused_s, refused);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 0; w < (int)(blockDim.x >> 5); ++w) taken = max(taken, red[w]);
-      a.result[0] = (int32_t)(nfree - taken);
-      a.result[1] = refused_s;
+    if (lane == 0) {
+      taken_s[warp] = taken;
+      refused_s[warp] = refused;
     }
   }
-  // new table entries: one warp per request
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  for (int b = blockIdx.x * warps + (threadIdx.x >> 5); b < a.nseq; b += gridDim.x * warps) {
-    const int64_t ctx = max(a.ctx[b], 0), add = max(a.add[b], 0);
-    if (first[b] < 0 || add == 0) continue;
-    const int64_t held = (ctx + P - 1) / P, need = (ctx + add + P - 1) / P - held;
-    for (int64_t j = lane; j < need; j += 32)
-      a.table[b * a.table_stride + held + j] = a.free_pages[nfree - 1 - first[b] - j];
-  }
-  // rows: the request is the first whose end lies behind the row
-  for (int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; r < a.max_rows;
-       r += (int64_t)gridDim.x * blockDim.x) {
-    int lo = 0, hi = a.nseq;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (end[mid] > r) hi = mid;
-      else lo = mid + 1;
+  longer = __syncthreads_or(longer);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    for (int w = 1; w < nwarps; ++w) {
+      taken = max(taken, taken_s[w]);
+      refused += refused_s[w];
     }
-    int64_t slot = -1, pos = 0;
-    if (lo < a.nseq && first[lo] >= 0) {
-      const int64_t ctx = max(a.ctx[lo], 0), held = (ctx + P - 1) / P;
-      pos = ctx + r - (lo > 0 ? end[lo - 1] : 0);
-      const int64_t pg = pos / P;
-      const int32_t page = pg < held ? a.table[lo * a.table_stride + pg]
-                                     : a.free_pages[nfree - 1 - first[lo] - (pg - held)];
-      if (page >= 0 && (uint32_t)page < a.num_pages) slot = (int64_t)page * P + pos % P;
-    }
-    a.slots[r] = slot;
-    a.positions[r] = (int32_t)pos;
-    a.row_seq[r] = lo < a.nseq ? lo : -1;
+    a.result[0] = (int32_t)(nfree - taken);
+    a.result[1] = refused;
   }
+  const int rows = (int)min(before.rows, (int64_t)a.max_rows);
+  if (longer) {
+    // new table entries, a warp for each request
+#pragma unroll 1
+    for (int b = warp * gridDim.x + blockIdx.x; b < a.nseq; b += gridDim.x * nwarps) {
+      const Span sp = spans[b];
+      if (!(sp.ctx & kLong) || sp.first < 0) continue;
+      const uint32_t ctx = sp.ctx & ~kLong, add = a.add[b];
+      const uint32_t held = ceil_div(ctx, P), need = ceil_div(ctx + add, P) - held;
+#pragma unroll 1
+      for (uint32_t j = lane; j < need; j += 32)
+        a.table[b * a.table_stride + held + j] = a.free_pages[nfree - 1 - sp.first - (int)j];
+    }
+    // rows: of the last request that begins at or before the row
+#pragma unroll 2
+    for (int r = blockIdx.x * blockDim.x + threadIdx.x; r < rows; r += gridDim.x * blockDim.x) {
+      int lo = 0, hi = a.nseq;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (spans[mid].start <= r) lo = mid;
+        else hi = mid;
+      }
+      const Span sp = spans[lo];
+      if (!(sp.ctx & kLong)) continue;
+      const uint32_t ctx = sp.ctx & ~kLong, pos = ctx + (r - sp.start), pg = pos / P;
+      if (sp.first < 0) row(r, lo, 0, 0, -1);
+      else row(r, lo, pos, pos - pg * P, page_of(lo, pg, ceil_div(ctx, P), sp.first));
+    }
+  }
+  // rows behind the last request's
+  for (int64_t r = (int64_t)rows + blockIdx.x * blockDim.x + threadIdx.x; r < a.max_rows;
+       r += gridDim.x * blockDim.x)
+    row((int)r, -1, 0, 0, -1);
 }
 
 // ------------------------------------------------------- norm, rotate, store
@@ -350,34 +391,34 @@ int myos_dev_paged_tables(int32_t* d_block_table, size_t table_stride, size_t ma
       max_blocks == 0 || max_blocks > 0x7fffffff || table_stride < max_blocks ||
       table_stride > ((size_t)1 << 40) || max_rows > 0x7fffffff || free_cap > 0x7fffffff)
     return MYOS_ERR_SHAPE;
-  const size_t smem = 8 * nseq;
+  const size_t smem = sizeof(Span) * nseq;
   static std::atomic<uint64_t> raised{0};
   if (smem > 48 * 1024 &&
-      raise_smem_limit((const void*)k_paged_tables, 8 * 16384, &raised) != cudaSuccess)
+      raise_smem_limit((const void*)k_paged_tables, sizeof(Span) * 16384, &raised) != cudaSuccess)
     return MYOS_ERR_CUDA;
   TablesArgs a;
   a.table = d_block_table;
   a.table_stride = (int64_t)table_stride;
-  a.max_blocks = (int64_t)max_blocks;
+  a.max_blocks = (int)max_blocks;
   a.ctx = d_ctx_lens;
   a.add = d_new_lens;
   a.nseq = (int)nseq;
   a.free_pages = d_free_pages;
-  a.free_cap = (int64_t)free_cap;
+  a.free_cap = (int)free_cap;
   a.num_free = d_num_free;
   a.page_size = page_size;
   a.num_pages = num_pages;
   a.slots = d_slots;
   a.positions = d_positions;
   a.row_seq = d_row_seq;
-  a.max_rows = (int64_t)max_rows;
+  a.max_rows = (int)max_rows;
   a.kv_lens = d_kv_lens;
   a.seq_starts = d_seq_starts;
   a.result = d_result;
-  const int threads = nseq <= 256 && max_rows <= 4096 ? 256 : 1024;
-  const size_t work = max_rows > nseq ? max_rows : nseq;
-  size_t grid = (work + threads - 1) / threads;
-  if (grid > 148) grid = 148;
+  // a small batch in small blocks: the barrier waits for fewer warps
+  const int threads = nseq <= 32 && max_rows <= 64 ? 32 : nseq <= 256 && max_rows <= 4096 ? 256 : 1024;
+  size_t grid = ((max_rows > nseq ? max_rows : nseq) + threads - 1) / threads;
+  if (grid > (size_t)sm_count()) grid = sm_count();
   k_paged_tables<<<(int)grid, threads, smem, (cudaStream_t)stream>>>(a);
   return counted(cudaGetLastError()) == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
 }
