@@ -70,6 +70,8 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
   if (a.ids && ranks > 1)  // the first block's memory is written to below: it has to have started
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  pdl_launch();
+  pdl_wait();
   const int64_t row = blockIdx.x / ranks;
   const myos_logit_controls_args& c = a.c;
   const float* x = a.logits + row * a.logits_stride;
@@ -387,18 +389,8 @@ cudaError_t launch_controls(LogitArgs a, size_t rows, cudaStream_t st) {
   const cudaError_t e = raise_smem_limit((const void*)k_logit_controls<kThreads>,
                                          bytes(kMaxChunk, kMostRoom, true), &raised);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return counted(cudaLaunchKernelEx(&cfg, k_logit_controls<kThreads>, a));
+  return counted(launch_pdl(k_logit_controls<kThreads>, dim3((unsigned)(rows * cluster)), kThreads,
+                            smem, st, cluster, a));
 }
 
 }  // namespace

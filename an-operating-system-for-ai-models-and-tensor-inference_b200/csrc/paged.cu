@@ -107,6 +107,8 @@ __global__ void __launch_bounds__(1024) k_paged_tables(const TablesArgs a) {
   __shared__ int refused_s[32];
   const uint32_t P = a.page_size;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  pdl_launch();
+  pdl_wait();
   const int nfree = min(max(*a.num_free, 0), a.free_cap);
   const int64_t room = (int64_t)a.max_blocks * P;
   Sums before = {0, 0};  // of the requests of earlier rounds
@@ -295,6 +297,8 @@ __global__ void __launch_bounds__(kStoreThreads) k_paged_store(const StoreArgs a
   const int c0 = 4 * (turn ? j : 2 * pairs + 2 * (j - pairs));
   const int c1 = turn ? c0 + 4 * pairs : c0 + 4;
   const bool norm = a.q_gamma || a.k_gamma;
+  pdl_launch();
+  pdl_wait();
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float* src = a.qkv + row * a.qkv_stride;
     const int64_t slot = a.slots[row];
@@ -376,8 +380,8 @@ cudaError_t launch_store(const StoreArgs& a, const myos_paged_kv* kv, cudaStream
   const int parts = (a.hq + 2 * (int)kv->num_kv_heads + per - 1) / per;
   dim3 grid((unsigned)(a.rows < most ? a.rows : most));
   while ((int)grid.y < parts && grid.x * (grid.y + 1) <= most / 2) ++grid.y;
-  k_paged_store<KT, 2><<<grid, kStoreThreads, 0, st>>>(a, paged_view<KT>(kv));
-  return counted(cudaGetLastError());
+  return counted(
+      launch_pdl(k_paged_store<KT, 2>, grid, kStoreThreads, 0, st, 1, a, paged_view<KT>(kv)));
 }
 
 }  // namespace
@@ -439,8 +443,9 @@ int myos_dev_paged_tables(int32_t* d_block_table, size_t table_stride, size_t ma
   const int threads = nseq <= 32 && max_rows <= 64 ? 32 : nseq <= 256 && max_rows <= 4096 ? 256 : 1024;
   size_t grid = ((max_rows > nseq ? max_rows : nseq) + threads - 1) / threads;
   if (grid > (size_t)sm_count()) grid = sm_count();
-  k_paged_tables<<<(int)grid, threads, smem, (cudaStream_t)stream>>>(a);
-  return counted(cudaGetLastError()) == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
+  const cudaError_t e =
+      launch_pdl(k_paged_tables, dim3((unsigned)grid), threads, smem, (cudaStream_t)stream, 1, a);
+  return counted(e) == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
 }
 
 int myos_dev_qk_norm_rope_store(float* d_q, size_t q_stride, const float* d_qkv,

@@ -51,6 +51,32 @@ inline cudaError_t raise_smem_limit(const void* kernel, size_t bytes, std::atomi
   return e;
 }
 
+// Launches with a programmatic edge to the previous kernel of the stream: the
+// blocks are placed while its last ones run, and wait for its end and its
+// memory (pdl_wait) before their first global access. cluster: blocks of one
+// thread-block cluster.
+template <class... P, class... A>
+inline cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, size_t smem,
+                              cudaStream_t st, int cluster, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cluster > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Multiprocessors of the current device (148 where it cannot be asked).
 int sm_count();
 

@@ -651,9 +651,13 @@ constexpr size_t attn_smem() {
          (kWarps - 1) * W::kRegs * 32 * 4;
 }
 
+// Blocks resident on a multiprocessor, by shared memory (55, 108 or 216 KB each).
+template <int DH>
+constexpr int kResident = DH == 64 ? 4 : DH == 128 ? 2 : 1;
+
 // kFull: head_dim is DH itself (else the chunks behind it are zero-filled).
 template <class W, int DH, bool kFull>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, kResident<DH>)
     k_paged_attn(const PagedAttnArgs a, const PagedKv<typename W::KT> kv) {
   using KT = typename W::KT;
   constexpr int T = W::kKeys * kWarps, kThreads = kWarps * 32;
@@ -672,6 +676,8 @@ __global__ void __launch_bounds__(kWarps * 32)
   const uint32_t me = blockIdx.x;
   float* swap = reinterpret_cast<float*>(smem + kStages * kStageBytes);
   if (threadIdx.x < 2) ready[threadIdx.x] = 0;
+  pdl_launch();
+  pdl_wait();
 
   // this block's share [lo, hi) of the tiles (fewer than 2^31 in all), and
   // where it begins
@@ -917,12 +923,12 @@ cudaError_t launch(PagedAttnArgs a, const myos_paged_kv* kv, void* work, cudaStr
   int64_t keys = a.max_keys;
   if (a.window > 0 && (int64_t)a.window + T < keys) keys = (int64_t)a.window + T;
   const int64_t most = (int64_t)a.nseq * kv->num_kv_heads * ((keys + T - 1) / T);
-  int64_t grid = (int64_t)sm_count() * (smem <= 110 * 1024 ? 2 : 1);
+  static_assert((smem + 1536) * kResident<DH> <= 228 * 1024);
+  int64_t grid = (int64_t)sm_count() * kResident<DH>;
   if (grid > kMaxShares) grid = kMaxShares;
   if (grid > most) grid = most;
-  k_paged_attn<W, DH, kFull>
-      <<<(int)grid, kWarps * 32, smem, st>>>(a, paged_view<typename W::KT>(kv));
-  return counted(cudaGetLastError());
+  return counted(launch_pdl(k_paged_attn<W, DH, kFull>, dim3((unsigned)grid), kWarps * 32, smem, st,
+                            1, a, paged_view<typename W::KT>(kv)));
 }
 
 template <int DH>
