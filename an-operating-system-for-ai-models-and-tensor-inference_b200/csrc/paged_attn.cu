@@ -568,8 +568,9 @@ MYOS_DEV void advance(const PagedAttnArgs& a, int heads, Cursor* c) {
 
 // The meeting of several blocks costs about as much as kJoinTiles tiles (2 us),
 // and each of its parts (0.06 us) about a sixth of one: an item of L tiles is
-// soonest done in sqrt(kPartsPerTile * L) shares.
-constexpr int kJoinTiles = 5, kPartsPerTile = 6;
+// soonest done in sqrt(kPartsPerTile * L) shares. A second piece in a share
+// costs kPieceTiles.
+constexpr int kJoinTiles = 5, kPartsPerTile = 6, kPieceTiles = 4;
 
 // The parts of one split item: shares first .. last. All but the first share
 // begin inside the item, so their part is their first piece (slot 0); the
@@ -724,22 +725,32 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<DH>)
     longest = max(longest, longs[w]);
   }
   total *= heads;
-  // n shares, none of them empty; or one for each item, where that is sooner done
+  // n equal shares, none of them empty; or each item in k of its own, where its
+  // longest is not much longer than an equal share
   const uint32_t items = (uint32_t)a.nseq * heads;
   const uint32_t best = items * sqrtf(kPartsPerTile * ((float)total / items));
   const uint32_t n = max(1u, min(min(gridDim.x, total), best));
   Shares shares;
   shares.cut(total, n);
-  const bool by_item = items <= gridDim.x && (uint32_t)longest <= shares.each + kJoinTiles;
-  uint32_t lo = 0, hi = 0;
+  const bool alone = (uint32_t)longest <= shares.each + kJoinTiles;
+  const uint32_t k = alone ? 1u : max(1u, n / items);
+  const bool by_item = items <= gridDim.x &&
+                       (alone || ((uint32_t)longest + k - 1) / k <= shares.each + kPieceTiles);
+  uint32_t lo = 0, hi = 0, first = 0, last = 0;  // and the item's shares, by item
   Cursor ahead;
   if (by_item) {
-    if (me >= items) return;
-    ahead.b = me / heads;
-    ahead.h = me - ahead.b * heads;
+    const uint32_t item = me / k, at = me - item * k;
+    if (item >= items) return;
+    ahead.b = item / heads;
+    ahead.h = item - ahead.b * heads;
     span_of<T>(a, ahead.b, &ahead);
-    ahead.t = ahead.t0;
-    hi = ahead.t1 - ahead.t0;
+    const uint32_t tiles = ahead.t1 - ahead.t0, cuts = min(k, tiles);
+    if (at >= cuts) return;
+    lo = at * tiles / cuts;
+    hi = (at + 1) * tiles / cuts;
+    ahead.t = ahead.t0 + lo;
+    first = item * k;
+    last = first + cuts - 1;
   } else {
     if (me < n) {
       lo = shares.begin(me);
@@ -868,9 +879,9 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<DH>)
         if (warp == 0) w.put_lse(a.lse ? a.lse + (int64_t)c.b * a.hq + head : nullptr, G);
       } else {
         Split sp;
-        sp.first = (int)shares.of(i0);
-        sp.last = (int)shares.of(i1 - 1);
-        sp.second = i0 >= shares.begin(sp.first);
+        sp.first = (int)(by_item ? first : shares.of(i0));
+        sp.last = (int)(by_item ? last : shares.of(i1 - 1));
+        sp.second = !by_item && i0 >= shares.begin(sp.first);
         sp.b = c.b;
         sp.h = c.h;
         float* part = part_of<DH>(a.parts, sp, (int)me);
