@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
       if (hashed) {
 #pragma unroll 1
         for (int k = tid; k < listed; k += kThreads)
-          enter(list[k].x & ~kSeen, list[k].x & kSeen, list[k].y);
+          enter((list[k].x & ~kSeen) - (uint32_t)base, list[k].x & kSeen, list[k].y);
       } else {
         all_of_row([&](int32_t id, uint32_t flag, uint32_t e) {
           const int l = place(id);
@@ -426,10 +426,10 @@ extern "C" int myos_dev_logit_controls(float* d_out, size_t out_stride, const fl
     if ((words & 3) != 0) return MYOS_ERR_ARG;
     if (!c->history && (c->repetition || c->frequency || c->presence)) return MYOS_ERR_ARG;
     if (c->bias_starts && (!c->bias_ids || !c->bias_vals)) return MYOS_ERR_ARG;
-    if (c->history && (c->history_width > 0x7fffffff || c->history_stride < c->history_width ||
+    if (c->history && (c->history_width > 0x40000000 || c->history_stride < c->history_width ||
                        c->history_stride > ((uint64_t)1 << 40)))
       return MYOS_ERR_SHAPE;
-    if (c->num_bias > 0x7fffffff) return MYOS_ERR_SHAPE;
+    if (c->num_bias > 0x40000000) return MYOS_ERR_SHAPE;
     if (c->mask && (c->mask_stride < (vocab + 31) / 32 || c->mask_stride > ((uint64_t)1 << 40) ||
                     c->num_masks > 0x7fffffff || (!c->mask_rows && c->num_masks < rows)))
       return MYOS_ERR_SHAPE;

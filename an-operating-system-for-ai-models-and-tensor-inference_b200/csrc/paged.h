@@ -48,6 +48,7 @@ inline cudaError_t raise_smem_limit(const void* kernel, size_t bytes, std::atomi
   if (bit && (done->load(std::memory_order_acquire) & bit)) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e == cudaSuccess) done->fetch_or(bit, std::memory_order_release);
+  else cudaGetLastError();
   return e;
 }
 
@@ -74,7 +75,9 @@ inline cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, size
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   }
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) cudaGetLastError();  // reported here, not by a later call
+  return e;
 }
 
 // Multiprocessors of the current device (148 where it cannot be asked).

@@ -521,7 +521,10 @@ def check_ids(out, ids):
 
 @pytest.mark.parametrize("rows,vocab,width,nbias", [
     (1, 1, 1, 1), (1, 151936, 300, 0), (3, 152064, 500, 40), (5, 8192, 64, 9), (4, 8193, 700, 9),
-    (70, 1001, 33, 5), (2, 33, 0, 0), (300, 97, 50, 3), (2, 262147, 2000, 100)])
+    (70, 1001, 33, 5), (2, 33, 0, 0), (300, 97, 50, 3), (2, 262147, 2000, 100),
+    (250, 70001, 40, 3),     # a block's ids in several passes
+    (2, 5003, 20000, 9),     # more tokens than the table has room for: chunk by chunk
+    (3, 9001, 50, 4000)])    # more biases
 @pytest.mark.parametrize("strided", [False, True])
 def test_logits(dev, rows, vocab, width, nbias, strided):
     rng = np.random.default_rng(rows + vocab)

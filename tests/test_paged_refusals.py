@@ -70,6 +70,7 @@ def test_a_cache_out_of_form_is_refused(over, code):
     (dict(q_stride=128), _lib.ERR_SHAPE), (dict(out_stride=128), _lib.ERR_SHAPE),
     (dict(max_blocks=0), _lib.ERR_SHAPE), (dict(table_stride=7), _lib.ERR_SHAPE),
     (dict(max_blocks=1 << 30, table_stride=1 << 30), _lib.ERR_SHAPE),
+    (dict(max_blocks=1 << 20, table_stride=1 << 20, nseq=4096), _lib.ERR_SHAPE),  # 2^32 tiles of 32 keys
     (dict(q=BASE + 4), _lib.ERR_ARG), (dict(out=BASE + 8), _lib.ERR_ARG),
     (dict(q_stride=12 * 128 + 2), _lib.ERR_ARG), (dict(lens=BASE + 2), _lib.ERR_ARG),
     (dict(work=BASE + 4), _lib.ERR_ARG),
@@ -144,6 +145,8 @@ def logits(c=None, **over):
     (None, dict(out=BASE + (1 << 30), out_stride=1004), _lib.ERR_ARG),
     (dict(repetition=BASE), {}, _lib.ERR_ARG),   # penalties without a history
     (dict(history=BASE, history_width=8, history_stride=7), {}, _lib.ERR_SHAPE),
+    (dict(history=BASE, history_width=1 << 31, history_stride=1 << 31), {}, _lib.ERR_SHAPE),
+    (dict(bias_starts=BASE, bias_ids=BASE, bias_vals=BASE, num_bias=1 << 31), {}, _lib.ERR_SHAPE),
     (dict(bias_starts=BASE), {}, _lib.ERR_ARG),
     (dict(bias_starts=BASE + 1, bias_ids=BASE, bias_vals=BASE), {}, _lib.ERR_ARG),
     (dict(mask=BASE, mask_stride=31, num_masks=4), {}, _lib.ERR_SHAPE),
@@ -158,6 +161,12 @@ def test_no_rows_is_no_work():
     assert store(rows=0, q=None) == _lib.OK
     assert tables(nseq=0, table=None) == _lib.OK
     assert logits(rows=0, x=None) == _lib.OK
+
+
+@pytest.mark.skipif(os.path.exists("/dev/nvidiactl") or os.path.exists("/dev/nvidia0"), reason="no-GPU behaviour")
+def test_no_gpu_is_an_error():
+    for st in (attn(), store(), tables(), logits()):
+        assert st == _lib.ERR_CUDA
 
 
 def test_python_layer_refuses_host_tensors():
