@@ -29,11 +29,14 @@ struct LogitArgs {
 // number, and the whole history is looked through for each. The blocks' best ids
 // meet in the first block's shared memory.
 //
-// What this replaces: tables of one word an id, chunk by chunk, with the
-// penalties in the pass over all ids, 59 instructions an id (64 rows of 152064:
-// 52 us), and with the touched ids computed before that pass from lists, 40
-// instructions (39 us): zeroing and reading the tables and looking through the
-// lists for every chunk cost more than the pass.
+// Everything before the pass is latency (row parameters, tokens, table), so it
+// is kept off the memory's back: the table is cleared before the launch's
+// dependency, the first tokens and logits and the mask are on their way while
+// the row's lengths come. 64 rows of 152064 with every control (79 MB): 27 us;
+// with tables of one word an id, chunk by chunk, and the penalties in the pass
+// over all ids 52 us (59 instructions an id, nearly every warp went through the
+// divisions), with the touched ids computed before that pass 39 us. The pass
+// itself, without controls, takes 19 us; 12 us is the memory's share.
 constexpr int kMaxCluster = 8;
 constexpr int kMaxChunk = 65536, kRun = 128, kRunWords = kRun / 32 + 1;
 static_assert(kRunWords <= 8);
@@ -58,7 +61,7 @@ MYOS_DEV void better(float& v, int& i, float ov, int oi) {
 }
 
 template <int kThreads>
-__global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) {
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(const LogitArgs a) {
   extern __shared__ __align__(16) uint32_t tables[];
   __shared__ float best_v[32];
   __shared__ int best_i[32];
@@ -70,10 +73,33 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
   if (a.ids && ranks > 1)  // the first block's memory is written to below: it has to have started
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  pdl_launch();
-  pdl_wait();
   const int64_t row = blockIdx.x / ranks;
   const myos_logit_controls_args& c = a.c;
+  // the chunk's touched ids, a bit each; the table: an id's place among the
+  // block's, the history's word, 1 + its last bias entry; the mask's words; the
+  // list; the slots in use
+  const uint32_t slots = a.slots;
+  uint32_t* key = tables;
+  uint32_t* word = key + slots;
+  uint32_t* bias = word + slots;
+  uint32_t* bits = bias + slots;
+  uint32_t* mask_s = bits + (slots ? a.chunk / 32 : 0);
+  uint2* list = reinterpret_cast<uint2*>(mask_s + (c.mask ? (a.chunk / kRun * kRunWords + 2) & ~1 : 0));
+  uint16_t* used = reinterpret_cast<uint16_t*>(list + a.room);
+  auto clear_tables = [&]() {
+    const uint4 none = make_uint4(0, 0, 0, 0), no_id = make_uint4(kNoId, kNoId, kNoId, kNoId);
+#pragma unroll 1
+    for (int k = tid; k < (int)slots / 4; k += kThreads) reinterpret_cast<uint4*>(key)[k] = no_id;
+    // word, bias and bits lie behind one another
+#pragma unroll 1
+    for (int k = tid; k < (int)slots / 2 + a.chunk / 128; k += kThreads)
+      reinterpret_cast<uint4*>(word)[k] = none;
+    if (tid == 0) in_use = 0;
+  };
+  if (slots) clear_tables();
+  if (tid == 0) listed = 0;
+  pdl_launch();
+  pdl_wait();
   const float* x = a.logits + row * a.logits_stride;
   float* y = a.out ? a.out + row * a.out_stride : nullptr;
   // Ids count from `shift` on, so that groups of four lie on 16 bytes of x.
@@ -82,7 +108,14 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
 
   int hist = 0, prompt = 0;
   float rep = 1.f, freq = 0.f, pres = 0.f;
+  const int32_t* said = c.history + row * (int64_t)c.history_stride;
+  // the row's first tokens on their way before its length is known
+  constexpr int kBatch = 4;
+  int32_t early[kBatch];
   if (c.history && (c.repetition || c.frequency || c.presence)) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      early[k] = tid + k * kThreads < (int)c.history_width ? said[tid + k * kThreads] : -1;
     hist = (int)c.history_width;
     if (c.history_lens) hist = min(hist, max(c.history_lens[row], 0));
     if (c.prompt_lens) prompt = c.prompt_lens[row];
@@ -90,7 +123,6 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
     if (c.frequency) freq = c.frequency[row];
     if (c.presence) pres = c.presence[row];
   }
-  const int32_t* said = c.history + row * (int64_t)c.history_stride;
   int e0 = 0, e1 = 0;
   if (c.bias_starts) {
     e0 = min(max(c.bias_starts[row], 0), (int)c.num_bias);
@@ -102,17 +134,6 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
     const int64_t g = c.mask_rows ? c.mask_rows[row] : row;
     if (g >= 0 && g < (int64_t)c.num_masks) mask = c.mask + g * (int64_t)c.mask_stride;
   }
-  // the chunk's touched ids, a bit each; the table: an id's place among the
-  // block's, the history's word, 1 + its last bias entry; the slots in use
-  const uint32_t slots = a.slots;
-  uint32_t* key = tables;
-  uint32_t* word = key + slots;
-  uint32_t* bias = word + slots;
-  uint32_t* bits = bias + slots;
-  uint32_t* mask_s = bits + (slots ? a.chunk / 32 : 0);
-  uint2* list = reinterpret_cast<uint2*>(mask_s + (c.mask ? (a.chunk / kRun * kRunWords + 2) & ~1 : 0));
-  uint16_t* used = reinterpret_cast<uint16_t*>(list + a.room);
-
   // The block's ids: place l is id (l / kRun * ranks + rank) * kRun + l % kRun - shift.
   const uint32_t log_ranks = __ffs(ranks) - 1;
   const int runs = (a.vocab + shift + kRun - 1) / kRun;
@@ -142,28 +163,44 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
   };
   // All tokens f(id, kSeen or 0, 0) and biases f(id, 0, 1 + entry) of the row,
   // whole warps at a time (id -1: none).
-  constexpr int kBatch = 4;
   const int warp_at = tid & ~31;
+  bool fresh = true;  // `early` still holds the first tokens
   auto all_of_row = [&](auto&& f) {
 #pragma unroll 1
     for (int i0 = warp_at; i0 < hist; i0 += kBatch * kThreads) {
-      int32_t id[kBatch];
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         const int i = i0 + lane + k * kThreads;
-        id[k] = i < hist ? said[i] : -1;
+        if (i0 > warp_at || !fresh) early[k] = i < hist ? said[i] : -1;
       }
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k)
-        f(id[k], i0 + lane + k * kThreads < prompt ? kSeen : 0u, 0u);
+      for (int k = 0; k < kBatch; ++k) {
+        const int i = i0 + lane + k * kThreads;
+        f(i < hist ? early[k] : -1, i < prompt ? kSeen : 0u, 0u);
+      }
     }
 #pragma unroll 1
     for (int e = e0 + warp_at; e < e1; e += kThreads)
       f(e + lane < e1 ? c.bias_ids[e + lane] : -1, 0u, (uint32_t)(e + lane - e0 + 1));
   };
+  // The pass: a thread's next kUnroll groups are always on their way, the first
+  // ones while the row's tokens are listed and sorted.
+  constexpr int kUnroll = 2;
+  static_assert(4 * kThreads % kRun == 0);
+  const int far = (4 * kThreads) << log_ranks;  // ids from a thread's group to its next
+  float4 v[kUnroll];
+  auto fetch = [&](float4& to, int l, int i, int n) {
+    if ((uint32_t)i < whole && l < n) to = *reinterpret_cast<const float4*>(x + i);
+  };
+  auto fetch_first = [&](int base, int n) {
+    const int i0 = id_at(base + 4 * tid);
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) fetch(v[k], 4 * (tid + k * kThreads), i0 + k * far, n);
+  };
+  fetch_first(0, min(a.chunk, places));
+
   bool hashed = true;
   if (touched) {
-    if (tid == 0) listed = 0;
     __syncthreads();
     all_of_row([&](int32_t id, uint32_t flag, uint32_t e) {
       const int l = place(id);
@@ -176,12 +213,18 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
     });
     __syncthreads();
     hashed = listed <= a.room;
+    fresh = false;
   }
   const int step = hashed ? a.chunk : min(a.chunk, (int)slots & ~(kRun - 1));
 #pragma unroll 1
   for (int base = 0; base < places; base += step) {
     const int n = min(step, places - base);
-    if (base > 0) __syncthreads();
+    if (base > 0) {
+      __syncthreads();
+      fetch_first(base, n);
+    } else if (step < a.chunk) {
+      fetch_first(0, n);  // a shorter pass than was taken for granted
+    }
     if (mask) {
       // the mask's words of each run, from the one with its first id on; that id
       // is the word's bit -shift % 32 in every run
@@ -189,20 +232,19 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
 #pragma unroll 1
       for (int k = tid; k < n / kRun * 8; k += kThreads) {  // eight threads a run
         const int at = k & 7, w = (id_at(base + (k >> 3) * kRun) >> 5) + at;  // -1: before the row
+        const bool in = (uint32_t)w < (uint32_t)all;
         if (at < kRunWords)
-          mask_s[(k >> 3) * kRunWords + at] = (uint32_t)w < (uint32_t)all ? mask[w] : 0u;
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                           smem_u32(mask_s + (k >> 3) * kRunWords + at)),
+                       "l"(mask + (in ? w : 0)), "r"(in ? 4 : 0)
+                       : "memory");
       }
     }
     if (touched) {
-      const uint4 none = make_uint4(0, 0, 0, 0), no_id = make_uint4(kNoId, kNoId, kNoId, kNoId);
-#pragma unroll 1
-      for (int k = tid; k < (int)slots / 4; k += kThreads) reinterpret_cast<uint4*>(key)[k] = no_id;
-      // word, bias and bits lie behind one another
-#pragma unroll 1
-      for (int k = tid; k < (int)slots / 2 + a.chunk / 128; k += kThreads)
-        reinterpret_cast<uint4*>(word)[k] = none;
-      if (tid == 0) in_use = 0;
-      __syncthreads();
+      if (base > 0) {
+        clear_tables();
+        __syncthreads();
+      }
       // a token (kSeen or 0: of the prompt or the output) or a bias entry of place l
       auto enter = [&](uint32_t l, uint32_t flag, uint32_t e) {
         if (l >= (uint32_t)n) return;
@@ -233,6 +275,7 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
         });
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (touched || mask) __syncthreads();
     // the mask's bits from place l on, at least four of them
     const int lead = -shift & 31;
@@ -242,26 +285,18 @@ __global__ void __launch_bounds__(kThreads) k_logit_controls(const LogitArgs a) 
       return __funnelshift_r(w[0], w[1], at & 31);  // a run's last word is not needed at its end
     };
 
-    constexpr int kUnroll = 4;
-    static_assert(4 * kThreads % kRun == 0);
-    const int far = (4 * kThreads) << log_ranks;  // from a thread's group to its next
+    int i0 = id_at(base + 4 * tid);
 #pragma unroll 1
-    for (int l0 = 4 * tid; l0 < n; l0 += 4 * kUnroll * kThreads) {
-      const int i0 = id_at(base + l0);
-      float4 v[kUnroll];
-#pragma unroll
-      for (int k = 0; k < kUnroll; ++k) {
-        const int i = i0 + k * far;
-        if ((uint32_t)i < whole && l0 + 4 * k * kThreads < n)
-          v[k] = *reinterpret_cast<const float4*>(x + i);
-      }
+    for (int l0 = 4 * tid; l0 < n; l0 += 4 * kUnroll * kThreads, i0 += kUnroll * far) {
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
         const int l = l0 + 4 * k * kThreads, i = i0 + k * far;
-        if (l >= n) break;
+        const float4 now = v[k];
+        fetch(v[k], l + 4 * kUnroll * kThreads, i + kUnroll * far, n);
+        if (l >= n) continue;
         const uint32_t b4 = touched ? bits[l >> 5] >> (l & 31) & 15u : 0u;  // l: a multiple of 4
         if ((uint32_t)i < whole) {
-          float r[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          float r[4] = {now.x, now.y, now.z, now.w};
           if (mask) {
             const uint32_t m = allowed(l);
 #pragma unroll
@@ -435,9 +470,10 @@ extern "C" int myos_dev_logit_controls(float* d_out, size_t out_stride, const fl
       return MYOS_ERR_SHAPE;
     a.c = *c;
   }
-  // Few rows: larger blocks, each through its ids in one or two rounds of loads
-  // (12 rows of 151936: 9.5 us against 12 us in blocks of 512).
-  const cudaError_t e = rows * kMaxCluster <= (size_t)sm_count()
+  // Few rows: larger blocks, as long as their clusters are placed at once, a
+  // block to a multiprocessor (with 18 rows they are not: 18.2 us of 151936 ids,
+  // against 9.8 us for 12 rows and 13.3 us for 24 in blocks of 512).
+  const cudaError_t e = rows * kMaxCluster <= (size_t)sm_count() * 7 / 8
                             ? launch_controls<1024>(a, rows, (cudaStream_t)stream)
                             : launch_controls<512>(a, rows, (cudaStream_t)stream);
   return e == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
