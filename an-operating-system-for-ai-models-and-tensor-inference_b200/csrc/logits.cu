@@ -471,9 +471,9 @@ extern "C" int myos_dev_logit_controls(float* d_out, size_t out_stride, const fl
     a.c = *c;
   }
   // Few rows: larger blocks, as long as their clusters are placed at once, a
-  // block to a multiprocessor (with 18 rows they are not: 18.2 us of 151936 ids,
-  // against 9.8 us for 12 rows and 13.3 us for 24 in blocks of 512).
-  const cudaError_t e = rows * kMaxCluster <= (size_t)sm_count() * 7 / 8
+  // block to a multiprocessor (with 16 rows they are not: 17.4 us of 151936 ids,
+  // against 9.8 us for 12 rows and 12.7 us for 18 in blocks of 512).
+  const cudaError_t e = rows * kMaxCluster <= (size_t)sm_count() * 2 / 3
                             ? launch_controls<1024>(a, rows, (cudaStream_t)stream)
                             : launch_controls<512>(a, rows, (cudaStream_t)stream);
   return e == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
