@@ -239,8 +239,9 @@ __global__ void __launch_bounds__(1024) k_paged_tables(const TablesArgs a) {
 // lane's cosines and sines serve all the heads it comes to, and its loads of
 // kHeads heads are in flight together; of few rows, several blocks take one.
 // Bound by memory: 16001 rows of 40/8 heads of 128 with norms into a bf16 cache
-// take 154 us, 5.6 TB/s (4 heads in flight: 167 us, fewer blocks fit; one head a
-// time over all rows' heads in turn: 205 us).
+// (860 MB) take 139 us, 6.2 TB/s, 0.94 of a copy. Full occupancy carries it, 16
+// blocks of 128 (14: 148 us; 8 of 256: 147 us; with a row's position loaded in
+// its own turn 156 us; 4 heads in flight, fewer blocks: 167 us).
 struct StoreArgs {
   float* q;
   const float* qkv;
@@ -284,7 +285,7 @@ MYOS_DEV float rot_hi(float x, float y, float c, float s) {
   return __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
 }
 
-constexpr int kStoreThreads = 256;
+constexpr int kStoreThreads = 128;
 
 template <class KT, int kHeads>
 __global__ void __launch_bounds__(kStoreThreads) k_paged_store(const StoreArgs a, const PagedKv<KT> kv) {
@@ -299,13 +300,19 @@ __global__ void __launch_bounds__(kStoreThreads) k_paged_store(const StoreArgs a
   const bool norm = a.q_gamma || a.k_gamma;
   pdl_launch();
   pdl_wait();
+  // a row's slot and position are loaded a row ahead: its cosines need them first
+  int64_t next_slot = a.slots[blockIdx.x];
+  int next_pos = a.rot > 0 ? a.positions[blockIdx.x] : 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float* src = a.qkv + row * a.qkv_stride;
-    const int64_t slot = a.slots[row];
+    const int64_t slot = next_slot, pos = next_pos;
+    if (row + gridDim.x < a.rows) {
+      next_slot = a.slots[row + gridDim.x];
+      if (a.rot > 0) next_pos = a.positions[row + gridDim.x];
+    }
     float4 cs = make_float4(0.f, 0.f, 0.f, 0.f), sn = cs;
     bool placed = true;
     if (a.rot > 0) {
-      const int64_t pos = a.positions[row];
       placed = pos >= 0 && pos < a.num_pos;
       if (placed && turn && on) {
         cs = *reinterpret_cast<const float4*>(a.cos_t + pos * (a.rot / 2) + c0);
@@ -374,7 +381,7 @@ __global__ void __launch_bounds__(kStoreThreads) k_paged_store(const StoreArgs a
 
 template <class KT>
 cudaError_t launch_store(const StoreArgs& a, const myos_paged_kv* kv, cudaStream_t st) {
-  constexpr int kResident = 8;  // blocks a multiprocessor
+  constexpr int kResident = 16;  // blocks a multiprocessor
   const int64_t most = (int64_t)sm_count() * kResident;
   const int per = kStoreThreads >> a.lanes_log2;
   const int parts = (a.hq + 2 * (int)kv->num_kv_heads + per - 1) / per;
