@@ -203,6 +203,45 @@ def test_attention_far_into_a_large_cache(dev):
     check_attention(out, lse, plain_attention(q.double().cpu().numpy(), ks, ks, d**-0.5, kept(lens)))
 
 
+def test_attention_of_many_short_sequences(dev):
+    """More sequences than a block has threads, many of them empty."""
+    rng = np.random.default_rng(12)
+    torch.manual_seed(12)
+    hq, hkv, d, page, n = 2, 2, 64, 4, 3000
+    lens = rng.integers(0, 6, n) * (rng.random(n) < 0.7)
+    k, v = cache(rng, int((-(-lens // page)).sum()) + 1, hkv, page, d, "bf16")
+    table, ks, vs = fill_cache(rng, k, v, lens.tolist(), page)
+    q = torch.randn(n, hq, d, device="cuda")
+    out, lse = attend(dev, q, dev.PagedKV(k, v), i32(table), i32(lens))
+    check_attention(out, lse, plain_attention(q.double().cpu().numpy(), ks, vs, d**-0.5, kept(lens.tolist())))
+
+
+def test_attention_on_two_streams_at_once(dev):
+    """Calls that run at the same time, each with a work buffer of its own."""
+    rng = np.random.default_rng(13)
+    torch.manual_seed(13)
+    hq, hkv, d, page = 12, 2, 128, 16
+    lens = [[4000, 300, 1], [2500, 2501, 17]]
+    sets = []
+    for n in lens:
+        k, v = cache(rng, sum(-(-m // page) for m in n), hkv, page, d, "bf16")
+        table, ks, vs = fill_cache(rng, k, v, n, page)
+        q = torch.randn(3, hq, d, device="cuda")
+        work = torch.zeros(dev.WORK_BYTES, dtype=torch.uint8, device="cuda")
+        want = plain_attention(q.double().cpu().numpy(), ks, vs, d**-0.5, kept(n))
+        sets.append((q, dev.PagedKV(k, v), i32(table), i32(n), work, want, torch.cuda.Stream()))
+    outs = [torch.zeros(50, 3, hq, d, device="cuda") for _ in sets]
+    torch.cuda.synchronize()
+    for i in range(50):
+        for (q, kv, table, n, work, _, st), o in zip(sets, outs):
+            dev.paged_attention(o[i], q, kv, table, n, work, stream=st)
+    torch.cuda.synchronize()
+    for (q, kv, table, n, work, want, st), o in zip(sets, outs):
+        assert (np.abs(o[0].double().cpu().numpy() - want[0]) <= want[2]).all()
+        assert (o.view(torch.int32) == o[0].view(torch.int32)).all()
+        assert not work[: 16 * 1024].any()  # the arrival counts are back at zero
+
+
 def test_attention_extremes(dev):
     """Scores far apart (one key takes all the weight) and large equal ones."""
     hq, hkv, d, page = 8, 1, 64, 16
@@ -597,6 +636,21 @@ def test_logits_parts_alone(dev):
     with pytest.raises(myos.MyosError) as e:
         dev.logit_controls(out, t, mask=torch.zeros(3, 15, dtype=torch.int32, device="cuda"))
     assert e.value.code == _lib.ERR_SHAPE
+
+
+def test_logits_rows_far_apart(dev):
+    """Rows more than 2^31 elements apart."""
+    rng = np.random.default_rng(4)
+    far, vocab = (1 << 31) + 64, 1000
+    buf = torch.empty(far + vocab, device="cuda")
+    x = buf.as_strided((2, vocab), (far, 1))
+    host = rng.standard_normal((2, vocab)).astype(np.float32)
+    x.copy_(torch.from_numpy(host).cuda())
+    hist, ids = rng.integers(0, vocab, (2, 30)), torch.zeros(2, dtype=torch.int32, device="cuda")
+    f = torch.tensor([0.5, 0.25], device="cuda")
+    dev.logit_controls(x, x, history=i32(hist), presence=f, ids=ids)
+    want, tol = plain_logits(host, hist, [0, 0], [30, 30], None, None, f.cpu().numpy(), [[], []], None)
+    check_logits(x, ids, want, tol)
 
 
 @pytest.mark.parametrize("vocab", [5, 40000])
