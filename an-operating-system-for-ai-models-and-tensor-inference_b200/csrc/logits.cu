@@ -109,12 +109,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
   int hist = 0, prompt = 0;
   float rep = 1.f, freq = 0.f, pres = 0.f;
   const int32_t* said = c.history + row * (int64_t)c.history_stride;
-  // the row's first tokens on their way before its length is known
-  constexpr int kBatch = 4;
-  int32_t early[kBatch];
+  // the row's first 4096 tokens on their way before its length is known
+  constexpr int kEarly = 4096 / kThreads;
+  int32_t early[kEarly];
   if (c.history && (c.repetition || c.frequency || c.presence)) {
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k)
+    for (int k = 0; k < kEarly; ++k)
       early[k] = tid + k * kThreads < (int)c.history_width ? said[tid + k * kThreads] : -1;
     hist = (int)c.history_width;
     if (c.history_lens) hist = min(hist, max(c.history_lens[row], 0));
@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
     e0 = min(max(c.bias_starts[row], 0), (int)c.num_bias);
     e1 = min(max(c.bias_starts[row + 1], 0), (int)c.num_bias);
   }
+  const int32_t early_bias = e0 + tid < e1 ? c.bias_ids[e0 + tid] : -1;
   const bool touched = hist > 0 || e1 > e0;
   const uint32_t* mask = nullptr;
   if (c.mask) {
@@ -161,26 +162,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
     const bool ours = (uint32_t)id < (uint32_t)a.vocab && (run & (ranks - 1)) == rank;
     return ours ? (int)((run >> log_ranks) * kRun + t % kRun) : -1;
   };
-  // All tokens f(id, kSeen or 0, 0) and biases f(id, 0, 1 + entry) of the row,
-  // whole warps at a time (id -1: none).
+  // The row's tokens from i0 on f(id, kSeen or 0, 0) and biases from entry b0 on
+  // f(id, 0, 1 + entry), whole warps at a time (id -1: none).
   const int warp_at = tid & ~31;
-  bool fresh = true;  // `early` still holds the first tokens
-  auto all_of_row = [&](auto&& f) {
+  auto rest_of_row = [&](int i0, int b0, auto&& f) {
 #pragma unroll 1
-    for (int i0 = warp_at; i0 < hist; i0 += kBatch * kThreads) {
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int i = i0 + lane + k * kThreads;
-        if (i0 > warp_at || !fresh) early[k] = i < hist ? said[i] : -1;
-      }
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int i = i0 + lane + k * kThreads;
-        f(i < hist ? early[k] : -1, i < prompt ? kSeen : 0u, 0u);
-      }
-    }
+    for (int i = i0 + warp_at; i < hist; i += kThreads)
+      f(i + lane < hist ? said[i + lane] : -1, i + lane < prompt ? kSeen : 0u, 0u);
 #pragma unroll 1
-    for (int e = e0 + warp_at; e < e1; e += kThreads)
+    for (int e = e0 + b0 + warp_at; e < e1; e += kThreads)
       f(e + lane < e1 ? c.bias_ids[e + lane] : -1, 0u, (uint32_t)(e + lane - e0 + 1));
   };
   // The pass: a thread's next kUnroll groups are always on their way, the first
@@ -202,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
   bool hashed = true;
   if (touched) {
     __syncthreads();
-    all_of_row([&](int32_t id, uint32_t flag, uint32_t e) {
+    auto note = [&](int32_t id, uint32_t flag, uint32_t e) {
       const int l = place(id);
       const uint32_t who = __ballot_sync(0xffffffffu, l >= 0);
       if (who == 0) return;
@@ -210,10 +200,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
       if (lane == 0) at = atomicAdd(&listed, __popc(who));
       at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
       if (l >= 0 && at < a.room) list[at] = make_uint2((uint32_t)l | flag, e);
-    });
+    };
+#pragma unroll
+    for (int k = 0; k < kEarly; ++k) {
+      const int i = tid + k * kThreads;
+      if (k * kThreads < hist) note(i < hist ? early[k] : -1, i < prompt ? kSeen : 0u, 0u);
+    }
+    if (e1 > e0) note(early_bias, 0u, (uint32_t)(tid + 1));
+    rest_of_row(kEarly * kThreads, kThreads, note);
     __syncthreads();
     hashed = listed <= a.room;
-    fresh = false;
   }
   const int step = hashed ? a.chunk : min(a.chunk, (int)slots & ~(kRun - 1));
 #pragma unroll 1
@@ -245,33 +241,42 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
         clear_tables();
         __syncthreads();
       }
-      // a token (kSeen or 0: of the prompt or the output) or a bias entry of place l
+      // a token (kSeen or 0: of the prompt or the output) or a bias entry of place
+      // l, or none (l from n on); a whole warp at a time
       auto enter = [&](uint32_t l, uint32_t flag, uint32_t e) {
-        if (l >= (uint32_t)n) return;
-        uint32_t h = hashed ? __umulhi(l * 2654435761u, slots) : l;
-        for (;;) {
-          const uint32_t was = atomicCAS(&key[h], kNoId, l);
-          if (was == kNoId) {
-            atomicOr(&bits[l >> 5], 1u << (l & 31));
-            used[atomicAdd(&in_use, 1)] = (uint16_t)h;
-            break;
+        uint32_t h = 0;
+        bool fresh_slot = false;
+        if (l < (uint32_t)n) {
+          h = hashed ? __umulhi(l * 2654435761u, slots) : l;
+          for (;;) {
+            const uint32_t was = atomicCAS(&key[h], kNoId, l);
+            fresh_slot = was == kNoId;
+            if (fresh_slot || was == l) break;
+            if (++h == slots) h = 0;
           }
-          if (was == l) break;
-          if (++h == slots) h = 0;
+          // the last entry of an id counts: entries leave their number, the largest stays
+          if (e) atomicMax(&bias[h], e);
+          else if (flag) atomicOr(&word[h], kSeen);
+          else atomicAdd(&word[h], 1u);
+          if (fresh_slot) atomicOr(&bits[l >> 5], 1u << (l & 31));
         }
-        // the last entry of an id counts: entries leave their number, the largest stays
-        if (e) atomicMax(&bias[h], e);
-        else if (flag) atomicOr(&word[h], kSeen);
-        else atomicAdd(&word[h], 1u);
+        const uint32_t who = __ballot_sync(0xffffffffu, fresh_slot);
+        if (who == 0) return;
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&in_use, __popc(who));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+        if (fresh_slot) used[at] = (uint16_t)h;
       };
       if (hashed) {
 #pragma unroll 1
-        for (int k = tid; k < listed; k += kThreads)
-          enter((list[k].x & ~kSeen) - (uint32_t)base, list[k].x & kSeen, list[k].y);
+        for (int k = warp_at; k < listed; k += kThreads) {
+          const uint2 t = k + lane < listed ? list[k + lane] : make_uint2(kNoId, 0u);
+          enter(t.x == kNoId ? kNoId : (t.x & ~kSeen) - (uint32_t)base, t.x & kSeen, t.y);
+        }
       } else {
-        all_of_row([&](int32_t id, uint32_t flag, uint32_t e) {
+        rest_of_row(0, 0, [&](int32_t id, uint32_t flag, uint32_t e) {
           const int l = place(id);
-          if (l >= base) enter((uint32_t)(l - base), flag, e);
+          enter(l >= base ? (uint32_t)(l - base) : kNoId, flag, e);
         });
       }
     }
