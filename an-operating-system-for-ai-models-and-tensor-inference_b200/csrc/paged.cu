@@ -55,7 +55,8 @@ namespace {
 // or two rows (decode) is written by the thread that scanned it, which has
 // looked its last page up meanwhile; the rows of longer ones find their request
 // by a binary search. What is left is latency: two loads on one another
-// (lengths, then pages), one barrier, the stores.
+// (lengths, then pages), one barrier, the stores. A new page's first slot is a
+// row of the step, and that row writes the page's table entry.
 struct TablesArgs {
   int32_t* table;
   int64_t table_stride;
@@ -171,10 +172,10 @@ __global__ void __launch_bounds__(1024) k_paged_tables(const TablesArgs a) {
         row(r, b, 0, 0, -1);
         continue;
       }
-      const uint32_t pos = ctx + (r - start), pg = pos / P;
+      const uint32_t pos = ctx + (r - start), pg = pos / P, in = pos - pg * P;
       const int32_t page = look && pg == ctx / P ? last : page_of(b, pg, held, first);
-      if (pg >= held && pos % P == 0) a.table[b * a.table_stride + pg] = page;
-      row(r, b, pos, pos - pg * P, page);
+      if (pg >= held && in == 0) a.table[b * a.table_stride + pg] = page;
+      row(r, b, pos, in, page);
     }
   }
   if (blockIdx.x == 0) {
@@ -199,17 +200,6 @@ __global__ void __launch_bounds__(1024) k_paged_tables(const TablesArgs a) {
   }
   const int rows = (int)min(before.rows, (int64_t)a.max_rows);
   if (longer) {
-    // new table entries, a warp for each request
-#pragma unroll 1
-    for (int b = warp * gridDim.x + blockIdx.x; b < a.nseq; b += gridDim.x * nwarps) {
-      const Span sp = spans[b];
-      if (!(sp.ctx & kLong) || sp.first < 0) continue;
-      const uint32_t ctx = sp.ctx & ~kLong, add = a.add[b];
-      const uint32_t held = ceil_div(ctx, P), need = ceil_div(ctx + add, P) - held;
-#pragma unroll 1
-      for (uint32_t j = lane; j < need; j += 32)
-        a.table[b * a.table_stride + held + j] = a.free_pages[nfree - 1 - sp.first - (int)j];
-    }
     // rows: of the last request that begins at or before the row
 #pragma unroll 2
     for (int r = blockIdx.x * blockDim.x + threadIdx.x; r < rows; r += gridDim.x * blockDim.x) {
@@ -222,8 +212,14 @@ __global__ void __launch_bounds__(1024) k_paged_tables(const TablesArgs a) {
       const Span sp = spans[lo];
       if (!(sp.ctx & kLong)) continue;
       const uint32_t ctx = sp.ctx & ~kLong, pos = ctx + (r - sp.start), pg = pos / P;
-      if (sp.first < 0) row(r, lo, 0, 0, -1);
-      else row(r, lo, pos, pos - pg * P, page_of(lo, pg, ceil_div(ctx, P), sp.first));
+      if (sp.first < 0) {
+        row(r, lo, 0, 0, -1);
+        continue;
+      }
+      const uint32_t held = ceil_div(ctx, P), in = pos - pg * P;
+      const int32_t page = page_of(lo, pg, held, sp.first);
+      if (pg >= held && in == 0) a.table[lo * a.table_stride + pg] = page;
+      row(r, lo, pos, in, page);
     }
   }
   // rows behind the last request's
