@@ -129,6 +129,8 @@ ATTN = [
     (28, 4, 128, 16, "f32", [1000, 1, 65], 1, False),   # a window of the newest key alone
     (32, 4, 64, 16, "bf16", [640] * 70, 0, False),      # more sequences than SMs / heads
     (16, 2, 128, 16, "bf16", [5000], 0, False),         # one long sequence over many blocks
+    (12, 2, 128, 16, "bf16", [700, 650, 690, 10] * 3, 0, False),  # several shares an item, some left empty
+    (4, 2, 256, 16, "f32", [300, 290, 280], 0, False),
     (2, 1, 64, 512, "bf16", [70001, 3], 0, False),
     (2, 2, 64, 512, "f32", [70001, 3], 50000, True),
 ]
