@@ -32,7 +32,7 @@ struct LogitArgs {
 // Everything before the pass is latency (row parameters, tokens, table), so it
 // is kept off the memory's back: the table is cleared before the launch's
 // dependency, the first tokens and logits and the mask are on their way while
-// the row's lengths come. 64 rows of 152064 with every control (79 MB): 27 us;
+// the row's lengths come. 64 rows of 152064 with every control (79 MB): 26 us;
 // with tables of one word an id, chunk by chunk, and the penalties in the pass
 // over all ids 52 us (59 instructions an id, nearly every warp went through the
 // divisions), with the touched ids computed before that pass 39 us. The pass

@@ -235,9 +235,11 @@ __global__ void __launch_bounds__(1024) k_paged_tables(const TablesArgs a) {
 // lane's cosines and sines serve all the heads it comes to, and its loads of
 // kHeads heads are in flight together; of few rows, several blocks take one.
 // Bound by memory: 16001 rows of 40/8 heads of 128 with norms into a bf16 cache
-// (860 MB) take 139 us, 6.2 TB/s, 0.94 of a copy. Full occupancy carries it, 16
-// blocks of 128 (14: 148 us; 8 of 256: 147 us; with a row's position loaded in
-// its own turn 156 us; 4 heads in flight, fewer blocks: 167 us).
+// (860 MB) take 139 us, 6.2 TB/s, 0.94 of a copy. Its 63 registers a thread let 8
+// blocks of 128 reside; the grid is twice that, 16 a multiprocessor (14: 148 us,
+// 32: 142 us; blocks of 256: 147 us). Registers capped for 10 or 12 resident
+// blocks: 154 and 187 us; a row's position loaded in its own turn: 156 us; 4
+// heads in flight: 167 us.
 struct StoreArgs {
   float* q;
   const float* qkv;
