@@ -779,8 +779,10 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<DH>)
       span_of<T>(a, ahead.b, &ahead);
       const uint32_t tiles = ahead.t1 - ahead.t0, cuts = min(k, tiles);
       if (at < cuts) {
-        lo = at * tiles / cuts;
-        hi = (at + 1) * tiles / cuts;
+        Shares own;  // at * tiles may pass 32 bits
+        own.cut(tiles, cuts);
+        lo = own.begin(at);
+        hi = own.begin(at + 1);
         ahead.t = ahead.t0 + lo;
         member = at % group;
         members = min(group, cuts - (at - member));

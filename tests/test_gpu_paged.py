@@ -205,6 +205,34 @@ def test_attention_far_into_a_large_cache(dev):
     check_attention(out, lse, plain_attention(q.double().cpu().numpy(), ks, ks, d**-0.5, kept(lens)))
 
 
+def test_attention_over_more_tiles_than_a_product_of_32_bits_holds(dev):
+    """592 shares of 7.5 million tiles: three pages, over and over in the table.
+
+    A share's warp adds up one part of 8 keys of about 7.5e6 / 592 tiles, one
+    rounding (a whole step at most, in the tensor core) each, and one for each
+    share that is joined: (12670 + 592 + 64) 2 U of the sum of the weights, and
+    of that of the weighted values.
+    """
+    torch.manual_seed(14)
+    d, page, blocks = 8, 1024, 234375
+    k, v = (torch.randn(3, 1, page, d, device="cuda") for _ in range(2))
+    q = torch.randn(1, 2, d, device="cuda")
+    order = np.arange(blocks) % 3
+    n = blocks * page - 100
+    out, lse = attend(dev, q, dev.PagedKV(k, v), i32(order[None]), i32([n]))
+    times = np.bincount(order, minlength=3)[:, None] * np.ones((3, page))
+    times[order[-1], page - 100 :] -= 1
+    w = times.reshape(-1)
+    k64, v64 = (x.double().cpu().numpy().reshape(-1, d) for x in (k, v))
+    s = q[0].double().cpu().numpy() @ k64.T * d**-0.5
+    e = w * np.exp(s - s.max(1, keepdims=True))
+    want = e @ v64 / e.sum(1, keepdims=True)
+    tol = (12670 + 592 + 64) * 2 * U
+    most = e @ np.abs(v64) / e.sum(1, keepdims=True)
+    assert (np.abs(out[0].double().cpu().numpy() - want) <= tol * (most + np.abs(want)) * 1.01).all()
+    assert (np.abs(lse[0].double().cpu().numpy() - np.log(e.sum(1)) - s.max(1)) <= tol * 1.01 + 1e-5).all()
+
+
 def test_attention_of_many_short_sequences(dev):
     """More sequences than a block has threads, many of them empty."""
     rng = np.random.default_rng(12)
