@@ -179,15 +179,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
   static_assert(4 * kThreads % kRun == 0);
   const int far = (4 * kThreads) << log_ranks;  // ids from a thread's group to its next
   float4 v[kUnroll];
-  auto fetch = [&](float4& to, int l, int i, int n) {
-    if ((uint32_t)i < whole && l < n) to = *reinterpret_cast<const float4*>(x + i);
+  auto fetch = [&](float4& to, int i) {  // of the row, if not of this chunk
+    if ((uint32_t)i < whole) to = *reinterpret_cast<const float4*>(x + i);
   };
-  auto fetch_first = [&](int base, int n) {
+  auto fetch_first = [&](int base) {
     const int i0 = id_at(base + 4 * tid);
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) fetch(v[k], 4 * (tid + k * kThreads), i0 + k * far, n);
+    for (int k = 0; k < kUnroll; ++k) fetch(v[k], i0 + k * far);
   };
-  fetch_first(0, min(a.chunk, places));
+  fetch_first(0);
 
   bool hashed = true;
   if (touched) {
@@ -217,9 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
     const int n = min(step, places - base);
     if (base > 0) {
       __syncthreads();
-      fetch_first(base, n);
-    } else if (step < a.chunk) {
-      fetch_first(0, n);  // a shorter pass than was taken for granted
+      fetch_first(base);
     }
     if (mask) {
       // the mask's words of each run, from the one with its first id on; that id
@@ -290,20 +288,26 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
       return __funnelshift_r(w[0], w[1], at & 31);  // a run's last word is not needed at its end
     };
 
-    int i0 = id_at(base + 4 * tid);
+    // A warp's groups are one run of ids, so a thread's place in its run, and with
+    // it the bits' position in their words, is the same in all its groups.
+    static_assert(kRun == 4 * 32);
+    int i = id_at(base + 4 * tid);
+    const uint32_t* bits_at = bits + (tid >> 3);
+    const uint32_t* mask_at = mask_s + (tid >> 5) * kRunWords + ((4 * lane + lead) >> 5);
+    const int bit = 4 * tid & 31, mask_bit = (4 * lane + lead) & 31;
 #pragma unroll 1
-    for (int l0 = 4 * tid; l0 < n; l0 += 4 * kUnroll * kThreads, i0 += kUnroll * far) {
+    for (int l0 = 4 * tid; l0 < n; l0 += 4 * kUnroll * kThreads) {
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
-        const int l = l0 + 4 * k * kThreads, i = i0 + k * far;
+        if (k > 0 && l0 + 4 * k * kThreads >= n) break;
         const float4 now = v[k];
-        fetch(v[k], l + 4 * kUnroll * kThreads, i + kUnroll * far, n);
-        if (l >= n) continue;
-        const uint32_t b4 = touched ? bits[l >> 5] >> (l & 31) & 15u : 0u;  // l: a multiple of 4
+        fetch(v[k], i + kUnroll * far);
+        const uint32_t b4 = touched ? bits_at[k * (kThreads / 8)] >> bit & 15u : 0u;
         if ((uint32_t)i < whole) {
           float r[4] = {now.x, now.y, now.z, now.w};
           if (mask) {
-            const uint32_t m = allowed(l);
+            const uint32_t* w = mask_at + k * (kThreads / 32 * kRunWords);
+            const uint32_t m = __funnelshift_r(w[0], w[1], mask_bit);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               if (!(m >> j & 1u)) r[j] = -INFINITY;
@@ -334,12 +338,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
             const int id = i + j;
             if ((uint32_t)id >= (uint32_t)a.vocab) continue;
             float r = x[id];
-            if (mask && !(allowed(l + j) & 1u)) r = -INFINITY;
+            if (mask && !(allowed(l0 + 4 * k * kThreads + j) & 1u)) r = -INFINITY;
             if (y) y[id] = r;
             if (!(b4 >> j & 1u)) take(r, id);
           }
         }
+        i += far;
       }
+      bits_at += kUnroll * (kThreads / 8);
+      mask_at += kUnroll * (kThreads / 32 * kRunWords);
     }
     if (!touched) continue;
     __syncthreads();
