@@ -1,6 +1,7 @@
 // Logits under the requests' controls (penalties for repeated tokens, biases,
 // grammar masks) and the greedy id.
 #include "common.cuh"
+#include "cp_async.cuh"
 #include "kernels.h"
 #include "paged.h"
 
@@ -32,7 +33,7 @@ struct LogitArgs {
 // Everything before the pass is latency (row parameters, tokens, table), so it
 // is kept off the memory's back: the table is cleared before the launch's
 // dependency, the first tokens and logits and the mask are on their way while
-// the row's lengths come. 64 rows of 152064 with every control (79 MB): 26 us;
+// the row's lengths come. 64 rows of 152064 with every control (79 MB): 24 us;
 // with tables of one word an id, chunk by chunk, and the penalties in the pass
 // over all ids 52 us (59 instructions an id, nearly every warp went through the
 // divisions), with the touched ids computed before that pass 39 us. The pass
@@ -60,7 +61,7 @@ MYOS_DEV void better(float& v, int& i, float ov, int oi) {
   }
 }
 
-template <int kThreads>
+template <int kThreads, int kDepth, int kUnroll>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(const LogitArgs a) {
   extern __shared__ __align__(16) uint32_t tables[];
   __shared__ float best_v[32];
@@ -79,7 +80,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
   // block's, the history's word, 1 + its last bias entry; the mask's words; the
   // list; the slots in use
   const uint32_t slots = a.slots;
-  uint32_t* key = tables;
+  float4* ring = reinterpret_cast<float4*>(tables) + tid;  // slot t at t * kThreads
+  uint32_t* key = tables + kDepth * kThreads * 4;
   uint32_t* word = key + slots;
   uint32_t* bias = word + slots;
   uint32_t* bits = bias + slots;
@@ -173,21 +175,31 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
     for (int e = e0 + b0 + warp_at; e < e1; e += kThreads)
       f(e + lane < e1 ? c.bias_ids[e + lane] : -1, 0u, (uint32_t)(e + lane - e0 + 1));
   };
-  // The pass: a thread's next kUnroll groups are always on their way, the first
-  // ones while the row's tokens are listed and sorted.
-  constexpr int kUnroll = 2;
-  static_assert(4 * kThreads % kRun == 0);
+  // The pass: a thread's next kAhead groups are always on their way, to its own
+  // slots of the ring (long slices) or to registers (kDepth 0), the first ones
+  // while the row's tokens are listed and sorted. With four slots 64 rows of
+  // 152064 take 23.5 us, with registers for two 25.6; 128 of 151936 36.6 and 38.9;
+  // 333 of 32003 29.7 and 33.8. Of few groups the ring's extra steps cost more than
+  // its depth gives: 16 rows of 151936 (9 groups a thread) 11.9 and 11.3 us.
+  constexpr int kAhead = kDepth > 0 ? kDepth : kUnroll;
+  static_assert(4 * kThreads % kRun == 0 && kAhead % kUnroll == 0);
   const int far = (4 * kThreads) << log_ranks;  // ids from a thread's group to its next
   float4 v[kUnroll];
-  auto fetch = [&](float4& to, int i) {  // of the row, if not of this chunk
-    if ((uint32_t)i < whole) to = *reinterpret_cast<const float4*>(x + i);
+  auto fetch = [&](int at, int l, int i, int n) {
+    const bool in = l < n && (uint32_t)i < whole;
+    if constexpr (kDepth > 0) {
+      if (in) cp_async16(smem_u32(ring + at * kThreads), x + i, true);
+      cp_commit();
+    } else {
+      if (in) v[at] = *reinterpret_cast<const float4*>(x + i);
+    }
   };
-  auto fetch_first = [&](int base) {
+  auto fetch_first = [&](int base, int n) {
     const int i0 = id_at(base + 4 * tid);
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) fetch(v[k], i0 + k * far);
+    for (int t = 0; t < kAhead; ++t) fetch(t, 4 * (tid + t * kThreads), i0 + t * far, n);
   };
-  fetch_first(0);
+  fetch_first(0, min(a.chunk, places));
 
   bool hashed = true;
   if (touched) {
@@ -217,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
     const int n = min(step, places - base);
     if (base > 0) {
       __syncthreads();
-      fetch_first(base);
+      fetch_first(base, n);
     }
     if (mask) {
       // the mask's words of each run, from the one with its first id on; that id
@@ -295,13 +307,21 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
     const uint32_t* bits_at = bits + (tid >> 3);
     const uint32_t* mask_at = mask_s + (tid >> 5) * kRunWords + ((4 * lane + lead) >> 5);
     const int bit = 4 * tid & 31, mask_bit = (4 * lane + lead) & 31;
+    int slot = 0;
 #pragma unroll 1
     for (int l0 = 4 * tid; l0 < n; l0 += 4 * kUnroll * kThreads) {
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
-        if (k > 0 && l0 + 4 * k * kThreads >= n) break;
-        const float4 now = v[k];
-        fetch(v[k], i + kUnroll * far);
+        const int l = l0 + 4 * k * kThreads;
+        if (k > 0 && l >= n) break;
+        float4 now;
+        if constexpr (kDepth > 0) {
+          cp_wait<kDepth - 1>();
+          now = ring[(slot + k) * kThreads];
+        } else {
+          now = v[k];
+          fetch(k, l + 4 * kAhead * kThreads, i + kAhead * far, n);
+        }
         const uint32_t b4 = touched ? bits_at[k * (kThreads / 8)] >> bit & 15u : 0u;
         if ((uint32_t)i < whole) {
           float r[4] = {now.x, now.y, now.z, now.w};
@@ -338,13 +358,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
             const int id = i + j;
             if ((uint32_t)id >= (uint32_t)a.vocab) continue;
             float r = x[id];
-            if (mask && !(allowed(l0 + 4 * k * kThreads + j) & 1u)) r = -INFINITY;
+            if (mask && !(allowed(l + j) & 1u)) r = -INFINITY;
             if (y) y[id] = r;
             if (!(b4 >> j & 1u)) take(r, id);
           }
         }
+        if constexpr (kDepth > 0)  // into the slot that has been read
+          fetch(slot + k, l + 4 * kAhead * kThreads, i + kAhead * far, n);
         i += far;
       }
+      slot = slot + kUnroll < kAhead ? slot + kUnroll : 0;
       bits_at += kUnroll * (kThreads / 8);
       mask_at += kUnroll * (kThreads / 32 * kRunWords);
     }
@@ -403,25 +426,31 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
   if (tid == 0) a.ids[row] = bv == -INFINITY ? 0u : (uint32_t)bi;
 }
 
+// As many blocks a row as are resident at once, with 2048 ids at least.
 template <int kThreads>
-cudaError_t launch_controls(LogitArgs a, size_t rows, cudaStream_t st) {
-  // As many blocks a row as are resident at once, with 2048 ids at least
+int cluster_of(const LogitArgs& a, size_t rows) {
   int cluster = kMaxCluster;
   while (cluster > 1 &&
          (rows * cluster > (size_t)sm_count() * 1024 / kThreads || a.vocab / cluster < 2048))
     cluster /= 2;
+  return cluster;
+}
+
+template <int kThreads, int kDepth, int kUnroll>
+cudaError_t launch_controls(LogitArgs a, size_t rows, int cluster, cudaStream_t st) {
   const int most = ((a.vocab + 3 + kRun - 1) / kRun + cluster - 1) / cluster * kRun;
   const int passes = (most + kMaxChunk - 1) / kMaxChunk;
   a.chunk = ((most / kRun + passes - 1) / passes) * kRun;
   const bool pen = a.c.history && (a.c.repetition || a.c.frequency || a.c.presence);
-  // a table for three times a block's share of the longest history and of the mean
-  // number of biases, and four slots for five entries
+  // a list for three times (beside a ring, so that two blocks fit a multiprocessor,
+  // twice) a block's share of the longest history and of the mean number of biases,
+  // and five slots of the table for four of its entries
   size_t share = 0;
   if (pen) share += a.c.history_width;
   if (a.c.bias_starts) share += a.c.num_bias / rows + 32;
   constexpr size_t kLeastRoom = 512, kMostRoom = 5120;
   static_assert(kLeastRoom * 5 / 4 >= kRun && kMostRoom * 5 / 4 <= 65536);
-  size_t room = share == 0 ? 0 : 3 * share / cluster;
+  size_t room = share == 0 ? 0 : (kDepth > 0 ? 2 : 3) * share / cluster;
   if (room > kMostRoom) room = kMostRoom;
   if (room > 0 && room < kLeastRoom) room = kLeastRoom;
   room = (room + 15) & ~(size_t)15;
@@ -429,15 +458,15 @@ cudaError_t launch_controls(LogitArgs a, size_t rows, cudaStream_t st) {
   a.slots = (int)(room + room / 4);
   const auto bytes = [](size_t chunk, size_t room, bool mask) {
     return (room ? chunk / 8 : 0) + (mask ? 4 * (chunk / kRun * kRunWords + 2) : 0) +
-           14 * (room + room / 4) + 8 * room;
+           14 * (room + room / 4) + 8 * room + 16 * kDepth * kThreads;
   };
   const size_t smem = bytes(a.chunk, room, a.c.mask);
   static std::atomic<uint64_t> raised{0};
-  const cudaError_t e = raise_smem_limit((const void*)k_logit_controls<kThreads>,
+  const cudaError_t e = raise_smem_limit((const void*)k_logit_controls<kThreads, kDepth, kUnroll>,
                                          bytes(kMaxChunk, kMostRoom, true), &raised);
   if (e != cudaSuccess) return e;
-  return counted(launch_pdl(k_logit_controls<kThreads>, dim3((unsigned)(rows * cluster)), kThreads,
-                            smem, st, cluster, a));
+  return counted(launch_pdl(k_logit_controls<kThreads, kDepth, kUnroll>,
+                            dim3((unsigned)(rows * cluster)), kThreads, smem, st, cluster, a));
 }
 
 }  // namespace
@@ -485,8 +514,15 @@ extern "C" int myos_dev_logit_controls(float* d_out, size_t out_stride, const fl
   // Few rows: larger blocks, as long as their clusters are placed at once, a
   // block to a multiprocessor (with 16 rows they are not: 17.4 us of 151936 ids,
   // against 9.8 us for 12 rows and 12.7 us for 18 in blocks of 512).
-  const cudaError_t e = rows * kMaxCluster <= (size_t)sm_count() * 2 / 3
-                            ? launch_controls<1024>(a, rows, (cudaStream_t)stream)
-                            : launch_controls<512>(a, rows, (cudaStream_t)stream);
+  // One group a thread and turn there: 12 rows 8.5 us, two groups 8.9 us.
+  const cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e;
+  if (rows * kMaxCluster <= (size_t)sm_count() * 2 / 3) {
+    e = launch_controls<1024, 0, 1>(a, rows, cluster_of<1024>(a, rows), st);
+  } else {
+    const int cluster = cluster_of<512>(a, rows);
+    e = a.vocab / cluster >= 12 * 4 * 512 ? launch_controls<512, 4, 2>(a, rows, cluster, st)
+                                          : launch_controls<512, 0, 2>(a, rows, cluster, st);
+  }
   return e == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
 }

@@ -20,6 +20,7 @@
 // eight rows: a lane stays with one or two rows of a tile, and all its
 // addresses are one base each and constants.
 #include "common.cuh"
+#include "cp_async.cuh"
 #include "kernels.h"
 #include "paged.h"
 
@@ -47,17 +48,6 @@ struct PagedAttnArgs {
   unsigned* arrived;  // [shares], zero between launches
   float* parts;       // [shares][2][8 * DH + 16]
 };
-
-MYOS_DEV void cp_async16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(on ? 16 : 0)
-               : "memory");
-}
-MYOS_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-MYOS_DEV void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 MYOS_DEV void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"

@@ -668,6 +668,37 @@ def test_logits_parts_alone(dev):
     assert e.value.code == _lib.ERR_SHAPE
 
 
+@pytest.mark.parametrize("rows,vocab,width,most,nbias", [
+    (64, 100003, 3000, 90, 5),   # a row's tokens all in one run of ids: chunk by chunk in one of its blocks
+    (160, 30011, 200, 30011, 3000),  # one row with nearly all the biases
+    (333, 24577, 1, 24577, 0), (75, 60000, 0, 1, 0)])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_logits_of_long_slices(dev, rows, vocab, width, most, nbias, pad):
+    rng = np.random.default_rng(rows + vocab)
+    buf = torch.from_numpy(rng.standard_normal((rows, vocab + pad)).astype(np.float32) * 5).cuda()
+    logits, x = buf[:, pad:], buf[:, pad:].cpu().numpy()
+    hist, hlen = rng.integers(0, most, (rows, max(width, 1))), [width] * rows
+    plen = rng.integers(0, width + 1, rows)
+    rep, freq, pres = (rng.uniform(a, b, rows).astype(np.float32) for a, b in ((0.8, 1.6), (-0.5, 0.7), (0, 0.9)))
+    bias = [[(int(t), 1.5) for t in rng.permutation(vocab)[: nbias if r == 1 else min(nbias, 3)]] for r in range(rows)]
+    bits = rng.random((rows, vocab)) < 0.7
+    words = np.packbits(np.pad(bits, ((0, 0), (0, -vocab % 32))), axis=1, bitorder="little").view(np.int32)
+    f = lambda a: torch.from_numpy(np.asarray(a, np.float32)).cuda()  # noqa: E731
+    flat = [e for b in bias for e in b] + [(0, 0.0)]
+    args = dict(history=i32(hist), prompt_lens=i32(plen), hist_lens=i32(hlen), repetition=f(rep), frequency=f(freq),
+                presence=f(pres), bias_starts=i32(np.cumsum([0] + [len(b) for b in bias])),
+                bias_ids=i32([t for t, _ in flat]), bias_vals=f([b for _, b in flat]),
+                mask=torch.from_numpy(words).cuda())
+    want, tol = plain_logits(x, hist, plen, hlen, rep, freq, pres, bias, list(bits))
+    out, ids = torch.full((rows, vocab), 3.0, device="cuda"), torch.zeros(rows, dtype=torch.int32, device="cuda")
+    dev.logit_controls(out, logits, ids=ids, **args)
+    check_logits(out, ids, want, tol)
+    ends = buf[:, :pad].clone()
+    again = torch.zeros_like(ids)
+    dev.logit_controls(logits, logits, ids=again, **args)  # in place
+    assert torch.equal(logits, out) and torch.equal(again, ids) and torch.equal(buf[:, :pad], ends)
+
+
 def test_logits_rows_far_apart(dev):
     """Rows more than 2^31 elements apart."""
     rng = np.random.default_rng(4)
