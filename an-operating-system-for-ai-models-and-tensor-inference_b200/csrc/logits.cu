@@ -37,7 +37,7 @@ struct LogitArgs {
 // with tables of one word an id, chunk by chunk, and the penalties in the pass
 // over all ids 52 us (59 instructions an id, nearly every warp went through the
 // divisions), with the touched ids computed before that pass 39 us. The pass
-// itself, without controls, takes 19 us; 12 us is the memory's share.
+// itself, without controls, takes 18.5 us; 12 us is the memory's share.
 constexpr int kMaxCluster = 8;
 constexpr int kMaxChunk = 65536, kRun = 128, kRunWords = kRun / 32 + 1;
 static_assert(kRunWords <= 8);
@@ -512,9 +512,9 @@ extern "C" int myos_dev_logit_controls(float* d_out, size_t out_stride, const fl
     a.c = *c;
   }
   // Few rows: larger blocks, as long as their clusters are placed at once, a
-  // block to a multiprocessor (with 16 rows they are not: 17.4 us of 151936 ids,
-  // against 9.8 us for 12 rows and 12.7 us for 18 in blocks of 512).
-  // One group a thread and turn there: 12 rows 8.5 us, two groups 8.9 us.
+  // block to a multiprocessor (with 16 rows of 151936 they are not: 17.4 us, in
+  // blocks of 512 12.1, before the pass's later steps). 12 rows take 8.6 us with one
+  // group a thread and turn, with two 8.9.
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   if (rows * kMaxCluster <= (size_t)sm_count() * 2 / 3) {
