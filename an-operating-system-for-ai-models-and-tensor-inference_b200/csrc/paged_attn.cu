@@ -300,22 +300,38 @@ struct Bf16Warp : WarpState<DH> {
   using KT = __nv_bfloat16;
   using WarpState<DH>::o;
   static constexpr int kKeys = 16, kSteps = DH / 16;
-  static constexpr bool kLate = DH > 128;  // queries split at each use: registers
-  Split3 q[kLate ? 1 : kSteps][2];
-  float2 raw[kLate ? kSteps : 1][2];
+  // The queries' terms: in registers, or (kShared, longer heads) for all warps in
+  // the swap space, which is free while the tiles go by (16 x 8192 keys of 16/4
+  // heads of 256: 111 us, f32 206; split again for each tile 120 and 236).
+  static constexpr bool kShared = DH > 128;
+  static constexpr int kRoom = kShared ? kSteps * 32 * 24 : 0;
+  Split3 q[kShared ? 1 : kSteps][2];
+  const uint32_t* room;
 
-  MYOS_DEV void begin(const float* q_row, int G, int d) {
+  MYOS_DEV void begin(const float* q_row, int G, int d, float* swap) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = (lane & 3) * 2;
+    auto load = [&](int at) -> Split3 {
+      float2 x = make_float2(0.f, 0.f);
+      if (g < G && at < d) x = *reinterpret_cast<const float2*>(q_row + g * d + at);
+      return split3(x.x, x.y);
+    };
+    if constexpr (kShared) {
+      uint32_t* to = reinterpret_cast<uint32_t*>(swap);
+      room = to;
+      __syncthreads();  // the states of the piece before have been read
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int at = 16 * k + 8 * u + c;
-        float2 x = make_float2(0.f, 0.f);
-        if (g < G && at < d) x = *reinterpret_cast<const float2*>(q_row + g * d + at);
-        if constexpr (kLate) raw[k][u] = x;
-        else q[k][u] = split3(x.x, x.y);
+      for (int k = threadIdx.x >> 5; k < kSteps; k += kWarps) {
+        const Split3 q0 = load(16 * k + c), q1 = load(16 * k + 8 + c);
+        reinterpret_cast<uint4*>(to)[k * 32 + lane] = make_uint4(q0.hi, q0.mid, q1.hi, q1.mid);
+        reinterpret_cast<uint2*>(to + kSteps * 128)[k * 32 + lane] = make_uint2(q0.lo, q1.lo);
       }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) q[k][u] = load(16 * k + 8 * u + c);
+    }
     this->clear();
   }
 
@@ -340,9 +356,11 @@ struct Bf16Warp : WarpState<DH> {
         uint32_t b[4];
         ldmatrix4(b, (base ^ ((2 * k & 6) << 4)) + (k >> 2) * 128);
         Split3 q0, q1;
-        if constexpr (kLate) {
-          q0 = split3(raw[k][0].x, raw[k][0].y);
-          q1 = split3(raw[k][1].x, raw[k][1].y);
+        if constexpr (kShared) {
+          const uint4 h = reinterpret_cast<const uint4*>(room)[k * 32 + lane];
+          const uint2 l = reinterpret_cast<const uint2*>(room + kSteps * 128)[k * 32 + lane];
+          q0 = Split3{h.x, h.y, l.x};
+          q1 = Split3{h.z, h.w, l.y};
         } else {
           q0 = q[k][0];
           q1 = q[k][1];
@@ -417,9 +435,10 @@ struct F32Warp : WarpState<DH> {
   using KT = float;
   using WarpState<DH>::o;
   static constexpr int kKeys = 8, kChunks = DH / 16;
-  static constexpr bool kLate = DH > 128;
-  uint32_t q[kLate ? 1 : kChunks][8];
-  float4 raw[kLate ? kChunks : 1];
+  static constexpr bool kShared = DH > 128;  // as above
+  static constexpr int kRoom = kShared ? kChunks * 32 * 32 : 0;
+  uint32_t q[kShared ? 1 : kChunks][8];
+  const uint32_t* room;
 
   static MYOS_DEV void split_q(const float4& x, uint32_t (&y)[8]) {
     split2(x.x, y[0], y[1]);
@@ -427,15 +446,28 @@ struct F32Warp : WarpState<DH> {
     split2(x.z, y[4], y[5]);
     split2(x.w, y[6], y[7]);
   }
-  MYOS_DEV void begin(const float* q_row, int G, int d) {
+  MYOS_DEV void begin(const float* q_row, int G, int d, float* swap) {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-#pragma unroll
-    for (int k = 0; k < kChunks; ++k) {
-      const int at = 16 * k + 4 * c;
+    auto load = [&](int at, uint32_t (&y)[8]) {
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (g < G && at < d) x = *reinterpret_cast<const float4*>(q_row + g * d + at);
-      if constexpr (kLate) raw[k] = x;
-      else split_q(x, q[k]);
+      split_q(x, y);
+    };
+    if constexpr (kShared) {
+      uint4* to = reinterpret_cast<uint4*>(swap);
+      room = reinterpret_cast<const uint32_t*>(swap);
+      __syncthreads();  // the states of the piece before have been read
+#pragma unroll
+      for (int k = threadIdx.x >> 5; k < kChunks; k += kWarps) {
+        uint32_t y[8];
+        load(16 * k + 4 * c, y);
+        to[k * 64 + lane] = make_uint4(y[0], y[1], y[2], y[3]);
+        to[k * 64 + 32 + lane] = make_uint4(y[4], y[5], y[6], y[7]);
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) load(16 * k + 4 * c, q[k]);
     }
     this->clear();
   }
@@ -465,8 +497,11 @@ struct F32Warp : WarpState<DH> {
         lds4(x, (base ^ ((4 * k & 4) << 4)) + (k >> 1) * 128);
         uint32_t y[8], qs[8];
         split_q(x, y);
-        if constexpr (kLate) {
-          split_q(raw[k], qs);
+        if constexpr (kShared) {
+          const uint4 l = reinterpret_cast<const uint4*>(room)[k * 64 + lane];
+          const uint4 h = reinterpret_cast<const uint4*>(room)[k * 64 + 32 + lane];
+          qs[0] = l.x, qs[1] = l.y, qs[2] = l.z, qs[3] = l.w;
+          qs[4] = h.x, qs[5] = h.y, qs[6] = h.z, qs[7] = h.w;
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) qs[i] = q[k][i];
@@ -662,6 +697,7 @@ __device__ __noinline__ void join_parts(const float* parts, const Split ps, floa
 
 template <class W, int DH>
 constexpr size_t attn_smem() {
+  static_assert(W::kRoom <= (kWarps - 1) * W::kRegs * 32 * 4);  // in the swap space
   return (size_t)kStages * kWarps * 2 * W::kKeys * DH * sizeof(typename W::KT) +
          (kWarps - 1) * W::kRegs * 32 * 4;
 }
@@ -889,7 +925,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<DH>)
     // one piece: the tiles of item (c.b, c.h) from c.t on in this share
     const uint32_t i0 = i - (c.t - c.t0), i1 = i0 + (c.t1 - c.t0);
     W w;
-    w.begin(a.q + c.b * a.q_stride + (int64_t)c.h * G * d, G, d);
+    w.begin(a.q + c.b * a.q_stride + (int64_t)c.h * G * d, G, d, swap);
 #pragma unroll 1
     for (const uint32_t end = min(hi, i1); i < end; ++i) {
       cp_wait<kStages - 2>();

@@ -186,6 +186,14 @@ def test_attention_of_strided_rows_and_bad_pages(dev, kvt):
     torch.testing.assert_close(b[1], b[0], rtol=1e-5, atol=1e-5)
 
 
+@pytest.mark.parametrize("kvt", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [136, 192, 256])
+@pytest.mark.parametrize("lens", [[2500] + [30, 0, 41, 7] * 30, [400] * 40, [900, 3]], ids=["pieces", "items", "few"])
+def test_attention_of_long_heads(dev, kvt, d, lens):
+    """Heads past 128 dims: shares of many pieces, whole items, a few long ones."""
+    test_attention(dev, (10, 2, d, 16, kvt, lens, 0, False))
+
+
 def test_attention_far_into_a_large_cache(dev):
     """Element offsets past 32 bits: the pages lie behind 2^32 elements."""
     rng = np.random.default_rng(6)
