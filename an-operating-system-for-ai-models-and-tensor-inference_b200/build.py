@@ -45,7 +45,7 @@ CUDA_SOURCES = ["kernels.cu", "engine.cu", "ops.cu", "noalloc.cu",
                 "prefill.cu", "gemm_sm100.cu", "paged.cu", "paged_attn.cu", "logits.cu",
                 "safetensors.cpp", "tp.cpp"]
 HEADERS = ["common.cuh", "cp_async.cuh", "kernels.h", "safetensors.h", "prefill.h",
-           "gemm_sm100.h", "paged.h", "tp.h"]
+           "gemm_sm100.h", "logits_plan.h", "paged.h", "tp.h"]
 
 
 def nvcc() -> str:

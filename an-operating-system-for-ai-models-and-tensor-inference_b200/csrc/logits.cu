@@ -3,6 +3,7 @@
 #include "common.cuh"
 #include "cp_async.cuh"
 #include "kernels.h"
+#include "logits_plan.h"
 #include "paged.h"
 
 namespace myos {
@@ -38,9 +39,6 @@ struct LogitArgs {
 // over all ids 52 us (59 instructions an id, nearly every warp went through the
 // divisions), with the touched ids computed before that pass 39 us. The pass
 // itself, without controls, takes 18.5 us; 12 us is the memory's share.
-constexpr int kMaxCluster = 8;
-constexpr int kMaxChunk = 65536, kRun = 128, kRunWords = kRun / 32 + 1;
-static_assert(kRunWords <= 8);
 constexpr uint32_t kSeen = 0x80000000u;  // in the prompt; the low bits count the output
 constexpr uint32_t kNoId = 0xffffffffu;
 
@@ -131,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
     e1 = min(max(c.bias_starts[row + 1], 0), (int)c.num_bias);
   }
   const int32_t early_bias = e0 + tid < e1 ? c.bias_ids[e0 + tid] : -1;
-  const bool touched = hist > 0 || e1 > e0;
+  const bool touched = slots > 0 && (hist > 0 || e1 > e0);  // the plan has slots for either
   const uint32_t* mask = nullptr;
   if (c.mask) {
     const int64_t g = c.mask_rows ? c.mask_rows[row] : row;
@@ -223,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
     __syncthreads();
     hashed = listed <= a.room;
   }
-  const int step = hashed ? a.chunk : min(a.chunk, (int)slots & ~(kRun - 1));
+  const int step = logit_step(hashed, a.chunk, (int)slots);
 #pragma unroll 1
   for (int base = 0; base < places; base += step) {
     const int n = min(step, places - base);
@@ -426,47 +424,22 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) k_logit_controls(co
   if (tid == 0) a.ids[row] = bv == -INFINITY ? 0u : (uint32_t)bi;
 }
 
-// As many blocks a row as are resident at once, with 2048 ids at least.
-template <int kThreads>
-int cluster_of(const LogitArgs& a, size_t rows) {
-  int cluster = kMaxCluster;
-  while (cluster > 1 &&
-         (rows * cluster > (size_t)sm_count() * 1024 / kThreads || a.vocab / cluster < 2048))
-    cluster /= 2;
-  return cluster;
-}
-
 template <int kThreads, int kDepth, int kUnroll>
 cudaError_t launch_controls(LogitArgs a, size_t rows, int cluster, cudaStream_t st) {
-  const int most = ((a.vocab + 3 + kRun - 1) / kRun + cluster - 1) / cluster * kRun;
-  const int passes = (most + kMaxChunk - 1) / kMaxChunk;
-  a.chunk = ((most / kRun + passes - 1) / passes) * kRun;
   const bool pen = a.c.history && (a.c.repetition || a.c.frequency || a.c.presence);
-  // a list for three times (beside a ring, so that two blocks fit a multiprocessor,
-  // twice) a block's share of the longest history and of the mean number of biases,
-  // and five slots of the table for four of its entries
-  size_t share = 0;
-  if (pen) share += a.c.history_width;
-  if (a.c.bias_starts) share += a.c.num_bias / rows + 32;
-  constexpr size_t kLeastRoom = 512, kMostRoom = 5120;
-  static_assert(kLeastRoom * 5 / 4 >= kRun && kMostRoom * 5 / 4 <= 65536);
-  size_t room = share == 0 ? 0 : (kDepth > 0 ? 2 : 3) * share / cluster;
-  if (room > kMostRoom) room = kMostRoom;
-  if (room > 0 && room < kLeastRoom) room = kLeastRoom;
-  room = (room + 15) & ~(size_t)15;
-  a.room = (int)room;
-  a.slots = (int)(room + room / 4);
-  const auto bytes = [](size_t chunk, size_t room, bool mask) {
-    return (room ? chunk / 8 : 0) + (mask ? 4 * (chunk / kRun * kRunWords + 2) : 0) +
-           14 * (room + room / 4) + 8 * room + 16 * kDepth * kThreads;
-  };
-  const size_t smem = bytes(a.chunk, room, a.c.mask);
+  const LogitPlan p = logit_plan(kThreads, kDepth, cluster, a.vocab, rows,
+                                 pen ? a.c.history_width : 0, a.c.bias_starts != nullptr,
+                                 a.c.num_bias, a.c.mask != nullptr);
+  a.chunk = p.chunk;
+  a.slots = p.slots;
+  a.room = p.room;
   static std::atomic<uint64_t> raised{0};
   const cudaError_t e = raise_smem_limit((const void*)k_logit_controls<kThreads, kDepth, kUnroll>,
-                                         bytes(kMaxChunk, kMostRoom, true), &raised);
+                                         logit_smem(kMaxChunk, kMostRoom, true, kThreads, kDepth),
+                                         &raised);
   if (e != cudaSuccess) return e;
   return counted(launch_pdl(k_logit_controls<kThreads, kDepth, kUnroll>,
-                            dim3((unsigned)(rows * cluster)), kThreads, smem, st, cluster, a));
+                            dim3((unsigned)(rows * cluster)), kThreads, p.smem, st, cluster, a));
 }
 
 }  // namespace
@@ -518,9 +491,9 @@ extern "C" int myos_dev_logit_controls(float* d_out, size_t out_stride, const fl
   const cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   if (rows * kMaxCluster <= (size_t)sm_count() * 2 / 3) {
-    e = launch_controls<1024, 0, 1>(a, rows, cluster_of<1024>(a, rows), st);
+    e = launch_controls<1024, 0, 1>(a, rows, logit_cluster(rows, a.vocab, 1024, sm_count()), st);
   } else {
-    const int cluster = cluster_of<512>(a, rows);
+    const int cluster = logit_cluster(rows, a.vocab, 512, sm_count());
     e = a.vocab / cluster >= 12 * 4 * 512 ? launch_controls<512, 4, 2>(a, rows, cluster, st)
                                           : launch_controls<512, 0, 2>(a, rows, cluster, st);
   }
