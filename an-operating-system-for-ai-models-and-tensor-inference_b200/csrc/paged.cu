@@ -200,26 +200,28 @@ __global__ void __launch_bounds__(1024) k_paged_tables(const TablesArgs a) {
   }
   const int rows = (int)min(before.rows, (int64_t)a.max_rows);
   if (longer) {
-    // rows: of the last request that begins at or before the row
+    // rows: of the last request that begins at or before the row (a step past 2^31
+    // rows is still below 2^32)
 #pragma unroll 2
-    for (int r = blockIdx.x * blockDim.x + threadIdx.x; r < rows; r += gridDim.x * blockDim.x) {
+    for (uint32_t r = blockIdx.x * blockDim.x + threadIdx.x; r < (uint32_t)rows;
+         r += gridDim.x * blockDim.x) {
       int lo = 0, hi = a.nseq;
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (spans[mid].start <= r) lo = mid;
+        if ((uint32_t)spans[mid].start <= r) lo = mid;
         else hi = mid;
       }
       const Span sp = spans[lo];
       if (!(sp.ctx & kLong)) continue;
       const uint32_t ctx = sp.ctx & ~kLong, pos = ctx + (r - sp.start), pg = pos / P;
       if (sp.first < 0) {
-        row(r, lo, 0, 0, -1);
+        row((int)r, lo, 0, 0, -1);
         continue;
       }
       const uint32_t held = ceil_div(ctx, P), in = pos - pg * P;
       const int32_t page = page_of(lo, pg, held, sp.first);
       if (pg >= held && in == 0) a.table[lo * a.table_stride + pg] = page;
-      row(r, lo, pos, in, page);
+      row((int)r, lo, pos, in, page);
     }
   }
   // rows behind the last request's

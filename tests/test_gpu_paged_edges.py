@@ -1,5 +1,5 @@
 """Calls of the paged serving operators at the edges of what their documentation
-allows: histories of few tokens.
+allows: histories of few tokens, rows near 2^31.
 """
 import numpy as np
 import pytest
@@ -36,3 +36,27 @@ def test_penalties_of_short_histories_without_biases(dev, rows, vocab, width):
     assert torch.equal(only, ids)
     dev.logit_controls(t, t, **args)  # in place
     assert torch.equal(t, out)
+
+
+# ---------------------------------------------------------------- tables
+def test_tables_of_as_many_rows_as_are_allowed(dev):
+    """One prompt that fills a row buffer of 2^31 - 1 rows (34 GB of outputs): the
+    threads' strides from row to row go past 2^31 at its end."""
+    rows, page = 2**31 - 1, 65536
+    blocks = 2**31 // page
+    torch.cuda.empty_cache()
+    free = torch.from_numpy(np.random.default_rng(1).permutation(blocks).astype(np.int32)).cuda()
+    table = torch.full((1, blocks), -1, dtype=torch.int32, device="cuda")
+    slots = torch.full((rows,), -9, dtype=torch.int64, device="cuda")
+    pos, seq = (torch.full((rows,), -9, dtype=torch.int32, device="cuda") for _ in range(2))
+    lens, starts, result = (torch.full((n,), -9, dtype=torch.int32, device="cuda") for n in (1, 2, 2))
+    dev.paged_tables(table, i32([0]), i32([rows]), free, i32([blocks]), page, blocks, slots, pos, seq, lens, starts, result)
+    assert torch.equal(table[0], free.flip(0))
+    assert lens.tolist() == [rows] and starts.tolist() == [0, rows] and result.tolist() == [0, 0]
+    step = 1 << 27
+    for r0 in range(0, rows, step):
+        r = torch.arange(r0, min(rows, r0 + step), device="cuda")
+        assert (pos[r0 : r0 + step] == r).all() and (seq[r0 : r0 + step] == 0).all()
+        assert (slots[r0 : r0 + step] == table[0, r // page].long() * page + r % page).all()
+    del table, slots, pos, seq, r
+    torch.cuda.empty_cache()
