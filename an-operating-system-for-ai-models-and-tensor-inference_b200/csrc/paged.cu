@@ -424,7 +424,8 @@ int myos_dev_paged_tables(int32_t* d_block_table, size_t table_stride, size_t ma
     return MYOS_ERR_SHAPE;
   const size_t smem = sizeof(Span) * nseq;
   static std::atomic<uint64_t> raised{0};
-  if (smem > 48 * 1024 &&
+  // 48 KB unless it is raised, the kernel's own shared memory (1.4 KB) included
+  if (smem > 40 * 1024 &&
       raise_smem_limit((const void*)k_paged_tables, sizeof(Span) * 16384, &raised) != cudaSuccess)
     return MYOS_ERR_CUDA;
   TablesArgs a;

@@ -1,8 +1,15 @@
 """Calls of the paged serving operators at the edges of what their documentation
-allows: histories of few tokens, rows near 2^31.
+allows: histories of few tokens, rows near 2^31, tables near
+the shared-memory limit.
 """
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
+
+import myos
 
 torch = pytest.importorskip("torch")
 
@@ -60,3 +67,25 @@ def test_tables_of_as_many_rows_as_are_allowed(dev):
         assert (slots[r0 : r0 + step] == table[0, r // page].long() * page + r % page).all()
     del table, slots, pos, seq, r
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n", [3900, 3978, 3979, 4000, 4096, 4097])
+def test_tables_of_batches_near_48_kb_of_shared_memory(n):
+    """Each batch as a process's first call: the kernel's own shared memory and
+    the requests' together pass the limit that holds unless it is raised."""
+    code = f"""if 1:
+        import torch
+        from myos import dev
+        n, page, blocks = {n}, 16, 2
+        i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+        table, free = i32(n, blocks) - 1, torch.arange(n, dtype=torch.int32, device="cuda")
+        slots, out = torch.zeros(n, dtype=torch.int64, device="cuda"), [i32(n), i32(n), i32(n), i32(n + 1), i32(2)]
+        dev.paged_tables(table, i32(n), i32(n) + 1, free, i32(1) + n, page, n, slots, *out)
+        r = torch.arange(n, device="cuda")
+        assert torch.equal(table[:, 0].long(), n - 1 - r) and (table[:, 1] == -1).all()
+        assert torch.equal(slots, (n - 1 - r) * page) and (out[0] == 0).all() and torch.equal(out[1].long(), r)
+        assert (out[2] == 1).all() and torch.equal(out[3][1:].long(), r + 1) and out[4].tolist() == [0, 0]
+    """
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       env={**os.environ, "PYTHONPATH": os.path.dirname(os.path.dirname(myos.__file__))})
+    assert r.returncode == 0, r.stderr[-2000:]
