@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(1024) k_paged_tables(const TablesArgs a) {
   pdl_launch();
   pdl_wait();
   const int nfree = min(max(*a.num_free, 0), a.free_cap);
-  const int64_t room = (int64_t)a.max_blocks * P;
+  const int64_t room = min((int64_t)a.max_blocks * P, (int64_t)0x7fffffff);  // lengths are int32
   Sums before = {0, 0};  // of the requests of earlier rounds
   int64_t taken = 0;
   int refused = 0, longer = 0;

@@ -401,10 +401,11 @@ typedef struct myos_paged_kv {
  * [0 .. *d_num_free) (free_cap entries; *d_num_free is clipped to it), in
  * request order, and are appended to the table row in place.
  * A request is admitted when its tokens fit the table row (max_blocks *
- * page_size) and the row buffer (max_rows), and the pages needed by the
- * requests up to and including it (those that fit) do not exceed *d_num_free;
- * a request that needs no page is not held up by the free list. A refused
- * request keeps its length, takes no page, and its rows get slot -1. Outputs:
+ * page_size, and at most 2^31 - 1) and the row buffer (max_rows), and the pages
+ * needed by the requests up to and including it (those that fit) do not exceed
+ * *d_num_free; a request that needs no page is not held up by the free list. A
+ * refused request keeps its length, takes no page, and its rows get slot -1.
+ * Outputs:
  * per row d_slots (page * page_size + slot in page; -1: none, also where the
  * page id is outside 0 .. num_pages), d_positions (0 without a slot's
  * request), d_row_seq (the request; -1 for rows behind the last one, whose

@@ -1,5 +1,5 @@
 """Calls of the paged serving operators at the edges of what their documentation
-allows: histories of few tokens, rows near 2^31, tables near
+allows: histories of few tokens, lengths and rows near 2^31, tables near
 the shared-memory limit.
 """
 import os
@@ -89,3 +89,22 @@ def test_tables_of_batches_near_48_kb_of_shared_memory(n):
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
                        env={**os.environ, "PYTHONPATH": os.path.dirname(os.path.dirname(myos.__file__))})
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_tables_of_lengths_that_reach_31_bits(dev):
+    """A table row with room for more than 2^31 - 1 tokens: a request grows to that
+    length, and past it is refused like one that its row has no room for."""
+    page, blocks, top = 65536, 32769, 2**31 - 1
+    num_pages = 2 * blocks
+    table = torch.arange(blocks, dtype=torch.int32, device="cuda").repeat(6, 1)
+    ctx, new = [top, top - 1, top - 3, top - 2, 5, top], [1, 1, 3, 3, top, 0]
+    rows = 10
+    i = lambda n: torch.full((n,), 99, dtype=torch.int32, device="cuda")  # noqa: E731
+    slots, pos, seq = torch.full((rows,), 99, dtype=torch.int64, device="cuda"), i(rows), i(rows)
+    lens, starts, result = i(6), i(7), i(2)
+    dev.paged_tables(table, i32(ctx), i32(new), i32([0]), i32([0]), page, num_pages, slots, pos, seq, lens, starts, result)
+    assert lens.tolist() == [top, top, top, top - 2, 5, top]
+    assert starts.tolist() == [0, 1, 2, 5, 8, 10, 10] and result.tolist() == [0, 3]
+    assert pos.tolist() == [0, top - 1, top - 3, top - 2, top - 1] + [0] * 5
+    assert slots.tolist() == [-1, top - 1, top - 3, top - 2, top - 1] + [-1] * 5
+    assert seq.tolist() == [0, 1, 2, 2, 2, 3, 3, 3, 4, 4]
