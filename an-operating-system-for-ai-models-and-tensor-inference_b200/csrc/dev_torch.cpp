@@ -181,12 +181,46 @@ PyObject* guarded(F&& body) {
 }
 
 // ------------------------------------------------------------------- PagedKV
+// The two tensors; what they hold is looked up at each call (0.05 us), so a
+// tensor that was given other memory, strides or sizes goes by those.
 struct PagedKv {
   PyObject_HEAD PyObject* k;
   PyObject* v;
+};
+
+struct KvView {
   int dev, heads, dim;
   myos_paged_kv c;
 };
+
+KvView kv_view(PyObject* ko, PyObject* vo) {
+  Call call(ko, "k");
+  const Tensor& k = call.get(ko, "k", {kF32, kBF16});
+  const Tensor& v = call.get(vo, "v", {kF32, kBF16});
+  if (k.dim() != 4)
+    refuse(MYOS_ERR_SHAPE, "k: [pages, heads, slots, dim] wanted, got " + shape_text(k.sizes()));
+  if (v.sizes() != k.sizes() || v.strides() != k.strides() || v.scalar_type() != k.scalar_type())
+    refuse(MYOS_ERR_ARG, "k and v differ in shape, strides or dtype");
+  int64_t size[4], st[4];
+  for (int i = 0; i < 4; ++i) {
+    size[i] = k.size(i);
+    st[i] = k.stride(i);
+    if (size[i] > 0x7fffffff) refuse(MYOS_ERR_SHAPE, "k: " + shape_text(k.sizes()));
+  }
+  if (size[3] > 1 && st[3] != 1) refuse(MYOS_ERR_ARG, "the last dimension is not contiguous");
+  // a dimension of one element has no stride of its own
+  int64_t least = size[3];
+  for (int i = 1; i < 3; ++i)
+    if (size[i] > 1 && st[i] > least) least = st[i];
+  for (int i = 0; i < 3; ++i)
+    if (size[i] <= 1) st[i] = least;
+  return {call.dev,
+          (int)size[1],
+          (int)size[3],
+          {k.data_ptr(),       v.data_ptr(),      (uint64_t)st[0],   (uint64_t)st[1],
+           (uint64_t)st[2],    (uint32_t)size[0], (uint32_t)size[2], (uint32_t)size[1],
+           (uint32_t)size[3],  k.scalar_type() == kF32 ? MYOS_KV_F32 : MYOS_KV_BF16, 0}};
+}
 
 void kv_free(PagedKv* self) {
   Py_XDECREF(self->k);
@@ -199,34 +233,9 @@ int kv_init(PagedKv* self, PyObject* args, PyObject* kw) {
   PyObject *ko, *vo;
   if (!PyArg_ParseTupleAndKeywords(args, kw, "OO", const_cast<char**>(names), &ko, &vo)) return -1;
   PyObject* ok = guarded([&]() -> PyObject* {
-    Call call(ko, "k");
-    const Tensor& k = call.get(ko, "k", {kF32, kBF16});
-    const Tensor& v = call.get(vo, "v", {kF32, kBF16});
-    if (k.dim() != 4)
-      refuse(MYOS_ERR_SHAPE, "k: [pages, heads, slots, dim] wanted, got " + shape_text(k.sizes()));
-    if (v.sizes() != k.sizes() || v.strides() != k.strides() || v.scalar_type() != k.scalar_type())
-      refuse(MYOS_ERR_ARG, "k and v differ in shape, strides or dtype");
-    int64_t size[4], st[4];
-    for (int i = 0; i < 4; ++i) {
-      size[i] = k.size(i);
-      st[i] = k.stride(i);
-      if (size[i] > 0x7fffffff) refuse(MYOS_ERR_SHAPE, "k: " + shape_text(k.sizes()));
-    }
-    if (size[3] > 1 && st[3] != 1) refuse(MYOS_ERR_ARG, "the last dimension is not contiguous");
-    // a dimension of one element has no stride of its own
-    int64_t least = size[3];
-    for (int i = 1; i < 3; ++i)
-      if (size[i] > 1 && st[i] > least) least = st[i];
-    for (int i = 0; i < 3; ++i)
-      if (size[i] <= 1) st[i] = least;
+    kv_view(ko, vo);
     Py_XSETREF(self->k, Py_NewRef(ko));
     Py_XSETREF(self->v, Py_NewRef(vo));
-    self->dev = call.dev;
-    self->heads = (int)size[1];
-    self->dim = (int)size[3];
-    self->c = {k.data_ptr(),       v.data_ptr(),      (uint64_t)st[0],   (uint64_t)st[1],
-               (uint64_t)st[2],    (uint32_t)size[0], (uint32_t)size[2], (uint32_t)size[1],
-               (uint32_t)size[3],  k.scalar_type() == kF32 ? MYOS_KV_F32 : MYOS_KV_BF16, 0};
     return Py_None;
   });
   return ok ? 0 : -1;
@@ -234,24 +243,28 @@ int kv_init(PagedKv* self, PyObject* args, PyObject* kw) {
 
 PyObject* kv_get_k(PagedKv* s, void*) { return Py_NewRef(s->k ? s->k : Py_None); }
 PyObject* kv_get_v(PagedKv* s, void*) { return Py_NewRef(s->v ? s->v : Py_None); }
-PyObject* kv_get_dev(PagedKv* s, void*) { return PyLong_FromLong(s->dev); }
-PyObject* kv_get_heads(PagedKv* s, void*) { return PyLong_FromLong(s->heads); }
-PyObject* kv_get_dim(PagedKv* s, void*) { return PyLong_FromLong(s->dim); }
+PyObject* kv_get_int(PagedKv* s, void* which) {
+  return guarded([&]() -> PyObject* {
+    const KvView kv = kv_view(s->k, s->v);
+    const int fields[] = {kv.dev, kv.heads, kv.dim};
+    return PyLong_FromLong(fields[(intptr_t)which]);
+  });
+}
 
 PyGetSetDef kv_fields[] = {
     {"k", (getter)kv_get_k, nullptr, "the K tensor", nullptr},
     {"v", (getter)kv_get_v, nullptr, "the V tensor", nullptr},
-    {"dev", (getter)kv_get_dev, nullptr, "the device's ordinal", nullptr},
-    {"num_kv_heads", (getter)kv_get_heads, nullptr, nullptr, nullptr},
-    {"head_dim", (getter)kv_get_dim, nullptr, nullptr, nullptr},
+    {"dev", (getter)kv_get_int, nullptr, "the device's ordinal", nullptr},
+    {"num_kv_heads", (getter)kv_get_int, nullptr, nullptr, (void*)1},
+    {"head_dim", (getter)kv_get_int, nullptr, nullptr, (void*)2},
     {nullptr, nullptr, nullptr, nullptr, nullptr}};
 
 PyTypeObject kv_type = {PyVarObject_HEAD_INIT(nullptr, 0) "myos.dev.PagedKV"};
 
-const PagedKv& kv_of(PyObject* o, int dev) {
+KvView kv_of(PyObject* o, int dev) {
   if (!o || !PyObject_TypeCheck(o, &kv_type) || !((PagedKv*)o)->k)
     refuse(MYOS_ERR_ARG, "kv: not a PagedKV");
-  const PagedKv& kv = *(PagedKv*)o;
+  const KvView kv = kv_view(((PagedKv*)o)->k, ((PagedKv*)o)->v);
   if (kv.dev != dev)
     refuse(MYOS_ERR_ARG, "kv: on cuda:" + std::to_string(kv.dev) + ", not cuda:" + std::to_string(dev));
   return kv;
@@ -298,7 +311,7 @@ PyObject* qk_norm_rope_store(PyObject*, PyObject* const* args, Py_ssize_t nargs,
     PyObject* o[N];
     parse("qk_norm_rope_store", args, nargs, kwnames, names, N, COS, o);
     Call c(o[QKV], "qkv");
-    const PagedKv& kv = kv_of(o[KV], c.dev);
+    const KvView kv = kv_of(o[KV], c.dev);
     const Tensor& q = c.get(o[Q], "q_out", {kF32});
     if (q.dim() != 3) refuse(MYOS_ERR_SHAPE, "q_out: [rows, num_q_heads, head_dim] wanted");
     const int64_t rows = q.size(0), hq = q.size(1), d = kv.dim;
@@ -339,7 +352,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs, Py
     PyObject* o[N];
     parse("paged_attention", args, nargs, kwnames, names, N, SCALE, o);
     Call c(o[Q], "q");
-    const PagedKv& kv = kv_of(o[KV], c.dev);
+    const KvView kv = kv_of(o[KV], c.dev);
     const Tensor& q = c.get(o[Q], "q", {kF32});
     if (q.dim() != 3) refuse(MYOS_ERR_SHAPE, "q: [nseq, num_q_heads, head_dim] wanted");
     const int64_t nseq = q.size(0), hq = q.size(1);
@@ -478,7 +491,8 @@ constexpr char k_doc_PagedKV[] =
     "One layer's paged cache: k and v as [num_pages, num_kv_heads, page_size,\n"
     "head_dim] views, f32 or bf16, with the same strides (a cache kept as\n"
     "[num_pages, page_size, num_kv_heads, head_dim] is passed as\n"
-    "t.permute(0, 2, 1, 3)). Holds the tensors, copies nothing.\n";
+    "t.permute(0, 2, 1, 3)). Holds the tensors, copies nothing; each call takes\n"
+    "their memory, strides and sizes as they are then.\n";
 
 #define METHOD(f) \
   {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL | METH_KEYWORDS, k_doc_##f}

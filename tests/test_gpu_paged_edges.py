@@ -1,6 +1,6 @@
 """Calls of the paged serving operators at the edges of what their documentation
 allows: histories of few tokens, lengths and rows near 2^31, tables near
-the shared-memory limit.
+the shared-memory limit, caches whose tensors got other memory.
 """
 import os
 import subprocess
@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 
 import myos
+from myos import _lib
 
 torch = pytest.importorskip("torch")
 
@@ -108,3 +109,57 @@ def test_tables_of_lengths_that_reach_31_bits(dev):
     assert pos.tolist() == [0, top - 1, top - 3, top - 2, top - 1] + [0] * 5
     assert slots.tolist() == [-1, top - 1, top - 3, top - 2, top - 1] + [-1] * 5
     assert seq.tolist() == [0, 1, 2, 2, 2, 3, 3, 3, 4, 4]
+
+
+# ---------------------------------------------------------------- the cache object
+def test_a_cache_goes_by_its_tensors_as_they_are_at_the_call(dev):
+    """PagedKV holds its tensors: memory, strides and shape are theirs at each
+    call, also after they were given other ones."""
+    torch.manual_seed(3)
+    pages, hkv, page, d, hq, rows = 4, 2, 16, 64, 4, 10
+    shape = (pages, hkv, page, d)
+    k, v = torch.zeros(shape, device="cuda"), torch.zeros(shape, device="cuda")
+    kv = dev.PagedKV(k, v)
+    qkv, q = torch.randn(rows, (hq + 2 * hkv) * d, device="cuda"), torch.zeros(rows, hq, d, device="cuda")
+    pos, slots = i32(np.arange(rows)), torch.arange(rows, device="cuda")
+    table, lens, work = i32([[0, 1, 2, 3]]), i32([rows]), torch.zeros(dev.WORK_BYTES, dtype=torch.uint8, device="cuda")
+
+    def attention():
+        out = torch.zeros(1, hq, d, device="cuda")
+        dev.paged_attention(out, q[:1], kv, table, lens, work)
+        return out
+
+    dev.qk_norm_rope_store(q, qkv, kv, pos, slots)
+    first = attention()
+    olds = k.data, v.data  # the old memory stays allocated
+    before = [t.clone() for t in olds]
+    k.data, v.data = torch.zeros(shape, device="cuda"), torch.zeros(shape, device="cuda")
+    assert not attention().any()
+    dev.qk_norm_rope_store(q, qkv * 2, kv, pos, slots)
+    assert torch.equal(k, before[0] * 2) and torch.equal(v, before[1] * 2)
+    assert torch.equal(olds[0], before[0]) and torch.equal(olds[1], before[1])
+    # other strides, a larger cache, another dtype
+    nhd = [torch.zeros(pages + 3, page, hkv, d, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    k.data, v.data = (t.permute(0, 2, 1, 3) for t in nhd)
+    dev.qk_norm_rope_store(q, qkv, kv, pos, slots + (pages + 2) * page)
+    assert torch.equal(nhd[0][pages + 2, :rows], before[0][0, :, :rows].transpose(0, 1).bfloat16())
+    table.fill_(pages + 2)
+    torch.testing.assert_close(attention(), first, rtol=2**-6, atol=2**-6)  # K and V rounded to bf16
+    # k alone was changed: refused, nothing is written
+    kept = nhd[1].clone()
+    k.data = torch.zeros(shape, device="cuda")
+    for call in (attention, lambda: dev.qk_norm_rope_store(q, qkv, kv, pos, slots)):
+        with pytest.raises(myos.MyosError) as e:
+            call()
+        assert e.value.code == _lib.ERR_ARG
+    assert not k.any() and torch.equal(nhd[1], kept)
+
+
+def test_a_cache_without_memory_is_refused(dev):
+    k, v = (torch.zeros(4, 2, 16, 64, device="cuda") for _ in range(2))
+    kv = dev.PagedKV(k, v)
+    k.untyped_storage().resize_(0)
+    out, work = torch.zeros(1, 4, 64, device="cuda"), torch.zeros(dev.WORK_BYTES, dtype=torch.uint8, device="cuda")
+    with pytest.raises(myos.MyosError) as e:
+        dev.paged_attention(out, out, kv, i32([[0]]), i32([1]), work)
+    assert e.value.code == _lib.ERR_ARG
