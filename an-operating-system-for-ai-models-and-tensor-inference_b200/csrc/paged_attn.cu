@@ -279,15 +279,16 @@ struct WarpState {
   }
   // 1 / l, or 0 without a key. l is at least 1 (the largest weight), at most the
   // number of keys: an approximate reciprocal and one Newton step, no special cases.
+  // A NaN query's l is NaN, and so are its out and lse.
   MYOS_DEV float inverse() const {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(l));
-    return l > 0.f ? fmaf(r, fmaf(-l, r, 1.0f), r) : 0.f;
+    return l == 0.f ? 0.f : fmaf(r, fmaf(-l, r, 1.0f), r);
   }
   MYOS_DEV void put_lse(float* lse, int G) const {
     const int lane = threadIdx.x & 31;
     if (lse && (lane & 3) == 0 && (lane >> 2) < G)
-      lse[lane >> 2] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      lse[lane >> 2] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
   }
 };
 

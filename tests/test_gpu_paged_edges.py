@@ -1,6 +1,8 @@
 """Calls of the paged serving operators at the edges of what their documentation
 allows: histories of few tokens, lengths and rows near 2^31, tables near
-the shared-memory limit, caches whose tensors got other memory.
+the shared-memory limit, caches whose tensors got other memory, NaN queries.
+
+Tolerances as in test_gpu_paged.py (u = 2^-24, half a step of f32).
 """
 import os
 import subprocess
@@ -14,7 +16,8 @@ from myos import _lib
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_paged import check_logits, dev, i32, plain_logits  # noqa: E402,F401
+from test_gpu_paged import (U, attend, cache, check_attention, check_logits, dev, fill_cache,  # noqa: E402,F401
+                            i32, kept, plain_attention, plain_logits)
 
 pytestmark = pytest.mark.gpu
 
@@ -163,3 +166,29 @@ def test_a_cache_without_memory_is_refused(dev):
     with pytest.raises(myos.MyosError) as e:
         dev.paged_attention(out, out, kv, i32([[0]]), i32([1]), work)
     assert e.value.code == _lib.ERR_ARG
+
+
+# ---------------------------------------------------------------- attention
+@pytest.mark.parametrize("kvt", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_nan_query_has_a_nan_lse(dev, kvt, d):
+    """The store marks a row whose position has no angles with a NaN query: its
+    attention is NaN in out and lse, not that of an empty sequence, however its
+    keys are split; the other rows and heads do not see it."""
+    rng = np.random.default_rng(d)
+    torch.manual_seed(d)
+    hq, hkv, page, lens = 6, 2, 16, [5000, 5000, 40, 40, 0, 1, 1]
+    k, v = cache(rng, sum(-(-n // page) for n in lens), hkv, page, d, kvt)
+    table, ks, vs = fill_cache(rng, k, v, lens, page)
+    q = torch.randn(len(lens), hq, d, device="cuda")
+    q[1], q[3], q[4], q[6, 2] = float("nan"), float("nan"), float("nan"), float("nan")
+    nan = torch.isnan(q[:, :, 0])
+    nan[4] = False  # no keys: zeros and -inf
+    out, lse = attend(dev, q, dev.PagedKV(k, v), i32(table), i32(lens))
+    assert torch.isnan(out[nan]).all() and torch.isnan(lse[nan]).all()
+    assert not torch.isnan(out[~nan]).any() and not torch.isnan(lse[~nan]).any()
+    clean = torch.nan_to_num(q)
+    want = plain_attention(clean.double().cpu().numpy(), ks, vs, d**-0.5, kept(lens))
+    for x, y in ((out, want[0]), (lse, want[1])):
+        x[nan] = torch.from_numpy(y).cuda()[nan].float()
+    check_attention(out, lse, want[:2] + tuple(t + 2 * U * np.abs(np.nan_to_num(w, neginf=0)) for t, w in zip(want[2:], want)))
