@@ -411,6 +411,11 @@ PyObject* logit_controls(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyO
     a.repetition = fl(REP, rows);
     a.frequency = fl(FREQ, rows);
     a.presence = fl(PRES, rows);
+    // no tokens: an empty tensor has no address, and the penalties nothing to do
+    if (o[HIST] && a.history_width == 0) {
+      a.history = nullptr;
+      a.repetition = a.frequency = a.presence = nullptr;
+    }
     if (o[BSTARTS]) {
       if (!o[BIDS] || !o[BVALS])
         refuse(MYOS_ERR_ARG, "bias_starts, bias_ids and bias_vals come together");

@@ -1,5 +1,5 @@
 """Calls of the paged serving operators at the edges of what their documentation
-allows: histories of few tokens, lengths and rows near 2^31, tables near
+allows: histories of no or few tokens, lengths and rows near 2^31, tables near
 the shared-memory limit, caches whose tensors got other memory, NaN queries.
 
 Tolerances as in test_gpu_paged.py (u = 2^-24, half a step of f32).
@@ -192,3 +192,21 @@ def test_a_nan_query_has_a_nan_lse(dev, kvt, d):
     for x, y in ((out, want[0]), (lse, want[1])):
         x[nan] = torch.from_numpy(y).cuda()[nan].float()
     check_attention(out, lse, want[:2] + tuple(t + 2 * U * np.abs(np.nan_to_num(w, neginf=0)) for t, w in zip(want[2:], want)))
+
+
+@pytest.mark.parametrize("view", [False, True])
+def test_penalties_of_a_history_without_columns(dev, view):
+    """No token so far: the penalties change nothing, biases still count."""
+    rng = np.random.default_rng(9)
+    x = rng.standard_normal((3, 20001)).astype(np.float32)
+    t = torch.from_numpy(x).cuda()
+    hist = i32(np.zeros((3, 5)))[:, :0] if view else torch.empty(3, 0, dtype=torch.int32, device="cuda")
+    two = torch.full((3,), 2.0, device="cuda")
+    out, ids = torch.zeros_like(t), torch.zeros(3, dtype=torch.int32, device="cuda")
+    zero = i32([0, 0, 0])
+    dev.logit_controls(out, t, history=hist, prompt_lens=zero, hist_lens=zero, repetition=two, frequency=two,
+                       presence=two, ids=ids)
+    assert torch.equal(out, t) and ids.tolist() == x.argmax(1).tolist()
+    dev.logit_controls(out, t, history=hist, repetition=two, bias_starts=i32([0, 1, 1, 2]), bias_ids=i32([20000, 7]),
+                       bias_vals=torch.tensor([50.0, 50.0], device="cuda"), ids=ids)
+    assert ids.tolist() == [20000, int(x[1].argmax()), 7]
