@@ -430,6 +430,8 @@ PyObject* logit_controls(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyO
       const Tensor& m = c.get(o[MASK], "mask", {kI32, kU32});
       if (m.dim() != 2 || m.size(1) * 32 < vocab)
         refuse(MYOS_ERR_SHAPE, "mask: fewer bits than the vocabulary");
+      // asked here too: a mask of no rows has no address, which to the C call is no mask
+      if (!o[MROWS] && m.size(0) < rows) refuse(MYOS_ERR_SHAPE, "mask: fewer rows than logits");
       a.mask = (uint32_t*)c.rows(o[MASK], "mask", {kI32, kU32}, m.sizes(), &st2);
       a.mask_stride = st2;
       a.num_masks = (uint64_t)m.size(0);

@@ -210,3 +210,15 @@ def test_penalties_of_a_history_without_columns(dev, view):
     dev.logit_controls(out, t, history=hist, repetition=two, bias_starts=i32([0, 1, 1, 2]), bias_ids=i32([20000, 7]),
                        bias_vals=torch.tensor([50.0, 50.0], device="cuda"), ids=ids)
     assert ids.tolist() == [20000, int(x[1].argmax()), 7]
+
+
+def test_a_mask_tensor_of_too_few_rows_is_refused(dev):
+    """Row r uses mask r where mask_rows is not given: also where there is none."""
+    t, out = torch.zeros(3, 100, device="cuda"), torch.full((3, 100), 5.0, device="cuda")
+    for n in (0, 1, 2):
+        with pytest.raises(myos.MyosError) as e:
+            dev.logit_controls(out, t, mask=torch.zeros(n, 4, dtype=torch.int32, device="cuda"))
+        assert e.value.code == _lib.ERR_SHAPE and (out == 5).all()
+    # named, a mask outside them is none
+    dev.logit_controls(out, t, mask=torch.zeros(0, 4, dtype=torch.int32, device="cuda"), mask_rows=i32([0, -1, 2]))
+    assert torch.equal(out, t)
