@@ -1,5 +1,6 @@
 """Build the in-tree native libraries with nvcc / g++. PyTorch is needed only by
-the last one, the tensor binding, which is left out where torch is not installed.
+the last one, the tensor binding, which is left out where torch is not installed
+or the binding cannot be built against it.
 
 Outputs (git-ignored, carried to the GPU box with the tree):
   lib/libmyos_cuda.so   CUDA kernels + the C ABI of include/myos_cuda.h (sm_100a)
@@ -103,23 +104,43 @@ def build(force: bool = False, verbose: bool = False) -> dict:
         _run(["g++", "-O2", "-std=c++17", "-I" + INCLUDE, "-o", cli_bin, cli_src,
               "-L" + LIB, "-lmyos_cuda", "-Wl,-rpath,$ORIGIN", "-pthread"])
     out = {"cuda": so, "synth": synth_so, "cli": cli_bin}
-    torch = importlib.util.find_spec("torch")
-    if torch is not None:
-        root = torch.submodule_search_locations[0]
-        dev_src = os.path.join(CSRC, "dev_torch.cpp")
-        dev_so = os.path.join(LIB, "_myos_dev.so")
-        if force or _stale(dev_so, [dev_src, os.path.join(INCLUDE, "myos_cuda.h"),
-                                    os.path.join(root, "version.py")]):
-            cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
-            inc = [os.path.join(root, "include"),
-                   os.path.join(root, "include", "torch", "csrc", "api", "include"),
-                   os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
-            _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
-                 + ["-I" + d for d in inc] + [dev_src, "-o", dev_so, "-L" + LIB, "-lmyos_cuda",
-                 "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
-                 "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
+    dev_so = build_binding(force)
+    if dev_so:
         out["dev"] = dev_so
     return out
+
+
+def build_binding(force: bool = False):
+    """lib/_myos_dev.so against the installed torch, or None: without a torch, or
+    with one that it cannot be built against (a CPU-only build, another C++ ABI).
+    Everything else works without it; myos.dev then names the missing file."""
+    torch = importlib.util.find_spec("torch")
+    if torch is None or not torch.submodule_search_locations:
+        return None
+    root = torch.submodule_search_locations[0]
+    dev_src = os.path.join(CSRC, "dev_torch.cpp")
+    dev_so = os.path.join(LIB, "_myos_dev.so")
+    version = os.path.join(root, "version.py")
+    deps = [dev_src, os.path.join(INCLUDE, "myos_cuda.h")]
+    if os.path.exists(version):
+        deps.append(version)
+    if not force and not _stale(dev_so, deps):
+        return dev_so
+    if os.path.exists(dev_so):
+        os.remove(dev_so)  # of another source or torch: not to be loaded if this build fails
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    inc = [os.path.join(root, "include"),
+           os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    try:
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
+             + ["-I" + d for d in inc] + [dev_src, "-o", dev_so, "-L" + LIB, "-lmyos_cuda",
+             "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+             "-ltorch_python", "-Wl,-rpath,$ORIGIN"])
+    except RuntimeError as e:
+        sys.stderr.write(f"myos.dev is left out, its binding does not build against {root}: {e}\n")
+        return None
+    return dev_so
 
 
 if __name__ == "__main__":
