@@ -175,7 +175,9 @@ MYOS_DEV float weight_of(float m, float top) { return top == -INFINITY ? 0.f : e
 // of the same heads, so a lane's c0, c1 and c2, c3 belong to one head
 // (lane / 4) and are added up. The tensor core truncates its f32 sums, so no
 // long chain runs through it: four steps of a score, one tile of an output;
-// the rest are f32 adds, rounded to nearest.
+// the rest are f32 adds, rounded to nearest. (The products with a side's last
+// term, at most 2^-11 of the others, go through in one chain of all steps, 32 at
+// most: what that cuts off is below 1/64 of a step of the scores' terms.)
 //
 // o[2 t + i] is value i of column tile t (8 of the head's dims).
 template <int DH>
@@ -303,7 +305,7 @@ struct Bf16Warp : WarpState<DH> {
   static constexpr int kKeys = 16, kSteps = DH / 16;
   // The queries' terms: in registers, or (kShared, longer heads) for all warps in
   // the swap space, which is free while the tiles go by (16 x 8192 keys of 16/4
-  // heads of 256: 111 us, f32 206; split again for each tile 120 and 236).
+  // heads of 256: 110 us, f32 210; split again for each tile 9 and 30 us more).
   static constexpr bool kShared = DH > 128;
   static constexpr int kRoom = kShared ? kSteps * 32 * 24 : 0;
   Split3 q[kShared ? 1 : kSteps][2];
@@ -345,11 +347,16 @@ struct Bf16Warp : WarpState<DH> {
     const int lane = threadIdx.x & 31, c = (lane & 3) * 2;
     float s[4];
     {
-      float a[2][2][4], lo[2][4];
+      constexpr int kSums = DH > 128 ? 4 : 2;  // of four steps each
+      float a[2][kSums][4], lo[2][4];
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[n][0][i] = a[n][1][i] = lo[n][i] = 0.f;
+        for (int i = 0; i < 4; ++i) {
+          lo[n][i] = 0.f;
+#pragma unroll
+          for (int u = 0; u < kSums; ++u) a[n][u][i] = 0.f;
+        }
       const int row = (lane & 7) + ((lane >> 4) << 3);
       const uint32_t base = ks + row * (DH * 2) + ((((lane >> 3) & 1) ^ (row & 7)) << 4);
 #pragma unroll
@@ -369,13 +376,20 @@ struct Bf16Warp : WarpState<DH> {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           mma16816(lo[n], q0.lo, 0u, q1.lo, 0u, b[2 * n], b[2 * n + 1]);
-          mma16816(a[n][(k >> 2) & 1], q0.hi, q0.mid, q1.hi, q1.mid, b[2 * n], b[2 * n + 1]);
+          mma16816(a[n][(k >> 2) & (kSums - 1)], q0.hi, q0.mid, q1.hi, q1.mid, b[2 * n], b[2 * n + 1]);
         }
       }
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          if constexpr (kSums == 4) {
+#pragma unroll
+            for (int u = i; u < 4; u += 2) {
+              a[n][0][u] += a[n][2][u];
+              a[n][1][u] += a[n][3][u];
+            }
+          }
           const float x = (a[n][0][i] + a[n][1][i]) + ((a[n][0][i + 2] + a[n][1][i + 2]) + lo[n][i]);
           s[2 * n + i] = (ok >> (8 * n + c + i)) & 1u ? x * scale2 : -INFINITY;
         }
@@ -483,7 +497,7 @@ struct F32Warp : WarpState<DH> {
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     float s[2];
     {
-      constexpr int kChains = DH / 32 < 4 ? DH / 32 : 4;
+      constexpr int kChains = DH / 32;  // of four steps each
       float a[kChains][4], lo[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -515,9 +529,16 @@ struct F32Warp : WarpState<DH> {
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        if constexpr (kChains == 8) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            a[n][i] += a[n + 4][i];
+            a[n][i + 2] += a[n + 4][i + 2];
+          }
+        }
         float x = a[0][i], y = a[0][i + 2];
 #pragma unroll
-        for (int n = 1; n < kChains; ++n) {
+        for (int n = 1; n < (kChains < 4 ? kChains : 4); ++n) {
           x += a[n][i];
           y += a[n][i + 2];
         }

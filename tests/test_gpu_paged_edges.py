@@ -222,3 +222,31 @@ def test_a_mask_tensor_of_too_few_rows_is_refused(dev):
     # named, a mask outside them is none
     dev.logit_controls(out, t, mask=torch.zeros(0, 4, dtype=torch.int32, device="cuda"), mask_rows=i32([0, -1, 2]))
     assert torch.equal(out, t)
+
+
+@pytest.mark.parametrize("kvt", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_score_leaves_the_tensor_core_after_four_steps(dev, kvt, d):
+    """The tensor core cuts its f32 sums off: one product of 1 and, in each other
+    step, one a little below a step of 1 (2 u), which a sum that holds the 1
+    loses. The score of a single key is its log-sum-exp.
+
+    Four steps lose three of them (6 u); the sums are joined with roundings of u
+    each, at most 4; the products with log2 e and ln 2 round twice, and the two
+    constants are off by 0.25 u together: 12.25 u.
+    """
+    first, step = 2.0**-12, 8 if kvt == "f32" else 16
+    small = (2 - 2.0 ** (-10 if kvt == "f32" else -7)) * first  # one term of a key
+    q, k = torch.zeros(1, 1, d, device="cuda"), torch.zeros(d)
+    # a step of an f32 cache takes values 4 c and 4 c + 1, or 4 c + 2 and 4 c + 3, of 16
+    at = torch.arange(0, d, step) if kvt == "bf16" else torch.tensor([16 * (s // 2) + 2 * (s % 2) for s in range(d // 8)])
+    q[0, 0, at.cuda()], k[at] = first, small
+    q[0, 0, 0], k[0] = 1, 1
+    kc, vc = cache(None, 1, 1, 16, d, kvt, fill=0.0)
+    kc[0, 0, 0] = k.cuda().to(kc.dtype)
+    vc[0, 0, 0] = 1
+    out, lse = attend(dev, q, dev.PagedKV(kc, vc), i32([[0]]), i32([1]), scale=1.0)
+    exact = 1 + (len(at) - 1) * first * small
+    assert (out == 1).all()
+    off = abs(lse.double().item() - exact) / U
+    assert off <= 12.25, off
