@@ -88,14 +88,6 @@ MYOS_DEV void mma1688(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-MYOS_DEV void mma1688_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                           uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
 MYOS_DEV void lds4(float4& x, uint32_t addr) {
   asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
                : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
@@ -434,11 +426,24 @@ MYOS_DEV void split2(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
+// x without its last bits.
+MYOS_DEV float cut(float x, int bits) {
+  return __uint_as_float(__float_as_uint(x) & (0xffffffffu << bits));
+}
 
-// f32 cache, 8 keys a tile: both sides as two tf32 terms, all four products
-// (hi and lo of the queries in the A operand's two halves, hi and lo of the
-// keys in two mma). On the FMA units a tile cost 1700 instructions, and 64
-// sequences of 512 to 640 keys (12/2 heads of 128) took 37 us.
+// f32 cache, 8 keys a tile. Keys and queries enter as two tf32 terms, all four
+// products (hi and lo of the queries in the A operand's two halves, hi and lo of
+// the keys in two mma): a step of a factor can be lost, which is less than the
+// scores' own f32 sums round. Values enter exactly, so that a key that takes all
+// the weight gives its value: 11 bits in tf32 by both terms of the weights, the
+// other 13 as two bf16 terms (8 and 5 bits), side by side along the summed index
+// of one mma, by 16 bits of the weights (off by 2^-26 of a product). As two tf32
+// terms the values lost their last bit and the kernel took 2 to 6 % less (64
+// sequences of 512 to 640 keys of 12/2 heads of 128: 21.3 us, exact 22.2; 16 x
+// 8192 of 40/8: 175.5 and 178.8, of 8/8 of 64: 94 and 99, of 16/4 of 256: 210 and
+// 217). A third tf32 product takes 5 to 11 % more than two, three bf16 terms of
+// keys and values alike 3 to 18.
+// On the FMA units a tile cost 1700 instructions, and the 64 sequences took 37 us.
 //
 // The order in which an mma takes its summed index is free, as long as both
 // operands agree: step s of a score sums dims 16 (s / 2) + 4 c + 2 (s % 2) and
@@ -550,24 +555,40 @@ struct F32Warp : WarpState<DH> {
     uint32_t w[4];
     split2(s[0], w[0], w[1]);
     split2(s[1], w[2], w[3]);
+    const uint32_t w_hi = pack_top(s[0], s[1]);
+    const uint32_t w_mid = pack_top(s[0] - top_bits(s[0]), s[1] - top_bits(s[1]));
     // rows 2 c and 2 c + 1 have the same exchange
     const uint32_t base = vs + 2 * c * (DH * 4) + ((g ^ flip_v(2 * c)) << 4);
+    // Column tiles whose two mma, one upon the other, go in turn: four (64 x 640
+    // above 22.1 us, one by one 23.3), where the registers hold them (128 x 300
+    // keys of 32/8 heads of 64: 25.4 us, one by one 24.1).
+    constexpr int kTurn = DH > 64 ? 4 : 1;
 #pragma unroll
     for (int j = 0; j < DH / 32; ++j) {
-      float4 x, y;
-      lds4(x, base + j * 128);
-      lds4(y, base + j * 128 + DH * 4);
-      uint32_t u[8], v[8];
-      split_q(x, u);
-      split_q(y, v);
+      float4 x4, y4;
+      lds4(x4, base + j * 128);
+      lds4(y4, base + j * 128 + DH * 4);
+      const float x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float t[4];
-        mma1688_zero(t, w[0], w[1], w[2], w[3], u[2 * e + 1], v[2 * e + 1]);
-        mma1688(t, w[0], w[1], w[2], w[3], u[2 * e], v[2 * e]);
-        float* r = &o[8 * j + 2 * e];
-        r[0] = fmaf(r[0], keep, t[0] + t[2]);
-        r[1] = fmaf(r[1], keep, t[1] + t[3]);
+      for (int e0 = 0; e0 < 4; e0 += kTurn) {
+        float t[kTurn][4], x0[kTurn], y0[kTurn];
+#pragma unroll
+        for (int n = 0; n < kTurn; ++n) {
+          const float xe = x[e0 + n], ye = y[e0 + n], x1 = cut(xe, 5), y1 = cut(ye, 5);
+          x0[n] = cut(xe, 13);
+          y0[n] = cut(ye, 13);
+          mma16816_zero(t[n], w_hi, w_mid, w_hi, w_mid, pack_top(x1 - x0[n], y1 - y0[n]),
+                        pack_top(xe - x1, ye - y1));
+        }
+#pragma unroll
+        for (int n = 0; n < kTurn; ++n)
+          mma1688(t[n], w[0], w[1], w[2], w[3], __float_as_uint(x0[n]), __float_as_uint(y0[n]));
+#pragma unroll
+        for (int n = 0; n < kTurn; ++n) {
+          float* r = &o[8 * j + 2 * (e0 + n)];
+          r[0] = fmaf(r[0], keep, t[n][0] + t[n][2]);
+          r[1] = fmaf(r[1], keep, t[n][1] + t[n][3]);
+        }
       }
     }
   }

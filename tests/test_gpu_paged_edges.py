@@ -250,3 +250,21 @@ def test_a_score_leaves_the_tensor_core_after_four_steps(dev, kvt, d):
     assert (out == 1).all()
     off = abs(lse.double().item() - exact) / U
     assert off <= 12.25, off
+
+
+@pytest.mark.parametrize("kvt", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [8, 64, 128, 256])
+def test_a_single_key_gives_its_value_exactly(dev, kvt, d):
+    """One key has the weight 1: out is V, all 24 bits of it, also where the other
+    keys of a window or of a table are left out."""
+    torch.manual_seed(d)
+    n, hkv, page = 40, 2, 16
+    k, v = (torch.randn(n, hkv, page, d, device="cuda").to(torch.float32 if kvt == "f32" else torch.bfloat16) for _ in range(2))
+    v[0], v[1, :, 0], v[2, :, 0] = v[0] * 1e30, v[1, :, 0] * 1e-30, 1 - 2.0**-24
+    q = torch.randn(n, 8, d, device="cuda")
+    table = torch.arange(n, dtype=torch.int32, device="cuda")[:, None]
+    kv = dev.PagedKV(k, v)
+    out, _ = attend(dev, q, kv, table, i32([1] * n))
+    assert torch.equal(out, v[:, :, 0].float().repeat_interleave(4, 1))
+    out, _ = attend(dev, q, kv, table, i32([7] * n), window=1)
+    assert torch.equal(out, v[:, :, 6].float().repeat_interleave(4, 1))
