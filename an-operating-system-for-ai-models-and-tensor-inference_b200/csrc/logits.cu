@@ -479,6 +479,10 @@ extern "C" int myos_dev_logit_controls(float* d_out, size_t out_stride, const fl
                        c->history_stride > ((uint64_t)1 << 40)))
       return MYOS_ERR_SHAPE;
     if (c->num_bias > 0x40000000) return MYOS_ERR_SHAPE;
+    // a block counts the entries of its list in 31 bits
+    if (c->bias_starts && (c->repetition || c->frequency || c->presence) &&
+        c->history_width + c->num_bias > 0x7fffffff)
+      return MYOS_ERR_SHAPE;
     if (c->mask && (c->mask_stride < (vocab + 31) / 32 || c->mask_stride > ((uint64_t)1 << 40) ||
                     c->num_masks > 0x7fffffff || (!c->mask_rows && c->num_masks < rows)))
       return MYOS_ERR_SHAPE;

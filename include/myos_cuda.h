@@ -510,7 +510,8 @@ typedef struct myos_logit_controls_args {
  * id of the result (myos_greedy_token's rule: the first maximum; NaN and -inf
  * never win, a row of nothing else gives 0). d_out receives the controlled
  * logits (may be d_logits with the same stride: in place; null: only the ids),
- * d_ids the ids (null: none); not both null. c null: no controls. */
+ * d_ids the ids (null: none); not both null. c null: no controls. vocab,
+ * history_width and num_bias are at most 2^30, the last two together below 2^31. */
 int myos_dev_logit_controls(float* d_out, size_t out_stride, const float* d_logits,
                             size_t logits_stride, size_t rows, size_t vocab,
                             const myos_logit_controls_args* c, uint32_t* d_ids, void* stream);
