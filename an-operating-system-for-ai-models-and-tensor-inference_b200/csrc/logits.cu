@@ -31,6 +31,14 @@ struct LogitArgs {
 // number, and the whole history is looked through for each. The blocks' best ids
 // meet in the first block's shared memory.
 //
+// The list has 5120 entries at most, of tokens, not of distinct ones. A row's
+// history passes it from about 5 thousand tokens on where a row has one block, 10
+// where it has two, 20 where it has four, sooner where few ids make most of it,
+// and from there the time grows with the history times the steps: 64 rows of
+// 152064 with 4096, 8192, 16384 and 32768 tokens take 23, 45, 136 and 304 us, 256
+// rows with 4096 and 8192 94 and 310 us; 64 rows that each said one token 4096
+// times 77 us.
+//
 // Everything before the pass is latency (row parameters, tokens, table), so it
 // is kept off the memory's back: the table is cleared before the launch's
 // dependency, the first tokens and logits and the mask are on their way while

@@ -9,13 +9,15 @@
 // of keys, and the tiles, in one row, into equal shares, one per block: the
 // lengths live on the device, so each block finds its share itself from a scan
 // of them, and no split has to be chosen on the host. An item that lies in one
-// share is finished there; else each block leaves its part in the work buffer
-// and the last to arrive joins them, in the order of the shares (the same bits
+// share is finished there. Where there are blocks for two shares of every item,
+// the items get equal numbers of shares, and neighbouring ones meet in a pair of
+// blocks' shared memory. What is left in parts goes through the work buffer: the
+// last block to arrive joins them, in the order of the shares (the same bits
 // whoever is last). A block has at most two parts, its first and its last
 // piece, so the buffer's size does not depend on the batch.
 //
 // Each warp streams keys of its own through its own stages of shared memory
-// (cp.async, three deep, pages looked up one tile ahead), so warps never wait
+// (cp.async, three deep, pages looked up two tiles ahead), so warps never wait
 // for one another inside an item. A copy instruction takes 64 bytes of each of
 // eight rows: a lane stays with one or two rows of a tile, and all its
 // addresses are one base each and constants.
@@ -747,9 +749,15 @@ constexpr size_t attn_smem() {
 
 // Blocks resident on a multiprocessor, by shared memory (55, 108 or 216 KB each),
 // and blocks of a cluster, in launches of at least so many for each item: two
-// shares of one meet through the pair's shared memory, not the work buffer (64 x
-// 640: 21.3 instead of 22.7 us in f32, 14.3 instead of 15.6 in bf16). Clusters of
-// 4 are not all placed at once: 32 ragged sequences took 380 us instead of 281.
+// shares of one meet through the pair's shared memory, not the work buffer. That
+// gains where many items are split (64 x 640 of 12/2 heads of 128, 22.2 us instead
+// of 23.7 in f32 and 14.1 instead of 15.3 in bf16; 1 x 32768 of 40/8 31.4 instead
+// of 33.2; 16 x 8192 f32 of 16/4 of 256 216 instead of 223) and loses up to 9 % of
+// a few short ones, whose launch by cluster takes longer (1 x 128 5.7 instead of
+// 5.6, 8 x 1024 10.9 instead of 10.0, 1 x 4097 11.3 instead of 10.7, 2 x 500 f32 of
+// 40/8 10.5 instead of 9.7): the lengths that tell them apart are the device's.
+// Clusters of 4 are not all placed at once: 32 ragged sequences took 380 us
+// instead of 281.
 template <int DH>
 constexpr int kResident = DH == 64 ? 4 : DH == 128 ? 2 : 1;
 constexpr int kCluster = 2;

@@ -358,9 +358,11 @@ int myos_dev_gqa_attn_f32_noalloc(float* d_y, const float* d_q, const float* d_k
  *
  * Common rules: the calls run on the current device, on `stream` (0: the
  * default stream) of that device, and every pointer is memory of that device.
- * They allocate nothing, do not synchronize, and can be captured into a graph;
- * the first call on a device belongs outside a capture (it raises the kernels'
- * shared-memory limits). Arguments that the host can see are checked before
+ * They allocate nothing, do not synchronize, and can be captured into a graph.
+ * A kernel's first call on a device loads it and raises its shared-memory limit,
+ * which belongs outside a capture; there are several kernels to a call (by cache
+ * type and head_dim, by rows and vocabulary), so make one call of each shape that
+ * will be captured. Arguments that the host can see are checked before
  * any device work: MYOS_ERR_ARG for null pointers, invalid options and
  * misaligned addresses or strides, MYOS_ERR_SHAPE for sizes. What only the
  * device can see (lengths, page ids, slots, positions, token ids) is checked
