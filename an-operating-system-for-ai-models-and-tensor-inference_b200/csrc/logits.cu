@@ -46,7 +46,7 @@ struct LogitArgs {
 // with tables of one word an id, chunk by chunk, and the penalties in the pass
 // over all ids 52 us (59 instructions an id, nearly every warp went through the
 // divisions), with the touched ids computed before that pass 39 us. The pass
-// itself, without controls, takes 18.5 us; 12 us is the memory's share.
+// itself, without controls, takes 17.9 us; 12 us is the memory's share.
 constexpr uint32_t kSeen = 0x80000000u;  // in the prompt; the low bits count the output
 constexpr uint32_t kNoId = 0xffffffffu;
 
