@@ -460,8 +460,9 @@ int myos_dev_qk_norm_rope_store(float* d_q, size_t q_stride, const float* d_qkv,
  * the natural log of the sum of exp(scale * q . k). Keys of a page whose table
  * entry is outside the cache are left out. A sequence with no keys gives zeros
  * and lse -inf. Slots behind len are never read, whatever they hold; the keys
- * and values that are attended to, q and scale are finite, but for a query head
- * of NaN (the store's mark of a row without angles), whose out and lse are NaN.
+ * and values that are attended to, q and scale are finite (keys of an f32 cache
+ * and q with it below 2^128 - 2^116), but for a query head of NaN (the store's
+ * mark of a row without angles), whose out and lse are NaN.
  * d_work: MYOS_PAGED_WORK_BYTES of device memory, 16-byte aligned, zeroed once
  * before its first use; each call leaves it ready for the next. Calls that may
  * run at the same time (other streams, graphs) need buffers of their own.
