@@ -71,7 +71,8 @@ def draw(rng):
         rows, k = _log(rng, 1, 4097), _log(rng, 64, 13824)
         most = min(151936, 4097 * 5120 * 27648 // (rows * k), 151936 * 1536 // k, 4097 * 27648 // rows // (2 if x == "f32" else 1))
         return {"op": op, "rows": rows, "k": k, "n": _log(rng, 64, max(64, most)), "bias": rng.random() < 0.5, "out": x}
-    width = rng.choice([1536, 5120, 8960, 13824, _log(rng, 100, 16384)])
+    width = rng.choice([8960, 13824] if op == "swiglu" else [1536, 5120, 8960, 13824])
+    width = rng.choice([width, width, width, _log(rng, 100, 16384)])
     case = {"op": op, "rows": _log(rng, 1, 8191 * 5120 // width), "width": width, "x": x}
     return {**case, "add": rng.random() < 0.7} if op == "norm" else case
 
