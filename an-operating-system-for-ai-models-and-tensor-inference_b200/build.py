@@ -44,7 +44,7 @@ def cutlass_include() -> list:
     raise RuntimeError("CUTLASS headers (sm100 collectives) not found")
 CUDA_SOURCES = ["kernels.cu", "engine.cu", "ops.cu", "noalloc.cu",
                 "prefill.cu", "gemm_sm100.cu", "paged.cu", "paged_attn.cu", "logits.cu",
-                "safetensors.cpp", "tp.cpp"]
+                "row_quant.cu", "matmul_i8.cu", "safetensors.cpp", "tp.cpp"]
 HEADERS = ["common.cuh", "cp_async.cuh", "kernels.h", "safetensors.h", "prefill.h",
            "gemm_sm100.h", "logits_plan.h", "paged.h", "tp.h"]
 

@@ -137,7 +137,9 @@ struct Call {
 
 constexpr ScalarType kF32 = ScalarType::Float, kI32 = ScalarType::Int, kI64 = ScalarType::Long,
                      kBF16 = ScalarType::BFloat16, kU8 = ScalarType::Byte,
-                     kU32 = ScalarType::UInt32;
+                     kU32 = ScalarType::UInt32, kI8 = ScalarType::Char;
+
+int32_t dtype_of(const Tensor& t) { return t.scalar_type() == kF32 ? MYOS_F32 : MYOS_BF16; }
 
 void* stream_of(PyObject* o, int dev) {
   if (!o) return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
@@ -447,6 +449,125 @@ PyObject* logit_controls(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyO
   });
 }
 
+// rows [rows, width] of x in 8 bits: q [rows, width], scales [rows]. width: of q.
+struct Rows {
+  int8_t* q;
+  float* scales;
+  const void* x;
+  size_t q_stride, x_stride;
+  int64_t rows, width;
+  int32_t x_dtype;
+};
+
+Rows rows_of(const Call& c, PyObject* q, PyObject* scales, PyObject* x, const char* what, int64_t times) {
+  const Tensor& t = c.get(q, "q", {kI8});
+  if (t.dim() != 2) refuse(MYOS_ERR_SHAPE, "q: [rows, width] wanted, got " + shape_text(t.sizes()));
+  Rows r;
+  r.rows = t.size(0);
+  r.width = t.size(1);
+  r.q = (int8_t*)c.rows(q, "q", {kI8}, {r.rows, r.width}, &r.q_stride);
+  r.x = c.rows(x, what, {kF32, kBF16}, {r.rows, times * r.width}, &r.x_stride);
+  r.x_dtype = dtype_of(c.get(x, what, {kF32, kBF16}));
+  r.scales = (float*)c.vec(scales, "scales", {kF32}, r.rows);
+  return r;
+}
+
+PyObject* add_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  return guarded([&]() -> PyObject* {
+    enum { Q, SCALES, X, GAMMA, RESIDUAL, TOTAL, EPS, STREAM, N };
+    static const char* const names[N] = {"q",        "scales", "x",   "gamma",
+                                         "residual", "total",  "eps", "stream"};
+    PyObject* o[N];
+    parse("add_norm_quant", args, nargs, kwnames, names, N, RESIDUAL, o);
+    Call c(o[Q], "q");
+    const Rows r = rows_of(c, o[Q], o[SCALES], o[X], "x", 1);
+    void* gamma = c.vec(o[GAMMA], "gamma", {kBF16}, r.width);
+    size_t res_stride = 0, total_stride = 0;
+    void* res = o[RESIDUAL]
+                    ? c.rows(o[RESIDUAL], "residual", {kF32}, {r.rows, r.width}, &res_stride)
+                    : nullptr;
+    void* total = o[TOTAL] ? c.rows(o[TOTAL], "total", {kF32}, {r.rows, r.width}, &total_stride)
+                           : nullptr;
+    const float eps = o[EPS] ? f32(o[EPS]) : 1e-6f;
+    void* st = stream_of(o[STREAM], c.dev);
+    run("add_norm_quant", c.dev, [&] {
+      return myos_dev_add_norm_quant(r.q, r.q_stride, r.scales, (float*)total, total_stride, r.x,
+                                     r.x_dtype, r.x_stride, (float*)res, res_stride, gamma, eps,
+                                     (size_t)r.rows, (size_t)r.width, st);
+    });
+    Py_RETURN_NONE;
+  });
+}
+
+PyObject* quant_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  return guarded([&]() -> PyObject* {
+    enum { Q, SCALES, X, STREAM, N };
+    static const char* const names[N] = {"q", "scales", "x", "stream"};
+    PyObject* o[N];
+    parse("quant_rows", args, nargs, kwnames, names, N, STREAM, o);
+    Call c(o[Q], "q");
+    const Rows r = rows_of(c, o[Q], o[SCALES], o[X], "x", 1);
+    void* st = stream_of(o[STREAM], c.dev);
+    run("quant_rows", c.dev, [&] {
+      return myos_dev_quant_rows(r.q, r.q_stride, r.scales, r.x, r.x_dtype, r.x_stride,
+                                 (size_t)r.rows, (size_t)r.width, st);
+    });
+    Py_RETURN_NONE;
+  });
+}
+
+PyObject* swiglu_quant(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  return guarded([&]() -> PyObject* {
+    enum { Q, SCALES, X, STREAM, N };
+    static const char* const names[N] = {"q", "scales", "gate_up", "stream"};
+    PyObject* o[N];
+    parse("swiglu_quant", args, nargs, kwnames, names, N, STREAM, o);
+    Call c(o[Q], "q");
+    const Rows r = rows_of(c, o[Q], o[SCALES], o[X], "gate_up", 2);
+    void* st = stream_of(o[STREAM], c.dev);
+    run("swiglu_quant", c.dev, [&] {
+      return myos_dev_swiglu_quant(r.q, r.q_stride, r.scales, r.x, r.x_dtype, r.x_stride,
+                                   (size_t)r.rows, (size_t)r.width, st);
+    });
+    Py_RETURN_NONE;
+  });
+}
+
+PyObject* matmul_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs, PyObject* kwnames) {
+  return guarded([&]() -> PyObject* {
+    enum { OUT, A, AS, W, WS, BIAS, STREAM, N };
+    static const char* const names[N] = {"out", "a", "a_scales", "w", "w_scales", "bias", "stream"};
+    PyObject* o[N];
+    parse("matmul_i8", args, nargs, kwnames, names, N, BIAS, o);
+    Call c(o[OUT], "out");
+    const Tensor& a = c.get(o[A], "a", {kI8});
+    const Tensor& w = c.get(o[W], "w", {kI8});
+    if (a.dim() != 2) refuse(MYOS_ERR_SHAPE, "a: [rows, k] wanted, got " + shape_text(a.sizes()));
+    if (w.dim() != 2 || w.size(1) != a.size(1))
+      refuse(MYOS_ERR_SHAPE, "w: [channels, " + std::to_string(a.size(1)) + "] wanted, got " +
+                                 shape_text(w.sizes()));
+    const int64_t rows = a.size(0), k = a.size(1), channels = w.size(0);
+    size_t out_stride, a_stride, w_stride;
+    void* out = c.rows(o[OUT], "out", {kF32, kBF16}, {rows, channels}, &out_stride);
+    void* ap = c.rows(o[A], "a", {kI8}, {rows, k}, &a_stride);
+    void* wp = c.rows(o[W], "w", {kI8}, {channels, k}, &w_stride);
+    // a single row has no stride of its own, and need not be a multiple of 16 long
+    if (rows == 1) a_stride = (size_t)((k + 15) / 16 * 16);
+    if (channels == 1) w_stride = (size_t)((k + 15) / 16 * 16);
+    void* as = c.vec(o[AS], "a_scales", {kF32}, rows);
+    void* ws = c.vec(o[WS], "w_scales", {kF32}, channels);
+    void* bias = c.vec(o[BIAS], "bias", {kF32}, channels);
+    const int32_t type = dtype_of(c.get(o[OUT], "out", {kF32, kBF16}));
+    void* st = stream_of(o[STREAM], c.dev);
+    run("matmul_i8", c.dev, [&] {
+      return myos_dev_matmul_i8(out, type, out_stride, (int8_t*)ap, a_stride, (float*)as,
+                                (int8_t*)wp, w_stride, (float*)ws, (float*)bias, (size_t)rows,
+                                (size_t)k, (size_t)channels, st);
+    });
+    Py_RETURN_NONE;
+  });
+}
+
 constexpr char k_doc_paged_tables[] =
     "paged_tables(block_table, ctx_lens, new_lens, free_pages, num_free, page_size, num_pages, slots, positions, row_seq, kv_lens, seq_starts, result, stream=None)\n"
     "--\n"
@@ -491,6 +612,40 @@ constexpr char k_doc_logit_controls[] =
     "of the result: myos_dev_logit_controls. out may be logits (in place) or\n"
     "None (only ids).\n";
 
+constexpr char k_doc_add_norm_quant[] =
+    "add_norm_quant(q, scales, x, gamma, residual=None, total=None, eps = 1e-6, stream=None)\n"
+    "--\n"
+    "\n"
+    "total = x + residual (f32; None: x), and the rows of its RMSNorm with gamma\n"
+    "(bf16 [width]) in 8 bits: q [rows, width] int8 and scales [rows], q * scale\n"
+    "standing for the value: myos_dev_add_norm_quant. x is f32 or bf16; total\n"
+    "(optional) receives the sum and may be residual, or an f32 x: in place.\n";
+
+constexpr char k_doc_quant_rows[] =
+    "quant_rows(q, scales, x, stream=None)\n"
+    "--\n"
+    "\n"
+    "The rows of x [rows, width] (f32 or bf16) in 8 bits: q [rows, width] int8\n"
+    "and scales [rows], the row's largest magnitude / 127: myos_dev_quant_rows.\n"
+    "For a weight [channels, k] that is a scale for each channel.\n";
+
+constexpr char k_doc_swiglu_quant[] =
+    "swiglu_quant(q, scales, gate_up, stream=None)\n"
+    "--\n"
+    "\n"
+    "silu(gate) * up in 8 bits: gate_up [rows, 2 width] (f32 or bf16) holds the\n"
+    "gate values of a row, then its up values; q [rows, width] int8 and scales\n"
+    "[rows]: myos_dev_swiglu_quant.\n";
+
+constexpr char k_doc_matmul_i8[] =
+    "matmul_i8(out, a, a_scales, w, w_scales, bias=None, stream=None)\n"
+    "--\n"
+    "\n"
+    "out [rows, channels] (f32 or bf16) = a w^T of int8 a [rows, k] and\n"
+    "w [channels, k], summed exactly, times a_scales [rows] and w_scales\n"
+    "[channels], plus bias [channels] (f32): myos_dev_matmul_i8. The rows of a\n"
+    "and w begin at multiples of 16 bytes (k itself need not be one).\n";
+
 constexpr char k_doc_PagedKV[] =
     "PagedKV(k, v)\n"
     "--\n"
@@ -504,7 +659,8 @@ constexpr char k_doc_PagedKV[] =
 #define METHOD(f) \
   {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL | METH_KEYWORDS, k_doc_##f}
 PyMethodDef methods[] = {METHOD(paged_tables), METHOD(qk_norm_rope_store), METHOD(paged_attention),
-                         METHOD(logit_controls), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(logit_controls), METHOD(add_norm_quant), METHOD(quant_rows),
+                         METHOD(swiglu_quant), METHOD(matmul_i8), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_myos_dev", nullptr, -1, methods,
                       nullptr,               nullptr,     nullptr, nullptr};

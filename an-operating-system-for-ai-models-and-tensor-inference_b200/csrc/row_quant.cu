@@ -1,0 +1,426 @@
+// Rows in 8 bits with a scale each: plain rows, silu(gate) * up, and the
+// residual's addition with RMSNorm (include/myos_cuda.h, "Projections in 8-bit
+// integers").
+//
+// The mathematics: y of the row, scale = f32(max|y| / 127), q = rint(y / scale).
+// A row's largest value and the nearest integer are where a rounding decides:
+// with y off by 2^-23 one value in some ten thousand lands one step away, and
+// which one depends on the order of the row's sum. So both are decided in 64
+// bits, but only where 32 leave them open: y is computed in f32 with a bound on
+// its error (kRel below), the values within that bound of the maximum, and those
+// within it of a border between two steps (about one in 10^4), are computed
+// again in f64 from the inputs. The sum of squares is f64 throughout.
+//
+// The memory bounds it: a row is read once into registers (a block per row, or a
+// warp where it has at most 1024 values), two meetings of the block, q and
+// scale out.
+#include <math.h>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "paged.h"
+
+namespace myos {
+namespace {
+
+enum { kQuant, kSwiglu, kNorm };
+
+struct RowArgs {
+  int8_t* q;
+  int64_t q_stride;
+  float* scales;
+  const void* x;
+  int64_t x_stride;
+  const float* residual;
+  int64_t residual_stride;
+  float* total;
+  int64_t total_stride;
+  const uint16_t* gamma;
+  float eps;
+  int rows, width;
+};
+
+constexpr float kSmallest = 1.17549435e-38f;  // 2^-126
+constexpr float kTiny = 7.8886e-31f;          // 2^-100: below it f32 products lose bits, all goes through f64
+
+MYOS_DEV float get(const float* p) { return *p; }
+MYOS_DEV float get(const uint16_t* p) { return bf16_at(p); }
+
+// 8 values at a 16-byte boundary. Plain loads: in place, x or the residual is written.
+MYOS_DEV void load8(const float* p, float* v) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+MYOS_DEV void load8(const uint16_t* p, float* v) {
+  const uint4 a = *reinterpret_cast<const uint4*>(p);
+  v[0] = bf16_lo(a.x), v[1] = bf16_hi(a.x), v[2] = bf16_lo(a.y), v[3] = bf16_hi(a.y);
+  v[4] = bf16_lo(a.z), v[5] = bf16_hi(a.z), v[6] = bf16_lo(a.w), v[7] = bf16_hi(a.w);
+}
+template <class T>
+MYOS_DEV void load_some(const T* p, float* v, int n) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = e < n ? get(p + e) : 0.0f;
+}
+
+MYOS_DEV double silu_up64(float g, float u) {
+  return (double)g / (1.0 + exp(-(double)g)) * (double)u;
+}
+
+// In f32, exp(-g) by the special function unit. The rounding of its argument
+// makes the result relatively off by |g| 2^-23 where g is negative, so values
+// below -8 (rare in a gate) go through f64; the rest is off by 1.6 x 2^-20 at
+// most: the argument 2^-20, ex2 2^-22, rcp 2^-23, a sum and two products 2^-24
+// each.
+MYOS_DEV float silu_up(float g, float u) {
+  if (!(g >= -8.0f)) return (float)silu_up64(g, u);
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * r * u;
+}
+
+// One row as a thread sees it.
+template <int KIND, class XT>
+struct Row {
+  const XT* x;
+  const float* residual;
+  float* total;
+  const uint16_t* gamma;
+  int width;
+
+  // y of one value in 64 bits, from the inputs. scale64: what the norm multiplies by.
+  MYOS_DEV double exact(int i, double inv) const {
+    if (KIND == kQuant) return (double)get(x + i);
+    if (KIND == kSwiglu) return silu_up64(get(x + i), get(x + width + i));
+    // in place the inputs are gone: the total was written by this thread
+    const float t = total ? total[i] : residual ? __fadd_rn(get(x + i), residual[i]) : get(x + i);
+    return (double)bf16_at(gamma + i) * ((double)t * inv);
+  }
+
+  // The f32 values that go with y (of the norm: gamma * total, without its
+  // factor), for 8 of the row from i on, n of them in it; adds the squares.
+  template <bool FULL>
+  MYOS_DEV void values(int i, int n, float* p, double& squares) const {
+    float a[8], b[8];
+    if (FULL) load8(x + i, a);
+    else load_some(x + i, a, n);
+    if (KIND == kQuant) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = a[e];
+    } else if (KIND == kSwiglu) {
+      if (FULL) load8(x + width + i, b);
+      else load_some(x + width + i, b, n);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = silu_up(a[e], b[e]);
+    } else {
+      if (residual) {
+        if (FULL) load8(residual + i, b);
+        else load_some(residual + i, b, n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = __fadd_rn(a[e], b[e]);
+      }
+      if (FULL) load8(gamma + i, b);
+      else load_some(gamma + i, b, n);
+      if (total) {
+        if (FULL) {
+          reinterpret_cast<float4*>(total + i)[0] = make_float4(a[0], a[1], a[2], a[3]);
+          reinterpret_cast<float4*>(total + i)[1] = make_float4(a[4], a[5], a[6], a[7]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < n) total[i + e] = a[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        squares += (double)a[e] * (double)a[e];
+        p[e] = __fmul_rn(a[e], b[e]);
+      }
+    }
+  }
+  // The f32 value of one, its inputs read again.
+  MYOS_DEV float value(int i) const {
+    if (KIND == kQuant) return get(x + i);
+    if (KIND == kSwiglu) return silu_up(get(x + i), get(x + width + i));
+    const float t = total ? total[i] : residual ? __fadd_rn(get(x + i), residual[i]) : get(x + i);
+    return __fmul_rn(t, bf16_at(gamma + i));
+  }
+};
+
+// What two f32 values may differ by, relatively, and be one value in 64 bits; also
+// more than a step's position is off by. gamma * total is one rounding, 1 / rms,
+// 1 / scale and the products with them one each; silu_up has its own.
+template <int KIND>
+constexpr float kRel = KIND == kSwiglu ? 3.8147e-6f : 9.5367e-7f;  // 2^-18, 2^-20
+
+// Magnitudes as integers: NaN above infinity above all others. The sign is taken
+// off the bits (arithmetic may leave a NaN's as it is).
+MYOS_DEV uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+MYOS_DEV uint64_t magnitude(double v) {
+  return (uint64_t)__double_as_longlong(v) & 0x7fffffffffffffffull;
+}
+
+template <int KIND, class XT, int C, bool VEC, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : 1024)
+    k_row_quant(const RowArgs a) {
+  __shared__ double sums[32];
+  __shared__ uint64_t tops64[32];
+  __shared__ uint32_t tops[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int64_t row = WARP ? (int64_t)blockIdx.x * warps + warp : blockIdx.x;
+  const int tid = WARP ? lane : threadIdx.x, team = WARP ? 32 : blockDim.x;
+  pdl_wait();
+  pdl_launch();
+  if (WARP && row >= a.rows) return;
+  Row<KIND, XT> r;
+  r.x = static_cast<const XT*>(a.x) + row * a.x_stride;
+  r.residual = KIND == kNorm && a.residual ? a.residual + row * a.residual_stride : nullptr;
+  r.total = KIND == kNorm && a.total ? a.total + row * a.total_stride : nullptr;
+  r.gamma = a.gamma;
+  r.width = a.width;
+  int8_t* const q = a.q + row * a.q_stride;
+
+  // ---- the row, its largest f32 value and its sum of squares
+  constexpr int kHeld = VEC ? C : 1;
+  float p[kHeld][8];
+  double squares = 0.0;
+  uint32_t top = 0;  // as bits: NaN above infinity above all others
+  if constexpr (VEC) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int i = (c * team + tid) * 8;
+      if (i + 8 <= a.width) {
+        r.template values<true>(i, 8, p[c], squares);
+      } else {
+        r.template values<false>(i, a.width - i, p[c], squares);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, magnitude(p[c][e]));
+    }
+  } else {
+    for (int i = tid; i < a.width; i += team) {
+      if (KIND == kNorm) {
+        const float t = r.residual ? __fadd_rn(get(r.x + i), r.residual[i]) : get(r.x + i);
+        if (r.total) r.total[i] = t;
+        squares += (double)t * (double)t;
+      }
+      top = max(top, magnitude(r.value(i)));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (KIND == kNorm) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (!WARP) {
+    if (lane == 0) {
+      sums[warp] = squares;
+      tops[warp] = top;
+    }
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, lane < warps ? tops[lane] : 0u);
+    if (KIND == kNorm) {
+      squares = lane < warps ? sums[lane] : 0.0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+    }
+  }
+  const double inv = KIND == kNorm ? 1.0 / sqrt(squares / a.width + (double)a.eps) : 1.0;
+  const float P = __uint_as_float(top);
+  const bool finite = top < 0x7f800000u;
+  // Nothing but zeros: scale 2^-126. (A product below f32's smallest number is 0
+  // as well, and a norm may still make it large.)
+  const bool zero = top == 0 && (KIND != kNorm || (squares == 0.0 && inv < 1e300));
+  const float rel = P < kTiny ? INFINITY : kRel<KIND>;
+
+  // ---- the largest value in 64 bits, of those that may be it
+  uint64_t most = 0;
+  if (KIND == kQuant) {
+    most = magnitude((double)P);
+  } else if (finite && !zero) {
+    const float least = P < kTiny ? 0.0f : P * (1.0f - kRel<KIND>);
+    if constexpr (VEC) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        uint32_t may = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) may |= fabsf(p[c][e]) >= least ? 1u << e : 0u;
+        while (may) {
+          const int i = (c * team + tid) * 8 + __ffs(may) - 1;
+          may &= may - 1;
+          if (i < a.width) most = max(most, magnitude(r.exact(i, inv)));
+        }
+      }
+    } else {
+      for (int i = tid; i < a.width; i += team)
+        if (fabsf(r.value(i)) >= least) most = max(most, magnitude(r.exact(i, inv)));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (!WARP) {
+      if (lane == 0) tops64[warp] = most;
+      __syncthreads();
+      most = lane < warps ? tops64[lane] : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+  }
+  const double top64 = __longlong_as_double((long long)most);
+  float scale = fmaxf((float)(top64 / 127.0), kSmallest);
+  if (!finite || !(top64 / 127.0 <= 3.4028234663852886e38)) scale = __uint_as_float(0x7fc00000u);
+  if (tid == 0) a.scales[row] = scale;
+
+  // ---- the steps
+  const bool good = scale == scale;
+  const float per = good ? (float)(inv / (double)scale) : 0.0f;
+  auto decide = [&](int i) {  // in 64 bits
+    return (int)rint(r.exact(i, inv) / (double)scale);
+  };
+  if constexpr (VEC) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int i = (c * team + tid) * 8;
+      if (i >= a.width) break;
+      uint32_t open = 0;
+      int s[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = p[c][e] * per, n = rintf(v);
+        s[e] = (int)n;
+        // how far from the border between two steps
+        if (!(0.5f - fabsf(v - n) > fabsf(v) * rel)) open |= 1u << e;
+        if (!good) s[e] = 0;
+      }
+      if (!good || zero) open = 0;
+      if (i + 8 <= a.width) {
+        uint2 w;
+        w.x = (s[0] & 255) | (s[1] & 255) << 8 | (s[2] & 255) << 16 | (uint32_t)s[3] << 24;
+        w.y = (s[4] & 255) | (s[5] & 255) << 8 | (s[6] & 255) << 16 | (uint32_t)s[7] << 24;
+        *reinterpret_cast<uint2*>(q + i) = w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i + e < a.width) q[i + e] = (int8_t)s[e];
+      }
+      while (open) {
+        const int j = i + __ffs(open) - 1;
+        open &= open - 1;
+        if (j < a.width) q[j] = (int8_t)decide(j);
+      }
+    }
+  } else {
+    for (int i = tid; i < a.width; i += team) {
+      const float v = r.value(i) * per, n = rintf(v);
+      const bool open = !(0.5f - fabsf(v - n) > fabsf(v) * rel);
+      q[i] = (int8_t)(!good || zero ? 0 : open ? decide(i) : (int)n);
+    }
+  }
+}
+
+template <int KIND, class XT, int C, bool VEC, bool WARP>
+cudaError_t launch(const RowArgs& a, int threads, cudaStream_t st) {
+  const int per = WARP ? threads / 32 : 1;
+  return counted(launch_pdl(k_row_quant<KIND, XT, C, VEC, WARP>,
+                            dim3((unsigned)((a.rows + (int64_t)per - 1) / per)), threads, 0, st, 1, a));
+}
+
+template <int KIND, class XT>
+cudaError_t launch_kind(const RowArgs& a, bool vec, cudaStream_t st) {
+  if (!vec || a.width > 32768) return launch<KIND, XT, 1, false, false>(a, 512, st);
+  if (a.width <= 256) return launch<KIND, XT, 1, true, true>(a, 128, st);
+  if (a.width <= 512) return launch<KIND, XT, 2, true, true>(a, 128, st);
+  if (a.width <= 1024) return launch<KIND, XT, 4, true, true>(a, 128, st);
+  const int chunks = (a.width + 7) / 8;
+  if (chunks <= 1024) return launch<KIND, XT, 1, true, false>(a, (chunks + 31) / 32 * 32, st);
+  if (chunks <= 2048) return launch<KIND, XT, 2, true, false>(a, (chunks + 63) / 64 * 32, st);
+  return launch<KIND, XT, 4, true, false>(a, (chunks + 127) / 128 * 32, st);
+}
+
+// The checks that the three calls share, and the launch.
+template <int KIND>
+int row_quant(RowArgs a, int32_t x_dtype, size_t q_stride, size_t x_stride, size_t rows,
+              size_t width, void* stream) {
+  if (x_dtype != MYOS_F32 && x_dtype != MYOS_BF16) return MYOS_ERR_ARG;
+  if (rows == 0) return MYOS_OK;
+  if (!a.q || !a.scales || !a.x) return MYOS_ERR_ARG;
+  const size_t most = (size_t)1 << 40, in = KIND == kSwiglu ? 2 * width : width;
+  if (rows > 0x7fffffff || width == 0 || width > MYOS_I8_MAX_K || q_stride < width ||
+      x_stride < in || q_stride > most || x_stride > most)
+    return MYOS_ERR_SHAPE;
+  const size_t size = x_dtype == MYOS_F32 ? 4 : 2;
+  if (!aligned(a.x, size) || !aligned(a.scales, 4)) return MYOS_ERR_ARG;
+  a.q_stride = (int64_t)q_stride;
+  a.x_stride = (int64_t)x_stride;
+  a.rows = (int)rows;
+  a.width = (int)width;
+  // whole vectors: 8 bytes of q, 16 of everything else (one row has no stride)
+  bool vec = aligned(a.q, 8) && aligned(a.x, 16) && aligned(a.gamma, 16) &&
+             aligned(a.residual, 16) && aligned(a.total, 16);
+  if (rows > 1)
+    vec &= q_stride % 8 == 0 && x_stride * size % 16 == 0 && a.residual_stride % 4 == 0 &&
+           a.total_stride % 4 == 0;
+  if (KIND == kSwiglu) vec &= width * size % 16 == 0;  // the up values
+  const cudaStream_t st = (cudaStream_t)stream;
+  const cudaError_t e = x_dtype == MYOS_F32 ? launch_kind<KIND, float>(a, vec, st)
+                                            : launch_kind<KIND, uint16_t>(a, vec, st);
+  return e == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
+}
+
+}  // namespace
+}  // namespace myos
+
+using namespace myos;
+
+extern "C" {
+
+int myos_dev_add_norm_quant(int8_t* d_q, size_t q_stride, float* d_scales, float* d_total,
+                            size_t total_stride, const void* d_x, int32_t x_dtype, size_t x_stride,
+                            const float* d_residual, size_t residual_stride, const void* d_gamma,
+                            float eps, size_t rows, size_t width, void* stream) {
+  if (rows > 0) {
+    if (!d_gamma || !(eps >= 0.0f)) return MYOS_ERR_ARG;
+    if (!aligned(d_gamma, 2) || !aligned(d_residual, 4) || !aligned(d_total, 4)) return MYOS_ERR_ARG;
+    const size_t most = (size_t)1 << 40;
+    if ((d_residual && (residual_stride < width || residual_stride > most)) ||
+        (d_total && (total_stride < width || total_stride > most)))
+      return MYOS_ERR_SHAPE;
+    if (d_total && rows > 1 &&
+        ((d_total == d_residual && total_stride != residual_stride) ||
+         (d_total == d_x && total_stride != x_stride)))
+      return MYOS_ERR_ARG;
+    if (d_total && d_total == d_x && x_dtype != MYOS_F32) return MYOS_ERR_ARG;
+  }
+  RowArgs a = {};
+  a.q = d_q;
+  a.scales = d_scales;
+  a.x = d_x;
+  a.residual = d_residual;
+  a.residual_stride = d_residual ? (int64_t)residual_stride : 0;
+  a.total = d_total;
+  a.total_stride = d_total ? (int64_t)total_stride : 0;
+  a.gamma = static_cast<const uint16_t*>(d_gamma);
+  a.eps = eps;
+  return row_quant<kNorm>(a, x_dtype, q_stride, x_stride, rows, width, stream);
+}
+
+int myos_dev_quant_rows(int8_t* d_q, size_t q_stride, float* d_scales, const void* d_x,
+                        int32_t x_dtype, size_t x_stride, size_t rows, size_t width, void* stream) {
+  RowArgs a = {};
+  a.q = d_q;
+  a.scales = d_scales;
+  a.x = d_x;
+  return row_quant<kQuant>(a, x_dtype, q_stride, x_stride, rows, width, stream);
+}
+
+int myos_dev_swiglu_quant(int8_t* d_q, size_t q_stride, float* d_scales, const void* d_x,
+                          int32_t x_dtype, size_t x_stride, size_t rows, size_t width,
+                          void* stream) {
+  RowArgs a = {};
+  a.q = d_q;
+  a.scales = d_scales;
+  a.x = d_x;
+  return row_quant<kSwiglu>(a, x_dtype, q_stride, x_stride, rows, width, stream);
+}
+
+}  // extern "C"

@@ -122,6 +122,7 @@ class LogitControls(C.Structure):
 
 
 PAGED_WORK_BYTES = 16 << 20  # MYOS_PAGED_WORK_BYTES
+I8_MAX_K = 131071  # MYOS_I8_MAX_K
 _dp = C.c_void_p  # a device pointer
 
 # Every symbol include/myos_cuda.h declares, with (restype, argtypes).
@@ -175,6 +176,13 @@ SIGNATURES = {
                                       sz, _dp, C.c_float, C.c_uint32, _dp, sz, _dp]),
     "myos_dev_logit_controls": (C.c_int, [_dp, sz, _dp, sz, sz, sz, C.POINTER(LogitControls),
                                           _dp, _dp]),
+    "myos_dev_add_norm_quant": (C.c_int, [_dp, sz, _dp, _dp, sz, _dp, C.c_int32, sz, _dp, sz, _dp,
+                                          C.c_float, sz, sz, _dp]),
+    "myos_dev_quant_rows": (C.c_int, [_dp, sz, _dp, _dp, C.c_int32, sz, sz, sz, _dp]),
+    "myos_dev_swiglu_quant": (C.c_int, [_dp, sz, _dp, _dp, C.c_int32, sz, sz, sz, _dp]),
+    "myos_dev_matmul_i8": (C.c_int, [_dp, C.c_int32, sz, _dp, sz, _dp, _dp, sz, _dp, _dp, sz, sz,
+                                     sz, _dp]),
+    "myos_dev_matmul_i8_status": (C.c_int, []),
     "myos_rope_table": (C.c_int, [_f32p, _f32p, sz, sz, C.c_float]),
 }
 

@@ -1,11 +1,16 @@
 """Operators on tensors already in device memory: one serving step over a
-paged KV cache (the device-pointer section of include/myos_cuda.h).
+paged KV cache, and its projections in 8-bit integers (the device-pointer
+sections of include/myos_cuda.h).
 
   PagedKV              one layer's paged cache, a view of its K and V tensors
   paged_tables         block tables, slot maps and positions from request lengths
   qk_norm_rope_store   per-head norm and rotation of q and k, K/V into the pages
   paged_attention      attention of one new token per sequence over the pages
   logit_controls       penalties, biases, grammar masks, and the greedy id
+  add_norm_quant       residual addition and RMSNorm, the rows in 8 bits with a scale each
+  quant_rows           rows (tokens, or a weight's channels) in 8 bits with a scale each
+  swiglu_quant         silu(gate) * up, the rows in 8 bits with a scale each
+  matmul_i8            product of 8-bit rows and channels, scaled, with a bias
   rope_table           cos and sin of the rotary angles (host arrays)
 
 Tensors are torch CUDA tensors, all on one device; the work runs there, on
@@ -51,6 +56,10 @@ paged_tables = _m.paged_tables
 qk_norm_rope_store = _m.qk_norm_rope_store
 paged_attention = _m.paged_attention
 logit_controls = _m.logit_controls
+add_norm_quant = _m.add_norm_quant
+quant_rows = _m.quant_rows
+swiglu_quant = _m.swiglu_quant
+matmul_i8 = _m.matmul_i8
 
 
 def rope_table(num_pos: int, rot_dim: int, theta: float):

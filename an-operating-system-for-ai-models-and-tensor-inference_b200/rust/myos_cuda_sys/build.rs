@@ -20,6 +20,8 @@ const SOURCES: &[&str] = &[
     "paged.cu",
     "paged_attn.cu",
     "logits.cu",
+    "row_quant.cu",
+    "matmul_i8.cu",
     "safetensors.cpp",
     "tp.cpp",
 ];

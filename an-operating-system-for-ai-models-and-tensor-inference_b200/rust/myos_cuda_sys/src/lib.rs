@@ -179,6 +179,11 @@ pub mod ffi {
         pub fn myos_dev_qk_norm_rope_store(d_q: *mut f32, q_stride: usize, d_qkv: *const f32, qkv_stride: usize, rows: usize, num_q_heads: usize, kv: *const myos_paged_kv, d_q_gamma: *const c_void, d_k_gamma: *const c_void, eps: f32, d_cos: *const f32, d_sin: *const f32, num_pos: usize, rot_dim: usize, d_positions: *const i32, d_slots: *const i64, stream: *mut c_void) -> c_int;
         pub fn myos_dev_paged_attn(d_out: *mut f32, out_stride: usize, d_lse: *mut f32, d_q: *const f32, q_stride: usize, nseq: usize, num_q_heads: usize, kv: *const myos_paged_kv, d_block_table: *const i32, table_stride: usize, max_blocks: usize, d_kv_lens: *const i32, scale: f32, window: u32, d_work: *mut c_void, work_bytes: usize, stream: *mut c_void) -> c_int;
         pub fn myos_dev_logit_controls(d_out: *mut f32, out_stride: usize, d_logits: *const f32, logits_stride: usize, rows: usize, vocab: usize, c: *const myos_logit_controls_args, d_ids: *mut u32, stream: *mut c_void) -> c_int;
+        pub fn myos_dev_add_norm_quant(d_q: *mut i8, q_stride: usize, d_scales: *mut f32, d_total: *mut f32, total_stride: usize, d_x: *const c_void, x_dtype: i32, x_stride: usize, d_residual: *const f32, residual_stride: usize, d_gamma: *const c_void, eps: f32, rows: usize, width: usize, stream: *mut c_void) -> c_int;
+        pub fn myos_dev_quant_rows(d_q: *mut i8, q_stride: usize, d_scales: *mut f32, d_x: *const c_void, x_dtype: i32, x_stride: usize, rows: usize, width: usize, stream: *mut c_void) -> c_int;
+        pub fn myos_dev_swiglu_quant(d_q: *mut i8, q_stride: usize, d_scales: *mut f32, d_x: *const c_void, x_dtype: i32, x_stride: usize, rows: usize, width: usize, stream: *mut c_void) -> c_int;
+        pub fn myos_dev_matmul_i8(d_out: *mut c_void, out_dtype: i32, out_stride: usize, d_a: *const i8, a_stride: usize, d_a_scales: *const f32, d_w: *const i8, w_stride: usize, d_w_scales: *const f32, d_bias: *const f32, rows: usize, k: usize, channels: usize, stream: *mut c_void) -> c_int;
+        pub fn myos_dev_matmul_i8_status() -> c_int;
         pub fn myos_rope_table(cos_out: *mut f32, sin_out: *mut f32, num_pos: usize, rot_dim: usize, theta: f32) -> c_int;
         pub fn myos_version() -> *const c_char;
     }

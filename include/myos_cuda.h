@@ -523,6 +523,75 @@ int myos_dev_logit_controls(float* d_out, size_t out_stride, const float* d_logi
  * built as tensor_core::rope_f32 builds its row (rope.rs:186-194). */
 int myos_rope_table(float* cos_out, float* sin_out, size_t num_pos, size_t rot_dim, float theta);
 
+/* ---------------------------------------------------------------------------
+ * Projections in 8-bit integers (device pointers). No counterpart in the
+ * reference, whose projections are bf16 weights times f32 rows
+ * (crates/tensor_core/src/bf16.rs:80-122). A layer of the serving step above
+ * with 8-bit weights is: the residual's addition and the norm, in 8 bits
+ * (myos_dev_add_norm_quant); q, k and v (myos_dev_matmul_i8); store and
+ * attention; the attention's rows in 8 bits (myos_dev_quant_rows); o_proj;
+ * addition and norm; gate and up; their SwiGLU in 8 bits
+ * (myos_dev_swiglu_quant); down_proj. A weight's channels are put in 8 bits
+ * once, by myos_dev_quant_rows.
+ *
+ * The common rules are those of the section above. A row of 8-bit values y has
+ * one scale: scale = max(max |y| / 127, 2^-126), rounded to f32, and
+ * q = y / scale rounded to the nearest integer, ties to even, so -127 .. 127:
+ * q * scale stands for y. Scales and q are those of y in 64-bit arithmetic from
+ * the inputs (y itself is rounded to nothing shorter on its way), whatever the
+ * order in which a row is summed: the same bits for every size and batch. A row
+ * with a y that f32 does not hold as a finite number (NaN, infinities, past its
+ * range) has scale NaN and q 0, so that all products with it are NaN.
+ * dtype arguments are MYOS_F32 or MYOS_BF16. Row strides count elements. Addresses are
+ * aligned to their elements; rows that begin at multiples of 16 bytes are faster.
+ * rows is below 2^31, a row's width at most MYOS_I8_MAX_K.
+ * ------------------------------------------------------------------------- */
+
+/* The longest row of 8-bit values: (2^31 - 1) / 128^2, where a sum of products
+ * still fits 32 bits. */
+#define MYOS_I8_MAX_K 131071u
+
+/* total = x + residual in f32 (rounded once; d_residual null: x), then the
+ * rows of RMSNorm with a BF16 weight d_gamma[width], gamma * (total /
+ * sqrt(mean(total^2) + eps)), in 8 bits: d_q and d_scales. x is f32 or bf16.
+ * d_total (nullable) receives total; it may be d_residual, or d_x where that is
+ * f32, each with the same stride: in place. */
+int myos_dev_add_norm_quant(int8_t* d_q, size_t q_stride, float* d_scales, float* d_total,
+                            size_t total_stride, const void* d_x, int32_t x_dtype, size_t x_stride,
+                            const float* d_residual, size_t residual_stride, const void* d_gamma,
+                            float eps, size_t rows, size_t width, void* stream);
+
+/* The rows of x (f32 or bf16) in 8 bits. For a weight [channels][k] the rows
+ * are its channels. */
+int myos_dev_quant_rows(int8_t* d_q, size_t q_stride, float* d_scales, const void* d_x,
+                        int32_t x_dtype, size_t x_stride, size_t rows, size_t width, void* stream);
+
+/* silu(gate) * up in 8 bits, silu(g) = g / (1 + exp(-g)): row r of d_x (f32 or
+ * bf16) holds width gate values, then width up values. */
+int myos_dev_swiglu_quant(int8_t* d_q, size_t q_stride, float* d_scales, const void* d_x,
+                          int32_t x_dtype, size_t x_stride, size_t rows, size_t width, void* stream);
+
+/* out[r][c] = (sum_i a[r][i] * w[c][i]) * a_scales[r] * w_scales[c] + bias[c]
+ * for rows rows of a, channels channels of w, k values each; d_bias (f32) may be
+ * null. The sum of products is exact in 32-bit integers (any 8-bit values, -128
+ * included), converted to f32, multiplied by a_scales[r], then by w_scales[c],
+ * and the bias added, each rounded to f32; out (f32 or bf16) is rounded from
+ * that. The same bits however the work is split. d_a, d_w and their row strides are
+ * multiples of 16 bytes (MYOS_ERR_ARG); k need not be one, what lies between k and the
+ * stride is neither read into the result nor required to be there. rows and
+ * channels are below 2^31 - 256. A wait inside the kernel is bounded: if one
+ * ran out, which only a fault elsewhere on the device can cause, the rows it
+ * served are NaN and myos_dev_matmul_i8_status says so. */
+int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const int8_t* d_a,
+                       size_t a_stride, const float* d_a_scales, const int8_t* d_w,
+                       size_t w_stride, const float* d_w_scales, const float* d_bias, size_t rows,
+                       size_t k, size_t channels, void* stream);
+
+/* MYOS_OK, or MYOS_ERR_TIMEOUT if a wait of a myos_dev_matmul_i8 on the current
+ * device has run out since the last such answer. Waits for the device; not for
+ * use in a capture. */
+int myos_dev_matmul_i8_status(void);
+
 /* Library version string and the build's target architecture. */
 const char* myos_version(void);
 
