@@ -46,7 +46,7 @@ CUDA_SOURCES = ["kernels.cu", "engine.cu", "ops.cu", "noalloc.cu",
                 "prefill.cu", "gemm_sm100.cu", "paged.cu", "paged_attn.cu", "logits.cu",
                 "row_quant.cu", "matmul_i8.cu", "safetensors.cpp", "tp.cpp"]
 HEADERS = ["common.cuh", "cp_async.cuh", "kernels.h", "safetensors.h", "prefill.h",
-           "gemm_sm100.h", "logits_plan.h", "paged.h", "tp.h"]
+           "gemm_sm100.h", "i8_plan.h", "logits_plan.h", "paged.h", "tcgen05.cuh", "tp.h"]
 
 
 def nvcc() -> str:

@@ -1,0 +1,42 @@
+// How a product of 8-bit rows and channels is cut into tiles (host arithmetic).
+#pragma once
+#include <stdint.h>
+
+namespace myos {
+
+constexpr int kI8Channels = 128;      // channels of a tile: the tensor core's M
+constexpr int kI8Step = 128;          // bytes of k of a stage: one swizzled row
+constexpr int kI8MaxRows = 256;       // rows of a tile at most: its N
+constexpr int kI8MaxStages = 12;
+constexpr int kI8StageBytes = 200 * 1024;  // of all stages together
+constexpr int kI8MaxSplit = 8;        // blocks that share a tile's k: a portable cluster
+
+struct I8Plan {
+  int tn;               // rows of a tile, a multiple of 16
+  int split;            // blocks (a cluster) along k
+  int stages;
+  int tiles_c, tiles_r;
+  int columns;          // of tensor memory: two accumulators, a power of two
+};
+
+inline int i8_ceil(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+inline I8Plan i8_plan(int64_t rows, int64_t k, int64_t channels, int sms) {
+  I8Plan p;
+  const int steps = i8_ceil(k, kI8Step);
+  p.tiles_c = i8_ceil(channels, kI8Channels);
+  p.tiles_r = i8_ceil(rows, kI8MaxRows);
+  p.tn = i8_ceil(i8_ceil(rows, p.tiles_r), 16) * 16;
+  p.tiles_r = i8_ceil(rows, p.tn);
+  const int64_t tiles = (int64_t)p.tiles_c * p.tiles_r;
+  p.split = 1;
+  while (p.split < kI8MaxSplit && p.split * 2 <= steps && tiles * p.split * 2 <= sms) p.split *= 2;
+  const int stage = (kI8Channels + p.tn) * kI8Step;
+  p.stages = kI8StageBytes / stage;
+  if (p.stages > kI8MaxStages) p.stages = kI8MaxStages;
+  p.columns = 32;
+  while (p.columns < 2 * p.tn) p.columns *= 2;
+  return p;
+}
+
+}  // namespace myos

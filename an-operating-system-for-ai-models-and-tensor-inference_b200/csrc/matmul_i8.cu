@@ -4,9 +4,22 @@
 //
 // The sum is exact in 32-bit integers, so it may be split and joined in any order
 // and gives the same bits.
-#include "common.cuh"
+//
+// A tile is 128 channels (the tensor core's M, the lanes of its memory) by up to
+// 256 rows (its N, the columns): a lane holds one channel, so a warp's store of
+// one row is 32 channels side by side, and few rows cost nothing but their own
+// columns. Six warps: copies (TMA, 128 bytes of k a stage), products (tcgen05,
+// 32 bytes of k each), and four that scale and store while the next tile's
+// products go into the other half of the tensor memory. Where there are fewer
+// tiles than multiprocessors, a cluster shares a tile's k and adds its parts
+// through shared memory.
+#include <cudaTypedefs.h>
+#include <math.h>
+
+#include "i8_plan.h"
 #include "kernels.h"
 #include "paged.h"
+#include "tcgen05.cuh"
 
 namespace myos {
 namespace {
@@ -14,15 +27,14 @@ namespace {
 struct MatArgs {
   void* out;
   int64_t out_stride;
-  const int8_t* a;
-  int64_t a_stride;
   const float* a_scales;
-  const int8_t* w;
-  int64_t w_stride;
   const float* w_scales;
   const float* bias;
-  int rows, k, channels;
+  int rows, channels, steps;
+  I8Plan plan;
 };
+
+__device__ uint32_t g_wait_failed;
 
 MYOS_DEV float scaled(int sum, float as, float ws, float bias) {
   return __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(sum), as), ws), bias);
@@ -30,57 +42,240 @@ MYOS_DEV float scaled(int sum, float as, float ws, float bias) {
 MYOS_DEV void put(float* p, float v) { *p = v; }
 MYOS_DEV void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// 16 bytes of a row from i on; zeros behind k.
-MYOS_DEV uint4 piece(const int8_t* row, int i, int k) {
-  if (i + 16 <= k) return *reinterpret_cast<const uint4*>(row + i);
-  uint32_t v[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int e = 0; e < 16; ++e)
-    if (i + e < k) v[e / 4] |= (uint32_t)(uint8_t)row[i + e] << (8 * (e % 4));
-  return make_uint4(v[0], v[1], v[2], v[3]);
+constexpr int kThreads = 192;
+constexpr int kGroup = 16;  // row tiles that share a channel tile's weights in L2 before the next
+
+// Tile t: its first channel and row.
+MYOS_DEV void tile_at(const I8Plan& p, int64_t t, int& c0, int& r0) {
+  const int64_t group = t / ((int64_t)kGroup * p.tiles_c);
+  const int first = (int)group * kGroup;
+  const int wide = min(kGroup, p.tiles_r - first);
+  const int64_t in = t - group * kGroup * p.tiles_c;
+  c0 = (int)(in / wide) * kI8Channels;
+  r0 = (first + (int)(in % wide)) * p.tn;
 }
 
-// 64 x 64 results a block, 4 x 4 a thread, 64 bytes of k at a time.
 template <class OT>
-__global__ void __launch_bounds__(256) k_matmul_i8(const MatArgs g) {
-  __shared__ uint32_t as[16][68], ws[16][68];
+__global__ void __launch_bounds__(kThreads, 1)
+    k_matmul_i8(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap amap,
+                const MatArgs g) {
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t full[kI8MaxStages], empty[kI8MaxStages], acc_full[2], acc_empty[2];
+  __shared__ float as[2][kI8MaxRows];
+  __shared__ uint32_t tmem_s;
+  __shared__ int dead;  // a wait of this block ran out
+  uint8_t* const smem = raw + (-smem_u32(raw) & 1023);
+  const I8Plan& p = g.plan;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t stage_bytes = (kI8Channels + p.tn) * kI8Step;
+  const int split = p.split, rank = split > 1 ? (int)cluster_rank() : 0;
+  const int k0 = (int)((int64_t)g.steps * rank / split);
+  const int k1 = (int)((int64_t)g.steps * (rank + 1) / split);
+  const int64_t tiles = (int64_t)p.tiles_c * p.tiles_r;
+  const int64_t tile0 = blockIdx.x / split, tile_step = gridDim.x / split;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 128);
+    }
+    dead = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc(&tmem_s, p.columns);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
   pdl_wait();
   pdl_launch();
-  const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
-  const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
-  const int lr = threadIdx.x / 4, lp = threadIdx.x % 4;
-  int sum[4][4] = {};
-  for (int k0 = 0; k0 < g.k; k0 += 64) {
-    const uint4 z = make_uint4(0, 0, 0, 0);
-    const uint4 x = r0 + lr < g.rows ? piece(g.a + (r0 + lr) * g.a_stride, k0 + lp * 16, g.k) : z;
-    const uint4 y =
-        c0 + lr < g.channels ? piece(g.w + (c0 + lr) * g.w_stride, k0 + lp * 16, g.k) : z;
-    as[lp * 4 + 0][lr] = x.x, as[lp * 4 + 1][lr] = x.y, as[lp * 4 + 2][lr] = x.z, as[lp * 4 + 3][lr] = x.w;
-    ws[lp * 4 + 0][lr] = y.x, ws[lp * 4 + 1][lr] = y.y, ws[lp * 4 + 2][lr] = y.z, ws[lp * 4 + 3][lr] = y.w;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          sum[r][c] = __dp4a((int)as[i][tr + 16 * r], (int)ws[i][tc + 16 * c], sum[r][c]);
+
+  if (warp == 0) {
+    if (lane == 0) {  // ---- copies
+      int s = 0, phase = 0, issued = 0;
+      bool ok = true;
+      for (int64_t t = tile0; ok && t < tiles; t += tile_step) {
+        int c0, r0;
+        tile_at(p, t, c0, r0);
+        for (int k = k0; k < k1; ++k) {
+          if (!mbar_wait(&empty[s], phase ^ 1, &g_wait_failed, kErrWaitEmpty)) {
+            ok = false;
+            break;
+          }
+          uint8_t* const at = smem + s * stage_bytes;
+          mbar_arrive_expect_tx(&full[s], stage_bytes);
+          tma_load_2d(at, &wmap, k * kI8Step, c0, &full[s]);
+          tma_load_2d(at + kI8Channels * kI8Step, &amap, k * kI8Step, r0, &full[s]);
+          ++issued;
+          if (++s == p.stages) s = 0, phase ^= 1;
+        }
+      }
+      if (!ok) {  // its copies in flight are waited for before the block ends
+        *(volatile int*)&dead = 1;
+        for (int n = min(issued, p.stages); n > 0; --n) {
+          if (--s < 0) s = p.stages - 1, phase ^= 1;
+          mbar_wait(&full[s], phase, &g_wait_failed, kErrWaitFull);
+        }
+      }
     }
-    __syncthreads();
-  }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {  // ---- products
+      const uint32_t shape = tc_i8_shape(kI8Channels, p.tn);
+      int s = 0, phase = 0, n = 0;
+      bool ok = true;
+      for (int64_t t = tile0; ok && t < tiles; t += tile_step, ++n) {
+        const int b = n & 1;
+        ok = mbar_wait(&acc_empty[b], (n >> 1 & 1) ^ 1, &g_wait_failed, kErrWaitEmpty);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + b * p.tn;
+        for (int k = k0; k < k1; ++k) {
+          ok = mbar_wait(&full[s], phase, &g_wait_failed, kErrWaitFull);
+          if (!ok) break;
+          tc_fence_after();
+          const uint8_t* const at = smem + s * stage_bytes;
+          const uint64_t wd = tc_operand(at), ad = tc_operand(at + kI8Channels * kI8Step);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int64_t col = c0 + tc + 16 * c;
-    if (col >= g.channels) continue;
-    const float scale = g.w_scales[col], bias = g.bias ? g.bias[col] : 0.0f;
+          for (int i = 0; i < kI8Step / 32; ++i)
+            tc_mma_i8(d, wd + 2 * i, ad + 2 * i, shape, k > k0 || i > 0);
+          tc_commit(&empty[s]);
+          if (++s == p.stages) s = 0, phase ^= 1;
+        }
+        if (ok) tc_commit(&acc_full[b]);
+      }
+      if (!ok) *(volatile int*)&dead = 1;
+    }
+    __syncwarp();
+  } else if (split == 1) {  // ---- scales and stores
+    const int quarter = warp % 4, tid = threadIdx.x - 64;
+    const float nan = __uint_as_float(0x7fc00000u);
+    bool ok = true;
+    int n = 0;
+    for (int64_t t = tile0; t < tiles; t += tile_step, ++n) {
+      int c0, r0;
+      tile_at(p, t, c0, r0);
+      const int b = n & 1, left = min(p.tn, g.rows - r0);
+      for (int j = tid; j < left; j += 128) as[b][j] = g.a_scales[r0 + j];
+      const int c = c0 + quarter * 32 + lane;
+      const bool on = c < g.channels;
+      const float ws = on ? g.w_scales[c] : 0.0f, bias = on && g.bias ? g.bias[c] : 0.0f;
+      named_sync(1, 128);
+      if (ok) ok = mbar_wait(&acc_full[b], n >> 1 & 1, &g_wait_failed, kErrWaitFull);
+      if (!ok) *(volatile int*)&dead = 1;
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      OT* o = static_cast<OT*>(g.out) + (int64_t)r0 * g.out_stride + c;
+      for (int j0 = 0; j0 < left; j0 += 16) {
+        int v[16];
+        tmem_load16(tmem + (quarter * 32 << 16) + b * p.tn + j0, v);
+        tmem_load_wait();
+        if (on) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t row = r0 + tr + 16 * r;
-      if (row < g.rows)
-        put(static_cast<OT*>(g.out) + row * g.out_stride + col,
-            scaled(sum[r][c], g.a_scales[row], scale, bias));
+          for (int j = 0; j < 16; ++j) {
+            if (j0 + j < left) {
+              const float y = scaled(v[j], as[b][j0 + j], ws, bias);
+              put(o + (int64_t)(j0 + j) * g.out_stride, ok ? y : nan);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(&acc_empty[b]);
     }
   }
+  if (split > 1) {  // ---- one tile, k shared by the cluster
+    int c0, r0;
+    tile_at(p, tile0, c0, r0);
+    const int left = min(p.tn, g.rows - r0);
+    int* const part = reinterpret_cast<int*>(smem);  // [row][channel], over the stages
+    if (warp >= 2) {
+      const int quarter = warp % 4;
+      bool ok = mbar_wait(&acc_full[0], 0, &g_wait_failed, kErrWaitFull);
+      if (!ok) *(volatile int*)&dead = 1;
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      if (ok) {
+        for (int j0 = 0; j0 < left; j0 += 16) {
+          int v[16];
+          tmem_load16(tmem + (quarter * 32 << 16) + j0, v);
+          tmem_load_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) part[(j0 + j) * kI8Channels + quarter * 32 + lane] = v[j];
+        }
+      }
+      tc_fence_before();
+    }
+    __syncwarp();
+    cluster_meet();
+    if (warp >= 2) {
+      const int ch = threadIdx.x - 64, c = c0 + ch;
+      const bool on = c < g.channels;
+      const float ws = on ? g.w_scales[c] : 0.0f, bias = on && g.bias ? g.bias[c] : 0.0f;
+      int bad = 0;
+      for (int q = 0; q < split; ++q) bad |= cluster_load(cluster_at(&dead, q));
+      const int j1 = left * (rank + 1) / split;
+      for (int j = left * rank / split; j < j1; ++j) {
+        int sum = 0;
+        for (int q = 0; q < split; ++q)
+          sum += cluster_load(cluster_at(part + j * kI8Channels + ch, q));
+        if (on)
+          put(static_cast<OT*>(g.out) + (int64_t)(r0 + j) * g.out_stride + c,
+              bad ? __uint_as_float(0x7fc00000u) : scaled(sum, g.a_scales[r0 + j], ws, bias));
+      }
+    }
+    __syncwarp();
+    cluster_meet();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_free(tmem, p.columns);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static std::atomic<void*> known{nullptr};
+  void* f = known.load(std::memory_order_acquire);
+  if (!f) {
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault,
+                                         &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    known.store(f, std::memory_order_release);
+  }
+  return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+}
+
+// Rows of k bytes in boxes of `box` rows by 128 bytes; what lies outside reads as 0.
+bool map_rows(CUtensorMap* map, const int8_t* p, int64_t k, int64_t rows, int64_t stride, int box) {
+  const auto encode = encoder();
+  if (!encode) return false;
+  const cuuint64_t size[2] = {(cuuint64_t)k, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride};
+  const cuuint32_t boxes[2] = {kI8Step, (cuuint32_t)box}, steps[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(p), size, strides, boxes,
+                steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class OT>
+cudaError_t launch(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap& amap, int sms,
+                   cudaStream_t st) {
+  constexpr size_t kSmem = kI8StageBytes + 1024;
+  static std::atomic<uint64_t> raised{0};
+  const cudaError_t e = raise_smem_limit((const void*)k_matmul_i8<OT>, kSmem, &raised);
+  if (e != cudaSuccess) return e;
+  const int64_t tiles = (int64_t)g.plan.tiles_c * g.plan.tiles_r;
+  const int64_t blocks = g.plan.split > 1 ? tiles * g.plan.split : tiles < sms ? tiles : sms;
+  return counted(launch_pdl(k_matmul_i8<OT>, dim3((unsigned)blocks), kThreads, kSmem, st,
+                            g.plan.split, wmap, amap, g));
 }
 
 }  // namespace
@@ -106,37 +301,39 @@ int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const 
       a_stride % 16 != 0 || w_stride % 16 != 0 || !aligned(d_a_scales, 4) ||
       !aligned(d_w_scales, 4) || !aligned(d_bias, 4))
     return MYOS_ERR_ARG;
+  const int sms = sm_count();
   MatArgs g;
   g.out = d_out;
   g.out_stride = (int64_t)out_stride;
-  g.a = d_a;
-  g.a_stride = (int64_t)a_stride;
   g.a_scales = d_a_scales;
-  g.w = d_w;
-  g.w_stride = (int64_t)w_stride;
   g.w_scales = d_w_scales;
   g.bias = d_bias;
   g.rows = (int)rows;
-  g.k = (int)k;
   g.channels = (int)channels;
+  g.steps = i8_ceil((int64_t)k, kI8Step);
+  g.plan = i8_plan((int64_t)rows, (int64_t)k, (int64_t)channels, sms);
+  CUtensorMap wmap, amap;
+  if (!map_rows(&wmap, d_w, (int64_t)k, (int64_t)channels, (int64_t)w_stride, kI8Channels) ||
+      !map_rows(&amap, d_a, (int64_t)k, (int64_t)rows, (int64_t)a_stride, g.plan.tn))
+    return MYOS_ERR_CUDA;
   const cudaStream_t st = (cudaStream_t)stream;
-  for (size_t r = 0; r < rows; r += 65535 * 64) {  // a grid's second side has at most 65535 blocks
-    MatArgs p = g;
-    const size_t n = rows - r < 65535 * 64 ? rows - r : 65535 * 64;
-    p.rows = (int)n;
-    p.a += r * a_stride;
-    p.a_scales += r;
-    p.out = static_cast<char*>(d_out) + r * out_stride * (out_dtype == MYOS_F32 ? 4 : 2);
-    const dim3 grid((unsigned)((channels + 63) / 64), (unsigned)((n + 63) / 64));
-    const cudaError_t e =
-        out_dtype == MYOS_F32
-            ? counted(launch_pdl(k_matmul_i8<float>, grid, 256, 0, st, 1, p))
-            : counted(launch_pdl(k_matmul_i8<__nv_bfloat16>, grid, 256, 0, st, 1, p));
-    if (e != cudaSuccess) return MYOS_ERR_CUDA;
-  }
-  return MYOS_OK;
+  const cudaError_t e = out_dtype == MYOS_F32 ? launch<float>(g, wmap, amap, sms, st)
+                                              : launch<__nv_bfloat16>(g, wmap, amap, sms, st);
+  return e == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
 }
 
-int myos_dev_matmul_i8_status(void) { return MYOS_OK; }
+int myos_dev_matmul_i8_status(void) {
+  uint32_t failed = 0, none = 0;
+  if (cudaMemcpyFromSymbol(&failed, g_wait_failed, sizeof failed) != cudaSuccess) {
+    cudaGetLastError();
+    return MYOS_ERR_CUDA;
+  }
+  if (failed == 0) return MYOS_OK;
+  if (cudaMemcpyToSymbol(g_wait_failed, &none, sizeof none) != cudaSuccess) {
+    cudaGetLastError();
+    return MYOS_ERR_CUDA;
+  }
+  return MYOS_ERR_TIMEOUT;
+}
 
 }  // extern "C"
