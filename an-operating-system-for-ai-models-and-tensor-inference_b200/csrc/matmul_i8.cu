@@ -42,6 +42,30 @@ MYOS_DEV float scaled(int sum, float as, float ws, float bias) {
 MYOS_DEV void put(float* p, float v) { *p = v; }
 MYOS_DEV void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// Up to 16 rows of one channel. Whole groups without a branch: the loads, products
+// and stores of 16 rows overlap (a row at a time they took 95 cycles each).
+template <class OT>
+MYOS_DEV void store16(OT* o, int64_t stride, const int* v, const float* as, float ws, float bias,
+                      int left, bool ok) {
+  if (left >= 16 && ok) {
+    float a[16];
+#pragma unroll
+    for (int j = 0; j < 16; j += 4)
+      *reinterpret_cast<float4*>(a + j) = *reinterpret_cast<const float4*>(as + j);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      put(o, scaled(v[j], a[j], ws, bias));
+      o += stride;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (j < left) put(o, ok ? scaled(v[j], as[j], ws, bias) : __uint_as_float(0x7fc00000u));
+      o += stride;
+    }
+  }
+}
+
 constexpr int kThreads = 192;
 constexpr int kGroup = 16;  // row tiles that share a channel tile's weights in L2 before the next
 
@@ -61,7 +85,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const MatArgs g) {
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[kI8MaxStages], empty[kI8MaxStages], acc_full[2], acc_empty[2];
-  __shared__ float as[2][kI8MaxRows];
+  __shared__ __align__(16) float as[2][kI8MaxRows];
   __shared__ uint32_t tmem_s;
   __shared__ int dead;  // a wait of this block ran out
   uint8_t* const smem = raw + (-smem_u32(raw) & 1023);
@@ -153,7 +177,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (split == 1) {  // ---- scales and stores
     const int quarter = warp % 4, tid = threadIdx.x - 64;
-    const float nan = __uint_as_float(0x7fc00000u);
     bool ok = true;
     int n = 0;
     for (int64_t t = tile0; t < tiles; t += tile_step, ++n) {
@@ -170,18 +193,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       OT* o = static_cast<OT*>(g.out) + (int64_t)r0 * g.out_stride + c;
-      for (int j0 = 0; j0 < left; j0 += 16) {
-        int v[16];
-        tmem_load16(tmem + (quarter * 32 << 16) + b * p.tn + j0, v);
-        tmem_load_wait();
-        if (on) {
+      // 16 rows at a time, the next 16 on their way from tensor memory meanwhile
+      const uint32_t from = tmem + (quarter * 32 << 16) + b * p.tn;
+      int v[2][16];
+      tmem_load16(from, v[0]);
+      for (int j0 = 0; j0 < left; j0 += 32) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (j0 + j < left) {
-              const float y = scaled(v[j], as[b][j0 + j], ws, bias);
-              put(o + (int64_t)(j0 + j) * g.out_stride, ok ? y : nan);
-            }
-          }
+        for (int h = 0; h < 2; ++h) {
+          const int j = j0 + 16 * h;
+          if (j >= left) break;
+          tmem_load_wait();
+          if (j + 16 < left) tmem_load16(from + j + 16, v[h ^ 1]);
+          store16(o, g.out_stride, v[h], &as[b][j], ws, bias, on ? left - j : 0, ok);
+          o += 16 * g.out_stride;
         }
       }
       tc_fence_before();
