@@ -63,7 +63,7 @@ MYOS_DEV void load_some(const T* p, float* v, int n) {
   for (int e = 0; e < 8; ++e) v[e] = e < n ? get(p + e) : 0.0f;
 }
 
-MYOS_DEV double silu_up64(float g, float u) {
+__device__ __noinline__ double silu_up64(float g, float u) {
   return (double)g / (1.0 + exp(-(double)g)) * (double)u;
 }
 
@@ -72,8 +72,8 @@ MYOS_DEV double silu_up64(float g, float u) {
 // below -8 (rare in a gate) go through f64; the rest is off by 1.6 x 2^-20 at
 // most: the argument 2^-20, ex2 2^-22, rcp 2^-23, a sum and two products 2^-24
 // each.
+MYOS_DEV bool silu_fast(float g) { return g >= -8.0f; }
 MYOS_DEV float silu_up(float g, float u) {
-  if (!(g >= -8.0f)) return (float)silu_up64(g, u);
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
@@ -111,8 +111,17 @@ struct Row {
     } else if (KIND == kSwiglu) {
       if (FULL) load8(x + width + i, b);
       else load_some(x + width + i, b, n);
+      bool fast = true;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = silu_up(a[e], b[e]);
+      for (int e = 0; e < 8; ++e) {
+        p[e] = silu_up(a[e], b[e]);
+        fast &= silu_fast(a[e]);
+      }
+      if (!fast) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!silu_fast(a[e])) p[e] = (float)silu_up64(a[e], b[e]);
+      }
     } else {
       if (residual) {
         if (FULL) load8(residual + i, b);
@@ -142,7 +151,10 @@ struct Row {
   // The f32 value of one, its inputs read again.
   MYOS_DEV float value(int i) const {
     if (KIND == kQuant) return get(x + i);
-    if (KIND == kSwiglu) return silu_up(get(x + i), get(x + width + i));
+    if (KIND == kSwiglu) {
+      const float g = get(x + i), u = get(x + width + i);
+      return silu_fast(g) ? silu_up(g, u) : (float)silu_up64(g, u);
+    }
     const float t = total ? total[i] : residual ? __fadd_rn(get(x + i), residual[i]) : get(x + i);
     return __fmul_rn(t, bf16_at(gamma + i));
   }
@@ -154,11 +166,25 @@ struct Row {
 template <int KIND>
 constexpr float kRel = KIND == kSwiglu ? 3.8147e-6f : 9.5367e-7f;  // 2^-18, 2^-20
 
-// Magnitudes as integers: NaN above infinity above all others. The sign is taken
-// off the bits (arithmetic may leave a NaN's as it is).
-MYOS_DEV uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// The larger magnitude, NaN above infinity above all others.
+MYOS_DEV float larger(float a, float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(v)));
+  return r;
+}
+// The same order among integers. The sign is taken off the bits (arithmetic may
+// leave a NaN's as it is).
 MYOS_DEV uint64_t magnitude(double v) {
   return (uint64_t)__double_as_longlong(v) & 0x7fffffffffffffffull;
+}
+
+// v rounded to the nearest integer, in the low byte. The addition rounds: the sum's
+// last bit is 1 (rint and its conversion run at a quarter of the rate). open: v is
+// so near the border between two steps that it may lie on its other side.
+MYOS_DEV uint32_t step(float v, float rel, bool& open) {
+  const float t = __fadd_rn(v, 12582912.0f), off = v - __fsub_rn(t, 12582912.0f);
+  open |= !(fabsf(off) < __fmaf_rn(-fabsf(v), rel, 0.5f));
+  return __float_as_uint(t);
 }
 
 template <int KIND, class XT, int C, bool VEC, bool WARP>
@@ -185,7 +211,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
   constexpr int kHeld = VEC ? C : 1;
   float p[kHeld][8];
   double squares = 0.0;
-  uint32_t top = 0;  // as bits: NaN above infinity above all others
+  float largest = 0.0f;
   if constexpr (VEC) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -196,7 +222,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
         r.template values<false>(i, a.width - i, p[c], squares);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, magnitude(p[c][e]));
+      for (int e = 0; e < 8; ++e) largest = larger(largest, p[c][e]);
     }
   } else {
     for (int i = tid; i < a.width; i += team) {
@@ -205,14 +231,14 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
         if (r.total) r.total[i] = t;
         squares += (double)t * (double)t;
       }
-      top = max(top, magnitude(r.value(i)));
+      largest = larger(largest, r.value(i));
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     if (KIND == kNorm) squares += __shfl_xor_sync(0xffffffffu, squares, o);
   }
-  top = __reduce_max_sync(0xffffffffu, top);
+  uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(largest) & 0x7fffffffu);
   if (!WARP) {
     if (lane == 0) {
       sums[warp] = squares;
@@ -282,37 +308,44 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
     for (int c = 0; c < C; ++c) {
       const int i = (c * team + tid) * 8;
       if (i >= a.width) break;
-      uint32_t open = 0;
-      int s[8];
+      uint32_t s[8];
+      bool open = false;  // whether any may lie on the other side of a border
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = p[c][e] * per, n = rintf(v);
-        s[e] = (int)n;
-        // how far from the border between two steps
-        if (!(0.5f - fabsf(v - n) > fabsf(v) * rel)) open |= 1u << e;
-        if (!good) s[e] = 0;
+      for (int e = 0; e < 8; ++e) s[e] = step(p[c][e] * per, rel, open);
+      if (!good || zero) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = 0;
+        open = false;
       }
-      if (!good || zero) open = 0;
       if (i + 8 <= a.width) {
         uint2 w;
-        w.x = (s[0] & 255) | (s[1] & 255) << 8 | (s[2] & 255) << 16 | (uint32_t)s[3] << 24;
-        w.y = (s[4] & 255) | (s[5] & 255) << 8 | (s[6] & 255) << 16 | (uint32_t)s[7] << 24;
+        w.x = __byte_perm(__byte_perm(s[0], s[1], 0x0040), __byte_perm(s[2], s[3], 0x0040), 0x5410);
+        w.y = __byte_perm(__byte_perm(s[4], s[5], 0x0040), __byte_perm(s[6], s[7], 0x0040), 0x5410);
         *reinterpret_cast<uint2*>(q + i) = w;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (i + e < a.width) q[i + e] = (int8_t)s[e];
       }
-      while (open) {
-        const int j = i + __ffs(open) - 1;
-        open &= open - 1;
-        if (j < a.width) q[j] = (int8_t)decide(j);
+      if (open) {
+        uint32_t which = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          bool o = false;
+          step(p[c][e] * per, rel, o);
+          which |= o ? 1u << e : 0u;
+        }
+        while (which) {
+          const int j = i + __ffs(which) - 1;
+          which &= which - 1;
+          if (j < a.width) q[j] = (int8_t)decide(j);
+        }
       }
     }
   } else {
     for (int i = tid; i < a.width; i += team) {
-      const float v = r.value(i) * per, n = rintf(v);
-      const bool open = !(0.5f - fabsf(v - n) > fabsf(v) * rel);
+      bool open = false;
+      const uint32_t n = step(r.value(i) * per, rel, open);
       q[i] = (int8_t)(!good || zero ? 0 : open ? decide(i) : (int)n);
     }
   }
@@ -332,9 +365,15 @@ cudaError_t launch_kind(const RowArgs& a, bool vec, cudaStream_t st) {
   if (a.width <= 512) return launch<KIND, XT, 2, true, true>(a, 128, st);
   if (a.width <= 1024) return launch<KIND, XT, 4, true, true>(a, 128, st);
   const int chunks = (a.width + 7) / 8;
-  if (chunks <= 1024) return launch<KIND, XT, 1, true, false>(a, (chunks + 31) / 32 * 32, st);
-  if (chunks <= 2048) return launch<KIND, XT, 2, true, false>(a, (chunks + 63) / 64 * 32, st);
-  return launch<KIND, XT, 4, true, false>(a, (chunks + 127) / 128 * 32, st);
+  // Few rows: as many threads as chunks, for the latency. Many: more chunks a thread,
+  // so that more rows are on their way at once (norm of 8191 x 5120 f32 with 1, 2, 4:
+  // 118, 99, 91 us; of 8191 x 1536: 32, 30, 36 us; of 512 x 5120: 11.3, 11.5, 11.3 us).
+  const int many = a.rows < 512 ? 1 : chunks <= 256 ? 2 : 4;
+  const int each = chunks > 2048 || many == 4 ? 4 : chunks > 1024 || many == 2 ? 2 : 1;
+  const int threads = (chunks + 32 * each - 1) / (32 * each) * 32;
+  if (each == 1) return launch<KIND, XT, 1, true, false>(a, threads, st);
+  if (each == 2) return launch<KIND, XT, 2, true, false>(a, threads, st);
+  return launch<KIND, XT, 4, true, false>(a, threads, st);
 }
 
 // The checks that the three calls share, and the launch.
