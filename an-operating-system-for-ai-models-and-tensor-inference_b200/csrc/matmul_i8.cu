@@ -16,6 +16,10 @@
 #include <cudaTypedefs.h>
 #include <math.h>
 
+#include <algorithm>
+#include <type_traits>
+#include <stdlib.h>
+
 #include "i8_plan.h"
 #include "kernels.h"
 #include "paged.h"
@@ -27,10 +31,14 @@ namespace {
 struct MatArgs {
   void* out;
   int64_t out_stride;
+  const int8_t* a;
+  int64_t a_stride;
+  const int8_t* w;
+  int64_t w_stride;
   const float* a_scales;
   const float* w_scales;
   const float* bias;
-  int rows, channels, steps;
+  int rows, k, channels, steps;
   I8Plan plan;
 };
 
@@ -41,6 +49,15 @@ MYOS_DEV float scaled(int sum, float as, float ws, float bias) {
 }
 MYOS_DEV void put(float* p, float v) { *p = v; }
 MYOS_DEV void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+MYOS_DEV void put4(float* p, const float* v) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+MYOS_DEV void put4(__nv_bfloat16* p, const float* v) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a),
+                                            *reinterpret_cast<const uint32_t*>(&b));
+}
 
 // Up to 16 rows of one channel. Whole groups without a branch: the loads, products
 // and stores of 16 rows overlap (a row at a time they took 95 cycles each).
@@ -80,14 +97,14 @@ MYOS_DEV void tile_at(const I8Plan& p, int64_t t, int& c0, int& r0) {
 }
 
 template <class OT>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads)
     k_matmul_i8(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap amap,
                 const MatArgs g) {
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[kI8MaxStages], empty[kI8MaxStages], acc_full[2], acc_empty[2];
   __shared__ __align__(16) float as[2][kI8MaxRows];
   __shared__ uint32_t tmem_s;
-  __shared__ int dead;  // a wait of this block ran out
+  __shared__ int dead, peer_dead;  // a wait of this block, of one of its cluster, ran out
   uint8_t* const smem = raw + (-smem_u32(raw) & 1023);
   const I8Plan& p = g.plan;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -107,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 128);
     }
-    dead = 0;
+    dead = peer_dead = 0;
     mbar_fence_init();
   }
   if (warp == 1) tmem_alloc(&tmem_s, p.columns);
@@ -213,52 +230,211 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   if (split > 1) {  // ---- one tile, k shared by the cluster
+    // Each block ends up with 128 / split of the channels, of all rows: every block
+    // stores its sums of them into its shared memory straight from tensor memory
+    // (stores answer nothing, so no load waits for another block). Sums of large
+    // tiles go over the stages, once every block is done with its own.
     int c0, r0;
     tile_at(p, tile0, c0, r0);
-    const int left = min(p.tn, g.rows - r0);
-    int* const part = reinterpret_cast<int*>(smem);  // [row][channel], over the stages
+    const int left = min(p.tn, g.rows - r0), wide = kI8Channels / split;
+    int* const sums = reinterpret_cast<int*>(smem + (p.apart ? p.stages * stage_bytes : 0));
+    const int tid = threadIdx.x - 64, quarter = warp % 4;
+    // what a thread adds up: 4 channels of every (128 / (wide / 4))th row
+    const int part = tid % (wide / 4) * 4, first = tid / (wide / 4), c = c0 + rank * wide + part;
+    float ws[4], bias[4];
+    bool ok = true;
     if (warp >= 2) {
-      const int quarter = warp % 4;
-      bool ok = mbar_wait(&acc_full[0], 0, &g_wait_failed, kErrWaitFull);
+      for (int j = tid; j < left; j += 128) as[0][j] = g.a_scales[r0 + j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ws[i] = c + i < g.channels ? g.w_scales[c + i] : 0.0f;
+        bias[i] = g.bias && c + i < g.channels ? g.bias[c + i] : 0.0f;
+      }
+      ok = mbar_wait(&acc_full[0], 0, &g_wait_failed, kErrWaitFull);
       if (!ok) *(volatile int*)&dead = 1;
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      if (ok) {
-        for (int j0 = 0; j0 < left; j0 += 16) {
-          int v[16];
-          tmem_load16(tmem + (quarter * 32 << 16) + j0, v);
-          tmem_load_wait();
+    }
+    __syncwarp();
+    if (!p.apart) cluster_meet();
+    if (warp >= 2 && ok) {
+      const int ch = quarter * 32 + lane;
+      uint32_t at = cluster_at(sums + (rank * p.tn) * wide + ch % wide, ch / wide);
+      const uint32_t from = tmem + (quarter * 32 << 16);
+      int v[2][16];
+      tmem_load16(from, v[0]);
+      for (int j0 = 0; j0 < left; j0 += 32) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) part[(j0 + j) * kI8Channels + quarter * 32 + lane] = v[j];
+        for (int h = 0; h < 2; ++h) {
+          const int jh = j0 + 16 * h;
+          if (jh >= left) break;
+          tmem_load_wait();
+          if (jh + 16 < left) tmem_load16(from + jh + 16, v[h ^ 1]);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) cluster_store(at + j * wide * 4, v[h][j]);
+          at += 16 * wide * 4;
         }
       }
       tc_fence_before();
     }
-    __syncwarp();
-    cluster_meet();
-    if (warp >= 2) {
-      const int ch = threadIdx.x - 64, c = c0 + ch;
-      const bool on = c < g.channels;
-      const float ws = on ? g.w_scales[c] : 0.0f, bias = on && g.bias ? g.bias[c] : 0.0f;
-      int bad = 0;
-      for (int q = 0; q < split; ++q) bad |= cluster_load(cluster_at(&dead, q));
-      const int j1 = left * (rank + 1) / split;
-      for (int j = left * rank / split; j < j1; ++j) {
-        int sum = 0;
-        for (int q = 0; q < split; ++q)
-          sum += cluster_load(cluster_at(part + j * kI8Channels + ch, q));
-        if (on)
-          put(static_cast<OT*>(g.out) + (int64_t)(r0 + j) * g.out_stride + c,
-              bad ? __uint_as_float(0x7fc00000u) : scaled(sum, g.a_scales[r0 + j], ws, bias));
+    if (tid == 0) {
+      for (int q = 0; q < split; ++q) {
+        if (*(volatile int*)&dead) cluster_store(cluster_at(&peer_dead, q), 1);
       }
     }
     __syncwarp();
     cluster_meet();
+    if (warp >= 2) {
+      OT* const o = static_cast<OT*>(g.out) + (int64_t)r0 * g.out_stride + c;
+      const int* const mine = sums + part;
+      const bool bad = peer_dead, whole = p.vec && c + 4 <= g.channels;
+      auto join = [&](auto blocks) {
+        constexpr int S = decltype(blocks)::value;
+        for (int j = first; j < left; j += 512 / (kI8Channels / S)) {
+          int4 v[S];
+#pragma unroll
+          for (int q = 0; q < S; ++q)
+            v[q] = *reinterpret_cast<const int4*>(mine + (q * p.tn + j) * (kI8Channels / S));
+#pragma unroll
+          for (int q = 1; q < S; ++q)
+            v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
+          const float x = bad ? __uint_as_float(0x7fc00000u) : as[0][j];
+          const float y[4] = {scaled(v[0].x, x, ws[0], bias[0]), scaled(v[0].y, x, ws[1], bias[1]),
+                              scaled(v[0].z, x, ws[2], bias[2]), scaled(v[0].w, x, ws[3], bias[3])};
+          OT* const to = o + (int64_t)j * g.out_stride;
+          if (whole) {
+            put4(to, y);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (c + i < g.channels) put(to + i, y[i]);
+          }
+        }
+      };
+      if (split == 2) join(std::integral_constant<int, 2>());
+      else if (split == 4) join(std::integral_constant<int, 4>());
+      else join(std::integral_constant<int, 8>());
+    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_free(tmem, p.columns);
+}
+
+// ---- up to 16 rows: the weights pass once, from memory into registers
+//
+// mma.sync of 16 rows by 8 channels by 32 bytes of k. The order of k inside the
+// sum is free, so a lane takes 16 bytes of a channel at once (4 lanes 64 bytes of
+// it side by side) and feeds them to two products, the rows' bytes in the same
+// order. The block's warps share k and meet once in shared memory.
+MYOS_DEV void mma_i8(int* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                     uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, "
+      "%9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 bytes of a row from i on; zeros from k on, where nothing is read.
+MYOS_DEV uint4 piece(const int8_t* row, int i, int k) {
+  if (i + 16 <= k) return ld_stream(reinterpret_cast<const uint4*>(row + i));
+  uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (i + e < k) v[e / 4] |= (uint32_t)(uint8_t)row[i + e] << (8 * (e % 4));
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+constexpr int kFewRows = 16;
+
+// NT: groups of 8 channels a block. U: 64-byte pieces of k at once. HI: rows 8 to 15.
+template <class OT, int NT, int U, bool HI>
+__global__ void __launch_bounds__(512) k_few_i8(const MatArgs g) {
+  constexpr int kTok = HI ? 16 : 8, kCh = NT * 8;
+  extern __shared__ int parts[];  // [warp][row][channel]
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+  const int gr = lane / 4, q = lane % 4;
+  const int c0 = (int)blockIdx.x * kCh;
+  const int blocks = (g.k + 63) / 64;
+  const int b0 = (int)((int64_t)blocks * warp / warps), b1 = (int)((int64_t)blocks * (warp + 1) / warps);
+  const int8_t* wp[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+    wp[n] = g.w + (int64_t)min(c0 + n * 8 + gr, g.channels - 1) * g.w_stride + q * 16;
+  const int8_t* const lo = g.a + (int64_t)min(gr, g.rows - 1) * g.a_stride + q * 16;
+  const int8_t* const hi = g.a + (int64_t)min(gr + 8, g.rows - 1) * g.a_stride + q * 16;
+  const bool has_lo = gr < g.rows, has_hi = HI && gr + 8 < g.rows;
+  int acc[NT][4] = {};
+  pdl_wait();
+  pdl_launch();
+  const uint4 z = make_uint4(0, 0, 0, 0);
+  for (int b = b0; b < b1; b += U) {
+    uint4 w[U][NT], x[U], y[U];
+    if ((b + U) * 64 <= g.k && b + U <= b1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          w[u][n] = ld_stream(reinterpret_cast<const uint4*>(wp[n] + (b + u) * 64));
+        x[u] = has_lo ? *reinterpret_cast<const uint4*>(lo + (b + u) * 64) : z;
+        y[u] = has_hi ? *reinterpret_cast<const uint4*>(hi + (b + u) * 64) : z;
+      }
+    } else {  // the last pieces of this warp, or of the row
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool in = b + u < b1;
+        const int left = g.k - q * 16;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) w[u][n] = in ? piece(wp[n], (b + u) * 64, left) : z;
+        x[u] = in && has_lo ? piece(lo, (b + u) * 64, left) : z;
+        y[u] = in && has_hi ? piece(hi, (b + u) * 64, left) : z;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        mma_i8(acc[n], x[u].x, y[u].x, x[u].y, y[u].y, w[u][n].x, w[u][n].y);
+        mma_i8(acc[n], x[u].z, y[u].z, x[u].w, y[u].w, w[u][n].z, w[u][n].w);
+      }
+  }
+  int* const mine = parts + warp * kTok * kCh;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    *reinterpret_cast<int2*>(mine + gr * kCh + n * 8 + q * 2) = make_int2(acc[n][0], acc[n][1]);
+    if (HI)
+      *reinterpret_cast<int2*>(mine + (gr + 8) * kCh + n * 8 + q * 2) = make_int2(acc[n][2], acc[n][3]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < g.rows * kCh; i += blockDim.x) {
+    const int r = i / kCh, c = c0 + i % kCh;
+    int sum = 0;
+    for (int p = 0; p < warps; ++p) sum += parts[p * kTok * kCh + i];
+    if (c < g.channels)
+      put(static_cast<OT*>(g.out) + (int64_t)r * g.out_stride + c,
+          scaled(sum, g.a_scales[r], g.w_scales[c], g.bias ? g.bias[c] : 0.0f));
+  }
+}
+
+template <class OT, int NT, int U>
+cudaError_t launch_few_of(const MatArgs& g, int warps, cudaStream_t st) {
+  const bool hi = g.rows > 8;
+  const size_t smem = (size_t)warps * (hi ? 16 : 8) * NT * 8 * 4;
+  const dim3 grid((unsigned)i8_ceil(g.channels, NT * 8));
+  return counted(hi ? launch_pdl(k_few_i8<OT, NT, U, true>, grid, warps * 32, smem, st, 1, g)
+                    : launch_pdl(k_few_i8<OT, NT, U, false>, grid, warps * 32, smem, st, 1, g));
+}
+template <class OT>
+cudaError_t launch_few(const MatArgs& g, int sms, cudaStream_t st) {
+  const char* e1 = getenv("FEW_NT"); const char* e2 = getenv("FEW_W");
+  int nt = e1 ? atoi(e1) : 0, w = e2 ? atoi(e2) : 0;
+  if (!w) w = 8;
+  if (!nt) nt = i8_ceil(g.channels, 32) * w >= sms * 32 ? 4 : i8_ceil(g.channels, 16) * w >= sms * 32 ? 2 : 1;
+  if (nt == 4) return launch_few_of<OT, 4, 3>(g, w, st);
+  if (nt == 2) return launch_few_of<OT, 2, 4>(g, w, st);
+  return launch_few_of<OT, 1, 6>(g, w, st);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -292,13 +468,13 @@ bool map_rows(CUtensorMap* map, const int8_t* p, int64_t k, int64_t rows, int64_
 template <class OT>
 cudaError_t launch(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap& amap, int sms,
                    cudaStream_t st) {
-  constexpr size_t kSmem = kI8StageBytes + 1024;
   static std::atomic<uint64_t> raised{0};
-  const cudaError_t e = raise_smem_limit((const void*)k_matmul_i8<OT>, kSmem, &raised);
+  const cudaError_t e = raise_smem_limit((const void*)k_matmul_i8<OT>, kI8Smem + 1024, &raised);
   if (e != cudaSuccess) return e;
+  const size_t smem = (g.plan.two ? kI8SmemTwo : kI8Smem) + 1024;
   const int64_t tiles = (int64_t)g.plan.tiles_c * g.plan.tiles_r;
-  const int64_t blocks = g.plan.split > 1 ? tiles * g.plan.split : tiles < sms ? tiles : sms;
-  return counted(launch_pdl(k_matmul_i8<OT>, dim3((unsigned)blocks), kThreads, kSmem, st,
+  const int64_t blocks = g.plan.split > 1 ? tiles * g.plan.split : std::min<int64_t>(tiles, sms * (g.plan.two ? 2 : 1));
+  return counted(launch_pdl(k_matmul_i8<OT>, dim3((unsigned)blocks), kThreads, smem, st,
                             g.plan.split, wmap, amap, g));
 }
 
@@ -329,13 +505,25 @@ int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const 
   MatArgs g;
   g.out = d_out;
   g.out_stride = (int64_t)out_stride;
+  g.a = d_a;
+  g.a_stride = (int64_t)a_stride;
+  g.w = d_w;
+  g.w_stride = (int64_t)w_stride;
+  g.k = (int)k;
   g.a_scales = d_a_scales;
   g.w_scales = d_w_scales;
   g.bias = d_bias;
   g.rows = (int)rows;
   g.channels = (int)channels;
   g.steps = i8_ceil((int64_t)k, kI8Step);
+  const size_t size = out_dtype == MYOS_F32 ? 4 : 2;
   g.plan = i8_plan((int64_t)rows, (int64_t)k, (int64_t)channels, sms);
+  g.plan.vec = aligned(d_out, 4 * size) && (rows == 1 || out_stride % 4 == 0);
+  if (rows <= kFewRows && !getenv("NO_FEW")) {
+    const cudaError_t e = out_dtype == MYOS_F32 ? launch_few<float>(g, sms, (cudaStream_t)stream)
+                                                : launch_few<__nv_bfloat16>(g, sms, (cudaStream_t)stream);
+    return e == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
+  }
   CUtensorMap wmap, amap;
   if (!map_rows(&wmap, d_w, (int64_t)k, (int64_t)channels, (int64_t)w_stride, kI8Channels) ||
       !map_rows(&amap, d_a, (int64_t)k, (int64_t)rows, (int64_t)a_stride, g.plan.tn))

@@ -90,10 +90,8 @@ MYOS_DEV uint32_t cluster_at(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
 }
-MYOS_DEV int cluster_load(uint32_t at) {
-  int v;
-  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-  return v;
+MYOS_DEV void cluster_store(uint32_t at, int v) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
 
 }  // namespace myos
