@@ -92,11 +92,11 @@ MYOS_DEV void tile_at(const I8Plan& p, int64_t t, int& c0, int& r0) {
   const int first = (int)group * kGroup;
   const int wide = min(kGroup, p.tiles_r - first);
   const int64_t in = t - group * kGroup * p.tiles_c;
-  c0 = (int)(in / wide) * kI8Channels;
+  c0 = (int)(in / wide) * p.tc;
   r0 = (first + (int)(in % wide)) * p.tn;
 }
 
-template <class OT>
+template <class OT, bool PAIR>
 __global__ void __launch_bounds__(kThreads)
     k_matmul_i8(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap amap,
                 const MatArgs g) {
@@ -108,12 +108,14 @@ __global__ void __launch_bounds__(kThreads)
   uint8_t* const smem = raw + (-smem_u32(raw) & 1023);
   const I8Plan& p = g.plan;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint32_t stage_bytes = (kI8Channels + p.tn) * kI8Step;
-  const int split = p.split, rank = split > 1 ? (int)cluster_rank() : 0;
-  const int k0 = (int)((int64_t)g.steps * rank / split);
-  const int k1 = (int)((int64_t)g.steps * (rank + 1) / split);
+  constexpr int kPair = PAIR ? 2 : 1;
+  const uint32_t stage_bytes = (kI8Channels + p.tn / kPair) * kI8Step;
+  const int split = PAIR ? 1 : p.split;
+  const int rank = PAIR || split > 1 ? (int)cluster_rank() : 0;
+  const int k0 = PAIR ? 0 : (int)((int64_t)g.steps * rank / split);
+  const int k1 = PAIR ? g.steps : (int)((int64_t)g.steps * (rank + 1) / split);
   const int64_t tiles = (int64_t)p.tiles_c * p.tiles_r;
-  const int64_t tile0 = blockIdx.x / split, tile_step = gridDim.x / split;
+  const int64_t tile0 = blockIdx.x / (kPair * split), tile_step = gridDim.x / (kPair * split);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -122,14 +124,17 @@ __global__ void __launch_bounds__(kThreads)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 128);
+      mbar_init(&acc_empty[b], 128 * kPair);
     }
     dead = peer_dead = 0;
     mbar_fence_init();
   }
-  if (warp == 1) tmem_alloc(&tmem_s, p.columns);
+  __syncwarp();
+  if (warp == 1) tmem_alloc<PAIR>(&tmem_s, p.columns);
   tc_fence_before();
-  __syncthreads();
+  // before a block's shared memory is written from another it has to be there
+  if (PAIR || split > 1) cluster_meet();
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_s;
   pdl_wait();
@@ -148,16 +153,25 @@ __global__ void __launch_bounds__(kThreads)
             break;
           }
           uint8_t* const at = smem + s * stage_bytes;
-          mbar_arrive_expect_tx(&full[s], stage_bytes);
-          tma_load_2d(at, &wmap, k * kI8Step, c0, &full[s]);
-          tma_load_2d(at + kI8Channels * kI8Step, &amap, k * kI8Step, r0, &full[s]);
+          if constexpr (PAIR) {
+            // both blocks' copies are counted where the products wait for them
+            const uint32_t bar = cluster_at(&full[s], 0);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * stage_bytes);
+            tma_load_2d_pair(at, &wmap, k * kI8Step, c0 + rank * kI8Channels, bar);
+            tma_load_2d_pair(at + kI8Channels * kI8Step, &amap, k * kI8Step, r0 + rank * (p.tn / 2),
+                             bar);
+          } else {
+            mbar_arrive_expect_tx(&full[s], stage_bytes);
+            tma_load_2d(at, &wmap, k * kI8Step, c0, &full[s]);
+            tma_load_2d(at + kI8Channels * kI8Step, &amap, k * kI8Step, r0, &full[s]);
+          }
           ++issued;
           if (++s == p.stages) s = 0, phase ^= 1;
         }
       }
       if (!ok) {  // its copies in flight are waited for before the block ends
         *(volatile int*)&dead = 1;
-        for (int n = min(issued, p.stages); n > 0; --n) {
+        for (int n = rank == 0 || !PAIR ? min(issued, p.stages) : 0; n > 0; --n) {
           if (--s < 0) s = p.stages - 1, phase ^= 1;
           mbar_wait(&full[s], phase, &g_wait_failed, kErrWaitFull);
         }
@@ -165,8 +179,8 @@ __global__ void __launch_bounds__(kThreads)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {  // ---- products
-      const uint32_t shape = tc_i8_shape(kI8Channels, p.tn);
+    if (lane == 0 && (!PAIR || rank == 0)) {  // ---- products
+      const uint32_t shape = tc_i8_shape(kPair * kI8Channels, p.tn);
       int s = 0, phase = 0, n = 0;
       bool ok = true;
       for (int64_t t = tile0; ok && t < tiles; t += tile_step, ++n) {
@@ -183,11 +197,11 @@ __global__ void __launch_bounds__(kThreads)
           const uint64_t wd = tc_operand(at), ad = tc_operand(at + kI8Channels * kI8Step);
 #pragma unroll
           for (int i = 0; i < kI8Step / 32; ++i)
-            tc_mma_i8(d, wd + 2 * i, ad + 2 * i, shape, k > k0 || i > 0);
-          tc_commit(&empty[s]);
+            tc_mma_i8<PAIR>(d, wd + 2 * i, ad + 2 * i, shape, k > k0 || i > 0);
+          tc_commit<PAIR>(&empty[s]);
           if (++s == p.stages) s = 0, phase ^= 1;
         }
-        if (ok) tc_commit(&acc_full[b]);
+        if (ok) tc_commit<PAIR>(&acc_full[b]);
       }
       if (!ok) *(volatile int*)&dead = 1;
     }
@@ -201,7 +215,7 @@ __global__ void __launch_bounds__(kThreads)
       tile_at(p, t, c0, r0);
       const int b = n & 1, left = min(p.tn, g.rows - r0);
       for (int j = tid; j < left; j += 128) as[b][j] = g.a_scales[r0 + j];
-      const int c = c0 + quarter * 32 + lane;
+      const int c = c0 + (PAIR ? rank * kI8Channels : 0) + quarter * 32 + lane;
       const bool on = c < g.channels;
       const float ws = on ? g.w_scales[c] : 0.0f, bias = on && g.bias ? g.bias[c] : 0.0f;
       named_sync(1, 128);
@@ -226,10 +240,11 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
       tc_fence_before();
-      mbar_arrive(&acc_empty[b]);
+      if (PAIR) cluster_arrive(cluster_at(&acc_empty[b], 0));
+      else mbar_arrive(&acc_empty[b]);
     }
   }
-  if (split > 1) {  // ---- one tile, k shared by the cluster
+  if (!PAIR && split > 1) {  // ---- one tile, k shared by the cluster
     // Each block ends up with 128 / split of the channels, of all rows: every block
     // stores its sums of them into its shared memory straight from tensor memory
     // (stores answer nothing, so no load waits for another block). Sums of large
@@ -316,10 +331,12 @@ __global__ void __launch_bounds__(kThreads)
       else join(std::integral_constant<int, 8>());
     }
   }
+  __syncwarp();
   tc_fence_before();
-  __syncthreads();
+  if (PAIR) cluster_meet();
+  else __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_free(tmem, p.columns);
+  if (warp == 1) tmem_free<PAIR>(tmem, p.columns);
 }
 
 // ---- up to 16 rows: the weights pass once, from memory into registers
@@ -465,17 +482,26 @@ bool map_rows(CUtensorMap* map, const int8_t* p, int64_t k, int64_t rows, int64_
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class OT>
+template <class OT, bool PAIR>
 cudaError_t launch(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap& amap, int sms,
                    cudaStream_t st) {
   static std::atomic<uint64_t> raised{0};
-  const cudaError_t e = raise_smem_limit((const void*)k_matmul_i8<OT>, kI8Smem + 1024, &raised);
+  const cudaError_t e =
+      raise_smem_limit((const void*)k_matmul_i8<OT, PAIR>, kI8Smem + 1024, &raised);
   if (e != cudaSuccess) return e;
   const size_t smem = (g.plan.two ? kI8SmemTwo : kI8Smem) + 1024;
   const int64_t tiles = (int64_t)g.plan.tiles_c * g.plan.tiles_r;
-  const int64_t blocks = g.plan.split > 1 ? tiles * g.plan.split : std::min<int64_t>(tiles, sms * (g.plan.two ? 2 : 1));
-  return counted(launch_pdl(k_matmul_i8<OT>, dim3((unsigned)blocks), kThreads, smem, st,
-                            g.plan.split, wmap, amap, g));
+  const int blocks_a_tile = PAIR ? 2 : g.plan.split;
+  const int64_t most = PAIR ? sms / 2 : sms * (g.plan.two ? 2 : 1);
+  const int64_t at_once = g.plan.split > 1 ? tiles : std::min(tiles, most);
+  return counted(launch_pdl(k_matmul_i8<OT, PAIR>, dim3((unsigned)(at_once * blocks_a_tile)),
+                            kThreads, smem, st, blocks_a_tile, wmap, amap, g));
+}
+template <class OT>
+cudaError_t launch_tiles(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap& amap,
+                         int sms, cudaStream_t st) {
+  return g.plan.pair ? launch<OT, true>(g, wmap, amap, sms, st)
+                     : launch<OT, false>(g, wmap, amap, sms, st);
 }
 
 }  // namespace
@@ -526,11 +552,12 @@ int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const 
   }
   CUtensorMap wmap, amap;
   if (!map_rows(&wmap, d_w, (int64_t)k, (int64_t)channels, (int64_t)w_stride, kI8Channels) ||
-      !map_rows(&amap, d_a, (int64_t)k, (int64_t)rows, (int64_t)a_stride, g.plan.tn))
+      !map_rows(&amap, d_a, (int64_t)k, (int64_t)rows, (int64_t)a_stride,
+                g.plan.tn / (g.plan.pair ? 2 : 1)))
     return MYOS_ERR_CUDA;
   const cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = out_dtype == MYOS_F32 ? launch<float>(g, wmap, amap, sms, st)
-                                              : launch<__nv_bfloat16>(g, wmap, amap, sms, st);
+  const cudaError_t e = out_dtype == MYOS_F32 ? launch_tiles<float>(g, wmap, amap, sms, st)
+                                              : launch_tiles<__nv_bfloat16>(g, wmap, amap, sms, st);
   return e == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
 }
 
