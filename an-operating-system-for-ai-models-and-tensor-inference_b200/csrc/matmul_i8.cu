@@ -18,7 +18,6 @@
 
 #include <algorithm>
 #include <type_traits>
-#include <stdlib.h>
 
 #include "i8_plan.h"
 #include "kernels.h"
@@ -84,14 +83,11 @@ MYOS_DEV void store16(OT* o, int64_t stride, const int* v, const float* as, floa
 }
 
 constexpr int kThreads = 192;
-constexpr int kGroup = 16;  // row tiles that share a channel tile's weights in L2 before the next
-
 // Tile t: its first channel and row.
 MYOS_DEV void tile_at(const I8Plan& p, int64_t t, int& c0, int& r0) {
-  const int64_t group = t / ((int64_t)kGroup * p.tiles_c);
-  const int first = (int)group * kGroup;
-  const int wide = min(kGroup, p.tiles_r - first);
-  const int64_t in = t - group * kGroup * p.tiles_c;
+  const int64_t each = (int64_t)p.group * p.tiles_c;
+  const int first = (int)(t / each) * p.group, wide = min(p.group, p.tiles_r - first);
+  const int64_t in = t % each;
   c0 = (int)(in / wide) * p.tc;
   r0 = (first + (int)(in % wide)) * p.tn;
 }
@@ -104,12 +100,15 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ uint64_t full[kI8MaxStages], empty[kI8MaxStages], acc_full[2], acc_empty[2];
   __shared__ __align__(16) float as[2][kI8MaxRows];
   __shared__ uint32_t tmem_s;
-  __shared__ int dead, peer_dead;  // a wait of this block, of one of its cluster, ran out
+  __shared__ int peer_dead;  // a wait of a block of the cluster ran out
   uint8_t* const smem = raw + (-smem_u32(raw) & 1023);
   const I8Plan& p = g.plan;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   constexpr int kPair = PAIR ? 2 : 1;
-  const uint32_t stage_bytes = (kI8Channels + p.tn / kPair) * kI8Step;
+  const int tr = p.tn / kPair;  // rows that a block copies
+  // rows of a tile that the tensor core takes: of the last one no more than there are
+  auto taken = [&](int r0) { return min(p.tn, (g.rows - r0 + 16 * kPair - 1) / (16 * kPair) * (16 * kPair)); };
+  const uint32_t stage_bytes = (kI8Channels + tr) * kI8Step;
   const int split = PAIR ? 1 : p.split;
   const int rank = PAIR || split > 1 ? (int)cluster_rank() : 0;
   const int k0 = PAIR ? 0 : (int)((int64_t)g.steps * rank / split);
@@ -126,15 +125,20 @@ __global__ void __launch_bounds__(kThreads)
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 128 * kPair);
     }
-    dead = peer_dead = 0;
+    peer_dead = 0;
     mbar_fence_init();
   }
   __syncwarp();
   if (warp == 1) tmem_alloc<PAIR>(&tmem_s, p.columns);
   tc_fence_before();
-  // before a block's shared memory is written from another it has to be there
-  if (PAIR || split > 1) cluster_meet();
-  else __syncthreads();
+  // before a block's shared memory is written from another it has to be there: a
+  // pair's at once, the others' before the sums go out
+  if (PAIR) {
+    cluster_meet();
+  } else {
+    if (split > 1) cluster_enter();
+    __syncthreads();
+  }
   tc_fence_after();
   const uint32_t tmem = tmem_s;
   pdl_wait();
@@ -147,6 +151,7 @@ __global__ void __launch_bounds__(kThreads)
       for (int64_t t = tile0; ok && t < tiles; t += tile_step) {
         int c0, r0;
         tile_at(p, t, c0, r0);
+        const int rank_r0 = PAIR && rank ? r0 + taken(r0) / 2 : r0;
         for (int k = k0; k < k1; ++k) {
           if (!mbar_wait(&empty[s], phase ^ 1, &g_wait_failed, kErrWaitEmpty)) {
             ok = false;
@@ -158,8 +163,7 @@ __global__ void __launch_bounds__(kThreads)
             const uint32_t bar = cluster_at(&full[s], 0);
             if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * stage_bytes);
             tma_load_2d_pair(at, &wmap, k * kI8Step, c0 + rank * kI8Channels, bar);
-            tma_load_2d_pair(at + kI8Channels * kI8Step, &amap, k * kI8Step, r0 + rank * (p.tn / 2),
-                             bar);
+            tma_load_2d_pair(at + kI8Channels * kI8Step, &amap, k * kI8Step, rank_r0, bar);
           } else {
             mbar_arrive_expect_tx(&full[s], stage_bytes);
             tma_load_2d(at, &wmap, k * kI8Step, c0, &full[s]);
@@ -170,7 +174,6 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
       if (!ok) {  // its copies in flight are waited for before the block ends
-        *(volatile int*)&dead = 1;
         for (int n = rank == 0 || !PAIR ? min(issued, p.stages) : 0; n > 0; --n) {
           if (--s < 0) s = p.stages - 1, phase ^= 1;
           mbar_wait(&full[s], phase, &g_wait_failed, kErrWaitFull);
@@ -180,7 +183,6 @@ __global__ void __launch_bounds__(kThreads)
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0 && (!PAIR || rank == 0)) {  // ---- products
-      const uint32_t shape = tc_i8_shape(kPair * kI8Channels, p.tn);
       int s = 0, phase = 0, n = 0;
       bool ok = true;
       for (int64_t t = tile0; ok && t < tiles; t += tile_step, ++n) {
@@ -188,6 +190,9 @@ __global__ void __launch_bounds__(kThreads)
         ok = mbar_wait(&acc_empty[b], (n >> 1 & 1) ^ 1, &g_wait_failed, kErrWaitEmpty);
         if (!ok) break;
         tc_fence_after();
+        int c0, r0;
+        tile_at(p, t, c0, r0);
+        const uint32_t shape = tc_i8_shape(kPair * kI8Channels, taken(r0));
         const uint32_t d = tmem + b * p.tn;
         for (int k = k0; k < k1; ++k) {
           ok = mbar_wait(&full[s], phase, &g_wait_failed, kErrWaitFull);
@@ -203,7 +208,6 @@ __global__ void __launch_bounds__(kThreads)
         }
         if (ok) tc_commit<PAIR>(&acc_full[b]);
       }
-      if (!ok) *(volatile int*)&dead = 1;
     }
     __syncwarp();
   } else if (split == 1) {  // ---- scales and stores
@@ -220,7 +224,6 @@ __global__ void __launch_bounds__(kThreads)
       const float ws = on ? g.w_scales[c] : 0.0f, bias = on && g.bias ? g.bias[c] : 0.0f;
       named_sync(1, 128);
       if (ok) ok = mbar_wait(&acc_full[b], n >> 1 & 1, &g_wait_failed, kErrWaitFull);
-      if (!ok) *(volatile int*)&dead = 1;
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       OT* o = static_cast<OT*>(g.out) + (int64_t)r0 * g.out_stride + c;
@@ -245,32 +248,33 @@ __global__ void __launch_bounds__(kThreads)
     }
   }
   if (!PAIR && split > 1) {  // ---- one tile, k shared by the cluster
-    // Each block ends up with 128 / split of the channels, of all rows: every block
+    // Each block ends up with i8_wide(split) of the channels, of all rows: every block
     // stores its sums of them into its shared memory straight from tensor memory
     // (stores answer nothing, so no load waits for another block). Sums of large
     // tiles go over the stages, once every block is done with its own.
     int c0, r0;
     tile_at(p, tile0, c0, r0);
-    const int left = min(p.tn, g.rows - r0), wide = kI8Channels / split;
+    const int left = min(p.tn, g.rows - r0), wide = i8_wide(split);
     int* const sums = reinterpret_cast<int*>(smem + (p.apart ? p.stages * stage_bytes : 0));
     const int tid = threadIdx.x - 64, quarter = warp % 4;
-    // what a thread adds up: 4 channels of every (128 / (wide / 4))th row
+    // what a thread adds up: 4 channels of one row in 128 / (wide / 4)
     const int part = tid % (wide / 4) * 4, first = tid / (wide / 4), c = c0 + rank * wide + part;
+    const int end = min(g.channels, c0 + kI8Channels);
     float ws[4], bias[4];
     bool ok = true;
     if (warp >= 2) {
       for (int j = tid; j < left; j += 128) as[0][j] = g.a_scales[r0 + j];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        ws[i] = c + i < g.channels ? g.w_scales[c + i] : 0.0f;
-        bias[i] = g.bias && c + i < g.channels ? g.bias[c + i] : 0.0f;
+        ws[i] = c + i < end ? g.w_scales[c + i] : 0.0f;
+        bias[i] = g.bias && c + i < end ? g.bias[c + i] : 0.0f;
       }
       ok = mbar_wait(&acc_full[0], 0, &g_wait_failed, kErrWaitFull);
-      if (!ok) *(volatile int*)&dead = 1;
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
     __syncwarp();
+    cluster_leave();  // of the start
     if (!p.apart) cluster_meet();
     if (warp >= 2 && ok) {
       const int ch = quarter * 32 + lane;
@@ -292,24 +296,22 @@ __global__ void __launch_bounds__(kThreads)
       }
       tc_fence_before();
     }
-    if (tid == 0) {
-      for (int q = 0; q < split; ++q) {
-        if (*(volatile int*)&dead) cluster_store(cluster_at(&peer_dead, q), 1);
-      }
-    }
+    if (warp >= 2 && !ok && lane == 0)
+      for (int q = 0; q < split; ++q) cluster_store(cluster_at(&peer_dead, q), 1);
     __syncwarp();
     cluster_meet();
     if (warp >= 2) {
       OT* const o = static_cast<OT*>(g.out) + (int64_t)r0 * g.out_stride + c;
       const int* const mine = sums + part;
-      const bool bad = peer_dead, whole = p.vec && c + 4 <= g.channels;
+      const bool bad = peer_dead, whole = p.vec && c + 4 <= end;
       auto join = [&](auto blocks) {
-        constexpr int S = decltype(blocks)::value;
-        for (int j = first; j < left; j += 512 / (kI8Channels / S)) {
+        constexpr int S = decltype(blocks)::value, kWide = i8_wide(S), kRows = 128 / (kWide / 4);
+        if (first >= kRows || c >= end) return;
+        for (int j = first; j < left; j += kRows) {
           int4 v[S];
 #pragma unroll
           for (int q = 0; q < S; ++q)
-            v[q] = *reinterpret_cast<const int4*>(mine + (q * p.tn + j) * (kI8Channels / S));
+            v[q] = *reinterpret_cast<const int4*>(mine + (q * p.tn + j) * kWide);
 #pragma unroll
           for (int q = 1; q < S; ++q)
             v[0].x += v[q].x, v[0].y += v[q].y, v[0].z += v[q].z, v[0].w += v[q].w;
@@ -322,13 +324,19 @@ __global__ void __launch_bounds__(kThreads)
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (c + i < g.channels) put(to + i, y[i]);
+              if (c + i < end) put(to + i, y[i]);
           }
         }
       };
-      if (split == 2) join(std::integral_constant<int, 2>());
-      else if (split == 4) join(std::integral_constant<int, 4>());
-      else join(std::integral_constant<int, 8>());
+      switch (split) {
+        case 2: join(std::integral_constant<int, 2>()); break;
+        case 3: join(std::integral_constant<int, 3>()); break;
+        case 4: join(std::integral_constant<int, 4>()); break;
+        case 5: join(std::integral_constant<int, 5>()); break;
+        case 6: join(std::integral_constant<int, 6>()); break;
+        case 7: join(std::integral_constant<int, 7>()); break;
+        default: join(std::integral_constant<int, 8>());
+      }
     }
   }
   __syncwarp();
@@ -363,8 +371,6 @@ MYOS_DEV uint4 piece(const int8_t* row, int i, int k) {
     if (i + e < k) v[e / 4] |= (uint32_t)(uint8_t)row[i + e] << (8 * (e % 4));
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
-
-constexpr int kFewRows = 16;
 
 // NT: groups of 8 channels a block. U: 64-byte pieces of k at once. HI: rows 8 to 15.
 template <class OT, int NT, int U, bool HI>
@@ -444,14 +450,10 @@ cudaError_t launch_few_of(const MatArgs& g, int warps, cudaStream_t st) {
                     : launch_pdl(k_few_i8<OT, NT, U, false>, grid, warps * 32, smem, st, 1, g));
 }
 template <class OT>
-cudaError_t launch_few(const MatArgs& g, int sms, cudaStream_t st) {
-  const char* e1 = getenv("FEW_NT"); const char* e2 = getenv("FEW_W");
-  int nt = e1 ? atoi(e1) : 0, w = e2 ? atoi(e2) : 0;
-  if (!w) w = 8;
-  if (!nt) nt = i8_ceil(g.channels, 32) * w >= sms * 32 ? 4 : i8_ceil(g.channels, 16) * w >= sms * 32 ? 2 : 1;
-  if (nt == 4) return launch_few_of<OT, 4, 3>(g, w, st);
-  if (nt == 2) return launch_few_of<OT, 2, 4>(g, w, st);
-  return launch_few_of<OT, 1, 6>(g, w, st);
+cudaError_t launch_few(const MatArgs& g, const I8Few& f, cudaStream_t st) {
+  if (f.groups == 4) return launch_few_of<OT, 4, 3>(g, f.warps, st);
+  if (f.groups == 2) return launch_few_of<OT, 2, 4>(g, f.warps, st);
+  return launch_few_of<OT, 1, 6>(g, f.warps, st);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -497,6 +499,46 @@ cudaError_t launch(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap&
   return counted(launch_pdl(k_matmul_i8<OT, PAIR>, dim3((unsigned)(at_once * blocks_a_tile)),
                             kThreads, smem, st, blocks_a_tile, wmap, amap, g));
 }
+// The clusters that the current device holds, asked once (clusters of more than the
+// blocks of one cluster share what a group of multiprocessors has over).
+I8Device this_device() {
+  static std::atomic<uint64_t> known[64][kI8MaxSplit + 1];
+  I8Device d = {};
+  d.sms = sm_count();
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return d;  // nothing is split
+  const void* const kernel = (const void*)k_matmul_i8<float, false>;
+  for (int s = 2; s <= kI8MaxSplit; ++s) {
+    uint64_t v = known[dev][s].load(std::memory_order_relaxed);
+    if (v == 0) {
+      int n[2] = {0, 0};
+      for (int two = 0; two < 2; ++two) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)s);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = (two ? kI8SmemTwo : kI8Smem) + 1024;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)s;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        static std::atomic<uint64_t> raised{0};
+        if (raise_smem_limit(kernel, kI8Smem + 1024, &raised) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n[two], kernel, &cfg) != cudaSuccess) {
+          cudaGetLastError();
+          n[two] = 0;
+        }
+      }
+      v = (uint64_t)1 << 63 | (uint64_t)(n[0] * s) << 31 | (uint64_t)(n[1] * s);
+      known[dev][s].store(v, std::memory_order_relaxed);
+    }
+    d.one[s] = (int)(v >> 31 & 0x7fffffff);
+    d.two[s] = (int)(v & 0x7fffffff);
+  }
+  return d;
+}
+
 template <class OT>
 cudaError_t launch_tiles(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap& amap,
                          int sms, cudaStream_t st) {
@@ -527,7 +569,6 @@ int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const 
       a_stride % 16 != 0 || w_stride % 16 != 0 || !aligned(d_a_scales, 4) ||
       !aligned(d_w_scales, 4) || !aligned(d_bias, 4))
     return MYOS_ERR_ARG;
-  const int sms = sm_count();
   MatArgs g;
   g.out = d_out;
   g.out_stride = (int64_t)out_stride;
@@ -541,15 +582,19 @@ int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const 
   g.bias = d_bias;
   g.rows = (int)rows;
   g.channels = (int)channels;
-  g.steps = i8_ceil((int64_t)k, kI8Step);
-  const size_t size = out_dtype == MYOS_F32 ? 4 : 2;
-  g.plan = i8_plan((int64_t)rows, (int64_t)k, (int64_t)channels, sms);
-  g.plan.vec = aligned(d_out, 4 * size) && (rows == 1 || out_stride % 4 == 0);
-  if (rows <= kFewRows && !getenv("NO_FEW")) {
-    const cudaError_t e = out_dtype == MYOS_F32 ? launch_few<float>(g, sms, (cudaStream_t)stream)
-                                                : launch_few<__nv_bfloat16>(g, sms, (cudaStream_t)stream);
+  g.steps = (int)i8_ceil((int64_t)k, kI8Step);
+  const I8Few few = i8_few((int64_t)rows, (int64_t)k, (int64_t)channels);
+  if (few.use) {
+    const cudaError_t e = out_dtype == MYOS_F32
+                              ? launch_few<float>(g, few, (cudaStream_t)stream)
+                              : launch_few<__nv_bfloat16>(g, few, (cudaStream_t)stream);
     return e == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
   }
+  const size_t size = out_dtype == MYOS_F32 ? 4 : 2;
+  const I8Device device = this_device();
+  const int sms = device.sms;
+  g.plan = i8_plan((int64_t)rows, (int64_t)k, (int64_t)channels, device);
+  g.plan.vec = aligned(d_out, 4 * size) && (rows == 1 || out_stride % 4 == 0);
   CUtensorMap wmap, amap;
   if (!map_rows(&wmap, d_w, (int64_t)k, (int64_t)channels, (int64_t)w_stride, kI8Channels) ||
       !map_rows(&amap, d_a, (int64_t)k, (int64_t)rows, (int64_t)a_stride,

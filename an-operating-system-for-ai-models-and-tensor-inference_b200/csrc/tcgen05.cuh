@@ -117,14 +117,12 @@ MYOS_DEV uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-MYOS_DEV uint32_t cluster_blocks() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
+// All threads of the cluster meet; in two parts, with work between them.
+MYOS_DEV void cluster_enter() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+MYOS_DEV void cluster_leave() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 MYOS_DEV void cluster_meet() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_enter();
+  cluster_leave();
 }
 // The address in block `rank` of the cluster of what lies at p in this one.
 MYOS_DEV uint32_t cluster_at(const void* p, uint32_t rank) {
