@@ -499,15 +499,18 @@ cudaError_t launch(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap&
   return counted(launch_pdl(k_matmul_i8<OT, PAIR>, dim3((unsigned)(at_once * blocks_a_tile)),
                             kThreads, smem, st, blocks_a_tile, wmap, amap, g));
 }
-// The clusters that the current device holds, asked once (clusters of more than the
-// blocks of one cluster share what a group of multiprocessors has over).
+// A kernel of k_matmul_i8's size: for that itself, as for any that takes tensor
+// memory, the occupancy calls answer one block a multiprocessor.
+__global__ void __launch_bounds__(kThreads) k_room() {}
+
+// The clusters that the current device holds, asked once.
 I8Device this_device() {
   static std::atomic<uint64_t> known[64][kI8MaxSplit + 1];
   I8Device d = {};
   d.sms = sm_count();
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return d;  // nothing is split
-  const void* const kernel = (const void*)k_matmul_i8<float, false>;
+  const void* const kernel = (const void*)k_room;
   for (int s = 2; s <= kI8MaxSplit; ++s) {
     uint64_t v = known[dev][s].load(std::memory_order_relaxed);
     if (v == 0) {
@@ -516,7 +519,7 @@ I8Device this_device() {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)s);
         cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = (two ? kI8SmemTwo : kI8Smem) + 1024;
+        cfg.dynamicSmemBytes = (two ? kI8SmemTwo : kI8Smem) + 4096;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = (unsigned)s;
@@ -524,7 +527,7 @@ I8Device this_device() {
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         static std::atomic<uint64_t> raised{0};
-        if (raise_smem_limit(kernel, kI8Smem + 1024, &raised) != cudaSuccess ||
+        if (raise_smem_limit(kernel, kI8Smem + 4096, &raised) != cudaSuccess ||
             cudaOccupancyMaxActiveClusters(&n[two], kernel, &cfg) != cudaSuccess) {
           cudaGetLastError();
           n[two] = 0;
