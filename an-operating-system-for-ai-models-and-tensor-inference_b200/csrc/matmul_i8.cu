@@ -83,6 +83,15 @@ MYOS_DEV void store16(OT* o, int64_t stride, const int* v, const float* as, floa
 }
 
 constexpr int kThreads = 192;
+
+// A whole warp's wait, its answer one for all lanes. Reading the clock takes some 0.3
+// us, so it begins with the 64th poll.
+MYOS_DEV bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t code) {
+  bool ok = false;
+  for (int i = 0; i < 64 && !ok; ++i) ok = mbar_try_wait(bar, parity);
+  if (!ok) ok = mbar_wait(bar, parity, &g_wait_failed, code);
+  return __all_sync(0xffffffffu, ok);
+}
 // Tile t: its first channel and row.
 MYOS_DEV void tile_at(const I8Plan& p, int64_t t, int& c0, int& r0) {
   const int64_t each = (int64_t)p.group * p.tiles_c;
@@ -103,7 +112,11 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ int peer_dead;  // a wait of a block of the cluster ran out
   uint8_t* const smem = raw + (-smem_u32(raw) & 1023);
   const I8Plan& p = g.plan;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // The copying and the issuing warp run as a whole, one lane of them acting: the
+  // tensor core's operands are registers of the warp, and a single lane's own values
+  // would have to be moved there one by one (390 cycles a step).
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  const bool acts = one_lane();
   constexpr int kPair = PAIR ? 2 : 1;
   const int tr = p.tn / kPair;  // rows that a block copies
   // rows of a tile that the tensor core takes: of the last one no more than there are
@@ -144,20 +157,18 @@ __global__ void __launch_bounds__(kThreads)
   pdl_wait();
   pdl_launch();
 
-  if (warp == 0) {
-    if (lane == 0) {  // ---- copies
-      int s = 0, phase = 0, issued = 0;
-      bool ok = true;
-      for (int64_t t = tile0; ok && t < tiles; t += tile_step) {
-        int c0, r0;
-        tile_at(p, t, c0, r0);
-        const int rank_r0 = PAIR && rank ? r0 + taken(r0) / 2 : r0;
-        for (int k = k0; k < k1; ++k) {
-          if (!mbar_wait(&empty[s], phase ^ 1, &g_wait_failed, kErrWaitEmpty)) {
-            ok = false;
-            break;
-          }
-          uint8_t* const at = smem + s * stage_bytes;
+  if (warp == 0) {  // ---- copies
+    int s = 0, phase = 0, issued = 0;
+    bool ok = true;
+    for (int64_t t = tile0; ok && t < tiles; t += tile_step) {
+      int c0, r0;
+      tile_at(p, t, c0, r0);
+      const int rank_r0 = PAIR && rank ? r0 + taken(r0) / 2 : r0;
+      for (int k = k0; k < k1; ++k) {
+        ok = warp_wait(&empty[s], phase ^ 1, kErrWaitEmpty);
+        if (!ok) break;
+        uint8_t* const at = smem + s * stage_bytes;
+        if (acts) {
           if constexpr (PAIR) {
             // both blocks' copies are counted where the products wait for them
             const uint32_t bar = cluster_at(&full[s], 0);
@@ -169,47 +180,47 @@ __global__ void __launch_bounds__(kThreads)
             tma_load_2d(at, &wmap, k * kI8Step, c0, &full[s]);
             tma_load_2d(at + kI8Channels * kI8Step, &amap, k * kI8Step, r0, &full[s]);
           }
-          ++issued;
-          if (++s == p.stages) s = 0, phase ^= 1;
         }
-      }
-      if (!ok) {  // its copies in flight are waited for before the block ends
-        for (int n = rank == 0 || !PAIR ? min(issued, p.stages) : 0; n > 0; --n) {
-          if (--s < 0) s = p.stages - 1, phase ^= 1;
-          mbar_wait(&full[s], phase, &g_wait_failed, kErrWaitFull);
-        }
+        __syncwarp();
+        ++issued;
+        if (++s == p.stages) s = 0, phase ^= 1;
       }
     }
-    __syncwarp();
-  } else if (warp == 1) {
-    if (lane == 0 && (!PAIR || rank == 0)) {  // ---- products
-      int s = 0, phase = 0, n = 0;
-      bool ok = true;
-      for (int64_t t = tile0; ok && t < tiles; t += tile_step, ++n) {
-        const int b = n & 1;
-        ok = mbar_wait(&acc_empty[b], (n >> 1 & 1) ^ 1, &g_wait_failed, kErrWaitEmpty);
+    if (!ok) {  // the copies in flight are waited for before the block ends
+      for (int n = rank == 0 || !PAIR ? min(issued, p.stages) : 0; n > 0; --n) {
+        if (--s < 0) s = p.stages - 1, phase ^= 1;
+        warp_wait(&full[s], phase, kErrWaitFull);
+      }
+    }
+  } else if (warp == 1) {  // ---- products
+    int s = 0, phase = 0, n = 0;
+    bool ok = !PAIR || rank == 0;
+    for (int64_t t = tile0; ok && t < tiles; t += tile_step, ++n) {
+      const int b = n & 1;
+      ok = warp_wait(&acc_empty[b], (n >> 1 & 1) ^ 1, kErrWaitEmpty);
+      if (!ok) break;
+      tc_fence_after();
+      int c0, r0;
+      tile_at(p, t, c0, r0);
+      const uint32_t shape = tc_i8_shape(kPair * kI8Channels, taken(r0));
+      const uint32_t d = tmem + b * p.tn;
+      for (int k = k0; k < k1; ++k) {
+        ok = warp_wait(&full[s], phase, kErrWaitFull);
         if (!ok) break;
         tc_fence_after();
-        int c0, r0;
-        tile_at(p, t, c0, r0);
-        const uint32_t shape = tc_i8_shape(kPair * kI8Channels, taken(r0));
-        const uint32_t d = tmem + b * p.tn;
-        for (int k = k0; k < k1; ++k) {
-          ok = mbar_wait(&full[s], phase, &g_wait_failed, kErrWaitFull);
-          if (!ok) break;
-          tc_fence_after();
-          const uint8_t* const at = smem + s * stage_bytes;
-          const uint64_t wd = tc_operand(at), ad = tc_operand(at + kI8Channels * kI8Step);
+        const uint8_t* const at = smem + s * stage_bytes;
+        const uint64_t wd = tc_operand(at), ad = tc_operand(at + kI8Channels * kI8Step);
+        if (acts) {
 #pragma unroll
           for (int i = 0; i < kI8Step / 32; ++i)
             tc_mma_i8<PAIR>(d, wd + 2 * i, ad + 2 * i, shape, k > k0 || i > 0);
           tc_commit<PAIR>(&empty[s]);
-          if (++s == p.stages) s = 0, phase ^= 1;
+          if (k + 1 == k1) tc_commit<PAIR>(&acc_full[b]);
         }
-        if (ok) tc_commit<PAIR>(&acc_full[b]);
+        __syncwarp();
+        if (++s == p.stages) s = 0, phase ^= 1;
       }
     }
-    __syncwarp();
   } else if (split == 1) {  // ---- scales and stores
     const int quarter = warp % 4, tid = threadIdx.x - 64;
     bool ok = true;
@@ -223,8 +234,7 @@ __global__ void __launch_bounds__(kThreads)
       const bool on = c < g.channels;
       const float ws = on ? g.w_scales[c] : 0.0f, bias = on && g.bias ? g.bias[c] : 0.0f;
       named_sync(1, 128);
-      if (ok) ok = mbar_wait(&acc_full[b], n >> 1 & 1, &g_wait_failed, kErrWaitFull);
-      ok = __all_sync(0xffffffffu, ok);
+      if (ok) ok = warp_wait(&acc_full[b], n >> 1 & 1, kErrWaitFull);
       tc_fence_after();
       OT* o = static_cast<OT*>(g.out) + (int64_t)r0 * g.out_stride + c;
       // 16 rows at a time, the next 16 on their way from tensor memory meanwhile
@@ -269,8 +279,7 @@ __global__ void __launch_bounds__(kThreads)
         ws[i] = c + i < end ? g.w_scales[c + i] : 0.0f;
         bias[i] = g.bias && c + i < end ? g.bias[c + i] : 0.0f;
       }
-      ok = mbar_wait(&acc_full[0], 0, &g_wait_failed, kErrWaitFull);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = warp_wait(&acc_full[0], 0, kErrWaitFull);
       tc_fence_after();
     }
     __syncwarp();

@@ -24,6 +24,13 @@ MYOS_DEV void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, 
       : "memory");
 }
 
+// One lane of a whole warp, the same each time.
+MYOS_DEV bool one_lane() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
+
 // Tensor memory: `columns` (a power of two, 32 .. 512) of 128 lanes x 32 bits, its
 // address into *dst (shared memory). One whole warp each.
 template <bool PAIR>
