@@ -72,49 +72,67 @@ struct I8Device {
   int one[kI8MaxSplit + 1], two[kI8MaxSplit + 1];
 };
 
-inline I8Plan i8_plan(int64_t rows, int64_t k, int64_t channels, const I8Device& d) {
-  I8Plan p = {};
-  const int64_t steps = i8_ceil(k, kI8Step);
-  // Pairs read a third less from L2 for the same products. They pay where they fill
-  // the device (4096 x 5120 x 27648: 490 -> 452; 512 x 5120 x 7168, 56 of 74 pairs:
-  // 22.8, 22.4; 1024 x 8960 x 1536, 24 pairs: 30.7, and 21.9 in split tiles).
-  const int64_t least_r = i8_ceil(rows, kI8MaxRows), pairs_c = i8_ceil(channels, 2 * kI8Channels);
-  p.pair = rows > kI8MaxRows && least_r * pairs_c >= d.sms / 2;
-  p.tc = p.pair ? 2 * kI8Channels : kI8Channels;
-  p.tiles_c = (int)i8_ceil(channels, p.tc);
-  const int unit = p.pair ? 32 : 16;
-  // Rows of a tile: the fewest tiles, or a few more that fill the last round better. A
-  // step costs its products (2 cycles a row) or its copies (59 bytes a cycle).
-  const int64_t places = p.pair ? d.sms / 2 : d.sms;
+// A step's time in a block that waits for its copies alone, in ns, and where pairs fill
+// the device and its power (8192 x 8192 x 8192).
+inline int64_t i8_step(bool pair, int64_t tn, bool filled) {
+  const int64_t copies = pair ? 175 + tn * 9 / 100 : 200 + tn * 3 / 4, products = tn * 8 / 5;
+  return filled && products > copies ? products : copies;
+}
+
+// Tiles of `unit` rows and their multiples: the fewest, or a few more that fill the last
+// round better (17 row tiles of 256 for 4097 rows, or 19 of 224).
+inline int64_t i8_rows(I8Plan& p, int64_t rows, int64_t places, int unit) {
+  const int64_t least_r = i8_ceil(rows, kI8MaxRows);
   int64_t best = 0;
-  for (int64_t r = least_r; r < least_r + 4 && (r == least_r || p.pair); ++r) {
+  for (int64_t r = least_r; r < least_r + 4; ++r) {
     const int64_t tn = i8_ceil(i8_ceil(rows, r), unit) * unit, n = i8_ceil(rows, tn);
-    const int64_t copies = (kI8Channels + tn / (p.pair ? 2 : 1)) * kI8Step / 59;
-    const int64_t cost = i8_ceil(n * p.tiles_c, places) * (copies > 2 * tn ? copies : 2 * tn);
-    if (best == 0 || cost < best) {
-      best = cost;
-      p.tn = (int)tn;
-      p.tiles_r = (int)n;
-    }
+    const int64_t rounds = i8_ceil(n * p.tiles_c, places);
+    const int64_t cost = rounds * i8_step(p.pair, tn, n * p.tiles_c >= places);
+    if (best != 0 && cost >= best) continue;
+    best = cost;
+    p.tn = (int)tn;
+    p.tiles_r = (int)n;
   }
-  const int64_t tiles = (int64_t)p.tiles_c * p.tiles_r;
-  p.two = !p.pair && p.tn <= 64;
-  // A multiprocessor takes weights from memory at some 49 GB/s, however many of its
-  // copies are on their way, so few tiles are split until every one has a part, if the
-  // shorter way (0.34 a step) saves what a cluster costs (0.5, and 0.012 a row).
-  // 64 x 13824 x 5120 in 1, 2, 4, 6 parts: 39.8, 26.9, 18.8, 18.4; 128 x 13824 x 5120 in
-  // 1, 2, 3: 40.8, 25.7, 21.0; 64 x 5120 x 27648 in 1, 2: 27.7, 34.3; 64 x 1536 x 2048
-  // in 1, 4, 8: 7.3, 5.0, 6.0.
+  return best;
+}
+
+inline I8Plan i8_plan(int64_t rows, int64_t k, int64_t channels, const I8Device& d) {
+  I8Plan p = {}, q = {};
+  const int64_t steps = i8_ceil(k, kI8Step);
+  // Pairs copy less for the same products: each block half of the rows. From 65 rows on
+  // they are the rule (256 x 5120 x 7168: 13.8 for 18.4; 128 x 1536 x 2048: 5.1 for 6.5).
+  q.pair = 1;
+  q.tc = 2 * kI8Channels;
+  q.tiles_c = (int)i8_ceil(channels, q.tc);
+  const int64_t paired = steps * i8_rows(q, rows, d.sms / 2, 32);
+  // Few tiles are split along k, if the shorter way saves what a cluster costs (1.2 us,
+  // and 14 ns a row): 64 x 13824 x 5120 in 1, 2, 3 parts 33.1, 18.4, 17.4; 64 x 5120 x
+  // 27648 in 1, 2: 27.0, 32.9; 64 x 1536 x 2048 in 1, 4, 8: 5.7, 4.8, 5.5; 128 x 13824 x
+  // 5120 in 1, 2, 3 and in pairs: 30.7, 21.5, 19.5, 23.3. Two blocks a multiprocessor
+  // only where there are more than multiprocessors: they have half the stages (64 x 5120
+  // x 7168 in 2 parts: 13.0 for 11.3).
+  p.tc = kI8Channels;
+  p.tiles_c = (int)i8_ceil(channels, p.tc);
+  p.tn = (int)i8_ceil(i8_ceil(rows, i8_ceil(rows, kI8MaxRows)), 16) * 16;
+  p.tiles_r = (int)i8_ceil(rows, p.tn);
+  const int64_t tiles = (int64_t)p.tiles_c * p.tiles_r, step = i8_step(false, p.tn, false);
   p.split = 1;
+  p.two = p.tn <= 64 && tiles > d.sms;
+  int64_t least = p.tn <= 64 ? steps * step : paired;
+  bool pair = p.tn > 64;
   const int parts[] = {2, 3, 4, 6, 8};
-  int64_t least = steps * 340;
   for (int s : parts) {
-    const int64_t most = p.two ? (d.two[s] < 5 * d.sms / 3 ? d.two[s] : 5 * d.sms / 3) : d.one[s];
-    const int64_t time = i8_ceil(steps, s) * 340 + 500 + 12 * p.tn;
-    if (p.pair || tiles * s > most || steps < 3 * s || time >= least) continue;
+    const int64_t n = tiles * s;
+    const bool two = n > d.one[s];
+    if (two && (p.tn > 64 || n > d.two[s] || n > 5 * d.sms / 3)) continue;
+    const int64_t time = i8_ceil(steps, s) * step * (two ? 2 : 1) + 1200 + 14 * p.tn;
+    if (steps < 3 * s || time >= least) continue;
     least = time;
     p.split = s;
+    p.two = two;
+    pair = false;
   }
+  if (pair) p = q, p.split = 1;
   const int stage = (kI8Channels + p.tn / (p.pair ? 2 : 1)) * kI8Step;
   const int sums = p.split * p.tn * i8_wide(p.split) * 4;
   p.apart = p.split > 1 && p.tn <= 64;
