@@ -75,7 +75,7 @@ struct I8Device {
 // A step's time in a block that waits for its copies alone, in ns, and where pairs fill
 // the device and its power (8192 x 8192 x 8192).
 inline int64_t i8_step(bool pair, int64_t tn, bool filled) {
-  const int64_t copies = pair ? 175 + tn * 9 / 100 : 200 + tn * 3 / 4, products = tn * 8 / 5;
+  const int64_t copies = pair ? 175 + tn * 9 / 100 : 200 + tn * 3 / 4, products = 20 + tn * 8 / 5;
   return filled && products > copies ? products : copies;
 }
 
