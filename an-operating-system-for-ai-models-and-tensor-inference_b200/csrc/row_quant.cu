@@ -160,16 +160,17 @@ struct Row {
   }
 };
 
-// What two f32 values may differ by, relatively, and be one value in 64 bits; also
-// more than a step's position is off by. gamma * total is one rounding, 1 / rms,
-// 1 / scale and the products with them one each; silu_up has its own.
+// How far an f32 value, or its position among the steps, may be from that in 64 bits,
+// relatively: a rounding each of gamma * total and of the factor that makes steps of it
+// (2^-24 each; four times that here); silu_up's own error beside them. The values that
+// may be the largest are within twice that of it.
 template <int KIND>
-constexpr float kRel = KIND == kSwiglu ? 3.8147e-6f : 9.5367e-7f;  // 2^-18, 2^-20
+constexpr float kRel = KIND == kSwiglu ? 1.9073e-6f : 2.3842e-7f;  // 2^-19, 2^-22
 
 // The larger magnitude, NaN above infinity above all others.
 MYOS_DEV float larger(float a, float v) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(v)));
+  asm("{\n .reg .f32 t;\n abs.f32 t, %2;\n max.NaN.f32 %0, %1, t;\n}" : "=f"(r) : "f"(a), "f"(v));
   return r;
 }
 // The same order among integers. The sign is taken off the bits (arithmetic may
@@ -178,12 +179,24 @@ MYOS_DEV uint64_t magnitude(double v) {
   return (uint64_t)__double_as_longlong(v) & 0x7fffffffffffffffull;
 }
 
-// v rounded to the nearest integer, in the low byte. The addition rounds: the sum's
-// last bit is 1 (rint and its conversion run at a quarter of the rate). open: v is
-// so near the border between two steps that it may lie on its other side.
-MYOS_DEV uint32_t step(float v, float rel, bool& open) {
-  const float t = __fadd_rn(v, 12582912.0f), off = v - __fsub_rn(t, 12582912.0f);
-  open |= !(fabsf(off) < __fmaf_rn(-fabsf(v), rel, 0.5f));
+// x / 127, correctly rounded: a quotient by the rounded reciprocal, its remainder
+// exactly, and the correction (Markstein's division).
+MYOS_DEV double over127(double x) {
+  const double y = 1.0 / 127.0, q = x * y;
+  return q < 1e300 ? fma(fma(-127.0, q, x), y, q) : q;
+}
+
+// p * per rounded to the nearest integer, in the low byte. The addition rounds: the
+// sum's last bit is 1 (rint and its conversion run at a quarter of the rate). open: it
+// is so near the border between two steps that it may lie on its other side.
+template <int KIND>
+MYOS_DEV uint32_t step(float p, float per, bool& open) {
+  const float t = __fmaf_rn(p, per, 12582912.0f), n = __fsub_rn(t, 12582912.0f);
+  const float off = __fmaf_rn(p, per, -n);
+  // of the silu the bound goes by the step: a bound for all would open four times as many
+  const float in = KIND == kSwiglu ? __fmaf_rn(-fabsf(n), kRel<KIND>, 0.5f - kRel<KIND>)
+                                   : 0.5f - 128.0f * kRel<KIND>;
+  open |= !(fabsf(off) < in);
   return __float_as_uint(t);
 }
 
@@ -252,23 +265,22 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
       for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
     }
   }
-  const double inv = KIND == kNorm ? 1.0 / sqrt(squares / a.width + (double)a.eps) : 1.0;
+  const double inv = KIND == kNorm ? rsqrt(squares / a.width + (double)a.eps) : 1.0;
   const float P = __uint_as_float(top);
   const bool finite = top < 0x7f800000u;
   // Nothing but zeros: scale 2^-126. (A product below f32's smallest number is 0
   // as well, and a norm may still make it large.)
   const bool zero = top == 0 && (KIND != kNorm || (squares == 0.0 && inv < 1e300));
-  const float rel = P < kTiny ? INFINITY : kRel<KIND>;
+  const bool tiny = P < kTiny;
 
   // ---- the largest value in 64 bits, of those that may be it
   uint64_t most = 0;
-  if (KIND == kQuant) {
-    most = magnitude((double)P);
-  } else if (finite && !zero) {
-    const float least = P < kTiny ? 0.0f : P * (1.0f - kRel<KIND>);
+  if (KIND != kQuant && finite && !zero) {
+    const float least = tiny ? 0.0f : P * (1.0f - 2.0f * kRel<KIND>);
     if constexpr (VEC) {
+      // (most threads have none)
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
+      for (int c = 0; c < C && largest >= least; ++c) {
         uint32_t may = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) may |= fabsf(p[c][e]) >= least ? 1u << e : 0u;
@@ -292,14 +304,17 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
       for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     }
   }
-  const double top64 = __longlong_as_double((long long)most);
-  float scale = fmaxf((float)(top64 / 127.0), kSmallest);
-  if (!finite || !(top64 / 127.0 <= 3.4028234663852886e38)) scale = __uint_as_float(0x7fc00000u);
+  float scale = fmaxf(KIND == kQuant ? __fdiv_rn(P, 127.0f)
+                                     : (float)over127(__longlong_as_double((long long)most)),
+                      kSmallest);
+  // fmaxf passes a NaN over; an infinite scale is none
+  if (!finite || most >= 0x7ff0000000000000ull || !(scale < INFINITY))
+    scale = __uint_as_float(0x7fc00000u);
   if (tid == 0) a.scales[row] = scale;
 
   // ---- the steps
   const bool good = scale == scale;
-  const float per = good ? (float)(inv / (double)scale) : 0.0f;
+  const float per = KIND == kNorm ? (float)(inv / (double)scale) : __frcp_rn(scale);
   auto decide = [&](int i) {  // in 64 bits
     return (int)rint(r.exact(i, inv) / (double)scale);
   };
@@ -308,14 +323,12 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
     for (int c = 0; c < C; ++c) {
       const int i = (c * team + tid) * 8;
       if (i >= a.width) break;
-      uint32_t s[8];
+      uint32_t s[8] = {};
       bool open = false;  // whether any may lie on the other side of a border
+      if (good && !zero) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = step(p[c][e] * per, rel, open);
-      if (!good || zero) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = 0;
-        open = false;
+        for (int e = 0; e < 8; ++e) s[e] = step<KIND>(p[c][e], per, open);
+        open |= tiny;
       }
       if (i + 8 <= a.width) {
         uint2 w;
@@ -331,8 +344,8 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
         uint32_t which = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          bool o = false;
-          step(p[c][e] * per, rel, o);
+          bool o = tiny;
+          step<KIND>(p[c][e], per, o);
           which |= o ? 1u << e : 0u;
         }
         while (which) {
@@ -344,8 +357,8 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
     }
   } else {
     for (int i = tid; i < a.width; i += team) {
-      bool open = false;
-      const uint32_t n = step(r.value(i) * per, rel, open);
+      bool open = tiny;
+      const uint32_t n = step<KIND>(r.value(i), per, open);
       q[i] = (int8_t)(!good || zero ? 0 : open ? decide(i) : (int)n);
     }
   }
