@@ -129,16 +129,18 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t tiles = (int64_t)p.tiles_c * p.tiles_r;
   const int64_t tile0 = blockIdx.x / (kPair * split), tile_step = gridDim.x / (kPair * split);
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+  if (warp == 0) {
+    if (lane < p.stages) {
+      mbar_init(&full[lane], 1);
+      mbar_init(&empty[lane], 1);
+    } else if (lane < p.stages + 2) {
+      mbar_init(&acc_full[lane - p.stages], 1);
+      mbar_init(&acc_empty[lane - p.stages], 128 * kPair);
+    } else if (lane == 31) {
+      peer_dead = 0;
+      tma_ahead(&wmap);
+      tma_ahead(&amap);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 128 * kPair);
-    }
-    peer_dead = 0;
     mbar_fence_init();
   }
   __syncwarp();
@@ -186,7 +188,13 @@ __global__ void __launch_bounds__(kThreads)
         if (++s == p.stages) s = 0, phase ^= 1;
       }
     }
-    if (!ok) {  // the copies in flight are waited for before the block ends
+    // The products' arrivals at the last stages come before the block ends (in a pair
+    // they are written from the other block).
+    for (int n = 0, last = s, turn = phase; ok && n < p.stages; ++n) {
+      ok = warp_wait(&empty[last], turn ^ 1, kErrWaitEmpty);
+      if (++last == p.stages) last = 0, turn ^= 1;
+    }
+    if (!ok) {  // the copies in flight are waited for as well
       for (int n = rank == 0 || !PAIR ? min(issued, p.stages) : 0; n > 0; --n) {
         if (--s < 0) s = p.stages - 1, phase ^= 1;
         warp_wait(&full[s], phase, kErrWaitFull);
@@ -253,8 +261,10 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
       tc_fence_before();
-      if (PAIR) cluster_arrive(cluster_at(&acc_empty[b], 0));
-      else mbar_arrive(&acc_empty[b]);
+      if (t + 2 * tile_step < tiles) {  // the products of a later tile wait for it
+        if (PAIR) cluster_arrive(cluster_at(&acc_empty[b], 0));
+        else mbar_arrive(&acc_empty[b]);
+      }
     }
   }
   if (!PAIR && split > 1) {  // ---- one tile, k shared by the cluster
@@ -350,7 +360,9 @@ __global__ void __launch_bounds__(kThreads)
   }
   __syncwarp();
   tc_fence_before();
-  if (PAIR) cluster_meet();
+  // a pair's memory is free when both are done with it; their results need not have
+  // arrived (waiting for that took 0.8 us)
+  if (PAIR) cluster_end();
   else __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_free<PAIR>(tmem, p.columns);

@@ -7,6 +7,10 @@
 
 namespace myos {
 
+// Brings a map (a kernel's parameter) to the copy engine.
+MYOS_DEV void tma_ahead(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 MYOS_DEV void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
@@ -129,6 +133,11 @@ MYOS_DEV void cluster_enter() { asm volatile("barrier.cluster.arrive.release.ali
 MYOS_DEV void cluster_leave() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 MYOS_DEV void cluster_meet() {
   cluster_enter();
+  cluster_leave();
+}
+// The same without an order of memory.
+MYOS_DEV void cluster_end() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   cluster_leave();
 }
 // The address in block `rank` of the cluster of what lies at p in this one.
