@@ -104,7 +104,7 @@ inline I8Plan i8_plan(int64_t rows, int64_t k, int64_t channels, const I8Device&
   q.pair = 1;
   q.tc = 2 * kI8Channels;
   q.tiles_c = (int)i8_ceil(channels, q.tc);
-  const int64_t paired = steps * i8_rows(q, rows, d.sms / 2, 32);
+  const int64_t pairs = d.one[2] / 2, paired = pairs ? steps * i8_rows(q, rows, pairs, 32) : 0;
   // Few tiles are split along k, if the shorter way saves what a cluster costs (1.2 us,
   // and 14 ns a row): 64 x 13824 x 5120 in 1, 2, 3 parts 33.1, 18.4, 17.4; 64 x 5120 x
   // 27648 in 1, 2: 27.0, 32.9; 64 x 1536 x 2048 in 1, 4, 8: 5.7, 4.8, 5.5; 128 x 13824 x
@@ -118,8 +118,8 @@ inline I8Plan i8_plan(int64_t rows, int64_t k, int64_t channels, const I8Device&
   const int64_t tiles = (int64_t)p.tiles_c * p.tiles_r, step = i8_step(false, p.tn, false);
   p.split = 1;
   p.two = p.tn <= 64 && tiles > d.sms;
-  int64_t least = p.tn <= 64 ? steps * step : paired;
-  bool pair = p.tn > 64;
+  bool pair = p.tn > 64 && pairs > 0;
+  int64_t least = pair ? paired : i8_ceil(tiles, d.sms) * steps * step;
   const int parts[] = {2, 3, 4, 6, 8};
   for (int s : parts) {
     const int64_t n = tiles * s;

@@ -506,8 +506,8 @@ bool map_rows(CUtensorMap* map, const int8_t* p, int64_t k, int64_t rows, int64_
 }
 
 template <class OT, bool PAIR>
-cudaError_t launch(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap& amap, int sms,
-                   cudaStream_t st) {
+cudaError_t launch(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap& amap,
+                   const I8Device& d, cudaStream_t st) {
   static std::atomic<uint64_t> raised{0};
   const cudaError_t e =
       raise_smem_limit((const void*)k_matmul_i8<OT, PAIR>, kI8Smem + 1024, &raised);
@@ -515,7 +515,7 @@ cudaError_t launch(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap&
   const size_t smem = (g.plan.two ? kI8SmemTwo : kI8Smem) + 1024;
   const int64_t tiles = (int64_t)g.plan.tiles_c * g.plan.tiles_r;
   const int blocks_a_tile = PAIR ? 2 : g.plan.split;
-  const int64_t most = PAIR ? sms / 2 : sms * (g.plan.two ? 2 : 1);
+  const int64_t most = PAIR ? d.one[2] / 2 : d.sms * (g.plan.two ? 2 : 1);
   const int64_t at_once = g.plan.split > 1 ? tiles : std::min(tiles, most);
   return counted(launch_pdl(k_matmul_i8<OT, PAIR>, dim3((unsigned)(at_once * blocks_a_tile)),
                             kThreads, smem, st, blocks_a_tile, wmap, amap, g));
@@ -565,9 +565,9 @@ I8Device this_device() {
 
 template <class OT>
 cudaError_t launch_tiles(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap& amap,
-                         int sms, cudaStream_t st) {
-  return g.plan.pair ? launch<OT, true>(g, wmap, amap, sms, st)
-                     : launch<OT, false>(g, wmap, amap, sms, st);
+                         const I8Device& d, cudaStream_t st) {
+  return g.plan.pair ? launch<OT, true>(g, wmap, amap, d, st)
+                     : launch<OT, false>(g, wmap, amap, d, st);
 }
 
 }  // namespace
@@ -616,7 +616,6 @@ int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const 
   }
   const size_t size = out_dtype == MYOS_F32 ? 4 : 2;
   const I8Device device = this_device();
-  const int sms = device.sms;
   g.plan = i8_plan((int64_t)rows, (int64_t)k, (int64_t)channels, device);
   g.plan.vec = aligned(d_out, 4 * size) && (rows == 1 || out_stride % 4 == 0);
   CUtensorMap wmap, amap;
@@ -625,8 +624,8 @@ int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const 
                 g.plan.tn / (g.plan.pair ? 2 : 1)))
     return MYOS_ERR_CUDA;
   const cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = out_dtype == MYOS_F32 ? launch_tiles<float>(g, wmap, amap, sms, st)
-                                              : launch_tiles<__nv_bfloat16>(g, wmap, amap, sms, st);
+  const cudaError_t e = out_dtype == MYOS_F32 ? launch_tiles<float>(g, wmap, amap, device, st)
+                                              : launch_tiles<__nv_bfloat16>(g, wmap, amap, device, st);
   return e == cudaSuccess ? MYOS_OK : MYOS_ERR_CUDA;
 }
 
