@@ -57,6 +57,13 @@ MYOS_DEV void load8(const uint16_t* p, float* v) {
   v[0] = bf16_lo(a.x), v[1] = bf16_hi(a.x), v[2] = bf16_lo(a.y), v[3] = bf16_hi(a.y);
   v[4] = bf16_lo(a.z), v[5] = bf16_hi(a.z), v[6] = bf16_lo(a.w), v[7] = bf16_hi(a.w);
 }
+MYOS_DEV uint4 some8(const uint16_t* p, int n) {
+  uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < n) v[e / 2] |= (uint32_t)p[e] << (16 * (e % 2));
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
 template <class T>
 MYOS_DEV void load_some(const T* p, float* v, int n) {
 #pragma unroll
@@ -111,13 +118,13 @@ struct Row {
     } else if (KIND == kSwiglu) {
       if (FULL) load8(x + width + i, b);
       else load_some(x + width + i, b, n);
-      bool fast = true;
+      float lowest = a[0];  // (a NaN is one in p)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         p[e] = silu_up(a[e], b[e]);
-        fast &= silu_fast(a[e]);
+        lowest = fminf(lowest, a[e]);
       }
-      if (!fast) {
+      if (!silu_fast(lowest)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (!silu_fast(a[e])) p[e] = (float)silu_up64(a[e], b[e]);
@@ -179,6 +186,12 @@ MYOS_DEV uint64_t magnitude(double v) {
   return (uint64_t)__double_as_longlong(v) & 0x7fffffffffffffffull;
 }
 
+MYOS_DEV uint64_t warp_most(uint64_t v) {  // the upper halves, then the lower of those
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(v >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, v >> 32 == hi ? (uint32_t)v : 0u);
+  return (uint64_t)hi << 32 | lo;
+}
+
 // x / 127, correctly rounded: a quotient by the rounded reciprocal, its remainder
 // exactly, and the correction (Markstein's division).
 MYOS_DEV double over127(double x) {
@@ -187,18 +200,42 @@ MYOS_DEV double over127(double x) {
 }
 
 // p * per rounded to the nearest integer, in the low byte. The addition rounds: the
-// sum's last bit is 1 (rint and its conversion run at a quarter of the rate). open: it
-// is so near the border between two steps that it may lie on its other side.
+// sum's last bit is 1 (rint and its conversion run at a quarter of the rate). edge:
+// the largest distance from an integer, with what it may be wrong by; from kEdge on
+// a value may lie on the other side of the border between two steps.
+constexpr float kEdge = 0.5f;
 template <int KIND>
-MYOS_DEV uint32_t step(float p, float per, bool& open) {
+MYOS_DEV uint32_t step(float p, float per, float& edge) {
   const float t = __fmaf_rn(p, per, 12582912.0f), n = __fsub_rn(t, 12582912.0f);
   const float off = __fmaf_rn(p, per, -n);
   // of the silu the bound goes by the step: a bound for all would open four times as many
-  const float in = KIND == kSwiglu ? __fmaf_rn(-fabsf(n), kRel<KIND>, 0.5f - kRel<KIND>)
-                                   : 0.5f - 128.0f * kRel<KIND>;
-  open |= !(fabsf(off) < in);
+  edge = KIND == kSwiglu ? larger(edge, __fmaf_rn(fabsf(n), kRel<KIND>, fabsf(off) + kRel<KIND>))
+                         : larger(edge, off);
   return __float_as_uint(t);
 }
+template <int KIND>
+MYOS_DEV bool open(float edge) {
+  return !(edge < (KIND == kSwiglu ? kEdge : kEdge - 128.0f * kRel<KIND>));
+}
+
+// A chunk's 8 values between the passes: bf16 rows as they came, for more rows at once.
+template <int KIND, class XT>
+struct Held {
+  float v[8];
+  MYOS_DEV void keep(const float* p) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = p[e];
+  }
+  MYOS_DEV void take(float* p) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = v[e];
+  }
+};
+template <>
+struct Held<kQuant, uint16_t> {
+  uint4 v;
+  MYOS_DEV void take(float* p) const { load8(reinterpret_cast<const uint16_t*>(&v), p); }
+};
 
 template <int KIND, class XT, int C, bool VEC, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : 1024)
@@ -222,20 +259,28 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
 
   // ---- the row, its largest f32 value and its sum of squares
   constexpr int kHeld = VEC ? C : 1;
-  float p[kHeld][8];
+  Held<KIND, XT> held[kHeld];
   double squares = 0.0;
   float largest = 0.0f;
   if constexpr (VEC) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int i = (c * team + tid) * 8;
-      if (i + 8 <= a.width) {
-        r.template values<true>(i, 8, p[c], squares);
+      float p[8];
+      if constexpr (KIND == kQuant && sizeof(XT) == 2) {
+        held[c].v = i + 8 <= a.width ? *reinterpret_cast<const uint4*>(r.x + i)
+                                     : some8(r.x + i, a.width - i);
+        held[c].take(p);
       } else {
-        r.template values<false>(i, a.width - i, p[c], squares);
+        if (i + 8 <= a.width) {
+          r.template values<true>(i, 8, p, squares);
+        } else {
+          r.template values<false>(i, a.width - i, p, squares);
+        }
+        held[c].keep(p);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) largest = larger(largest, p[c][e]);
+      for (int e = 0; e < 8; ++e) largest = larger(largest, p[e]);
     }
   } else {
     for (int i = tid; i < a.width; i += team) {
@@ -273,35 +318,38 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
   const bool zero = top == 0 && (KIND != kNorm || (squares == 0.0 && inv < 1e300));
   const bool tiny = P < kTiny;
 
+  // the place of this thread's value n
+  auto place = [&](int n) { return ((n >> 3) * team + tid) * 8 + (n & 7); };
+
   // ---- the largest value in 64 bits, of those that may be it
   uint64_t most = 0;
   if (KIND != kQuant && finite && !zero) {
     const float least = tiny ? 0.0f : P * (1.0f - 2.0f * kRel<KIND>);
     if constexpr (VEC) {
-      // (most threads have none)
+      uint32_t may = 0;  // (most threads have none)
+      if (largest >= least) {
 #pragma unroll
-      for (int c = 0; c < C && largest >= least; ++c) {
-        uint32_t may = 0;
+        for (int c = 0; c < C; ++c) {
+          float p[8];
+          held[c].take(p);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) may |= fabsf(p[c][e]) >= least ? 1u << e : 0u;
-        while (may) {
-          const int i = (c * team + tid) * 8 + __ffs(may) - 1;
-          may &= may - 1;
-          if (i < a.width) most = max(most, magnitude(r.exact(i, inv)));
+          for (int e = 0; e < 8; ++e) may |= fabsf(p[e]) >= least ? 1u << (8 * c + e) : 0u;
         }
+      }
+      while (may) {
+        const int i = place(__ffs(may) - 1);
+        may &= may - 1;
+        if (i < a.width) most = max(most, magnitude(r.exact(i, inv)));
       }
     } else {
       for (int i = tid; i < a.width; i += team)
         if (fabsf(r.value(i)) >= least) most = max(most, magnitude(r.exact(i, inv)));
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    most = warp_most(most);
     if (!WARP) {
       if (lane == 0) tops64[warp] = most;
       __syncthreads();
-      most = lane < warps ? tops64[lane] : 0;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      most = warp_most(lane < warps ? tops64[lane] : 0);
     }
   }
   float scale = fmaxf(KIND == kQuant ? __fdiv_rn(P, 127.0f)
@@ -315,20 +363,43 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
   // ---- the steps
   const bool good = scale == scale;
   const float per = KIND == kNorm ? (float)(inv / (double)scale) : __frcp_rn(scale);
-  auto decide = [&](int i) {  // in 64 bits
-    return (int)rint(r.exact(i, inv) / (double)scale);
+  // Value i by its f32 value p: on which side of the nearest border it lies, exactly
+  // (a border times the scale has 32 bits; plain rows compare through one fma's sign).
+  auto decide = [&](int i, float p) {
+    if (tiny) return (int)rint(r.exact(i, inv) / (double)scale);
+    const float v = p * per, border = floorf(v) + 0.5f;
+    float side;
+    if (KIND == kQuant) {
+      side = __fmaf_rn(-border, scale, p);
+    } else {
+      const double d = r.exact(i, inv) - (double)border * (double)scale;
+      side = d > 0.0 ? 1.0f : d < 0.0 ? -1.0f : 0.0f;
+    }
+    const int below = (int)floorf(border);
+    return side > 0.0f || (side == 0.0f && (below & 1)) ? below + 1 : below;
   };
   if constexpr (VEC) {
+    uint32_t unsure = 0;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int i = (c * team + tid) * 8;
       if (i >= a.width) break;
       uint32_t s[8] = {};
-      bool open = false;  // whether any may lie on the other side of a border
+      float p[8], edge = 0.0f;
+      held[c].take(p);
       if (good && !zero) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = step<KIND>(p[c][e], per, open);
-        open |= tiny;
+        for (int e = 0; e < 8; ++e) s[e] = step<KIND>(p[e], per, edge);
+        if (tiny) {
+          unsure |= 255u << (8 * c);
+        } else if (open<KIND>(edge)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float one = 0.0f;
+            step<KIND>(p[e], per, one);
+            unsure |= open<KIND>(one) ? 1u << (8 * c + e) : 0u;
+          }
+        }
       }
       if (i + 8 <= a.width) {
         uint2 w;
@@ -340,26 +411,18 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
         for (int e = 0; e < 8; ++e)
           if (i + e < a.width) q[i + e] = (int8_t)s[e];
       }
-      if (open) {
-        uint32_t which = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          bool o = tiny;
-          step<KIND>(p[c][e], per, o);
-          which |= o ? 1u << e : 0u;
-        }
-        while (which) {
-          const int j = i + __ffs(which) - 1;
-          which &= which - 1;
-          if (j < a.width) q[j] = (int8_t)decide(j);
-        }
-      }
+    }
+    while (unsure) {
+      const int i = place(__ffs(unsure) - 1);
+      unsure &= unsure - 1;
+      if (i < a.width) q[i] = (int8_t)decide(i, r.value(i));
     }
   } else {
     for (int i = tid; i < a.width; i += team) {
-      bool open = tiny;
-      const uint32_t n = step<KIND>(r.value(i), per, open);
-      q[i] = (int8_t)(!good || zero ? 0 : open ? decide(i) : (int)n);
+      const float p = r.value(i);
+      float edge = 0.0f;
+      const uint32_t n = step<KIND>(p, per, edge);
+      q[i] = (int8_t)(!good || zero ? 0 : open<KIND>(edge) || tiny ? decide(i, p) : (int)n);
     }
   }
 }
