@@ -124,10 +124,15 @@ struct Row {
         p[e] = silu_up(a[e], b[e]);
         lowest = fminf(lowest, a[e]);
       }
-      if (!silu_fast(lowest)) {
+      if (!silu_fast(lowest)) {  // one place for the call: eight of them cost registers
+#pragma unroll 1
+        for (int f = 0; f < n && f < 8; ++f) {
+          const float g = get(x + i + f);
+          if (silu_fast(g)) continue;
+          const float y = (float)silu_up64(g, get(x + width + i + f));
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (!silu_fast(a[e])) p[e] = (float)silu_up64(a[e], b[e]);
+          for (int e = 0; e < 8; ++e) p[e] = e == f ? y : p[e];
+        }
       }
     } else {
       if (residual) {
@@ -237,9 +242,11 @@ struct Held<kQuant, uint16_t> {
   MYOS_DEV void take(float* p) const { load8(reinterpret_cast<const uint16_t*>(&v), p); }
 };
 
-template <int KIND, class XT, int C, bool VEC, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 1024)
+// SHARED: the values between the passes in shared memory.
+template <int KIND, class XT, int C, bool VEC, bool WARP, bool SHARED>
+__global__ void __launch_bounds__(WARP ? 128 : SHARED ? 512 : 1024, SHARED ? 3 : 1)
     k_row_quant(const RowArgs a) {
+  extern __shared__ float4 shared[];  // SHARED: [chunk][half][thread]
   __shared__ double sums[32];
   __shared__ uint64_t tops64[32];
   __shared__ uint32_t tops[32];
@@ -258,8 +265,24 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
   int8_t* const q = a.q + row * a.q_stride;
 
   // ---- the row, its largest f32 value and its sum of squares
-  constexpr int kHeld = VEC ? C : 1;
+  constexpr int kHeld = VEC && !SHARED ? C : 1;
   Held<KIND, XT> held[kHeld];
+  auto keep = [&](int c, const float* p) {
+    if constexpr (SHARED) {
+      shared[2 * c * team + tid] = make_float4(p[0], p[1], p[2], p[3]);
+      shared[(2 * c + 1) * team + tid] = make_float4(p[4], p[5], p[6], p[7]);
+    } else if constexpr (KIND != kQuant || sizeof(XT) == 4) {
+      held[c].keep(p);
+    }
+  };
+  auto take = [&](int c, float* p) {
+    if constexpr (SHARED) {
+      const float4 x = shared[2 * c * team + tid], y = shared[(2 * c + 1) * team + tid];
+      p[0] = x.x, p[1] = x.y, p[2] = x.z, p[3] = x.w, p[4] = y.x, p[5] = y.y, p[6] = y.z, p[7] = y.w;
+    } else {
+      held[c].take(p);
+    }
+  };
   double squares = 0.0;
   float largest = 0.0f;
   if constexpr (VEC) {
@@ -277,7 +300,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
         } else {
           r.template values<false>(i, a.width - i, p, squares);
         }
-        held[c].keep(p);
+        keep(c, p);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) largest = larger(largest, p[e]);
@@ -331,7 +354,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
           float p[8];
-          held[c].take(p);
+          take(c, p);
 #pragma unroll
           for (int e = 0; e < 8; ++e) may |= fabsf(p[e]) >= least ? 1u << (8 * c + e) : 0u;
         }
@@ -386,7 +409,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
       if (i >= a.width) break;
       uint32_t s[8] = {};
       float p[8], edge = 0.0f;
-      held[c].take(p);
+      take(c, p);
       if (good && !zero) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] = step<KIND>(p[e], per, edge);
@@ -427,11 +450,18 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024)
   }
 }
 
-template <int KIND, class XT, int C, bool VEC, bool WARP>
+template <int KIND, class XT, int C, bool VEC, bool WARP, bool SHARED = false>
 cudaError_t launch(const RowArgs& a, int threads, cudaStream_t st) {
   const int per = WARP ? threads / 32 : 1;
-  return counted(launch_pdl(k_row_quant<KIND, XT, C, VEC, WARP>,
-                            dim3((unsigned)((a.rows + (int64_t)per - 1) / per)), threads, 0, st, 1, a));
+  const auto kernel = k_row_quant<KIND, XT, C, VEC, WARP, SHARED>;
+  const size_t smem = SHARED ? (size_t)threads * C * 32 : 0;
+  if (SHARED) {
+    static std::atomic<uint64_t> raised{0};
+    const cudaError_t e = raise_smem_limit((const void*)kernel, 512 * C * 32, &raised);
+    if (e != cudaSuccess) return e;
+  }
+  return counted(launch_pdl(kernel, dim3((unsigned)((a.rows + (int64_t)per - 1) / per)), threads,
+                            smem, st, 1, a));
 }
 
 template <int KIND, class XT>
@@ -443,12 +473,17 @@ cudaError_t launch_kind(const RowArgs& a, bool vec, cudaStream_t st) {
   const int chunks = (a.width + 7) / 8;
   // Few rows: as many threads as chunks, for the latency. Many: more chunks a thread,
   // so that more rows are on their way at once (norm of 8191 x 5120 f32 with 1, 2, 4:
-  // 118, 99, 91 us; of 8191 x 1536: 32, 30, 36 us; of 512 x 5120: 11.3, 11.5, 11.3 us).
+  // 118, 99, 91 us; of 8191 x 1536: 32, 30, 36 us; of 512 x 5120: 11.3, 11.5, 11.3 us,
+  // at an earlier stage of the kernel).
   const int many = a.rows < 512 ? 1 : chunks <= 256 ? 2 : 4;
   const int each = chunks > 2048 || many == 4 ? 4 : chunks > 1024 || many == 2 ? 2 : 1;
   const int threads = (chunks + 32 * each - 1) / (32 * each) * 32;
   if (each == 1) return launch<KIND, XT, 1, true, false>(a, threads, st);
   if (each == 2) return launch<KIND, XT, 2, true, false>(a, threads, st);
+  // SwiGLU's values in shared memory: 40 registers a thread, three rows at once where
+  // held in registers there were two (4099 x 13824 bf16: 91, 84 us).
+  if constexpr (KIND == kSwiglu)
+    if (many == 4 && chunks <= 2048) return launch<KIND, XT, 4, true, false, true>(a, threads, st);
   return launch<KIND, XT, 4, true, false>(a, threads, st);
 }
 
