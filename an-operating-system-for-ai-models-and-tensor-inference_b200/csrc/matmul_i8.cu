@@ -3,16 +3,28 @@
 // (sum_i a[r][i] w[c][i]) a_scales[r] w_scales[c] + bias[c].
 //
 // The sum is exact in 32-bit integers, so it may be split and joined in any order
-// and gives the same bits.
+// and gives the same bits. Two kernels:
 //
-// A tile is 128 channels (the tensor core's M, the lanes of its memory) by up to
-// 256 rows (its N, the columns): a lane holds one channel, so a warp's store of
-// one row is 32 channels side by side, and few rows cost nothing but their own
-// columns. Six warps: copies (TMA, 128 bytes of k a stage), products (tcgen05,
-// 32 bytes of k each), and four that scale and store while the next tile's
-// products go into the other half of the tensor memory. Where there are fewer
-// tiles than multiprocessors, a cluster shares a tile's k and adds its parts
-// through shared memory.
+// k_few_i8, up to 16 rows: the weights' memory bounds it. mma.sync straight from
+// global memory, blocks of 8 to 32 channels, its warps sharing k (1 x 1536 x 151936:
+// 39.8 us, 5.9 TB/s, 0.9 of the copy rate; 1 x 1536 x 2048: 2.2 us).
+//
+// k_matmul_i8, tiles on tcgen05: 128 channels (the tensor core's M, the lanes of its
+// memory) by up to 256 rows (its N, the columns). A lane holds one channel, so a
+// warp's store of one row is 32 channels side by side, and few rows cost nothing but
+// their own columns. Six warps: copies (TMA, 128 bytes of k a stage), products
+// (tcgen05, 32 bytes of k each), and four that scale and store while the next tile's
+// products go into the other half of the tensor memory. From 65 rows on two blocks
+// make a tile of 256 channels, each copying half of the rows. Where tiles are few, a
+// cluster shares a tile's k and adds its parts through shared memory.
+//
+// What bounds it: of many rows the tensor cores and the device's power (4097 x 5120 x
+// 27648: 345 us with the tensor pipe busy 91% of the time at full clock; 360 to 430 in a
+// row of calls, where the clock falls under the power limit; 8192 x 8192 x 8192 340 us,
+// 3.2 x 10^15 operations a second). Of 64 x 13824 x 5120 (17.0 us) the weights' way to
+// 120 multiprocessors (11 us at the copy rate), a block's start and first copy (1.6 us)
+// and the cluster's sums. Of 333 x 5120 x 7168 (15.1 us) copies from L2, 29 KB a step
+// and block, 40 steps in 8 us, then 9.5 MB of results at once.
 #include <cudaTypedefs.h>
 #include <math.h>
 
@@ -84,14 +96,14 @@ MYOS_DEV void store16(OT* o, int64_t stride, const int* v, const float* as, floa
 
 constexpr int kThreads = 192;
 
-// A whole warp's wait, its answer one for all lanes. Reading the clock takes some 0.3
-// us, so it begins with the 64th poll.
+// A whole warp's wait, its answer one for all lanes; by the clock from the 64th poll on.
 MYOS_DEV bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t code) {
   bool ok = false;
   for (int i = 0; i < 64 && !ok; ++i) ok = mbar_try_wait(bar, parity);
   if (!ok) ok = mbar_wait(bar, parity, &g_wait_failed, code);
   return __all_sync(0xffffffffu, ok);
 }
+
 // Tile t: its first channel and row.
 MYOS_DEV void tile_at(const I8Plan& p, int64_t t, int& c0, int& r0) {
   const int64_t each = (int64_t)p.group * p.tiles_c;

@@ -11,6 +11,7 @@ sections of include/myos_cuda.h).
   quant_rows           rows (tokens, or a weight's channels) in 8 bits with a scale each
   swiglu_quant         silu(gate) * up, the rows in 8 bits with a scale each
   matmul_i8            product of 8-bit rows and channels, scaled, with a bias
+  matmul_i8_status     whether the waits inside matmul_i8 on a device all ended
   rope_table           cos and sin of the rotary angles (host arrays)
 
 Tensors are torch CUDA tensors, all on one device; the work runs there, on
@@ -31,7 +32,7 @@ import importlib.util
 import os
 
 import numpy as np
-import torch  # noqa: F401  (its libraries, which the extension links)
+import torch  # (also its libraries, which the extension links)
 
 from . import _lib
 from ._lib import MyosError
@@ -60,6 +61,15 @@ add_norm_quant = _m.add_norm_quant
 quant_rows = _m.quant_rows
 swiglu_quant = _m.swiglu_quant
 matmul_i8 = _m.matmul_i8
+
+
+def matmul_i8_status(device=None) -> None:
+    """Raises MyosError if a bounded wait inside a matmul_i8 on `device` (default: the
+    current one) has run out since the last such call; waits for the device."""
+    with torch.cuda.device(device):
+        st = _lib.load().myos_dev_matmul_i8_status()
+    if st != 0:
+        raise MyosError(st, "matmul_i8")
 
 
 def rope_table(num_pos: int, rot_dim: int, theta: float):

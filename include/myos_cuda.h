@@ -540,11 +540,12 @@ int myos_rope_table(float* cos_out, float* sin_out, size_t num_pos, size_t rot_d
  * q * scale stands for y. Scales and q are those of y in 64-bit arithmetic from
  * the inputs (y itself is rounded to nothing shorter on its way), whatever the
  * order in which a row is summed: the same bits for every size and batch. A row
- * with a y that f32 does not hold as a finite number (NaN, infinities, past its
- * range) has scale NaN and q 0, so that all products with it are NaN.
- * dtype arguments are MYOS_F32 or MYOS_BF16. Row strides count elements. Addresses are
- * aligned to their elements; rows that begin at multiples of 16 bytes are faster.
- * rows is below 2^31, a row's width at most MYOS_I8_MAX_K.
+ * with a y (or, of the norm, a gamma * total) that f32 does not hold as a finite
+ * number - NaN, infinities, past its range - has scale NaN and q 0, so that all
+ * products with it are NaN. dtype arguments are MYOS_F32 or MYOS_BF16. Row strides
+ * count elements. Addresses are aligned to their elements; rows that begin at
+ * multiples of 16 bytes (q: 8) are faster, and so are widths up to 32768. rows is
+ * below 2^31, a row's width at most MYOS_I8_MAX_K.
  * ------------------------------------------------------------------------- */
 
 /* The longest row of 8-bit values: (2^31 - 1) / 128^2, where a sum of products
@@ -577,11 +578,11 @@ int myos_dev_swiglu_quant(int8_t* d_q, size_t q_stride, float* d_scales, const v
  * included), converted to f32, multiplied by a_scales[r], then by w_scales[c],
  * and the bias added, each rounded to f32; out (f32 or bf16) is rounded from
  * that. The same bits however the work is split. d_a, d_w and their row strides are
- * multiples of 16 bytes (MYOS_ERR_ARG); k need not be one, what lies between k and the
- * stride is neither read into the result nor required to be there. rows and
- * channels are below 2^31 - 256. A wait inside the kernel is bounded: if one
- * ran out, which only a fault elsewhere on the device can cause, the rows it
- * served are NaN and myos_dev_matmul_i8_status says so. */
+ * multiples of 16 bytes (MYOS_ERR_ARG); k need not be one: what lies between k and
+ * the stride is not read. rows and channels are at most 2^31 - 256. The waits inside
+ * the kernel are bounded (about a second); were one to run out, the results it
+ * served are NaN and myos_dev_matmul_i8_status says so. The first call on a device
+ * asks it how many clusters it holds. */
 int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const int8_t* d_a,
                        size_t a_stride, const float* d_a_scales, const int8_t* d_w,
                        size_t w_stride, const float* d_w_scales, const float* d_bias, size_t rows,
