@@ -240,3 +240,79 @@ def test_the_same_call_again_gives_the_same_bits(dev):
         for o in outs:
             dev.matmul_i8(o, a, a_s, w, w_s)
         assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.parametrize("x", ["f32", "bf16"])
+@pytest.mark.parametrize("width", [129, 1025, 1520, 2047, 2056, 5000, 5120, 8192, 13824, 16383, 16384, 16392])
+def test_many_rows(dev, width, x):
+    """The forms that keep several rows on their way at once: 515 rows, some of them marked, zero or alike."""
+    dtype = torch.float32 if x == "f32" else torch.bfloat16
+    rng = np.random.default_rng(width)
+    rows, half = 515, width // 2
+    a = some(rng, rows, width)
+    a[7, width // 3], a[511, width - 1] = np.nan, -np.inf
+    a[100], a[101] = 3.0, -a[102]
+    pad = -width % 8
+    t = rows_of(rows, width, dtype, pad)
+    t.copy_(torch.from_numpy(a))
+    q, s = rows_of(rows, width, torch.int8, pad), torch.zeros(rows, device="cuda")
+    dev.quant_rows(q, s, t)
+    same(q, s, stepped(np64(t)))
+    res = rows_of(rows, width, torch.float32, pad)
+    res.copy_(torch.from_numpy(some(rng, rows, width)))
+    want = t.float() + res
+    g = torch.from_numpy(rng.standard_normal(width)).cuda().bfloat16()
+    dev.add_norm_quant(q, s, t, g, residual=res, total=res)
+    assert torch.equal(res.nan_to_num(1.0), want.nan_to_num(1.0))
+    same(q, s, stepped(norm64(np64(want), np64(g), 1e-6)))
+    if width % 2 == 0:
+        q2 = rows_of(rows, half, torch.int8, -half % 8)
+        dev.swiglu_quant(q2, s, t)
+        same(q2, s, stepped(swiglu64(np64(t))))
+    if width <= 8192:  # gate and up of this width each
+        gu = torch.cat([t, t.flip(1)], 1)
+        dev.swiglu_quant(q, s, gu)
+        same(q, s, stepped(swiglu64(np64(gu))))
+
+
+@pytest.mark.parametrize("rows,k,channels", [(4097, 13824, 700), (1300, 4100, 3000), (20000, 260, 300), (515, 1000, 20000)])
+def test_row_tiles_in_groups(dev, rows, k, channels):
+    """Row tiles that pass the weights in more than one group, ragged last tiles among them."""
+    rng = np.random.default_rng(rows)
+    a, w = ints(rng, rows, k, -k % 16), ints(rng, channels, k, -k % 16)
+    a_s, w_s = torch.rand(rows, device="cuda"), torch.rand(channels, device="cuda")
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.zeros(rows, channels, dtype=dtype, device="cuda")
+        dev.matmul_i8(out, a, a_s, w, w_s)
+        assert torch.equal(out.cpu(), product(a, a_s, w, w_s, None, dtype))
+
+
+def test_calls_on_two_streams_at_once(dev):
+    """Large and small products and rows interleaved on two streams: each its own results, again and again."""
+    rng = np.random.default_rng(9)
+    jobs = []
+    for rows, k, n in ((300, 2048, 4000), (64, 8960, 1536), (3, 5120, 7168), (1024, 640, 2000)):
+        a, w = ints(rng, rows, k), ints(rng, n, k)
+        a_s, w_s = torch.rand(rows, device="cuda"), torch.rand(n, device="cuda")
+        x = torch.from_numpy(some(rng, rows, k)).cuda()
+        q, s = rows_of(rows, k, torch.int8), torch.zeros(rows, device="cuda")
+        dev.quant_rows(q, s, x)
+        want = torch.zeros(rows, n, device="cuda")
+        dev.matmul_i8(want, a, a_s, w, w_s)
+        assert torch.equal(want.cpu(), product(a, a_s, w, w_s, None, torch.float32))
+        jobs.append((a, a_s, w, w_s, x, want, q.clone(), s.clone()))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(40):
+        a, a_s, w, w_s, x, want, q, s = jobs[i % 4 if i % 2 else 3 - i % 4]
+        o, q2, s2 = torch.empty_like(want), torch.empty_like(q), torch.empty_like(s)
+        outs.append((o, want, q2, q, s2, s))
+    torch.cuda.synchronize()
+    for i, (o, want, q2, q, s2, s) in enumerate(outs):
+        a, a_s, w, w_s, x = jobs[i % 4 if i % 2 else 3 - i % 4][:5]
+        dev.matmul_i8(o, a, a_s, w, w_s, stream=streams[i % 2])
+        dev.quant_rows(q2, s2, x, stream=streams[i % 2])
+    torch.cuda.synchronize()
+    for o, want, q2, q, s2, s in outs:
+        assert torch.equal(o, want) and torch.equal(q2, q) and torch.equal(s2, s)
