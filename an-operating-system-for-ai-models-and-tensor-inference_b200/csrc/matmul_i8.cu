@@ -396,7 +396,7 @@ MYOS_DEV void mma_i8(int* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
 }
 
 // 16 bytes of a row from i on; zeros from k on, where nothing is read.
-MYOS_DEV uint4 piece(const int8_t* row, int i, int k) {
+__device__ __noinline__ uint4 piece(const int8_t* row, int i, int k) {
   if (i + 16 <= k) return ld_stream(reinterpret_cast<const uint4*>(row + i));
   uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -426,9 +426,19 @@ __global__ void __launch_bounds__(512) k_few_i8(const MatArgs g) {
   pdl_wait();
   pdl_launch();
   const uint4 z = make_uint4(0, 0, 0, 0);
-  for (int b = b0; b < b1; b += U) {
+  auto multiply = [&](const uint4* w, const uint4& x, const uint4& y) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      mma_i8(acc[n], x.x, y.x, x.y, y.y, w[n].x, w[n].y);
+      mma_i8(acc[n], x.z, y.z, x.w, y.w, w[n].z, w[n].w);
+    }
+  };
+  const int whole = min(b1, g.k / 64);
+  for (int b = b0; b < whole; b += U) {
     uint4 w[U][NT], x[U], y[U];
-    if ((b + U) * 64 <= g.k && b + U <= b1) {
+    // (two branches that meet: without them the loads sink to their products, a few at
+    // a time, and 1 x 13824 x 5120 takes 21 us for 14)
+    if (b + U <= whole) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -437,24 +447,26 @@ __global__ void __launch_bounds__(512) k_few_i8(const MatArgs g) {
         x[u] = has_lo ? *reinterpret_cast<const uint4*>(lo + (b + u) * 64) : z;
         y[u] = has_hi ? *reinterpret_cast<const uint4*>(hi + (b + u) * 64) : z;
       }
-    } else {  // the last pieces of this warp, or of the row
+    } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const bool in = b + u < b1;
-        const int left = g.k - q * 16;
+        const int at = min(b + u, whole - 1) * 64;  // past the end the last again, times nothing
+        const bool in = b + u < whole;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) w[u][n] = in ? piece(wp[n], (b + u) * 64, left) : z;
-        x[u] = in && has_lo ? piece(lo, (b + u) * 64, left) : z;
-        y[u] = in && has_hi ? piece(hi, (b + u) * 64, left) : z;
+        for (int n = 0; n < NT; ++n) w[u][n] = ld_stream(reinterpret_cast<const uint4*>(wp[n] + at));
+        x[u] = in && has_lo ? *reinterpret_cast<const uint4*>(lo + at) : z;
+        y[u] = in && has_hi ? *reinterpret_cast<const uint4*>(hi + at) : z;
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) multiply(w[u], x[u], y[u]);
+  }
+  if (b1 > whole && b1 > b0) {  // the piece that k ends in
+    const int at = whole * 64, left = g.k - q * 16;
+    uint4 w[NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        mma_i8(acc[n], x[u].x, y[u].x, x[u].y, y[u].y, w[u][n].x, w[u][n].y);
-        mma_i8(acc[n], x[u].z, y[u].z, x[u].w, y[u].w, w[u][n].z, w[u][n].w);
-      }
+    for (int n = 0; n < NT; ++n) w[n] = piece(wp[n], at, left);
+    multiply(w, has_lo ? piece(lo, at, left) : z, has_hi ? piece(hi, at, left) : z);
   }
   int* const mine = parts + warp * kTok * kCh;
 #pragma unroll
