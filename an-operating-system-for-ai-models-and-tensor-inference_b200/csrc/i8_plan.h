@@ -42,6 +42,7 @@ inline I8Few i8_few(int64_t rows, int64_t k, int64_t channels) {
     if (i8_ceil(channels, 32) * f.warps < 1100) f.groups = 2;
   } else {
     f.warps = pieces > 40 ? 4 : 2;
+    if (pieces <= 16 && channels >= 27200) f.groups = 4;  // fewer blocks: 3 ns each
     if (i8_ceil(channels, 16) * 4 < 1700) {
       f.groups = 1;
       f.warps = i8_ceil(channels, 8) * 4 < 1200 && pieces > 48 ? 8 : 4;
@@ -105,34 +106,41 @@ inline I8Plan i8_plan(int64_t rows, int64_t k, int64_t channels, const I8Device&
   q.tc = 2 * kI8Channels;
   q.tiles_c = (int)i8_ceil(channels, q.tc);
   const int64_t pairs = d.one[2] / 2, paired = pairs ? steps * i8_rows(q, rows, pairs, 32) : 0;
-  // Few tiles are split along k, if the shorter way saves what a cluster costs (1.2 us,
-  // and 14 ns a row): 64 x 13824 x 5120 in 1, 2, 3 parts 33.1, 18.4, 17.4; 64 x 5120 x
-  // 27648 in 1, 2: 27.0, 32.9; 64 x 1536 x 2048 in 1, 4, 8: 5.7, 4.8, 5.5; 128 x 13824 x
-  // 5120 in 1, 2, 3 and in pairs: 30.7, 21.5, 19.5, 23.3. Two blocks a multiprocessor
-  // only where there are more than multiprocessors: they have half the stages (64 x 5120
-  // x 7168 in 2 parts: 13.0 for 11.3).
+  // Where tiles are few they are split along k, if the shorter way saves what a cluster
+  // costs (1.2 us, and 14 ns a row): 64 x 13824 x 5120 in 1, 2, 3 parts 33.1, 18.4, 17.4;
+  // 64 x 5120 x 27648 in 1, 2: 27.0, 32.9; 64 x 1536 x 2048 in 1, 4, 8: 5.7, 4.8, 5.5; 128
+  // x 13824 x 5120 in 1, 2, 3 and in pairs: 30.7, 21.5, 19.5, 23.3. Two blocks a
+  // multiprocessor only where there are more than multiprocessors: they have half the
+  // stages (64 x 5120 x 7168 in 2 parts: 13.0 for 11.3). Many rows of few channels are cut
+  // into smaller tiles as well (1745 x 7464 x 216: 13.4 in pairs, 9.3).
   p.tc = kI8Channels;
   p.tiles_c = (int)i8_ceil(channels, p.tc);
-  p.tn = (int)i8_ceil(i8_ceil(rows, i8_ceil(rows, kI8MaxRows)), 16) * 16;
-  p.tiles_r = (int)i8_ceil(rows, p.tn);
-  const int64_t tiles = (int64_t)p.tiles_c * p.tiles_r, step = i8_step(false, p.tn, false);
-  p.split = 1;
-  p.two = p.tn <= 64 && tiles > d.sms;
-  bool pair = p.tn > 64 && pairs > 0;
-  int64_t least = pair ? paired : i8_ceil(tiles, d.sms) * steps * step;
-  const int parts[] = {2, 3, 4, 6, 8};
-  for (int s : parts) {
-    const int64_t n = tiles * s;
-    const bool two = n > d.one[s];
-    if (two && (p.tn > 64 || n > d.two[s] || n > 5 * d.sms / 3)) continue;
-    const int64_t time = i8_ceil(steps, s) * step * (two ? 2 : 1) + 1200 + 14 * p.tn;
-    if (steps < 3 * s || time >= least) continue;
-    least = time;
-    p.split = s;
-    p.two = two;
-    pair = false;
+  int64_t least = 0;
+  const int parts[] = {1, 2, 3, 4, 6, 8};
+  for (int64_t r = i8_ceil(rows, kI8MaxRows); r == i8_ceil(rows, kI8MaxRows) || rows > 64; ++r) {
+    const int64_t tn = i8_ceil(i8_ceil(rows, r), 16) * 16, n_r = i8_ceil(rows, tn);
+    if (n_r < r && r > i8_ceil(rows, kI8MaxRows)) continue;  // the tiles of a smaller r
+    if ((tn < 64 || r > 2 * d.sms) && least != 0) break;
+    const int64_t tiles = p.tiles_c * n_r, step = i8_step(false, tn, false);
+    for (int s : parts) {
+      const int64_t n = tiles * s;
+      const bool two = s == 1 ? tn <= 64 && n > d.sms : n > d.one[s];
+      if (s > 1 && (steps < 3 * s || (two && (tn > 64 || n > d.two[s] || n > 5 * d.sms / 3)))) continue;
+      // of one part the tiles follow one another on a multiprocessor, of more they are all
+      // there at once; and all that is copied comes through L2, 12000 bytes a ns
+      int64_t time = i8_ceil(steps, s) * step * (s == 1 ? i8_ceil(n, d.sms) : two ? 2 : 1);
+      const int64_t l2 = tiles * steps * (kI8Channels + tn) * kI8Step / 12000;
+      if (time < l2) time = l2;
+      time += s == 1 ? 6 * tn : 1200 + 14 * tn;
+      if (least != 0 && time >= least) continue;
+      least = time;
+      p.tn = (int)tn;
+      p.tiles_r = (int)n_r;
+      p.split = s;
+      p.two = two;
+    }
   }
-  if (pair) p = q, p.split = 1;
+  if (rows > 64 && pairs > 0 && paired + 6 * q.tn <= least) p = q, p.split = 1;
   const int stage = (kI8Channels + p.tn / (p.pair ? 2 : 1)) * kI8Step;
   const int sums = p.split * p.tn * i8_wide(p.split) * 4;
   p.apart = p.split > 1 && p.tn <= 64;

@@ -396,7 +396,7 @@ MYOS_DEV void mma_i8(int* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
 }
 
 // 16 bytes of a row from i on; zeros from k on, where nothing is read.
-__device__ __noinline__ uint4 piece(const int8_t* row, int i, int k) {
+MYOS_DEV uint4 piece(const int8_t* row, int i, int k) {
   if (i + 16 <= k) return ld_stream(reinterpret_cast<const uint4*>(row + i));
   uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
