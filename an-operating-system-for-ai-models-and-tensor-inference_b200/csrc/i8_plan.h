@@ -26,8 +26,8 @@ struct I8Few {
 };
 
 // 9 to 16 rows read as many bytes of rows as of weights, so they take wide blocks,
-// and tiles from 64 MB of weights on (16 x 1536 x 151936: 48.7 here, 41.5 in tiles;
-// 16 x 5120 x 7168: 10.4, 11.3). Up to 8 rows the blocks are as small as still gives
+// and tiles from 64 MB of weights on (16 x 1536 x 151936: 48.7 here, 39.2 in tiles;
+// 16 x 5120 x 7168: 10.6, 11.3). Up to 8 rows the blocks are as small as still gives
 // each warp a few pieces of k, with some 1700 warps at least where the channels allow
 // it: 1 x 1536 x 17920 with 2, 4, 8 warps of 16 channels 6.4, 7.8, 10.3; 1 x 13824 x
 // 5120 with 4 warps of 8, 16, 32 channels 14.0, 18.1, 22.9; 1 x 8960 x 1536 with 4, 8
@@ -42,7 +42,8 @@ inline I8Few i8_few(int64_t rows, int64_t k, int64_t channels) {
     if (i8_ceil(channels, 32) * f.warps < 1100) f.groups = 2;
   } else {
     f.warps = pieces > 40 ? 4 : 2;
-    if (pieces <= 16 && channels >= 27200) f.groups = 4;  // fewer blocks: 3 ns each
+    // short rows: fewer blocks, which take 3 ns each (2 x 124 x 73276: 15.5, 11.3)
+    if (pieces <= 16 && channels >= 27200) f.groups = 4;
     if (i8_ceil(channels, 16) * 4 < 1700) {
       f.groups = 1;
       f.warps = i8_ceil(channels, 8) * 4 < 1200 && pieces > 48 ? 8 : 4;
@@ -112,7 +113,7 @@ inline I8Plan i8_plan(int64_t rows, int64_t k, int64_t channels, const I8Device&
   // x 13824 x 5120 in 1, 2, 3 and in pairs: 30.7, 21.5, 19.5, 23.3. Two blocks a
   // multiprocessor only where there are more than multiprocessors: they have half the
   // stages (64 x 5120 x 7168 in 2 parts: 13.0 for 11.3). Many rows of few channels are cut
-  // into smaller tiles as well (1745 x 7464 x 216: 13.4 in pairs, 9.3).
+  // into smaller tiles as well (4041 x 2775 x 83: 15.4 in pairs of 256 rows, 9.0).
   p.tc = kI8Channels;
   p.tiles_c = (int)i8_ceil(channels, p.tc);
   int64_t least = 0;

@@ -7,7 +7,7 @@
 //
 // k_few_i8, up to 16 rows: the weights' memory bounds it. mma.sync straight from
 // global memory, blocks of 8 to 32 channels, its warps sharing k (1 x 1536 x 151936:
-// 39.8 us, 5.9 TB/s, 0.9 of the copy rate; 1 x 1536 x 2048: 2.2 us).
+// 37.5 us, 6.2 TB/s, 0.95 of the copy rate; 1 x 1536 x 2048: 2.2 us).
 //
 // k_matmul_i8, tiles on tcgen05: 128 channels (the tensor core's M, the lanes of its
 // memory) by up to 256 rows (its N, the columns). A lane holds one channel, so a
