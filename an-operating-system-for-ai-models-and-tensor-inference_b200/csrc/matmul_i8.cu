@@ -359,13 +359,11 @@ __global__ void __launch_bounds__(kThreads)
           }
         }
       };
-      switch (split) {
+      switch (split) {  // i8_plan's parts
         case 2: join(std::integral_constant<int, 2>()); break;
         case 3: join(std::integral_constant<int, 3>()); break;
         case 4: join(std::integral_constant<int, 4>()); break;
-        case 5: join(std::integral_constant<int, 5>()); break;
         case 6: join(std::integral_constant<int, 6>()); break;
-        case 7: join(std::integral_constant<int, 7>()); break;
         default: join(std::integral_constant<int, 8>());
       }
     }

@@ -43,7 +43,7 @@ int main() {
           ok = ok && (int64_t)p.tiles_c * p.tc >= c && (int64_t)(p.tiles_c - 1) * p.tc < c;
           ok = ok && (int64_t)p.tiles_r * p.tn >= r && (int64_t)(p.tiles_r - 1) * p.tn < r;
           // every block of a cluster has k, and the whole cluster is resident at once
-          ok = ok && p.split >= 1 && p.split <= kI8MaxSplit && p.split <= steps && !(p.pair && p.split > 1);
+          ok = ok && p.split >= 1 && p.split <= kI8MaxSplit && p.split != 5 && p.split != 7 && p.split <= steps && !(p.pair && p.split > 1);
           if (p.split > 1) ok = ok && tiles * p.split <= (p.two ? d.two[p.split] : d.one[p.split]);
           ok = ok && !(p.two && (p.tn > 64 || p.pair)) && !(p.apart && p.split == 1);
           // shared memory: stages, and the sums behind or over them
