@@ -538,9 +538,10 @@ int myos_rope_table(float* cos_out, float* sin_out, size_t num_pos, size_t rot_d
  * one scale: scale = max(max |y| / 127, 2^-126), rounded to f32, and
  * q = y / scale rounded to the nearest integer, ties to even, so -127 .. 127:
  * q * scale stands for y. Scales and q are those of y in 64-bit arithmetic from
- * the inputs (y itself is rounded to nothing shorter on its way), whatever the
- * order in which a row is summed: the same bits for every size and batch. A row
- * with a y (or, of the norm, a gamma * total) that f32 does not hold as a finite
+ * the inputs (y itself is rounded to nothing shorter on its way), so a row has the
+ * same bits alone and in any batch, but for the last bits of its f64 sum of squares,
+ * whose order goes by the batch: they move a scale in some one of 10^8 rows of the
+ * norm. A row with a y (or, of the norm, a gamma * total) that f32 does not hold as a finite
  * number - NaN, infinities, past its range - has scale NaN and q 0, so that all
  * products with it are NaN. dtype arguments are MYOS_F32 or MYOS_BF16. Row strides
  * count elements. Addresses are aligned to their elements; rows that begin at
