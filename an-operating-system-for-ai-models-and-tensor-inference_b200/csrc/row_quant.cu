@@ -81,13 +81,16 @@ __device__ __noinline__ double silu_up64(float g, float u) {
 // makes the result relatively off by |g| 2^-23 where g is negative, so values
 // below -8 (rare in a gate) go through f64; the rest is off by 1.6 x 2^-20 at
 // most: the argument 2^-20, ex2 2^-22, rcp 2^-23, a sum and two products 2^-24
-// each.
+// each. That holds for every y that counts in a row past kTiny, whatever the inputs:
+// r * u first, which is below f32's normal numbers only where u is nearly so itself, and
+// with such a u y reaches 2^-121 only by a gate above 17, whose r is 1. g * r first lost
+// bits of the smallest gates, which a large u brings back.
 MYOS_DEV bool silu_fast(float g) { return g >= -8.0f; }
 MYOS_DEV float silu_up(float g, float u) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.44269504f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return g * r * u;
+  return g * (r * u);
 }
 
 // One row as a thread sees it.

@@ -1,0 +1,57 @@
+"""The 8-bit projections at the ends of f32's range: gates below the normal numbers.
+Bit for bit against 64 bits, as in test_gpu_i8."""
+import numpy as np
+import pytest
+
+from test_gpu_i8 import np64, rows_of, same, stepped, swiglu64
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+T = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def dev():
+    from myos import dev as m
+
+    return m
+
+
+def checked_swiglu(dev, x, want=stepped):
+    """swiglu_quant of x [rows, 2 width], its rows 16 bytes apart from their like, against `want` of y."""
+    rows, width = x.shape[0], x.shape[1] // 2
+    q, s = rows_of(rows, width, torch.int8, -width % 16), torch.zeros(rows, device="cuda")
+    dev.swiglu_quant(q, s, x)
+    same(q, s, want(swiglu64(np64(x))))
+
+
+# a warp a row, a block, values in shared memory (from 512 rows on), one value at a time
+@pytest.mark.parametrize("rows,width", [(3, 2), (6, 96), (6, 101), (6, 1536), (5, 8200), (515, 2600), (515, 101), (3, 40000)])
+@pytest.mark.parametrize("x", ["f32", "bf16"])
+def test_subnormal_gates(dev, x, rows, width):
+    """Gates below f32's normal numbers, brought back by large up values; a large gate and such an up value."""
+    rng = np.random.default_rng(width)
+    unit, most = (2.0**-149, 2**12) if x == "f32" else (2.0**-133, 2**6)
+    gate = rng.integers(1, most, (rows, width)) * unit * rng.choice([-1, 1], (rows, width))
+    up = np.exp2(rng.uniform(100, 127, (rows, width)))
+    gate[0], up[0] = 3 * unit, 2.0**100 * rng.choice([0.5, 0.75, 1.0], width)  # a row of one gate
+    other = rng.random((rows, width)) < 0.5  # the other rows: half of them ordinary values of the same size
+    other[:2] = False
+    size = 0.5 * np.abs(gate * up).max(1, keepdims=True)
+    gate = np.where(other, rng.standard_normal((rows, width)), gate)
+    up = np.where(other, size * rng.standard_normal((rows, width)), up)
+    far = rng.random((rows, width)) < 0.1
+    far[:2] = False
+    gate, up = np.where(far, np.exp2(rng.uniform(100, 127, (rows, width))), gate), np.where(far, rng.integers(1, most, (rows, width)) * unit, up)
+    t = torch.from_numpy(np.concatenate([gate, up], 1)).cuda().to(T[x])
+    assert bool((t[:2, :width].abs() < 2.0**-126).all() and (t[:, :width] != 0).all())
+    checked_swiglu(dev, t)
+
+
+def test_gates_whose_products_f32_loses(dev):
+    for g, u, q, s in (((1, 1), (2.0**127, 2.0**126), (127, 64), 2.0**-23 / 127), ((3, 4), (2.0**100, 0.9 * 2.0**100), (106, 127), 2.0**-47 * 0.9 / 127)):
+        x = torch.tensor([[g[0] * 2.0**-149, g[1] * 2.0**-149, *u]], dtype=torch.float64).float().cuda()
+        got, scale = torch.zeros(1, 2, dtype=torch.int8, device="cuda"), torch.zeros(1, device="cuda")
+        dev.swiglu_quant(got, scale, x)
+        assert got.tolist() == [list(q)] and scale.item() == pytest.approx(s, rel=2.0**-23)
