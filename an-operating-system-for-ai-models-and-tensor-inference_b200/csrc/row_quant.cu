@@ -45,6 +45,7 @@ struct RowArgs {
 
 constexpr float kSmallest = 1.17549435e-38f;  // 2^-126
 constexpr float kTiny = 7.8886e-31f;          // 2^-100: below it f32 products lose bits, all goes through f64
+constexpr uint64_t kPast = 0x47effffff0000000ull;  // f64's 2^128 - 2^103: rounds to no finite f32
 
 MYOS_DEV float get(const float* p) { return *p; }
 MYOS_DEV float get(const uint16_t* p) { return bf16_at(p); }
@@ -384,9 +385,8 @@ __global__ void __launch_bounds__(WARP ? 128 : SHARED ? 512 : 1024, SHARED ? 3 :
   float scale = fmaxf(KIND == kQuant ? __fdiv_rn(P, 127.0f)
                                      : (float)over127(__longlong_as_double((long long)most)),
                       kSmallest);
-  // fmaxf passes a NaN over; an infinite scale is none
-  if (!finite || most >= 0x7ff0000000000000ull || !(scale < INFINITY))
-    scale = __uint_as_float(0x7fc00000u);
+  // fmaxf passes a NaN over
+  if (!finite || most >= kPast) scale = __uint_as_float(0x7fc00000u);
   if (tid == 0) a.scales[row] = scale;
 
   // ---- the steps

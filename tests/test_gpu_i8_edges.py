@@ -1,9 +1,9 @@
-"""The 8-bit projections at the ends of f32's range: gates below the normal numbers.
-Bit for bit against 64 bits, as in test_gpu_i8."""
+"""The 8-bit projections at the ends of f32's range: gates below the normal numbers,
+rows past the largest. Bit for bit against 64 bits, as in test_gpu_i8."""
 import numpy as np
 import pytest
 
-from test_gpu_i8 import np64, rows_of, same, stepped, swiglu64
+from test_gpu_i8 import norm64, np64, rows_of, same, stepped, swiglu64
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,38 @@ def test_gates_whose_products_f32_loses(dev):
         got, scale = torch.zeros(1, 2, dtype=torch.int8, device="cuda"), torch.zeros(1, device="cuda")
         dev.swiglu_quant(got, scale, x)
         assert got.tolist() == [list(q)] and scale.item() == pytest.approx(s, rel=2.0**-23)
+
+
+# ---------------------------------------------------------------- past f32
+PAST = 2.0**128 - 2.0**103  # from here on f32 has no finite number
+
+
+def marked(y):
+    """`stepped`, a row with a y past f32 marked."""
+    q, s = stepped(y)
+    bad = ~(np.abs(y) < PAST).all(1)
+    q[bad], s[bad] = 0, np.nan
+    return q, s
+
+
+@pytest.mark.parametrize("width", [96, 101, 1536, 8200, 40000])
+@pytest.mark.parametrize("x", ["f32", "bf16"])
+def test_norms_past_f32(dev, x, width):
+    """y past f32 where gamma * total is not: such rows are marked, those that end just below are not."""
+    rows, at = 60, width // 3
+    ratio = np.concatenate([np.linspace(0.1, 9, 30), 2 * (1 + np.arange(-15, 15) * 2.0**-9)])  # y at the column, in 2^127
+    t = np.full((rows, width), 2.0**-10)
+    t[:, at] *= np.sqrt(ratio**2 * (width - 1) / (width - ratio**2))
+    t = torch.from_numpy(t).cuda().to(T[x])
+    g = torch.ones(width, device="cuda").bfloat16()
+    g[at] = 2.0**127
+    y = norm64(np64(t), np64(g), 0.0)
+    past = ~(np.abs(y) < PAST).all(1)
+    assert 10 < past.sum() < 50 and np.isfinite(y).all() and bool((t.float() * g.float()).isfinite().all())
+    q, s = rows_of(rows, width, torch.int8, -width % 16), torch.zeros(rows, device="cuda")
+    dev.add_norm_quant(q, s, t, g, eps=0.0)
+    same(q, s, marked(y))
+    total = torch.zeros(rows, width, device="cuda")
+    dev.add_norm_quant(q, s, t, g, residual=torch.zeros(rows, width, device="cuda"), total=total, eps=0.0)
+    assert torch.equal(total, t.float())
+    same(q, s, marked(y))
