@@ -342,11 +342,12 @@ __global__ void __launch_bounds__(WARP ? 128 : SHARED ? 512 : 1024, SHARED ? 3 :
   }
   const double inv = KIND == kNorm ? rsqrt(squares / a.width + (double)a.eps) : 1.0;
   const float P = __uint_as_float(top);
-  const bool finite = top < 0x7f800000u;
+  // A SwiGLU's f32 value may pass f32's range where y does not, and the other way round.
+  const bool finite = KIND == kSwiglu ? top <= 0x7f800000u : top < 0x7f800000u;
   // Nothing but zeros: scale 2^-126. (A product below f32's smallest number is 0
   // as well, and a norm may still make it large.)
   const bool zero = top == 0 && (KIND != kNorm || (squares == 0.0 && inv < 1e300));
-  const bool tiny = P < kTiny;
+  const bool all64 = P < kTiny || (KIND == kSwiglu && P >= 0x1p127f);  // the whole row in f64
 
   // the place of this thread's value n
   auto place = [&](int n) { return ((n >> 3) * team + tid) * 8 + (n & 7); };
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(WARP ? 128 : SHARED ? 512 : 1024, SHARED ? 3 :
   // ---- the largest value in 64 bits, of those that may be it
   uint64_t most = 0;
   if (KIND != kQuant && finite && !zero) {
-    const float least = tiny ? 0.0f : P * (1.0f - 2.0f * kRel<KIND>);
+    const float least = all64 ? 0.0f : P * (1.0f - 2.0f * kRel<KIND>);
     if constexpr (VEC) {
       uint32_t may = 0;  // (most threads have none)
       if (largest >= least) {
@@ -395,7 +396,7 @@ __global__ void __launch_bounds__(WARP ? 128 : SHARED ? 512 : 1024, SHARED ? 3 :
   // Value i by its f32 value p: on which side of the nearest border it lies, exactly
   // (a border times the scale has 32 bits; plain rows compare through one fma's sign).
   auto decide = [&](int i, float p) {
-    if (tiny) return (int)rint(r.exact(i, inv) / (double)scale);
+    if (all64) return (int)rint(r.exact(i, inv) / (double)scale);
     const float v = p * per, border = floorf(v) + 0.5f;
     float side;
     if (KIND == kQuant) {
@@ -419,7 +420,7 @@ __global__ void __launch_bounds__(WARP ? 128 : SHARED ? 512 : 1024, SHARED ? 3 :
       if (good && !zero) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] = step<KIND>(p[e], per, edge);
-        if (tiny) {
+        if (all64) {
           unsure |= 255u << (8 * c);
         } else if (open<KIND>(edge)) {
 #pragma unroll
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(WARP ? 128 : SHARED ? 512 : 1024, SHARED ? 3 :
       const float p = r.value(i);
       float edge = 0.0f;
       const uint32_t n = step<KIND>(p, per, edge);
-      q[i] = (int8_t)(!good || zero ? 0 : open<KIND>(edge) || tiny ? decide(i, p) : (int)n);
+      q[i] = (int8_t)(!good || zero ? 0 : open<KIND>(edge) || all64 ? decide(i, p) : (int)n);
     }
   }
 }

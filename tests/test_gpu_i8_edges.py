@@ -90,3 +90,20 @@ def test_norms_past_f32(dev, x, width):
     dev.add_norm_quant(q, s, t, g, residual=torch.zeros(rows, width, device="cuda"), total=total, eps=0.0)
     assert torch.equal(total, t.float())
     same(q, s, marked(y))
+
+
+@pytest.mark.parametrize("rows", [300, 3000])
+@pytest.mark.parametrize("width", [64, 101, 1536, 2600])
+def test_swiglu_next_to_the_largest_number(dev, rows, width):
+    """y on either side of f32's end, closer to it than an f32 product is to y."""
+    rng = np.random.default_rng(rows + width)
+    gate, up = rng.standard_normal((rows, width)), 1e37 * rng.standard_normal((rows, width))
+    at = rng.integers(0, width, rows)
+    g = rng.uniform(1.3, 4, rows).astype(np.float32).astype(np.float64)
+    u = (PAST / (g / (1 + np.exp(-g)))).astype(np.float32)
+    u = (u.view(np.int32) + rng.integers(-2, 3, rows).astype(np.int32)).view(np.float32)
+    gate[np.arange(rows), at], up[np.arange(rows), at] = g, u * rng.choice([-1, 1], rows)
+    t = torch.from_numpy(np.concatenate([gate, up], 1).astype(np.float32)).cuda()
+    y = np.abs(swiglu64(np64(t))).max(1)
+    assert 0.3 < (y < PAST).mean() < 0.7 and (np.abs(y / PAST - 1) < 2.0**-20).all()
+    checked_swiglu(dev, t, marked)
