@@ -29,6 +29,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 
 #include "i8_plan.h"
@@ -53,7 +54,10 @@ struct MatArgs {
   I8Plan plan;
 };
 
-__device__ uint32_t g_wait_failed;
+__device__ uint32_t g_wait_failed, g_wait_taken;
+
+// Reads and clears at once: what fails meanwhile is the next answer's.
+__global__ void k_take_failed() { g_wait_taken = atomicExch(&g_wait_failed, 0u); }
 
 MYOS_DEV float scaled(int sum, float as, float ws, float bias) {
   return __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(sum), as), ws), bias);
@@ -652,17 +656,22 @@ int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const 
 }
 
 int myos_dev_matmul_i8_status(void) {
-  uint32_t failed = 0, none = 0;
-  if (cudaMemcpyFromSymbol(&failed, g_wait_failed, sizeof failed) != cudaSuccess) {
+  static std::mutex one;  // callers share the answer's place
+  const std::lock_guard<std::mutex> hold(one);
+  uint32_t failed = 0;
+  // a copy from a symbol waits for the default stream, and that for no other that was
+  // made non-blocking
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) {
+    k_take_failed<<<1, 1>>>();
+    e = counted(cudaGetLastError());
+  }
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&failed, g_wait_taken, sizeof failed);
+  if (e != cudaSuccess) {
     cudaGetLastError();
     return MYOS_ERR_CUDA;
   }
-  if (failed == 0) return MYOS_OK;
-  if (cudaMemcpyToSymbol(g_wait_failed, &none, sizeof none) != cudaSuccess) {
-    cudaGetLastError();
-    return MYOS_ERR_CUDA;
-  }
-  return MYOS_ERR_TIMEOUT;
+  return failed ? MYOS_ERR_TIMEOUT : MYOS_OK;
 }
 
 }  // extern "C"

@@ -65,7 +65,7 @@ matmul_i8 = _m.matmul_i8
 
 def matmul_i8_status(device=None) -> None:
     """Raises MyosError if a bounded wait inside a matmul_i8 on `device` (default: the
-    current one) has run out since the last such call; waits for the device."""
+    current one) has run out since the last such call; waits for all its streams."""
     with torch.cuda.device(device):
         st = _lib.load().myos_dev_matmul_i8_status()
     if st != 0:

@@ -590,8 +590,8 @@ int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const 
                        size_t k, size_t channels, void* stream);
 
 /* MYOS_OK, or MYOS_ERR_TIMEOUT if a wait of a myos_dev_matmul_i8 on the current
- * device has run out since the last such answer. Waits for the device; not for
- * use in a capture. */
+ * device has run out since the last such answer. Waits for all streams of the device;
+ * not for use in a capture. */
 int myos_dev_matmul_i8_status(void);
 
 /* Library version string and the build's target architecture. */

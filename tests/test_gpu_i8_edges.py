@@ -1,5 +1,5 @@
 """The 8-bit projections at the ends of f32's range: gates below the normal numbers,
-rows past the largest. Bit for bit against 64 bits, as in test_gpu_i8."""
+rows past the largest. Bit for bit against 64 bits, as in test_gpu_i8. And the status."""
 import numpy as np
 import pytest
 
@@ -107,3 +107,18 @@ def test_swiglu_next_to_the_largest_number(dev, rows, width):
     y = np.abs(swiglu64(np64(t))).max(1)
     assert 0.3 < (y < PAST).mean() < 0.7 and (np.abs(y / PAST - 1) < 2.0**-20).all()
     checked_swiglu(dev, t, marked)
+
+
+# ---------------------------------------------------------------- the status
+def test_the_status_waits_for_every_stream(dev):
+    """A product on a stream that the default stream does not wait for is over when the status is known."""
+    a = torch.ones(4096, 4096, dtype=torch.int8, device="cuda")
+    one, out = torch.ones(4096, device="cuda"), torch.zeros(4096, 4096, device="cuda")
+    dev.matmul_i8(out, a, one, a, one)
+    dev.matmul_i8_status()
+    side = torch.cuda.Stream()
+    for _ in range(1000):
+        dev.matmul_i8(out, a, one, a, one, stream=side)
+    dev.matmul_i8_status()
+    assert side.query()
+    assert bool((out == 4096).all())
