@@ -25,6 +25,22 @@ MYOS_DEV uint4 ld_stream(const uint4* p) {
   return r;
 }
 
+// The same of memory that an earlier kernel of the stream may have written: not through
+// the read-only path, which is for what nobody writes while this kernel is resident (under
+// a programmatic edge the earlier kernel still does). p has to come from after_wait.
+MYOS_DEV uint4 ld_once(const uint4* p) {
+  uint4 r;
+  asm("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+      : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+      : "l"(p));
+  return r;
+}
+// After pdl_wait: the loads by p stay behind it, in whatever order among themselves.
+template <class T>
+MYOS_DEV void after_wait(const T*& p) {
+  asm volatile("" : "+l"(p));
+}
+
 MYOS_DEV float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

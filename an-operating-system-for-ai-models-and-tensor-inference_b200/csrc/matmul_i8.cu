@@ -399,7 +399,7 @@ MYOS_DEV void mma_i8(int* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
 
 // 16 bytes of a row from i on; zeros from k on, where nothing is read.
 MYOS_DEV uint4 piece(const int8_t* row, int i, int k) {
-  if (i + 16 <= k) return ld_stream(reinterpret_cast<const uint4*>(row + i));
+  if (i + 16 <= k) return *reinterpret_cast<const uint4*>(row + i);
   uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int e = 0; e < 16; ++e)
@@ -427,6 +427,8 @@ __global__ void __launch_bounds__(512) k_few_i8(const MatArgs g) {
   int acc[NT][4] = {};
   pdl_wait();
   pdl_launch();
+#pragma unroll
+  for (int n = 0; n < NT; ++n) after_wait(wp[n]);
   const uint4 z = make_uint4(0, 0, 0, 0);
   auto multiply = [&](const uint4* w, const uint4& x, const uint4& y) {
 #pragma unroll
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(512) k_few_i8(const MatArgs g) {
       for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-          w[u][n] = ld_stream(reinterpret_cast<const uint4*>(wp[n] + (b + u) * 64));
+          w[u][n] = ld_once(reinterpret_cast<const uint4*>(wp[n] + (b + u) * 64));
         x[u] = has_lo ? *reinterpret_cast<const uint4*>(lo + (b + u) * 64) : z;
         y[u] = has_hi ? *reinterpret_cast<const uint4*>(hi + (b + u) * 64) : z;
       }
@@ -455,7 +457,7 @@ __global__ void __launch_bounds__(512) k_few_i8(const MatArgs g) {
         const int at = min(b + u, whole - 1) * 64;  // past the end the last again, times nothing
         const bool in = b + u < whole;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) w[u][n] = ld_stream(reinterpret_cast<const uint4*>(wp[n] + at));
+        for (int n = 0; n < NT; ++n) w[u][n] = ld_once(reinterpret_cast<const uint4*>(wp[n] + at));
         x[u] = in && has_lo ? *reinterpret_cast<const uint4*>(lo + at) : z;
         y[u] = in && has_hi ? *reinterpret_cast<const uint4*>(hi + at) : z;
       }

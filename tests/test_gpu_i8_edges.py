@@ -1,5 +1,6 @@
 """The 8-bit projections at the ends of f32's range: gates below the normal numbers,
-rows past the largest. Bit for bit against 64 bits, as in test_gpu_i8. And the status."""
+rows past the largest. Bit for bit against 64 bits, as in test_gpu_i8.
+The status, and kernels one after another."""
 import numpy as np
 import pytest
 
@@ -122,3 +123,44 @@ def test_the_status_waits_for_every_stream(dev):
     dev.matmul_i8_status()
     assert side.query()
     assert bool((out == 4096).all())
+
+
+# ---------------------------------------------------------------- one kernel after another
+@pytest.mark.parametrize("rows", [1, 5, 8, 12, 16, 40, 300])
+@pytest.mark.parametrize("k,channels", [(100, 600), (1000, 333), (640, 1024), (4090, 512)])
+def test_products_of_what_the_kernel_before_wrote(dev, rows, k, channels):
+    """Weights and rows in 8 bits, then their product, again and again over the same buffers: each product
+    reads what the calls before it have just written."""
+    rng = np.random.default_rng(rows + k)
+    n = 12
+    x, w = (torch.from_numpy(rng.standard_normal((n, m, k)).astype(np.float32)).cuda() for m in (rows, channels))
+    q, s = rows_of(rows, k, torch.int8, -k % 16), torch.zeros(rows, device="cuda")
+    wq, ws = rows_of(channels, k, torch.int8, -k % 16), torch.zeros(channels, device="cuda")
+    out = torch.zeros(n, rows, channels, device="cuda")
+    want = []
+    for i in range(n):
+        a, b = stepped(np64(x[i])), stepped(np64(w[i]))
+        y = (a[0].astype(np.int64) @ b[0].astype(np.int64).T).astype(np.float32) * a[1][:, None] * b[1][None, :]
+        want.append(torch.from_numpy(y))
+
+    def chain(order):
+        for i in order:
+            dev.quant_rows(wq, ws, w[i])
+            dev.quant_rows(q, s, x[i])
+            dev.matmul_i8(out[i], q, s, wq, ws)
+            dev.quant_rows(q, s, x[(i + 1) % n])  # the rows alone anew, the weights as they are
+            dev.quant_rows(q, s, x[i])
+            dev.matmul_i8(out[i], q, s, wq, ws)
+
+    chain(range(n))
+    for i in range(n):
+        assert torch.equal(out[i].cpu(), want[i])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        chain(reversed(range(n)))
+    for _ in range(3):
+        out.zero_()
+        for _ in range(5):
+            g.replay()
+        for i in range(n):
+            assert torch.equal(out[i].cpu(), want[i])
