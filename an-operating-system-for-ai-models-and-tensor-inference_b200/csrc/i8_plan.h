@@ -13,6 +13,7 @@ constexpr int kI8MaxStages = 12;
 constexpr int kI8Smem = 200 * 1024;     // a block's stages,
 constexpr int kI8SmemTwo = 109 * 1024;  // where two blocks share a multiprocessor
 constexpr int kI8MaxSplit = 8;          // blocks that share a tile's k: a portable cluster
+constexpr int kI8Parts[] = {1, 2, 3, 4, 6, 8};
 constexpr int kI8FewRows = 16;
 
 inline int64_t i8_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -74,6 +75,25 @@ struct I8Device {
   int one[kI8MaxSplit + 1], two[kI8MaxSplit + 1];
 };
 
+// Fills in what the device holds in clusters. known: a word for each size (std::atomic, 0
+// at first). ask(s, two, &blocks): whether it could be asked; an answer that could not be
+// had counts as no room in this call, and is asked for again in the next.
+template <class Word, class Ask>
+inline void i8_room(I8Device& d, Word* known, const Ask& ask) {
+  for (int s : kI8Parts) {
+    if (s == 1) continue;
+    uint64_t v = known[s].load();
+    if (v == 0) {
+      int one = 0, two = 0;
+      const bool first = ask(s, false, &one), second = ask(s, true, &two);
+      v = (uint64_t)1 << 63 | (uint64_t)(first ? one : 0) << 31 | (uint64_t)(second ? two : 0);
+      if (first && second) known[s].store(v);
+    }
+    d.one[s] = (int)(v >> 31 & 0x7fffffff);
+    d.two[s] = (int)(v & 0x7fffffff);
+  }
+}
+
 // A step's time in a block that waits for its copies alone, in ns, and where pairs fill
 // the device and its power (8192 x 8192 x 8192).
 inline int64_t i8_step(bool pair, int64_t tn, bool filled) {
@@ -117,13 +137,12 @@ inline I8Plan i8_plan(int64_t rows, int64_t k, int64_t channels, const I8Device&
   p.tc = kI8Channels;
   p.tiles_c = (int)i8_ceil(channels, p.tc);
   int64_t least = 0;
-  const int parts[] = {1, 2, 3, 4, 6, 8};
   for (int64_t r = i8_ceil(rows, kI8MaxRows); r == i8_ceil(rows, kI8MaxRows) || rows > 64; ++r) {
     const int64_t tn = i8_ceil(i8_ceil(rows, r), 16) * 16, n_r = i8_ceil(rows, tn);
     if (n_r < r && r > i8_ceil(rows, kI8MaxRows)) continue;  // the tiles of a smaller r
     if ((tn < 64 || r > 2 * d.sms) && least != 0) break;
     const int64_t tiles = p.tiles_c * n_r, step = i8_step(false, tn, false);
-    for (int s : parts) {
+    for (int s : kI8Parts) {
       const int64_t n = tiles * s;
       const bool two = s == 1 ? tn <= 64 && n > d.sms : n > d.one[s];
       if (s > 1 && (steps < 3 * s || (two && (tn > 64 || n > d.two[s] || n > 5 * d.sms / 3)))) continue;

@@ -552,7 +552,7 @@ cudaError_t launch(const MatArgs& g, const CUtensorMap& wmap, const CUtensorMap&
 // memory, the occupancy calls answer one block a multiprocessor.
 __global__ void __launch_bounds__(kThreads) k_room() {}
 
-// The clusters that the current device holds, asked once.
+// The clusters that the current device holds.
 I8Device this_device() {
   static std::atomic<uint64_t> known[64][kI8MaxSplit + 1];
   I8Device d = {};
@@ -560,34 +560,27 @@ I8Device this_device() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return d;  // nothing is split
   const void* const kernel = (const void*)k_room;
-  for (int s = 2; s <= kI8MaxSplit; ++s) {
-    uint64_t v = known[dev][s].load(std::memory_order_relaxed);
-    if (v == 0) {
-      int n[2] = {0, 0};
-      for (int two = 0; two < 2; ++two) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)s);
-        cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = (two ? kI8SmemTwo : kI8Smem) + 4096;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)s;
-        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        static std::atomic<uint64_t> raised{0};
-        if (raise_smem_limit(kernel, kI8Smem + 4096, &raised) != cudaSuccess ||
-            cudaOccupancyMaxActiveClusters(&n[two], kernel, &cfg) != cudaSuccess) {
-          cudaGetLastError();
-          n[two] = 0;
-        }
-      }
-      v = (uint64_t)1 << 63 | (uint64_t)(n[0] * s) << 31 | (uint64_t)(n[1] * s);
-      known[dev][s].store(v, std::memory_order_relaxed);
+  i8_room(d, known[dev], [&](int s, bool two, int* blocks) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)s);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (two ? kI8SmemTwo : kI8Smem) + 4096;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)s;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    static std::atomic<uint64_t> raised{0};
+    int clusters = 0;
+    if (raise_smem_limit(kernel, kI8Smem + 4096, &raised) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
     }
-    d.one[s] = (int)(v >> 31 & 0x7fffffff);
-    d.two[s] = (int)(v & 0x7fffffff);
-  }
+    *blocks = clusters * s;
+    return true;
+  });
   return d;
 }
 
