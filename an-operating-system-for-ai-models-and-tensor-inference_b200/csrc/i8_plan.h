@@ -27,13 +27,13 @@ struct I8Few {
 };
 
 // 9 to 16 rows read as many bytes of rows as of weights, so they take wide blocks,
-// and tiles from 64 MB of weights on (16 x 1536 x 151936: 48.7 here, 39.2 in tiles;
-// 16 x 5120 x 7168: 10.6, 11.3). Up to 8 rows the blocks are as small as still gives
+// and tiles from 64 MB of weights on (16 x 1536 x 151936: 47.7 here, 39.5 in tiles;
+// 16 x 5120 x 7168: 10.3, 10.2). Up to 8 rows the blocks are as small as still gives
 // each warp a few pieces of k, with some 1700 warps at least where the channels allow
-// it: 1 x 1536 x 17920 with 2, 4, 8 warps of 16 channels 6.4, 7.8, 10.3; 1 x 13824 x
-// 5120 with 4 warps of 8, 16, 32 channels 14.0, 18.1, 22.9; 1 x 8960 x 1536 with 4, 8
-// warps of 8 channels 7.9, 5.7; 1 x 5120 x 27648 with 2, 4 warps of 16 channels 27.1,
-// 24.3.
+// it: 1 x 1536 x 17920 with 2, 4, 8 warps of 16 channels 6.5, 8.0, 9.8; 1 x 13824 x
+// 5120 with 4 warps of 8, 16, 32 channels 14.0, 17.5, 21.6; 1 x 8960 x 1536 with 4, 8
+// warps of 8 channels 7.5, 5.3; 1 x 5120 x 27648 with 2, 4 warps of 16 channels 28.9,
+// 25.3.
 inline I8Few i8_few(int64_t rows, int64_t k, int64_t channels) {
   I8Few f = {rows <= 8 || (rows <= kI8FewRows && k * channels < ((int64_t)64 << 20)), 2, 2};
   const int64_t pieces = i8_ceil(k, 64);
@@ -43,7 +43,7 @@ inline I8Few i8_few(int64_t rows, int64_t k, int64_t channels) {
     if (i8_ceil(channels, 32) * f.warps < 1100) f.groups = 2;
   } else {
     f.warps = pieces > 40 ? 4 : 2;
-    // short rows: fewer blocks, which take 3 ns each (2 x 124 x 73276: 15.5, 11.3)
+    // short rows: fewer blocks, which take 3 ns each (2 x 128 x 73276: 7.7, 5.9)
     if (pieces <= 16 && channels >= 27200) f.groups = 4;
     if (i8_ceil(channels, 16) * 4 < 1700) {
       f.groups = 1;

@@ -19,12 +19,13 @@
 // cluster shares a tile's k and adds its parts through shared memory.
 //
 // What bounds it: of many rows the tensor cores and the device's power (4097 x 5120 x
-// 27648: 345 us with the tensor pipe busy 91% of the time at full clock; 360 to 430 in a
-// row of calls, where the clock falls under the power limit; 8192 x 8192 x 8192 340 us,
-// 3.2 x 10^15 operations a second). Of 64 x 13824 x 5120 (17.0 us) the weights' way to
-// 120 multiprocessors (11 us at the copy rate), a block's start and first copy (1.6 us)
-// and the cluster's sums. Of 333 x 5120 x 7168 (15.1 us) copies from L2, 29 KB a step
-// and block, 40 steps in 8 us, then 9.5 MB of results at once.
+// 27648: 345 us cold under the profiler, the tensor pipe busy 91% of the time at full
+// clock; 380 to 425 in a row of calls, where the clock falls under the power limit; 8192
+// x 8192 x 8192 335 to 346 us, 3.2 x 10^15 operations a second). Of 64 x 13824 x 5120
+// (16.9 us) the weights' way to 120 multiprocessors (11 us at the copy rate), a block's
+// start and first copy (1.6 us) and the cluster's sums. Of 333 x 5120 x 7168 (15.1 us)
+// copies from L2, 29 KB a step and block, 40 steps in 8 us, then 9.5 MB of results at
+// once.
 #include <cudaTypedefs.h>
 #include <math.h>
 

@@ -14,9 +14,11 @@
 //
 // A row is read once into registers (a block per row, or a warp where it has at most
 // 1024 values), two meetings of the block, q and scale out. f32 rows are bound by the
-// memory (8191 x 5120: 6.25 TB/s for the norm, 6.6 for plain rows), bf16 rows by
-// instructions (27648 x 5120: 93 us, 4.6 TB/s; 4099 x 13824 SwiGLU: 84 us, 3.4), a few
-// rows by their latency (norm 1 x 1536: 2.3 us).
+// memory (8191 x 5120: 6.25 TB/s for the norm, 5.4 with bf16 x; 6.6 for plain rows), bf16
+// rows by instructions (27648 x 5120: 93 us, 4.6 TB/s), SwiGLU too (4099 x 13824 bf16:
+// 85 us, 3.3; f32: 106 us, 4.8), a few rows by their latency (norm 1 x 1536: 2.3 us). Of a
+// SwiGLU whose up values do not begin at 16 bytes, and of other rows that do not, a block
+// takes one value at a time, three times over: 4099 x 13823 bf16 367 us.
 #include <math.h>
 
 #include "common.cuh"
@@ -480,15 +482,16 @@ cudaError_t launch_kind(const RowArgs& a, bool vec, cudaStream_t st) {
   const int chunks = (a.width + 7) / 8;
   // Few rows: as many threads as chunks, for the latency. Many: more chunks a thread,
   // so that more rows are on their way at once (norm of 8191 x 5120 f32 with 1, 2, 4:
-  // 118, 99, 91 us; of 8191 x 1536: 32, 30, 36 us; of 512 x 5120: 11.3, 11.5, 11.3 us,
-  // at an earlier stage of the kernel).
+  // 104, 92, 87 us; of 8191 x 1536: 33, 29, 34 us; of 512 x 5120: 10.7, 10.6, 10.3 us; of
+  // 64 x 5120: 3.8, 3.9, 4.5 us; rows 27648 x 5120 bf16: 168, 111, 93 us).
   const int many = a.rows < 512 ? 1 : chunks <= 256 ? 2 : 4;
   const int each = chunks > 2048 || many == 4 ? 4 : chunks > 1024 || many == 2 ? 2 : 1;
   const int threads = (chunks + 32 * each - 1) / (32 * each) * 32;
   if (each == 1) return launch<KIND, XT, 1, true, false>(a, threads, st);
   if (each == 2) return launch<KIND, XT, 2, true, false>(a, threads, st);
-  // SwiGLU's values in shared memory: 40 registers a thread, three rows at once where
-  // held in registers there were two (4099 x 13824 bf16: 91, 84 us).
+  // SwiGLU's values in shared memory: 40 registers a thread (20 words of it spilled),
+  // three rows at once where held in registers there were two (4099 x 13824 bf16: 91, 85
+  // us; f32: 110, 106; 512 x 8960 f32: 14.3, 13.4).
   if constexpr (KIND == kSwiglu)
     if (many == 4 && chunks <= 2048) return launch<KIND, XT, 4, true, false, true>(a, threads, st);
   return launch<KIND, XT, 4, true, false>(a, threads, st);

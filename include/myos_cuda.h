@@ -539,14 +539,17 @@ int myos_rope_table(float* cos_out, float* sin_out, size_t num_pos, size_t rot_d
  * q = y / scale rounded to the nearest integer, ties to even, so -127 .. 127:
  * q * scale stands for y. Scales and q are those of y in 64-bit arithmetic from
  * the inputs (y itself is rounded to nothing shorter on its way), so a row has the
- * same bits alone and in any batch, but for the last bits of its f64 sum of squares,
- * whose order goes by the batch: they move a scale in some one of 10^8 rows of the
- * norm. A row with a y (or, of the norm, a gamma * total) that f32 does not hold as a finite
+ * same bits alone and in any batch, but for the last bits of the norm's factor in f64:
+ * the order of its sum of squares goes by the batch (and by the rows' alignment), which
+ * moves a scale in some one of 2 x 10^9 rows; and a y of the norm that lies on a border between two steps as far as
+ * f64 tells (a row of one value, an eps far above the squares) may go either way. A row with a y (or, of the norm, a gamma * total) that f32 does not hold as a finite
  * number - NaN, infinities, past its range - has scale NaN and q 0, so that all
  * products with it are NaN. dtype arguments are MYOS_F32 or MYOS_BF16. Row strides
  * count elements. Addresses are aligned to their elements; rows that begin at
- * multiples of 16 bytes (q: 8) are faster, and so are widths up to 32768. rows is
- * below 2^31, a row's width at most MYOS_I8_MAX_K.
+ * multiples of 16 bytes (q: 8) are faster, and so are widths up to 32768; of the
+ * SwiGLU the up values as well, so widths of whole 16 bytes (4099 rows of 13823 bf16
+ * values take four times as long as of 13824). rows is below 2^31, a row's width
+ * (the product's k) 1 .. MYOS_I8_MAX_K.
  * ------------------------------------------------------------------------- */
 
 /* The longest row of 8-bit values: (2^31 - 1) / 128^2, where a sum of products
@@ -580,10 +583,13 @@ int myos_dev_swiglu_quant(int8_t* d_q, size_t q_stride, float* d_scales, const v
  * and the bias added, each rounded to f32; out (f32 or bf16) is rounded from
  * that. The same bits however the work is split. d_a, d_w and their row strides are
  * multiples of 16 bytes (MYOS_ERR_ARG); k need not be one: what lies between k and
- * the stride is not read. rows and channels are at most 2^31 - 256. The waits inside
- * the kernel are bounded (about a second); were one to run out, the results it
- * served are NaN and myos_dev_matmul_i8_status says so. The first call on a device
- * asks it how many clusters it holds. */
+ * the stride is not read. rows and channels are at most 2^31 - 256. Each wait for
+ * copies or products inside the kernel is bounded by about a second; were one to run
+ * out, the results it served are NaN, myos_dev_matmul_i8_status says so, and the call
+ * may take some fifteen seconds (its copies in flight are waited for one by one). The
+ * meetings of a cluster's blocks and the allocation of tensor memory have no limit of
+ * their own: they wait for blocks whose waits have. The first call on a device asks it
+ * how many clusters it holds. */
 int myos_dev_matmul_i8(void* d_out, int32_t out_dtype, size_t out_stride, const int8_t* d_a,
                        size_t a_stride, const float* d_a_scales, const int8_t* d_w,
                        size_t w_stride, const float* d_w_scales, const float* d_bias, size_t rows,
