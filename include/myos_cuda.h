@@ -534,22 +534,22 @@ int myos_rope_table(float* cos_out, float* sin_out, size_t num_pos, size_t rot_d
  * (myos_dev_swiglu_quant); down_proj. A weight's channels are put in 8 bits
  * once, by myos_dev_quant_rows.
  *
- * The common rules are those of the section above. A row of 8-bit values y has
- * one scale: scale = max(max |y| / 127, 2^-126), rounded to f32, and
- * q = y / scale rounded to the nearest integer, ties to even, so -127 .. 127:
- * q * scale stands for y. Scales and q are those of y in 64-bit arithmetic from
- * the inputs (y itself is rounded to nothing shorter on its way), so a row has the
- * same bits alone and in any batch, but for the last bits of the norm's factor in f64:
- * the order of its sum of squares goes by the batch (and by the rows' alignment), which
- * moves a scale in some one of 2 x 10^9 rows; and a y of the norm that lies on a border between two steps as far as
- * f64 tells (a row of one value, an eps far above the squares) may go either way. A row with a y (or, of the norm, a gamma * total) that f32 does not hold as a finite
- * number - NaN, infinities, past its range - has scale NaN and q 0, so that all
- * products with it are NaN. dtype arguments are MYOS_F32 or MYOS_BF16. Row strides
- * count elements. Addresses are aligned to their elements; rows that begin at
- * multiples of 16 bytes (q: 8) are faster, and so are widths up to 32768; of the
- * SwiGLU the up values as well, so widths of whole 16 bytes (4099 rows of 13823 bf16
- * values take four times as long as of 13824). rows is below 2^31, a row's width
- * (the product's k) 1 .. MYOS_I8_MAX_K.
+ * The common rules are those of the section above. A row of 8-bit values y has one scale:
+ * scale = max(max |y| / 127, 2^-126), rounded to f32, and q = y / scale rounded to the
+ * nearest integer, ties to even, so -127 .. 127: q * scale stands for y. Scales and q are
+ * those of y in 64-bit arithmetic from the inputs (y itself is rounded to nothing shorter
+ * on its way), so a row has the same bits alone and in any batch, but for the last bits
+ * of the norm's factor in f64: the order of its sum of squares goes by the batch (and by
+ * the rows' alignment), which moves a scale in some one of 2 x 10^9 rows; and a y of the
+ * norm that lies on a border between two steps as far as f64 tells (a row of one value,
+ * an eps far above the squares) may go either way. A row with a y (or, of the norm, a
+ * gamma * total) that f32 does not hold as a finite number - NaN, infinities, past its
+ * range - has scale NaN and q 0, so that all products with it are NaN. dtype arguments
+ * are MYOS_F32 or MYOS_BF16. Row strides count elements. Addresses are aligned to their
+ * elements; rows that begin at multiples of 16 bytes (q: 8) are faster, and so are widths
+ * up to 32768; of the SwiGLU the up values as well, so widths of whole 16 bytes (4099
+ * rows of 13823 bf16 values take four times as long as of 13824). rows is below 2^31, a
+ * row's width (the product's k) 1 .. MYOS_I8_MAX_K.
  * ------------------------------------------------------------------------- */
 
 /* The longest row of 8-bit values: (2^31 - 1) / 128^2, where a sum of products
