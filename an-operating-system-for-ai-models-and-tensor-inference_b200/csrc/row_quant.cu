@@ -111,7 +111,8 @@ struct Row {
     if (KIND == kSwiglu) return silu_up64(get(x + i), get(x + width + i));
     // in place the inputs are gone: the total was written by this thread
     const float t = total ? total[i] : residual ? __fadd_rn(get(x + i), residual[i]) : get(x + i);
-    return (double)bf16_at(gamma + i) * ((double)t * inv);
+    // each product rounded: drawn into decide's difference, the last one would not be
+    return __dmul_rn((double)bf16_at(gamma + i), __dmul_rn((double)t, inv));
   }
 
   // The f32 values that go with y (of the norm: gamma * total, without its

@@ -1,5 +1,5 @@
 """The 8-bit projections at the ends of f32's range: gates below the normal numbers,
-rows past the largest. Bit for bit against 64 bits, as in test_gpu_i8.
+rows past the largest, borders between steps. Bit for bit against 64 bits, as in test_gpu_i8.
 The status, and kernels one after another."""
 import numpy as np
 import pytest
@@ -108,6 +108,28 @@ def test_swiglu_next_to_the_largest_number(dev, rows, width):
     y = np.abs(swiglu64(np64(t))).max(1)
     assert 0.3 < (y < PAST).mean() < 0.7 and (np.abs(y / PAST - 1) < 2.0**-20).all()
     checked_swiglu(dev, t, marked)
+
+
+# ---------------------------------------------------------------- on a border
+@pytest.mark.parametrize("width", [96, 101, 1536, 8200, 40000])
+@pytest.mark.parametrize("x", ["f32", "bf16"])
+def test_norms_on_a_border(dev, x, width):
+    """Rows whose factor is 1/5, which f64 does not hold, and whose y in f64 is on a border all the same: each
+    product is rounded, so a tie is one, and goes to the even step."""
+    rng = np.random.default_rng(width)
+    t = np.full((4, width), 5.0)
+    pairs = rng.permutation(width - 1)[: (width - 1) // 2 * 2] + 1
+    t[:, pairs[::2]], t[:, pairs[1::2]] = 1.0, 7.0  # 1 + 49 = 25 + 25
+    t *= rng.choice([-1, 1], (4, width))
+    g = 5.0 * rng.integers(0, 26, width) * rng.choice([-1, 1], width) / np.where(t[0] == 5, 5, 1)
+    g[0] = 254.0  # of a total of 5: the scale is 2
+    g = np.where(np.abs(g) * np.abs(t[0]) > 1270, 5.0, g)
+    t, g = torch.from_numpy(t).cuda().to(T[x]), torch.from_numpy(g).cuda().bfloat16()
+    y = norm64(np64(t), np64(g), 0.0)
+    assert (np.abs(y).max(1) == 254).all() and ((np.abs(y) % 2) == 1).sum() > width // 4
+    q, s = rows_of(4, width, torch.int8, -width % 16), torch.zeros(4, device="cuda")
+    dev.add_norm_quant(q, s, t, g, eps=0.0)
+    same(q, s, stepped(y))
 
 
 # ---------------------------------------------------------------- the status
