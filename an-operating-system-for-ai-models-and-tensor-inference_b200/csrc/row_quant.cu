@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(WARP ? 128 : SHARED ? 512 : 1024, SHARED ? 3 :
   // Nothing but zeros: scale 2^-126. (A product below f32's smallest number is 0
   // as well, and a norm may still make it large.)
   const bool zero = top == 0 && (KIND != kNorm || (squares == 0.0 && inv < 1e300));
-  const bool all64 = P < kTiny || (KIND == kSwiglu && P >= 0x1p127f);  // the whole row in f64
+  const bool all64 = P < kTiny || (KIND == kSwiglu && P == INFINITY);  // the steps all in f64
 
   // the place of this thread's value n
   auto place = [&](int n) { return ((n >> 3) * team + tid) * 8 + (n & 7); };
@@ -358,7 +358,8 @@ __global__ void __launch_bounds__(WARP ? 128 : SHARED ? 512 : 1024, SHARED ? 3 :
   // ---- the largest value in 64 bits, of those that may be it
   uint64_t most = 0;
   if (KIND != kQuant && finite && !zero) {
-    const float least = all64 ? 0.0f : P * (1.0f - 2.0f * kRel<KIND>);
+    const float least =
+        P < kTiny ? 0.0f : fminf(P, 3.40282347e38f) * (1.0f - 2.0f * kRel<KIND>);
     if constexpr (VEC) {
       uint32_t may = 0;  // (most threads have none)
       if (largest >= least) {
